@@ -53,6 +53,8 @@ extern "C" {
 #define TOKMIX_DTYPE_BF16 0
 #define TOKMIX_DTYPE_FP32 1
 #define TOKMIX_DTYPE_FP16 2
+#define TOKMIX_DTYPE_E4M3 3
+#define TOKMIX_DTYPE_INT8 4
 
 /* Causal / non-causal attention forward, bf16 in and out, fp32 softmax and accumulation.
  *
@@ -273,6 +275,76 @@ int tokmix_swiglu_input_quant(const void* x, void* out, void* x_fp8, float* x_sc
  * the column pairs (j, j + half); negative_sin != 0 negates sin.  head_dim, nope_dim multiples of 8. */
 int tokmix_qkv_part_rope(const void* qkv, const float* cos, const float* sin, void* out, int batch, int seq, int heads,
                          int head_dim, int q_heads, int kv_heads, int nope_dim, int negative_sin, void* stream);
+
+/* Residual addition, RMS norm and FP8 quantisation of a layer's input (between rms_norm,
+ * references/rms_norm.py:6-10, and the block quantisation of references/swiglu_input_quant.py:6-30; the
+ * reference has no fused form).  x, residual, residual_out: [rows, n] in `dtype` (bf16 or fp16);
+ * weight: [n]; y_fp8: [rows, n] e4m3.
+ *   h = T(x + residual), stored to residual_out;  u = h * weight (fp32)
+ *   inv_rms = 1 / sqrt(mean(h^2) + eps);  per group of `group` columns: a = max(max |u|, 2^-100)
+ *   y_fp8 = e4m3(u * (448 / a));  y_scale = a * inv_rms / 448
+ * so y_fp8 * y_scale is the normalised row.  group 32 or 128 (n a multiple of it): y_scale is
+ * [n / group, rows] as tokmix_swiglu_input_quant lays its scales out; group 0: one scale per row,
+ * y_scale [rows].  residual NULL: h = x, and residual_out is not used.  residual_out may equal
+ * residual or x.  n a multiple of 8, at most 65536; 16-byte aligned. */
+int tokmix_add_rms_norm_quant(const void* x, const void* residual, const void* weight, void* residual_out, void* y_fp8,
+                              float* y_scale, int rows, int n, int group, int dtype, float eps, void* stream);
+
+/* ---- a paged key/value cache held in 8 bits, and the decode attention that reads it (no counterpart
+ * in the reference, whose attention is prefill only) ---- */
+
+/* The cache and the sequences of one call.  k, v: [num_pages][heads_kv][page_size][head_dim] bytes
+ * (TOKMIX_DTYPE_E4M3 or TOKMIX_DTYPE_INT8); a (page, head) tile is contiguous, page and head strides
+ * are in bytes and multiples of 16.  k_scale, v_scale: [num_pages, heads_kv] fp32; a cached value is
+ * byte * scale.  block_table: [batch, max_pages] int32, rows table_stride apart: the pages of each
+ * sequence in order; entries behind a sequence's last page are not read.  seq_lens [batch]: tokens in
+ * the cache, those of this call included; new_lens [batch] (or NULL: every token of the call): how many
+ * of them are new, the last ones.  page_size 16, 32, 64 or 128; head_dim 64, 128 or 256.
+ * All of it is device memory of the current device, read when the kernels run. */
+typedef struct tokmix_kv8_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  long long k_page_stride, k_head_stride, v_page_stride, v_head_stride;
+  const int32_t* block_table;
+  long long table_stride;
+  const int32_t* seq_lens;
+  const int32_t* new_lens;
+  int num_pages, page_size, heads_kv, head_dim, dtype, batch, max_pages;
+} tokmix_kv8_cache;
+
+/* Appends new keys and values: row i < new_lens[b] of k, v [batch, tokens, heads_kv, head_dim] (bf16 or
+ * fp16, element strides given, head_dim contiguous, strides multiples of 8) becomes the token at position
+ * seq_lens[b] - new_lens[b] + i of sequence b.  Per (page, head), keys and values apart: the scale is the
+ * smallest power of two, at least 2^-100, with max |x| <= qmax * scale over the page's tokens (qmax 448
+ * for e4m3, 127 for int8); values are rounded to nearest, ties to even; where new tokens raise the scale,
+ * the page's older tokens are rounded again to it.  A page whose first slot is written starts afresh.  A
+ * value that is not finite makes its block's scale NaN until the page is started afresh.  No two
+ * sequences of a call may append to one page.
+ * Lengths that do not fit the call or the table, and table entries outside the pool, write nothing for
+ * that sequence (page) and set TOKMIX_DEV_BAD_ARGS in *status (device memory or mapped host memory). */
+int tokmix_kv8_append(const void* k, long long k_batch_stride, long long k_token_stride, long long k_head_stride,
+                      const void* v, long long v_batch_stride, long long v_token_stride, long long v_head_stride,
+                      int tokens, int io_dtype, const tokmix_kv8_cache* cache, uint32_t* status, void* stream);
+
+/* Attention of the newest tokens over the cache: row i < new_lens[b] of q [batch, tokens, heads_q,
+ * head_dim] (bf16 or fp16, element strides given) is the query at position p = seq_lens[b] - new_lens[b] + i
+ * and sees positions 0 .. p; out [batch, tokens, heads_q, head_dim] (contiguous, q's type) =
+ * softmax(q k^T * sm_scale) v in fp32, k and v as the cache holds them; query head h reads key/value
+ * head h / (heads_q / heads_kv).  lse (NULL or fp32 [batch, tokens, heads_q]): the natural logarithm of the
+ * row's sum of exponentials.  Rows i >= new_lens[b] give zeros and lse -infinity.
+ * 1 <= tokens <= 16.  workspace: tokmix_kv8_attention_workspace_bytes(...) bytes of device memory, 16-byte
+ * aligned, no initialisation, not shared by calls that may overlap.
+ * Lengths that do not fit give NaN for the sequence's rows, a table entry outside the pool NaN for the
+ * rows that see it; both set TOKMIX_DEV_BAD_ARGS in *status (device memory or mapped host memory). */
+int tokmix_kv8_attention(const void* q, long long q_batch_stride, long long q_token_stride, long long q_head_stride,
+                         void* out, float* lse, int tokens, int heads_q, int io_dtype, float sm_scale,
+                         const tokmix_kv8_cache* cache, void* workspace, long long workspace_bytes, uint32_t* status,
+                         void* stream);
+
+/* Workspace size of tokmix_kv8_attention in bytes on the current device (-1 for bad arguments). */
+long long tokmix_kv8_attention_workspace_bytes(int tokens, int heads_q, int heads_kv, int head_dim);
 
 /* Self-test of the bounded waits every pipelined kernel relies on: one small kernel waits on an
  * event that never happens -- which = 0: a transaction barrier whose bytes never land (a TMA load

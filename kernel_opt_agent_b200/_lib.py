@@ -10,6 +10,7 @@ reference's plugin modules report them: bad shapes / dtypes / devices raise ``Va
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import pathlib
@@ -30,6 +31,8 @@ LAYOUT_BSHD = 1
 DTYPE_BF16 = 0
 DTYPE_FP32 = 1
 DTYPE_FP16 = 2
+DTYPE_E4M3 = 3
+DTYPE_INT8 = 4
 
 DEV_STATUS_BITS = {
     0x1: "a TMA load never completed",
@@ -42,6 +45,7 @@ DEV_STATUS_BITS = {
 _VP = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
+_LL = ctypes.c_longlong
 SIGNATURES = {
     "tokmix_fa2_fwd": (_I, [_VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _I, _F, _VP, _VP]),
     "tokmix_gdn_prefill": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _F, _I, _VP,
@@ -63,6 +67,10 @@ SIGNATURES = {
     "tokmix_rms_norm": (_I, [_VP, _VP, _VP, _I, _I, _I, _F, _VP]),
     "tokmix_swiglu_input_quant": (_I, [_VP, _VP, _VP, _VP, _I, _I, _F, _VP]),
     "tokmix_qkv_part_rope": (_I, [_VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _I, _VP]),
+    "tokmix_add_rms_norm_quant": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _F, _VP]),
+    "tokmix_kv8_append": (_I, [_VP, _LL, _LL, _LL, _VP, _LL, _LL, _LL, _I, _I, _VP, _VP, _VP]),
+    "tokmix_kv8_attention": (_I, [_VP, _LL, _LL, _LL, _VP, _VP, _I, _I, _I, _F, _VP, _VP, _LL, _VP, _VP]),
+    "tokmix_kv8_attention_workspace_bytes": (_LL, [_I, _I, _I, _I]),
     "tokmix_selftest_wait_timeout": (_I, [_I, ctypes.c_longlong, _VP, _VP, _VP, _VP]),
     "tokmix_last_error": (ctypes.c_char_p, []),
     "tokmix_version": (ctypes.c_char_p, []),
@@ -74,6 +82,16 @@ class Stage1Inputs(ctypes.Structure):
     _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("dtype", ctypes.c_int),
                 ("a_log", ctypes.c_void_p), ("dt_bias", ctypes.c_void_p), ("qk_l2norm", ctypes.c_int),
                 ("l2norm_eps", ctypes.c_float), ("k_normed", ctypes.c_void_p)]
+
+
+class Kv8Cache(ctypes.Structure):
+    """tokmix_kv8_cache: a paged 8-bit key/value cache and the sequences of one call."""
+
+    _fields_ = [("k", _VP), ("v", _VP), ("k_scale", _VP), ("v_scale", _VP),
+                ("k_page_stride", _LL), ("k_head_stride", _LL), ("v_page_stride", _LL), ("v_head_stride", _LL),
+                ("block_table", _VP), ("table_stride", _LL), ("seq_lens", _VP), ("new_lens", _VP),
+                ("num_pages", _I), ("page_size", _I), ("heads_kv", _I), ("head_dim", _I), ("dtype", _I),
+                ("batch", _I), ("max_pages", _I)]
 
 
 _lib = None
@@ -215,6 +233,63 @@ def check_status(device: torch.device, what: str) -> None:
     if m is not None:
         m.copied = None
     raise_on_device_status(status_word(torch.device("cuda", idx)), what)
+
+
+class _HostStatus:
+    """A status word in pinned host memory that the kernels of a device store to when they meet bad
+    device-side arguments: looking at it costs no launch, copy or synchronisation, so every call
+    does, inside a graph capture too."""
+
+    def __init__(self):
+        self.tensor = torch.zeros(1, dtype=torch.int32).pin_memory()
+        self.ptr = self.tensor.data_ptr()
+        self.word = ctypes.c_uint32.from_address(self.ptr)
+
+
+_host_status: dict[int, _HostStatus] = {}
+
+
+def host_status_ptr(device: torch.device, what: str) -> int | None:
+    """Raises if an earlier launch on `device` stored a bit in the host status word (and clears it), else
+    its address for the next launch (None for a first call inside a graph capture, where it cannot be
+    allocated, and with TOKMIX_CHECK_STATUS=0)."""
+    if _STATUS_MODE == "off":
+        return None
+    h = _host_status.get(device.index)
+    if h is None:
+        if torch.cuda.is_current_stream_capturing():
+            return None
+        h = _host_status[device.index] = _HostStatus()
+    if h.word.value:
+        take_host_status(device, what)
+    return h.ptr
+
+
+def take_host_status(device: torch.device, what: str) -> None:
+    """Raises TokmixDeviceError if the host status word of `device` holds a bit; clears it first."""
+    h = _host_status.get(device.index)
+    if h is not None and h.word.value:
+        val, h.word.value = h.word.value, 0
+        _raise_for(val, what)
+
+
+def after_host_status_launch(device: torch.device, what: str) -> None:
+    """With TOKMIX_CHECK_STATUS=1, synchronise and check; otherwise the next call looks."""
+    if _STATUS_MODE == "sync" and not torch.cuda.is_current_stream_capturing():
+        torch.cuda.current_stream(device).synchronize()
+        take_host_status(device, what)
+
+
+def on_device(device: torch.device):
+    """Context in which `device` is current (free when it already is)."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def aligned(x: torch.Tensor) -> torch.Tensor:
+    """x itself if it is contiguous and starts on a 16-byte boundary, else a copy that is."""
+    if not x.is_contiguous():
+        return x.contiguous()
+    return x.clone() if x.data_ptr() % 16 else x
 
 
 def stream_ptr(device: torch.device) -> int:
