@@ -35,11 +35,13 @@ def make_cache(num_pages: int, heads_kv: int, page_size: int = 64, head_dim: int
     return [kv[0], kv[1], scale[0], scale[1]]
 
 
-def _tile_strides(name: str, t: torch.Tensor) -> tuple[int, int]:
+def _tile_strides(name: str, t: torch.Tensor, shape=None) -> tuple[int, int]:
     """(page, head) strides of a cache; refuses tiles that are not contiguous, aligned or apart."""
-    pages, heads, page, d = t.shape
+    pages, heads, page, d = shape or t.shape
     sp, sh, ss, sd = t.stride()
     tile = page * d
+    if sd == 1 and ss == d and sh == tile and sp == tile * heads and t.data_ptr() % 16 == 0:
+        return sp, sh  # contiguous
     if pages == 1:
         sp = max(sp, tile * heads) // 16 * 16
     if heads == 1:
@@ -54,39 +56,45 @@ def _tile_strides(name: str, t: torch.Tensor) -> tuple[int, int]:
 
 def cache_args(x: torch.Tensor, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, new_lens) -> _lib.Kv8Cache:
     """Checks a cache and a call's sequences against x [B, T, heads, D] (the new keys or the queries)."""
-    if x.ndim != 4 or k_cache.ndim != 4 or v_cache.shape != k_cache.shape:
+    shape = k_cache.shape
+    if x.ndim != 4 or len(shape) != 4 or v_cache.shape != shape:
         raise ValueError("new tokens must be [B, T, heads, D], k_cache and v_cache [num_pages, Hkv, page, D]")
-    num_pages, heads, page, d = k_cache.shape
-    if k_cache.dtype not in CACHE_DTYPES or v_cache.dtype != k_cache.dtype:
+    num_pages, heads, page, d = shape
+    batch = x.shape[0]
+    dtype = CACHE_DTYPES.get(k_cache.dtype)
+    if dtype is None or v_cache.dtype != k_cache.dtype:
         raise ValueError("k_cache and v_cache must both be float8_e4m3fn or both int8")
     if page not in PAGE_SIZES or d not in HEAD_DIMS or num_pages == 0 or heads == 0:
         raise ValueError(f"page size must be one of {PAGE_SIZES} and head_dim one of {HEAD_DIMS}")
     if x.dtype not in IO_DTYPES or x.shape[3] != d:
         raise ValueError("new tokens must be bfloat16 or float16 with the cache's head_dim")
     dev = x.device
-    tensors = (k_cache, v_cache, k_scale, v_scale, block_table, seq_lens)
-    if not x.is_cuda or any(t.device != dev for t in tensors) or (new_lens is not None and new_lens.device != dev):
+    if not x.is_cuda or k_cache.device != dev or v_cache.device != dev or k_scale.device != dev or (
+            v_scale.device != dev or block_table.device != dev or seq_lens.device != dev) or (
+            new_lens is not None and new_lens.device != dev):
         raise ValueError("all tensors must be CUDA tensors on one device")
-    for t in (k_scale, v_scale):
-        if t.dtype != torch.float32 or t.shape != (num_pages, heads) or not t.is_contiguous():
-            raise ValueError("k_scale and v_scale must be contiguous float32 [num_pages, Hkv]")
-    batch = x.shape[0]
-    if block_table.dtype != torch.int32 or block_table.ndim != 2 or block_table.shape[0] != batch or (
-            block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError("block_table must be int32 [B, max_pages] with contiguous rows")
-    for t in (seq_lens, new_lens):
-        if t is not None and (t.dtype != torch.int32 or t.shape != (batch,) or not t.is_contiguous()):
-            raise ValueError("seq_lens and new_lens must be contiguous int32 [B]")
+    f32, i32, per_page = torch.float32, torch.int32, (num_pages, heads)
+    if k_scale.dtype != f32 or v_scale.dtype != f32 or k_scale.shape != per_page or v_scale.shape != per_page or not (
+            k_scale.is_contiguous() and v_scale.is_contiguous()):
+        raise ValueError("k_scale and v_scale must be contiguous float32 [num_pages, Hkv]")
+    if block_table.dtype != i32 or block_table.ndim != 2 or block_table.shape[0] != batch:
+        raise ValueError("block_table must be int32 [B, max_pages]")
     max_pages = block_table.shape[1]
-    table_stride = block_table.stride(0) if batch > 1 else max_pages
-    if table_stride < max_pages:
-        raise ValueError("the rows of block_table must not overlap")
-    kp, kh = _tile_strides("k_cache", k_cache)
-    vp, vh = _tile_strides("v_cache", v_cache)
+    table_stride, along = block_table.stride()
+    if batch <= 1:
+        table_stride = max_pages
+    if table_stride < max_pages or (along != 1 and max_pages > 1):
+        raise ValueError("the rows of block_table must be contiguous and must not overlap")
+    if seq_lens.dtype != i32 or seq_lens.shape != (batch,) or not seq_lens.is_contiguous():
+        raise ValueError("seq_lens must be contiguous int32 [B]")
+    if new_lens is not None and (new_lens.dtype != i32 or new_lens.shape != (batch,) or not new_lens.is_contiguous()):
+        raise ValueError("new_lens must be contiguous int32 [B]")
+    kp, kh = _tile_strides("k_cache", k_cache, shape)
+    vp, vh = _tile_strides("v_cache", v_cache, shape)
     return _lib.Kv8Cache(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), kp, kh, vp,
                          vh, block_table.data_ptr(), table_stride, seq_lens.data_ptr(),
-                         new_lens.data_ptr() if new_lens is not None else None, num_pages, page, heads, d,
-                         CACHE_DTYPES[k_cache.dtype], batch, max_pages)
+                         new_lens.data_ptr() if new_lens is not None else None, num_pages, page, heads, d, dtype,
+                         batch, max_pages)
 
 
 def token_strides(x: torch.Tensor) -> tuple[torch.Tensor, tuple[int, int, int]]:

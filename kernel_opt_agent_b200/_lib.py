@@ -280,9 +280,12 @@ def after_host_status_launch(device: torch.device, what: str) -> None:
         take_host_status(device, what)
 
 
+_HERE = contextlib.nullcontext()
+
+
 def on_device(device: torch.device):
     """Context in which `device` is current (free when it already is)."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def aligned(x: torch.Tensor) -> torch.Tensor:
@@ -293,4 +296,5 @@ def aligned(x: torch.Tensor) -> torch.Tensor:
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream of `device` as an address (without making a Stream object, which costs 2 us)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)

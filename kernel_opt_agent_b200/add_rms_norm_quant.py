@@ -31,25 +31,25 @@ MAX_N = 65536
 
 def kernel_fn(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float = 1e-6, *,
               group: int | None = 128, inplace: bool = False):
-    if x.dtype not in _DTYPES or weight.dtype != x.dtype or x.ndim < 1:
+    dtype, shape, dev = x.dtype, x.shape, x.device
+    if dtype not in _DTYPES or weight.dtype != dtype or not shape:
         raise ValueError("x and weight must both be bfloat16 or both float16")
-    if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape):
+    if residual is not None and (residual.dtype != dtype or residual.shape != shape):
         raise ValueError("residual must have the shape and type of x")
-    dev = x.device
     if not x.is_cuda or weight.device != dev or (residual is not None and residual.device != dev):
         raise ValueError("x, residual and weight must be CUDA tensors on one device")
     if group not in (None, 32, 128):
         raise ValueError("group must be 32, 128 or None (one scale per row)")
-    n = x.shape[-1]
+    n = shape[-1]
     if n == 0 or n % (group or 8) != 0 or n > MAX_N:
         raise ValueError(f"the last dimension of x must be a multiple of {group or 8} and at most {MAX_N} (got {n})")
-    if tuple(weight.shape) != (n,):
+    if weight.shape != (n,):
         raise ValueError("weight must be [N], N the last dimension of x")
     if inplace and (residual is None or not residual.is_contiguous() or residual.data_ptr() % 16):
         raise ValueError("inplace=True needs a contiguous, 16-byte aligned residual")
     x, w = _lib.aligned(x), _lib.aligned(weight)
     rows = x.numel() // n
-    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
+    y = torch.empty_like(x, dtype=torch.float8_e4m3fn)
     y_scale = torch.empty((n // group, rows) if group else (rows,), dtype=torch.float32, device=dev)
     if residual is None:
         res, res_out = None, x
@@ -59,7 +59,7 @@ def kernel_fn(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tens
     with _lib.on_device(dev):
         rc = _lib.load().tokmix_add_rms_norm_quant(
             x.data_ptr(), res.data_ptr() if res is not None else None, w.data_ptr(), res_out.data_ptr(), y.data_ptr(),
-            y_scale.data_ptr(), rows, n, group or 0, _DTYPES[x.dtype], eps, _lib.stream_ptr(dev))
+            y_scale.data_ptr(), rows, n, group or 0, _DTYPES[dtype], eps, _lib.stream_ptr(dev))
     if rc:
         _lib.check(rc, "add_rms_norm_quant")
     return y, y_scale, res_out

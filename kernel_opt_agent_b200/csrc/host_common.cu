@@ -1,6 +1,7 @@
 // host_common.cu -- error reporting, tensor-map encoding and device queries for the C ABI.
 #include "host_common.h"
 
+#include <atomic>
 #include <cmath>
 
 #include <mutex>
@@ -78,11 +79,21 @@ bool encode_tiled(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void
   return true;
 }
 
+namespace {
+// attributes of a device do not change: asked once per device (0: not asked yet)
+constexpr int kCachedDevices = 64;
+std::atomic<int> g_sms[kCachedDevices];
+std::atomic<int> g_cc[kCachedDevices];
+}  // namespace
+
 int device_sm_count() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  int n = 0;
+  const bool cached = dev >= 0 && dev < kCachedDevices;
+  int n = cached ? g_sms[dev].load(std::memory_order_relaxed) : 0;
+  if (n > 0) return n;
   cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  if (cached) g_sms[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 
@@ -102,9 +113,12 @@ bool ensure_smem_attr(const void* func, int bytes) {
 int check_device() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return fail(TOKMIX_ERR_DEVICE, "no CUDA device");
+  const bool cached = dev >= 0 && dev < kCachedDevices;
+  if (cached && g_cc[dev].load(std::memory_order_relaxed) == 100) return TOKMIX_OK;
   int major = 0, minor = 0;
   cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
   cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
+  if (cached) g_cc[dev].store(10 * major + minor, std::memory_order_relaxed);
   if (major != 10 || minor != 0)
     return fail(TOKMIX_ERR_DEVICE, "libtokmix is built for sm_100a (B200); device %d is sm_%d%d", dev, major, minor);
   return TOKMIX_OK;

@@ -37,20 +37,21 @@ namespace kv8 {
 
 constexpr int kMaxTokens = 16;
 constexpr int kMaxBatch = 8192;  // the plan keeps batch + 1 words in shared memory
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
 constexpr float kShift = 14.0f;  // weights are held times 2^14
 constexpr int kJoinThreads = 256;
 constexpr int kMaxCtas = 148 * 8;
 
 template <int D, int NT>
 struct Shape {
-  static constexpr int kTok = 4096 / D;       // tokens per tile
+  static constexpr int kTok = D == 256 ? 16 : 32;  // tokens per tile
   static constexpr int kMt = kTok / 16;       // 16-token subtiles (a page holds whole ones)
   static constexpr int kRows = 8 * NT;        // query rows per unit
   static constexpr int kQStride = D + 8;      // halves between rows of q in shared memory (conflict-free 16-byte reads)
-  static constexpr int kCtasPerSm = NT == 1 ? 3 : 2;
-  static constexpr int kMergeBytes = kWarps * kRows * D * 4;
+  static constexpr int kStageBytes = 2 * kTok * D;   // a tile's keys and values
+  static constexpr int kStages = D == 64 ? 6 : 3;    // 24 KB in flight per warp
+  static constexpr int kWarpsPerSm = 8;
+  __host__ __device__ static constexpr int smem_bytes(int warps) { return warps * kStages * (kStageBytes + 8 * kMt) + kRows * kQStride * 2; }
+  static_assert(8 * D * 4 <= kStageBytes, "eight partial rows fit a stage");
 };
 
 struct AttnParams {
@@ -65,6 +66,7 @@ struct AttnParams {
   int bf16;
   float scale_log2;  // sm_scale * log2(e)
   int grid;          // CTAs of the attention kernel
+  int min_tiles;     // a CTA's range is at least this long
   uint32_t* status;
 };
 
@@ -117,9 +119,9 @@ __device__ __forceinline__ void make_plan(const AttnParams& p, uint32_t* prefix,
   __syncthreads();
 }
 
-// CTAs that take part: each has at least a tile per warp, so none is empty
+// CTAs that take part: none is empty
 __device__ __forceinline__ uint32_t active_ctas(const AttnParams& p, uint32_t total) {
-  return min(static_cast<uint32_t>(p.grid), max(1u, total / kWarps));
+  return min(static_cast<uint32_t>(p.grid), max(1u, total / p.min_tiles));
 }
 __device__ __forceinline__ uint32_t range_begin(uint32_t cta, uint32_t total, uint32_t ctas) {
   return static_cast<uint32_t>(static_cast<unsigned long long>(cta) * total / ctas);
@@ -130,17 +132,6 @@ __device__ __forceinline__ uint32_t cta_of(uint32_t t, uint32_t total, uint32_t 
 }
 
 // ------------------------------------------------------------------------------------ small pieces
-__device__ __forceinline__ uint4 ld16(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 ld8(const uint8_t* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
-}
-
 // four bytes -> four halves (two registers), exact
 template <bool E4M3>
 __device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -203,17 +194,79 @@ __device__ __forceinline__ float lse_of(float m, float sum) {
 }
 
 // ------------------------------------------------------------------------------------ attention
-template <int D, bool E4M3, int NT>
-__global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtasPerSm) attn_kernel(const AttnParams p) {
+// One unit's share of a CTA's range
+struct Segment {
+  Seq s;
+  int b, kvh, row0, rows_valid;  // rows row0 .. of the rows_valid of the sequence's key/value head
+  int t0, t1;                    // token tiles
+  bool whole;                    // all of the unit
+};
+
+// The tiles of a CTA's range in order, unit by unit
+template <int TOK, int ROWS>
+struct Walk {
+  uint32_t pos, stop;
+  int b;
+  __device__ __forceinline__ bool next(const AttnParams& p, const uint32_t* prefix, Segment& n) {
+    if (pos >= stop) return false;
+    while (prefix[b + 1] <= pos) ++b;
+    n.b = b;
+    n.s = load_seq(p.c, b, p.tokens);
+    const Unit u = unit_of<TOK, ROWS>(p, n.s);
+    const int off = static_cast<int>(pos - prefix[b]);
+    const int ui = off / u.tiles;
+    n.t0 = off - ui * u.tiles;
+    n.t1 = min(u.tiles, n.t0 + static_cast<int>(stop - pos));
+    n.kvh = ui / u.row_tiles;
+    n.row0 = (ui - n.kvh * u.row_tiles) * ROWS;
+    n.rows_valid = (n.s.end - n.s.start) * p.group;
+    n.whole = n.t0 == 0 && n.t1 == u.tiles;
+    pos += n.t1 - n.t0;
+    return true;
+  }
+};
+
+// Byte offset of 16-byte chunk c of token row r in a tile in shared memory: rows of D bytes, chunks permuted inside each
+// 128-byte line so that the reads below meet every bank once.  D >= 128: c ^ (r % 8).  D = 64 (two rows a line):
+// line chunk 4 (r % 2) + c, ^ 2 ((r / 2) % 4).
+template <int D>
+__device__ __forceinline__ int tile_chunk(int r, int c) {
+  if constexpr (D == 64) return (r >> 1) * 128 + ((((r & 1) << 2 | c) ^ (((r >> 1) & 3) << 1)) << 4);
+  return r * D + ((c ^ (r & 7)) << 4);
+}
+
+// 16-byte chunk of a partial row in shared memory: spread so that the four rows a store instruction meets fall into
+// different banks (a store's eight lanes hold rows 2 cq + e and chunks 4 g + x, or 2 g + x at D = 64)
+template <int D>
+__device__ __forceinline__ int merge_chunk(int row, int chunk) {
+  const int cq = (row >> 1) & 3;
+  return chunk ^ (D == 64 ? (cq & 1) | ((cq >> 1) << 2) : cq);
+}
+
+// Copies 16 bytes to shared memory, or zeros if !live (nothing is read then)
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const float* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+template <int D, bool E4M3, int NT, int W>
+__global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_kernel(const AttnParams p) {
   using S = Shape<D, NT>;
-  constexpr int TOK = S::kTok, MT = S::kMt, ROWS = S::kRows, J = D / 64;
+  constexpr int TOK = S::kTok, MT = S::kMt, ROWS = S::kRows, J = D / 64, STAGES = S::kStages;
   constexpr int kVec = D / 8;  // 16-byte vectors of a query row
-  extern __shared__ __align__(16) uint8_t smem[];
-  float* merge = reinterpret_cast<float*>(smem);                                   // [warp][row][D]
-  __half* qs = reinterpret_cast<__half*>(smem + S::kMergeBytes);                    // [row][kQStride]
-  uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + S::kMergeBytes + ROWS * S::kQStride * 2);
-  __shared__ float row_factor[ROWS], warp_m[kWarps][ROWS], warp_l[kWarps][ROWS], warp_v[kWarps];
-  __shared__ uint32_t scratch[kWarps];
+  constexpr int kThreads = 32 * W;
+  constexpr int kQv = (ROWS * kVec + kThreads - 1) / kThreads;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t* ring = smem + (threadIdx.x >> 5) * STAGES * S::kStageBytes;                 // this warp's [stage][keys, values]
+  float* scales = reinterpret_cast<float*>(smem + W * STAGES * S::kStageBytes) + (threadIdx.x >> 5) * STAGES * 2 * MT;
+  __half* qs = reinterpret_cast<__half*>(smem + W * STAGES * (S::kStageBytes + 8 * MT));  // [row][kQStride]
+  uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + S::smem_bytes(W));
+  __shared__ float row_factor[ROWS], warp_m[W][ROWS], warp_l[W][ROWS], warp_v[W];
+  __shared__ int warp_at[W];  // where in `smem` a warp's partial rows lie, -1: it had no tile of the segment
+  __shared__ uint32_t scratch[W];
 
   const View& c = p.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -225,49 +278,113 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtasPerSm) attn_kerne
   if (total == 0) return;
   const uint32_t ctas = active_ctas(p, total);
   if (blockIdx.x >= ctas) return;
-  uint32_t pos = range_begin(blockIdx.x, total, ctas);
-  const uint32_t stop = range_begin(blockIdx.x + 1, total, ctas);
-  int b = 0;
-  for (int hi = c.batch; hi - b > 1;) {  // the last b with prefix[b] <= pos
-    const int mid = (b + hi) >> 1;
-    if (prefix[mid] <= pos) b = mid; else hi = mid;
+  Walk<TOK, ROWS> walk;
+  walk.pos = range_begin(blockIdx.x, total, ctas);
+  walk.stop = range_begin(blockIdx.x + 1, total, ctas);
+  walk.b = 0;
+  for (int hi = c.batch; hi - walk.b > 1;) {  // the last sequence with prefix <= pos
+    const int mid = (walk.b + hi) >> 1;
+    if (prefix[mid] <= walk.pos) walk.b = mid; else hi = mid;
   }
 
-  for (bool first = true; pos < stop; first = false) {
-    while (prefix[b + 1] <= pos) ++b;
-    const Seq s = load_seq(c, b, p.tokens);
-    const Unit u = unit_of<TOK, ROWS>(p, s);
-    const int off = static_cast<int>(pos - prefix[b]);
-    const int ui = off / u.tiles;
-    const int t0 = off - ui * u.tiles;
-    const int t1 = min(u.tiles, t0 + static_cast<int>(stop - pos));
-    const int kvh = ui / u.row_tiles;
-    const int row0 = (ui - kvh * u.row_tiles) * ROWS;     // first row of the unit
-    const int rows_valid = (s.end - s.start) * p.group;   // rows of the sequence's key/value head
-    pos += t1 - t0;
-
-    // q rows into shared memory as scaled halves; rows behind the last are zero and never written out
-    for (int v = threadIdx.x; v < ROWS * kVec; v += kThreads) {
-      const int r = v / kVec, x = v % kVec;
-      const int row = row0 + r;
-      float f[8];
-      float amax = 0.0f;
-      if (row < rows_valid) {
-        const int i = row / p.group, h = kvh * p.group + row - i * p.group;
-        const long long at = b * p.q_sb + i * p.q_st + h * p.q_sh + x * 8;
-        const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + at));
-        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+  // ---- the loads run ahead of the products by up to STAGES tiles, across units; table entries by one more
+  Walk<TOK, ROWS> ahead = walk;
+  Segment ld{};         // unit of the next tile to load
+  int ld_t = 0;         // that tile
+  bool ld_live;         // false: no tile is left
+  int pid[MT];          // its pages
+  int ld_stage = 0;
+  auto find_tile = [&]() {
+    while (ld_live && ld_t >= ld.t1) {
+      ld_live = ahead.next(p, prefix, ld);
+      if (ld_live) ld_t = ld.t0 + warp;
+    }
+    if (ld_live) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 t = p.bf16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&ws[e]))
-                                  : __half22float2(*reinterpret_cast<const __half2*>(&ws[e]));
-          f[2 * e] = t.x;
-          f[2 * e + 1] = t.y;
-          amax = fmaxf(amax, fmaxf(fabsf(t.x), fabsf(t.y)));
+      for (int mt = 0; mt < MT; ++mt)  // behind the sequence's end: its last page
+        pid[mt] = __ldg(c.table + ld.b * c.table_stride + (min(ld_t * TOK + mt * 16, ld.s.end - 1) >> c.page_shift));
+    }
+  };
+  auto load_tile = [&]() {
+    if (ld_live) {
+      const uint32_t dst0 = smem_addr(ring + ld_stage * S::kStageBytes);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const int tok = ld_t * TOK + mt * 16;
+        const bool good = static_cast<unsigned>(pid[mt]) < static_cast<unsigned>(c.num_pages);
+        const long long pg = good ? pid[mt] : 0;
+        const int slot = (tok & (c.page - 1)) * D + lane * 16;
+        const uint8_t* ksrc = c.k + pg * c.k_page_stride + ld.kvh * c.k_head_stride + slot;
+        const uint8_t* vsrc = c.v + pg * c.v_page_stride + ld.kvh * c.v_head_stride + slot;
+        const int rows = good ? ld.s.end - tok : 0;  // token rows to read; zeros behind them
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const int r = (i * 32 + lane) / (D / 16), ch = lane % (D / 16);
+          const uint32_t dst = dst0 + mt * 16 * D + tile_chunk<D>(r, ch);
+          copy16(dst, ksrc + i * 512, r < rows);
+          copy16(dst + TOK * D, vsrc + i * 512, r < rows);
         }
-      } else {
+        float* sc = scales + ld_stage * 2 * MT + mt;
+        if (good) {
+          if (lane < 2) copy4(smem_addr(sc + lane * MT), (lane == 0 ? c.k_scale : c.v_scale) + pg * c.hkv + ld.kvh);
+        } else if (lane < 2) {  // NaN scores for the rows that see it
+          sc[lane * MT] = lane == 0 && tok < ld.s.end ? nan_f() : 0.0f;
+          if (lane == 0 && tok < ld.s.end) report_bad(p.status);
+        }
+      }
+      ld_t += W;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");  // an empty group too: the waits count groups
+    ld_stage = ld_stage == STAGES - 1 ? 0 : ld_stage + 1;
+    find_tile();
+  };
+  ld_live = ahead.next(p, prefix, ld);
+  ld_t = ld.t0 + warp;
+  find_tile();
+
+  uint4 qraw[kQv];
+  // q of a segment as it lies; rows behind the last are zero and never written out
+  auto load_q = [&](const Segment& n) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = 0.0f;
+    for (int k = 0; k < kQv; ++k) {
+      const int v = threadIdx.x + k * kThreads;
+      const int r = v / kVec, x = v % kVec, row = n.row0 + r;
+      qraw[k] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < ROWS && row < n.rows_valid) {
+        const int i = row / p.group, h = n.kvh * p.group + row - i * p.group;
+        const long long at = n.b * p.q_sb + i * p.q_st + h * p.q_sh + x * 8;
+        qraw[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + at));
+      }
+    }
+  };
+  Segment n;
+  bool more = walk.next(p, prefix, n);
+  load_q(n);
+#pragma unroll
+  for (int x = 0; x < STAGES; ++x) load_tile();
+  int stage = 0;
+
+  for (bool first = true; more; first = false) {
+    const Segment cur = n;
+    const Seq s = cur.s;
+    const int row0 = cur.row0, rows_valid = cur.rows_valid, t1 = cur.t1;
+
+    // q rows into shared memory as halves times a power of two, in the order the products take the head dimension:
+    // position 64 j + 16 cq + e holds dim 128 (j / 2) + 32 cq + 16 (j % 2) + e (D = 64: unchanged)
+#pragma unroll
+    for (int k = 0; k < kQv; ++k) {
+      const int v = threadIdx.x + k * kThreads;
+      const int r = v / kVec, x = v % kVec;
+      if ((k + 1) * kThreads > ROWS * kVec && r >= ROWS) break;  // whole warps
+      const uint32_t ws[4] = {qraw[k].x, qraw[k].y, qraw[k].z, qraw[k].w};
+      float f[8], amax = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 w = p.bf16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&ws[e]))
+                                : __half22float2(*reinterpret_cast<const __half2*>(&ws[e]));
+        f[2 * e] = w.x;
+        f[2 * e + 1] = w.y;
+        amax = fmaxf(amax, fmaxf(fabsf(w.x), fabsf(w.y)));
       }
 #pragma unroll
       for (int o = kVec / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
@@ -279,7 +396,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtasPerSm) attn_kerne
       hq.y = half2_bits(f[2] * up, f[3] * up);
       hq.z = half2_bits(f[4] * up, f[5] * up);
       hq.w = half2_bits(f[6] * up, f[7] * up);
-      *reinterpret_cast<uint4*>(qs + r * S::kQStride + x * 8) = hq;
+      const int at = D == 64 ? x * 8 : 64 * (2 * (x >> 4) + ((x >> 1) & 1)) + 16 * ((x >> 2) & 3) + 8 * (x & 1);
+      *reinterpret_cast<uint4*>(qs + r * S::kQStride + at) = hq;
     }
     __syncthreads();
 
@@ -309,97 +427,19 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtasPerSm) attn_kerne
         for (int e = 0; e < 4; ++e) acc[nt][x][e] = 0.0f;
     float vref = 0.0f;
 
-    const int32_t* trow = c.table + static_cast<long long>(b) * c.table_stride;
-    const uint8_t* kbase = c.k + kvh * c.k_head_stride + g * D + 16 * cq;
-    const uint8_t* vbase = c.v + kvh * c.v_head_stride + 2 * cq * D + (D == 64 ? 8 : 16) * g;
-    const float* ksb = c.k_scale + kvh;
-    const float* vsb = c.v_scale + kvh;
-
-    uint4 kr[8];
-    uint32_t vr[32];
-    int pid[MT];
-    float ks[MT], vs[MT], ksn[MT], vsn[MT];
-
-    // page of each 16-token subtile of tile t; -1: outside the pool, -2: behind the range or the sequence
-    auto load_pages = [&](int t) {
+    int t = cur.t0 + warp;
+    const bool any = t < t1;
+    for (; t < t1; t += W) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+      __syncwarp();
+      const uint8_t* kt = ring + stage * S::kStageBytes;
+      const uint8_t* vt = kt + TOK * D;
+      float ks[MT], vs[MT];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        const int tok = t * TOK + mt * 16;
-        pid[mt] = -2;
-        if (t < t1 && tok < s.end) {
-          pid[mt] = __ldg(trow + (tok >> c.page_shift));
-          if (static_cast<unsigned>(pid[mt]) >= static_cast<unsigned>(c.num_pages)) {
-            pid[mt] = -1;
-            if (lane == 0) report_bad(p.status);
-          }
-        }
+        ks[mt] = scales[stage * 2 * MT + mt];
+        vs[mt] = scales[stage * 2 * MT + MT + mt];
       }
-    };
-    auto load_keys = [&](int t) {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        if (pid[mt] >= 0) {
-          const int slot = (t * TOK + mt * 16) & (c.page - 1);
-          const uint8_t* src = kbase + pid[mt] * c.k_page_stride + slot * D;
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int j = 0; j < J; ++j) kr[(mt * 2 + half) * J + j] = ld16(src + half * 8 * D + j * 64);
-          ksn[mt] = __ldg(ksb + static_cast<long long>(pid[mt]) * c.hkv);
-          vsn[mt] = __ldg(vsb + static_cast<long long>(pid[mt]) * c.hkv);
-        } else {
-#pragma unroll
-          for (int x = 0; x < 2 * J; ++x) kr[mt * 2 * J + x] = make_uint4(0u, 0u, 0u, 0u);
-          ksn[mt] = pid[mt] == -1 ? nan_f() : 0.0f;  // NaN scores for the rows that see it
-          vsn[mt] = 0.0f;
-        }
-      }
-    };
-    // vr[(mt * 4 + i) * (D / 32) + ...]: token 2 cq + {0, 1, 8, 9}[i] of subtile mt, this lane's D / 8 dims
-    auto load_values = [&](int t) {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        if (pid[mt] >= 0) {
-          const int slot = (t * TOK + mt * 16) & (c.page - 1);
-          const uint8_t* src = vbase + pid[mt] * c.v_page_stride + slot * D;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint8_t* tp = src + ((i & 1) + (i >> 1) * 8) * D;
-            if constexpr (D == 64) {
-              const uint2 v = ld8(tp);
-              vr[(mt * 4 + i) * 2] = v.x;
-              vr[(mt * 4 + i) * 2 + 1] = v.y;
-            } else {
-#pragma unroll
-              for (int jj = 0; jj < D / 128; ++jj) {
-                const uint4 v = ld16(tp + jj * 128);
-                uint32_t* d = vr + (mt * 4 + i) * (D / 32) + jj * 4;
-                d[0] = v.x;
-                d[1] = v.y;
-                d[2] = v.z;
-                d[3] = v.w;
-              }
-            }
-          }
-        } else {
-#pragma unroll
-          for (int x = 0; x < D / 8; ++x) vr[mt * (D / 8) + x] = 0u;
-        }
-      }
-    };
-
-    int t = t0 + warp;
-    load_pages(t);
-    load_keys(t);
-    load_values(t);
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      ks[mt] = ksn[mt];
-      vs[mt] = vsn[mt];
-    }
-    load_pages(t + kWarps);
-
-    for (; t < t1; t += kWarps) {
       // scores: two accumulators per product shorten the dependent chain
       float sc[MT][NT][2][4];
 #pragma unroll
@@ -418,9 +458,11 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtasPerSm) attn_kerne
           qf[nt][0] = a.x; qf[nt][1] = a.y; qf[nt][2] = a.z; qf[nt][3] = a.w;
           qf[nt][4] = d.x; qf[nt][5] = d.y; qf[nt][6] = d.z; qf[nt][7] = d.w;
         }
+        const int ch = D == 64 ? cq : 8 * (j >> 1) + 2 * cq + (j & 1);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          const uint4 lo = kr[mt * 2 * J + j], hi = kr[(mt * 2 + 1) * J + j];
+          const uint4 lo = *reinterpret_cast<const uint4*>(kt + mt * 16 * D + tile_chunk<D>(g, ch));
+          const uint4 hi = *reinterpret_cast<const uint4*>(kt + mt * 16 * D + tile_chunk<D>(g + 8, ch));
           const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
@@ -432,8 +474,6 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtasPerSm) attn_kerne
           }
         }
       }
-      load_keys(t + kWarps);
-
       // softmax: a lane has tokens g and g + 8 of each subtile for its rows
       float top[NT][2];
       const bool tail = t * TOK + TOK > min_lim;
@@ -509,116 +549,142 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtasPerSm) attn_kerne
           }
         }
       }
-      // bytes behind the sequence's end may be anything, e4m3 NaN too, and 0 * NaN would stay
-      if (t * TOK + TOK > s.end) {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (t * TOK + mt * 16 + 2 * cq + (i & 1) + (i >> 1) * 8 >= s.end) {
-#pragma unroll
-              for (int x = 0; x < D / 32; ++x) vr[(mt * 4 + i) * (D / 32) + x] = 0u;
-            }
-      }
+      // o^T += v^T p^T: a lane has tokens 2 cq + {0, 1, 8, 9} of each subtile and D / 8 dims
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
+        const uint8_t* vm = vt + mt * 16 * D;
 #pragma unroll
-        for (int x = 0; x < D / 32; ++x) {
-          const uint32_t* w = vr + mt * (D / 8) + x;  // four dims of tokens 2cq, +1, +8, +9
-          const uint32_t t0w = w[0], t1w = w[D / 32], t8w = w[2 * (D / 32)], t9w = w[3 * (D / 32)];
+        for (int jj = 0; jj < (D + 127) / 128; ++jj) {
+          constexpr int X = D == 64 ? 2 : 4;  // words of four dims
+          uint32_t w[4][X];
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {  // dims 4x + 2y, 4x + 2y + 1
-            uint32_t a0, a1, a2, a3;
-            widen4<E4M3>(__byte_perm(t0w, t1w, y == 0 ? 0x5140 : 0x7362), a0, a1);
-            widen4<E4M3>(__byte_perm(t8w, t9w, y == 0 ? 0x5140 : 0x7362), a2, a3);
+          for (int i = 0; i < 4; ++i) {
+            const int r = 2 * cq + (i & 1) + (i >> 1) * 8;
+            if constexpr (D == 64) {
+              const uint2 v = *reinterpret_cast<const uint2*>(vm + tile_chunk<D>(r, g >> 1) + (g & 1) * 8);
+              w[i][0] = v.x;
+              w[i][1] = v.y;
+            } else {
+              const uint4 v = *reinterpret_cast<const uint4*>(vm + tile_chunk<D>(r, 8 * jj + g));
+              w[i][0] = v.x;
+              w[i][1] = v.y;
+              w[i][2] = v.z;
+              w[i][3] = v.w;
+            }
+          }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma16816(acc[nt][2 * x + y], a0, a1, a2, a3, pb[mt][nt][0], pb[mt][nt][1]);
+          for (int x = 0; x < X; ++x) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {  // dims 4x + 2y, 4x + 2y + 1
+              uint32_t a0, a1, a2, a3;
+              widen4<E4M3>(__byte_perm(w[0][x], w[1][x], y == 0 ? 0x5140 : 0x7362), a0, a1);
+              widen4<E4M3>(__byte_perm(w[2][x], w[3][x], y == 0 ? 0x5140 : 0x7362), a2, a3);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma16816(acc[nt][2 * (4 * jj + x) + y], a0, a1, a2, a3, pb[mt][nt][0], pb[mt][nt][1]);
+            }
           }
         }
       }
-      load_values(t + kWarps);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        ks[mt] = ksn[mt];
-        vs[mt] = vsn[mt];
+      __syncwarp();  // every lane has read the stage
+      if (t + W < t1) {
+        load_tile();
+        stage = stage == STAGES - 1 ? 0 : stage + 1;
       }
-      load_pages(t + 2 * kWarps);
     }
 
-    // join the four warps
+    more = walk.next(p, prefix, n);
+    if (more) load_q(n);  // on its way while this segment's warps are joined
+    // join the warps: 8 rows at a time through the stage each has just used up, which is loaded again afterwards
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      float* dst = reinterpret_cast<float*>(ring + stage * S::kStageBytes);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], o);
-        const int r = nt * 8 + 2 * cq + e;
+        const int r = 2 * cq + e;
         if (g == 0) {
-          warp_m[warp][r] = m[nt][e];
-          warp_l[warp][r] = l[nt][e];
+          warp_m[warp][nt * 8 + r] = m[nt][e];
+          warp_l[warp][nt * 8 + r] = l[nt][e];
         }
-        // dims of acc[2x], acc[2x + 1]: D 64: 8 g + 4 x; else 128 (x / 4) + 16 g + 4 (x % 4), four in a row
-        float* dst = merge + (warp * ROWS + r) * D + (D == 64 ? 8 : 16) * g;
+        if (any) {
+          // dims of acc[2x], acc[2x + 1]: D 64: 8 g + 4 x; else 128 (x / 4) + 16 g + 4 (x % 4), four in a row
 #pragma unroll
-        for (int x = 0; x < D / 32; ++x)
-          *reinterpret_cast<float4*>(dst + (D == 64 ? 4 * x : 128 * (x / 4) + 4 * (x % 4))) =
-              make_float4(acc[nt][2 * x][e], acc[nt][2 * x][2 + e], acc[nt][2 * x + 1][e], acc[nt][2 * x + 1][2 + e]);
+          for (int x = 0; x < D / 32; ++x) {
+            const int chunk = D == 64 ? 2 * g + x : 32 * (x / 4) + 4 * g + x % 4;
+            *reinterpret_cast<float4*>(dst + r * D + 4 * merge_chunk<D>(r, chunk)) =
+                make_float4(acc[nt][2 * x][e], acc[nt][2 * x][2 + e], acc[nt][2 * x + 1][e], acc[nt][2 * x + 1][2 + e]);
+          }
+        }
       }
+      if (lane == 0) {
+        warp_v[warp] = vref;
+        warp_at[warp] = any ? static_cast<int>(reinterpret_cast<uint8_t*>(dst) - smem) : -1;
+      }
+      __syncthreads();
+      const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (first ? 0 : 1);
+      constexpr int kOut = 8 * (D / 4);
+#pragma unroll
+      for (int k = 0; k < (kOut + kThreads - 1) / kThreads; ++k) {
+        const int v = threadIdx.x + k * kThreads;
+        const int r8 = v / (D / 4), x = v % (D / 4);
+        const int r = nt * 8 + r8, row = row0 + r;
+        if (v >= kOut || row >= rows_valid) break;
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) top = fmaxf(top, warp_m[i][r]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          if (warp_at[i] < 0) continue;
+          const float4 a = *reinterpret_cast<const float4*>(smem + warp_at[i] + r8 * D * 4 + 16 * merge_chunk<D>(r8, x));
+          const float w = ex2(warp_m[i][r] - ref);
+          sum += w * warp_l[i][r];
+          const float wv = w * warp_v[i];
+          o[0] += a.x * wv;
+          o[1] += a.y * wv;
+          o[2] += a.z * wv;
+          o[3] += a.w * wv;
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] *= inv;
+        if (cur.whole) {
+          const int i = row / p.group, h = cur.kvh * p.group + row - i * p.group;
+          const size_t orow = (static_cast<size_t>(cur.b) * p.tokens + i) * p.hq + h;
+          store_out4(p, orow * D + 4 * x, o);
+          if (p.lse != nullptr && x == 0) p.lse[orow] = lse_of(ref, sum);
+        } else {
+          *reinterpret_cast<float4*>(p.part_o + (slot * ROWS + r) * D + 4 * x) = make_float4(o[0], o[1], o[2], o[3]);
+          if (x == 0) p.part_ml[slot * ROWS + r] = make_float2(top, sum);
+        }
+      }
+      __syncthreads();
     }
-    if (lane == 0) warp_v[warp] = vref;
-    __syncthreads();
-    const bool whole = t0 == 0 && t1 == u.tiles;
-    const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (first ? 0 : 1);
-    for (int v = threadIdx.x; v < ROWS * (D / 4); v += kThreads) {
-      const int r = v / (D / 4), x = v % (D / 4);
-      const int row = row0 + r;
-      if (row >= rows_valid) continue;
-      float top = -INFINITY, sum = 0.0f, w[kWarps];
-#pragma unroll
-      for (int i = 0; i < kWarps; ++i) top = fmaxf(top, warp_m[i][r]);
-      const float ref = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-      for (int i = 0; i < kWarps; ++i) {
-        w[i] = ex2(warp_m[i][r] - ref);
-        sum += w[i] * warp_l[i][r];
-      }
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int i = 0; i < kWarps; ++i) {
-        const float4 a = *reinterpret_cast<const float4*>(merge + (i * ROWS + r) * D + 4 * x);
-        const float wi = w[i] * inv, vi = warp_v[i];
-        o[0] += a.x * wi * vi;
-        o[1] += a.y * wi * vi;
-        o[2] += a.z * wi * vi;
-        o[3] += a.w * wi * vi;
-      }
-      if (whole) {
-        const int i = row / p.group, h = kvh * p.group + row - i * p.group;
-        const size_t orow = (static_cast<size_t>(b) * p.tokens + i) * p.hq + h;
-        store_out4(p, orow * D + 4 * x, o);
-        if (p.lse != nullptr && x == 0) p.lse[orow] = lse_of(ref, sum);
-      } else {
-        *reinterpret_cast<float4*>(p.part_o + (slot * ROWS + r) * D + 4 * x) = make_float4(o[0], o[1], o[2], o[3]);
-        if (x == 0) p.part_ml[slot * ROWS + r] = make_float2(top, sum);
-      }
+    if (any) {
+      load_tile();
+      stage = stage == STAGES - 1 ? 0 : stage + 1;
     }
-    __syncthreads();  // before the next segment's q and sums
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // ------------------------------------------------------------------------------------ joining cut units
 // Rows of units that range borders cut (partials of CTAs c0 .. c1), rows that see nothing (zeros) and rows of
 // sequences whose lengths do not fit (NaN).  A CTA takes up to 8 rows, a warp each; a row with many partials is
-// joined by the whole CTA.
+// joined by the whole CTA, and where there are few rows by gridDim.y CTAs, each a share of the columns.
 template <int D, int NT>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, int rows_per_cta) {
   using S = Shape<D, NT>;
   constexpr int TOK = S::kTok, ROWS = S::kRows, kShort = 8;
-  constexpr int TPR = D / 4, PG = kJoinThreads / TPR;  // threads of a partial row, partials at a time
-  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int TPR = D / 4;               // threads of a row
+  const int tpr = TPR / gridDim.y;         // threads of this CTA's share of a row
+  const int pg_n = kJoinThreads / tpr;     // partials at a time
+  extern __shared__ __align__(128) uint8_t smem[];
   float* weight = reinterpret_cast<float*>(smem);                       // [kMaxCtas]
-  float4* sums = reinterpret_cast<float4*>(smem + kMaxCtas * 4);        // [PG][TPR]
+  float4* sums = reinterpret_cast<float4*>(smem + kMaxCtas * 4);        // [pg_n][tpr]
   uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + kMaxCtas * 4 + kJoinThreads * 16);
   __shared__ uint32_t scratch[kJoinThreads / 32];
   __shared__ float red[2][kJoinThreads / 32];
@@ -636,7 +702,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
   for (long long base = static_cast<long long>(blockIdx.x) * rows_per_cta; base < rows; base += step) {
     const long long row = base + warp;
     if (lane == 0) long_c1[warp] = 0;
-    if (warp < rows_per_cta && row < rows) {
+    if (warp < rows_per_cta && row < rows) {  // short rows: the first share's CTA does all of them
       const int h = static_cast<int>(row % p.hq);
       const int rest = static_cast<int>(row / p.hq);
       const int i = rest % p.tokens, b = rest / p.tokens;
@@ -644,8 +710,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
       if (!s.ok || i >= s.end - s.start) {
         const float f = s.ok ? 0.0f : nan_f();
         const float o[4] = {f, f, f, f};
-        for (int x = lane; x < TPR; x += 32) store_out4(p, static_cast<size_t>(row) * D + 4 * x, o);
-        if (p.lse != nullptr && lane == 0) p.lse[row] = s.ok ? -INFINITY : nan_f();
+        for (int x = lane; x < TPR && blockIdx.y == 0; x += 32) store_out4(p, static_cast<size_t>(row) * D + 4 * x, o);
+        if (p.lse != nullptr && lane == 0 && blockIdx.y == 0) p.lse[row] = s.ok ? -INFINITY : nan_f();
       } else {
         const Unit u = unit_of<TOK, ROWS>(p, s);
         const int kvh = h / p.group, r = i * p.group + h - kvh * p.group;
@@ -660,7 +726,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
             long_r[warp] = rr;
             long_row[warp] = row;
           }
-        } else if (c1 > c0) {
+        } else if (c1 > c0 && blockIdx.y == 0) {
           // the partial of CTA c: its first segment unless the unit began inside its range
           const uint32_t c = c0 + min(static_cast<uint32_t>(lane), c1 - c0);
           const size_t slot = 2 * static_cast<size_t>(c) + (range_begin(c, total, ctas) >= first ? 0 : 1);
@@ -710,10 +776,17 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
       if (c1 == 0) continue;
       const int n = static_cast<int>(c1 - c0) + 1, rr = long_r[k];
       const uint32_t first = long_t0[k];
+      // only the first CTA's partial may lie in its second slot
+      const size_t slot0 = 2 * static_cast<size_t>(c0) + (range_begin(c0, total, ctas) >= first ? 0 : 1);
+      auto slot_of = [&](int x) { return x == 0 ? slot0 : 2 * static_cast<size_t>(c0 + x); };
+      constexpr int M = (kMaxCtas + kJoinThreads - 1) / kJoinThreads;
+      float2 ml[M];
       float top = -INFINITY;
-      for (int x = threadIdx.x; x < n; x += kJoinThreads) {
-        const size_t slot = 2 * static_cast<size_t>(c0 + x) + (range_begin(c0 + x, total, ctas) >= first ? 0 : 1);
-        top = fmaxf(top, __ldcg(&p.part_ml[slot * ROWS + rr]).x);
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        const int x = threadIdx.x + i * kJoinThreads;
+        ml[i] = x < n ? __ldcg(&p.part_ml[slot_of(x) * ROWS + rr]) : make_float2(-INFINITY, 0.0f);
+        top = fmaxf(top, ml[i].x);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -723,11 +796,11 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
       for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, red[0][w]);
       const float ref = top == -INFINITY ? 0.0f : top;
       float sum = 0.0f;
-      for (int x = threadIdx.x; x < n; x += kJoinThreads) {
-        const size_t slot = 2 * static_cast<size_t>(c0 + x) + (range_begin(c0 + x, total, ctas) >= first ? 0 : 1);
-        const float2 ml = __ldcg(&p.part_ml[slot * ROWS + rr]);
-        const float w = ex2(ml.x - ref) * ml.y;
-        weight[x] = w;
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        const int x = threadIdx.x + i * kJoinThreads;
+        const float w = ex2(ml[i].x - ref) * ml[i].y;
+        if (x < n) weight[x] = w;
         sum += w;
       }
 #pragma unroll
@@ -738,31 +811,31 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
 #pragma unroll
       for (int w = 0; w < kJoinThreads / 32; ++w) sum += red[1][w];
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      const int x = threadIdx.x % TPR, pg = threadIdx.x / TPR;
+      const int x = threadIdx.x % tpr, pg = threadIdx.x / tpr;
+      const int col = (blockIdx.y * tpr + x) * 4;
       float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
-      for (int y = pg; y < n; y += PG) {
-        const size_t slot = 2 * static_cast<size_t>(c0 + y) + (range_begin(c0 + y, total, ctas) >= first ? 0 : 1);
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + (slot * ROWS + rr) * D) + x);
+      for (int y = pg; y < n; y += pg_n) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + (slot_of(y) * ROWS + rr) * D + col));
         const float w = weight[y] * inv;
         a.x += w * v.x;
         a.y += w * v.y;
         a.z += w * v.z;
         a.w += w * v.w;
       }
-      sums[pg * TPR + x] = a;
+      sums[pg * tpr + x] = a;
       __syncthreads();
       if (pg == 0) {
         float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int y = 0; y < PG; ++y) {
-          const float4 v = sums[y * TPR + x];
+        for (int y = 0; y < pg_n; ++y) {
+          const float4 v = sums[y * tpr + x];
           o[0] += v.x;
           o[1] += v.y;
           o[2] += v.z;
           o[3] += v.w;
         }
-        store_out4(p, static_cast<size_t>(long_row[k]) * D + 4 * x, o);
-        if (p.lse != nullptr && x == 0) p.lse[long_row[k]] = lse_of(ref, sum);
+        store_out4(p, static_cast<size_t>(long_row[k]) * D + col, o);
+        if (p.lse != nullptr && col == 0) p.lse[long_row[k]] = lse_of(ref, sum);
       }
       __syncthreads();  // before the next row's weights and sums
     }
@@ -770,38 +843,47 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
   }
 }
 
+#ifndef KV8_FEW
+#define KV8_FEW 1
+#endif
+#ifndef KV8_MIN_FEW
+#define KV8_MIN_FEW 8
+#endif
+constexpr int kSmallWarps = 4;
+
 template <int D, int NT>
 size_t workspace_bytes(int sms) {
   using S = Shape<D, NT>;
-  const size_t slots = 2 * static_cast<size_t>(sms) * S::kCtasPerSm;
+  const size_t slots = 2 * static_cast<size_t>(sms) * (S::kWarpsPerSm / kSmallWarps);
   return slots * S::kRows * (D * 4 + 8);
 }
 
-template <int D, bool E4M3, int NT>
-int launch_attn(const char* who, AttnParams& p, int sms, void* workspace, cudaStream_t s) {
+template <int D, bool E4M3, int NT, int W>
+int launch_with(const char* who, AttnParams& p, int sms, void* workspace, cudaStream_t s) {
   using S = Shape<D, NT>;
-  p.grid = sms * S::kCtasPerSm;
+  p.grid = sms * (S::kWarpsPerSm / W);
+  p.min_tiles = W == kSmallWarps ? kSmallWarps : KV8_MIN_FEW;
   if (p.grid > kMaxCtas) return fail(TOKMIX_ERR_UNSUPPORTED, "%s: more SMs than the kernel is planned for", who);
   const size_t slots = 2 * static_cast<size_t>(p.grid);
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + slots * S::kRows * D);
   const int plan = (p.c.batch + 1) * 4;
-  const int smem = S::kMergeBytes + S::kRows * S::kQStride * 2 + plan;
   const int join_smem = kMaxCtas * 4 + kJoinThreads * 16 + plan;
-  // limits for the largest batch, set once
-  const int plan_max = (kMaxBatch + 1) * 4;
-  auto* attn = attn_kernel<D, E4M3, NT>;
+  const int plan_max = (kMaxBatch + 1) * 4;  // the limit is set once, for the largest batch
+  const int attn_plan_max = W == kSmallWarps ? plan_max : (kMaxCtas + 1) * 4;  // large CTAs: at most a unit per SM
+  auto* attn = attn_kernel<D, E4M3, NT, W>;
   auto* join = join_kernel<D, NT>;
-  if (!ensure_smem_attr(reinterpret_cast<const void*>(attn), S::kMergeBytes + S::kRows * S::kQStride * 2 + plan_max) ||
+  if (!ensure_smem_attr(reinterpret_cast<const void*>(attn), S::smem_bytes(W) + attn_plan_max) ||
       !ensure_smem_attr(reinterpret_cast<const void*>(join), kMaxCtas * 4 + kJoinThreads * 16 + plan_max))
     return fail(TOKMIX_ERR_LAUNCH, "%s: cannot set the shared memory size", who);
-  attn<<<p.grid, kThreads, smem, s>>>(p);
+  attn<<<p.grid, 32 * W, S::smem_bytes(W) + plan, s>>>(p);
   if (const int rc = check_launch(who)) return rc;
   const long long rows = static_cast<long long>(p.c.batch) * p.tokens * p.hq;
   const int per = static_cast<int>(std::min<long long>(8, (rows + 2 * sms - 1) / (2 * sms)));
   const long long want = (rows + per - 1) / per;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(want, 4LL * sms)));
+  // with a row per CTA, rows of long sequences are shared by CTAs of 64 columns
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(want, 4LL * sms)), per == 1 ? D / 64 : 1);
   cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = static_cast<size_t>(join_smem);
   cfg.stream = s;
@@ -812,6 +894,15 @@ int launch_attn(const char* who, AttnParams& p, int sms, void* workspace, cudaSt
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, join, static_cast<const AttnParams>(p), per) != cudaSuccess) return check_launch(who);
   return check_launch(who);
+}
+
+template <int D, bool E4M3, int NT>
+int launch_attn(const char* who, AttnParams& p, int sms, void* workspace, cudaStream_t s) {
+  using S = Shape<D, NT>;
+  // few units: one CTA per SM leaves the fewest partial rows to join; many: small CTAs, whose unit changes overlap
+  const long long units = static_cast<long long>(p.c.batch) * p.c.hkv * ((p.tokens * p.group + S::kRows - 1) / S::kRows);
+  if (KV8_FEW && units <= sms) return launch_with<D, E4M3, NT, S::kWarpsPerSm>(who, p, sms, workspace, s);
+  return launch_with<D, E4M3, NT, kSmallWarps>(who, p, sms, workspace, s);
 }
 
 template <int D>

@@ -23,6 +23,7 @@ go through ``flash_attention_2`` (their keys and values enter the cache with ``k
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -33,6 +34,12 @@ from .kv8_append import check_device_status  # noqa: F401
 
 KERNEL_TYPE = "kv8_attention"
 MAX_TOKENS = 16
+
+
+@functools.cache
+def _workspace_bytes(tokens: int, hq: int, hkv: int, d: int, device: int) -> int:
+    """The workspace of a shape on a device (which is current)."""
+    return _lib.load().tokmix_kv8_attention_workspace_bytes(tokens, hq, hkv, d)
 
 
 def kernel_fn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -60,7 +67,7 @@ def kernel_fn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_s
     lib = _lib.load()
     with _lib.on_device(dev):
         status = _lib.host_status_ptr(dev, "kv8")
-        need = lib.tokmix_kv8_attention_workspace_bytes(max(tokens, 1), hq, cache.heads_kv, d)
+        need = _workspace_bytes(max(tokens, 1), hq, cache.heads_kv, d, dev.index)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)  # per call: calls may overlap on other streams
         rc = lib.tokmix_kv8_attention(q.data_ptr(), *qs, out.data_ptr(), lse.data_ptr() if return_lse else None, tokens,
                                       hq, _kv8.IO_DTYPES[q.dtype], sm_scale, _kv8.byref(cache), ws.data_ptr(), need,
