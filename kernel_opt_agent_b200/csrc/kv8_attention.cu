@@ -47,9 +47,9 @@ struct Shape {
   static constexpr int kMt = kTok / 16;       // 16-token subtiles (a page holds whole ones)
   static constexpr int kRows = 8 * NT;        // query rows per unit
   static constexpr int kQStride = D + 8;      // halves between rows of q in shared memory (conflict-free 16-byte reads)
-  static constexpr int kStageBytes = 2 * kTok * D;   // a tile's keys and values
-  static constexpr int kStages = D == 64 ? 6 : 3;    // 24 KB in flight per warp
-  static constexpr int kWarpsPerSm = 8;
+  static constexpr int kStageBytes = 2 * kTok * D;              // a tile's keys and values
+  static constexpr int kWarpsPerSm = NT == 1 ? 12 : 8;          // 168 or 255 registers a thread
+  static constexpr int kStages = (NT == 1 ? 16384 : 24576) / kStageBytes;  // 192 KB of tiles per SM
   __host__ __device__ static constexpr int smem_bytes(int warps) { return warps * kStages * (kStageBytes + 8 * kMt) + kRows * kQStride * 2; }
   static_assert(8 * D * 4 <= kStageBytes, "eight partial rows fit a stage");
 };
@@ -243,8 +243,11 @@ __device__ __forceinline__ int merge_chunk(int row, int chunk) {
   return chunk ^ (D == 64 ? (cq & 1) | ((cq >> 1) << 2) : cq);
 }
 
-// Copies 16 bytes to shared memory, or zeros if !live (nothing is read then)
-__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, bool live) {
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// the same, or zeros if !live (nothing is read then)
+__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const uint8_t* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void copy4(uint32_t dst, const float* src) {
@@ -265,7 +268,7 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
   __half* qs = reinterpret_cast<__half*>(smem + W * STAGES * (S::kStageBytes + 8 * MT));  // [row][kQStride]
   uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + S::smem_bytes(W));
   __shared__ float row_factor[ROWS], warp_m[W][ROWS], warp_l[W][ROWS], warp_v[W];
-  __shared__ int warp_at[W];  // where in `smem` a warp's partial rows lie, -1: it had no tile of the segment
+  __shared__ int warp_at[W];  // where in `smem` a warp's partial rows lie
   __shared__ uint32_t scratch[W];
 
   const View& c = p.c;
@@ -317,12 +320,21 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
         const uint8_t* ksrc = c.k + pg * c.k_page_stride + ld.kvh * c.k_head_stride + slot;
         const uint8_t* vsrc = c.v + pg * c.v_page_stride + ld.kvh * c.v_head_stride + slot;
         const int rows = good ? ld.s.end - tok : 0;  // token rows to read; zeros behind them
+        if (rows >= 16) {
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          const int r = (i * 32 + lane) / (D / 16), ch = lane % (D / 16);
-          const uint32_t dst = dst0 + mt * 16 * D + tile_chunk<D>(r, ch);
-          copy16(dst, ksrc + i * 512, r < rows);
-          copy16(dst + TOK * D, vsrc + i * 512, r < rows);
+          for (int i = 0; i < D / 32; ++i) {
+            const uint32_t dst = dst0 + mt * 16 * D + tile_chunk<D>((i * 32 + lane) / (D / 16), lane % (D / 16));
+            copy16(dst, ksrc + i * 512);
+            copy16(dst + TOK * D, vsrc + i * 512);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            const int r = (i * 32 + lane) / (D / 16);
+            const uint32_t dst = dst0 + mt * 16 * D + tile_chunk<D>(r, lane % (D / 16));
+            copy16_or_zero(dst, ksrc + i * 512, r < rows);
+            copy16_or_zero(dst + TOK * D, vsrc + i * 512, r < rows);
+          }
         }
         float* sc = scales + ld_stage * 2 * MT + mt;
         if (good) {
@@ -476,22 +488,30 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
       }
       // softmax: a lane has tokens g and g + 8 of each subtile for its rows
       float top[NT][2];
-      const bool tail = t * TOK + TOK > min_lim;
+      const bool tail = t * TOK + TOK > min_lim;  // some token is hidden from some row
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            sc[mt][nt][0][e] = (sc[mt][nt][0][e] + sc[mt][nt][1][e]) * (ks[mt] * factor[nt][e & 1]);
+      if (tail) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (t * TOK + mt * 16 + (e >> 1) * 8 + g >= lim[nt][e & 1]) sc[mt][nt][0][e] = -INFINITY;
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          top[nt][e] = -INFINITY;
+          top[nt][e] = fmaxf(sc[0][nt][0][e], sc[0][nt][0][2 + e]);
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              float& x = sc[mt][nt][0][half * 2 + e];
-              x = (x + sc[mt][nt][1][half * 2 + e]) * (ks[mt] * factor[nt][e]);
-              if (tail && t * TOK + mt * 16 + half * 8 + g >= lim[nt][e]) x = -INFINITY;
-              top[nt][e] = fmaxf(top[nt][e], x);
-            }
-          }
+          for (int mt = 1; mt < MT; ++mt) top[nt][e] = fmaxf(top[nt][e], fmaxf(sc[mt][nt][0][e], sc[mt][nt][0][2 + e]));
         }
       }
       bool grew = false;
@@ -532,20 +552,30 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
       }
       uint32_t pb[MT][NT][2];
 #pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float off[2] = {ref[nt][0] - kShift, ref[nt][1] - kShift};
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sc[mt][nt][0][e] = ex2(sc[mt][nt][0][e] - off[e & 1]);
+            l[nt][e & 1] += sc[mt][nt][0][e];
+          }
+      }
+#pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        const float rv = vref > 0.0f ? vs[mt] / vref : vs[mt] * 0.0f;
+        const float rv = vref > 0.0f ? __fdividef(vs[mt], vref) : vs[mt] * 0.0f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const float w0 = ex2(sc[mt][nt][0][half * 2] - (ref[nt][0] - kShift));
-            const float w1 = ex2(sc[mt][nt][0][half * 2 + 1] - (ref[nt][1] - kShift));
-            l[nt][0] += w0;
-            l[nt][1] += w1;
-            // a hidden token weighs nothing even where its block's scale is NaN
-            const float p0 = sc[mt][nt][0][half * 2] == -INFINITY ? 0.0f : w0 * rv;
-            const float p1 = sc[mt][nt][0][half * 2 + 1] == -INFINITY ? 0.0f : w1 * rv;
-            pb[mt][nt][half] = transpose8x8(half2_bits(p0, p1));
+            float w0 = sc[mt][nt][0][half * 2] * rv, w1 = sc[mt][nt][0][half * 2 + 1] * rv;
+            if (tail) {  // a hidden token weighs nothing even where its block's scale is NaN
+              const int tok = t * TOK + mt * 16 + half * 8 + g;
+              w0 = tok >= lim[nt][0] ? 0.0f : w0;
+              w1 = tok >= lim[nt][1] ? 0.0f : w1;
+            }
+            pb[mt][nt][half] = transpose8x8(half2_bits(w0, w1));
           }
         }
       }
@@ -620,10 +650,11 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
       }
       if (lane == 0) {
         warp_v[warp] = vref;
-        warp_at[warp] = any ? static_cast<int>(reinterpret_cast<uint8_t*>(dst) - smem) : -1;
+        warp_at[warp] = static_cast<int>(reinterpret_cast<uint8_t*>(dst) - smem);
       }
       __syncthreads();
       const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (first ? 0 : 1);
+      const int nw = min(W, t1 - cur.t0);  // warps that had a tile
       constexpr int kOut = 8 * (D / 4);
 #pragma unroll
       for (int k = 0; k < (kOut + kThreads - 1) / kThreads; ++k) {
@@ -631,14 +662,12 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
         const int r8 = v / (D / 4), x = v % (D / 4);
         const int r = nt * 8 + r8, row = row0 + r;
         if (v >= kOut || row >= rows_valid) break;
-        float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < W; ++i) top = fmaxf(top, warp_m[i][r]);
+        float top = warp_m[0][r], sum = 0.0f;
+        for (int i = 1; i < nw; ++i) top = fmaxf(top, warp_m[i][r]);
         const float ref = top == -INFINITY ? 0.0f : top;
         float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-          if (warp_at[i] < 0) continue;
+#pragma unroll 4
+        for (int i = 0; i < nw; ++i) {
           const float4 a = *reinterpret_cast<const float4*>(smem + warp_at[i] + r8 * D * 4 + 16 * merge_chunk<D>(r8, x));
           const float w = ex2(warp_m[i][r] - ref);
           sum += w * warp_l[i][r];
@@ -690,21 +719,24 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
   __shared__ float red[2][kJoinThreads / 32];
   __shared__ uint32_t long_c0[8], long_c1[8], long_t0[8];
   __shared__ int long_r[8];
-  __shared__ long long long_row[8];
+  __shared__ int long_row[8];
 
-  make_plan<TOK, ROWS, kJoinThreads>(p, prefix, scratch);  // reads only the call's inputs
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  make_plan<TOK, ROWS, kJoinThreads>(p, prefix, scratch);
   const uint32_t total = prefix[p.c.batch];
   const uint32_t ctas = active_ctas(p, total);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long rows = static_cast<long long>(p.c.batch) * p.tokens * p.hq;
-  const long long step = static_cast<long long>(gridDim.x) * rows_per_cta;
-  for (long long base = static_cast<long long>(blockIdx.x) * rows_per_cta; base < rows; base += step) {
-    const long long row = base + warp;
+  const int rows = p.c.batch * p.tokens * p.hq;
+  const int step = gridDim.x * rows_per_cta;
+  bool waited = false;  // the rows are found from the call's inputs alone, while the attention kernel still runs
+  auto wait_partials = [&]() {
+    if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+    waited = true;
+  };
+  for (int base = blockIdx.x * rows_per_cta; base < rows; base += step) {
+    const int row = base + warp;
     if (lane == 0) long_c1[warp] = 0;
     if (warp < rows_per_cta && row < rows) {  // short rows: the first share's CTA does all of them
-      const int h = static_cast<int>(row % p.hq);
-      const int rest = static_cast<int>(row / p.hq);
+      const int rest = row / p.hq, h = row - rest * p.hq;
       const int i = rest % p.tokens, b = rest / p.tokens;
       const Seq s = load_seq(p.c, b, p.tokens);
       if (!s.ok || i >= s.end - s.start) {
@@ -727,10 +759,11 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
             long_row[warp] = row;
           }
         } else if (c1 > c0 && blockIdx.y == 0) {
-          // the partial of CTA c: its first segment unless the unit began inside its range
-          const uint32_t c = c0 + min(static_cast<uint32_t>(lane), c1 - c0);
-          const size_t slot = 2 * static_cast<size_t>(c) + (range_begin(c, total, ctas) >= first ? 0 : 1);
-          const float2 ml = lane <= static_cast<int>(c1 - c0) ? p.part_ml[slot * ROWS + rr] : make_float2(-INFINITY, 0.0f);
+          // the partial of a CTA is its first segment's, unless the unit began inside the CTA's range
+          const uint32_t slot0 = 2 * c0 + (range_begin(c0, total, ctas) >= first ? 0 : 1);
+          const size_t slot = lane == 0 ? slot0 : 2 * (c0 + min(static_cast<uint32_t>(lane), c1 - c0));
+          wait_partials();
+          const float2 ml = lane <= static_cast<int>(c1 - c0) ? __ldcg(&p.part_ml[slot * ROWS + rr]) : make_float2(-INFINITY, 0.0f);
           float top = ml.x;
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -750,7 +783,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
           for (int k = 0; k < kShort; ++k) {
             if (k > static_cast<int>(c1 - c0)) break;
             const float wk = __shfl_sync(0xffffffffu, w, k) * inv;
-            const size_t sk = 2 * static_cast<size_t>(c0 + k) + (range_begin(c0 + k, total, ctas) >= first ? 0 : 1);
+            const size_t sk = k == 0 ? slot0 : 2 * (c0 + k);
             const float4* src = reinterpret_cast<const float4*>(p.part_o + (sk * ROWS + rr) * D);
 #pragma unroll
             for (int x = 0; x < X; ++x) {
@@ -774,6 +807,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
     for (int k = 0; k < rows_per_cta; ++k) {  // uniform over the CTA
       const uint32_t c0 = long_c0[k], c1 = long_c1[k];
       if (c1 == 0) continue;
+      wait_partials();
       const int n = static_cast<int>(c1 - c0) + 1, rr = long_r[k];
       const uint32_t first = long_t0[k];
       // only the first CTA's partial may lie in its second slot
@@ -841,6 +875,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
     }
     __syncthreads();  // before the next rows' descriptions
   }
+  wait_partials();
 }
 
 #ifndef KV8_FEW
@@ -901,7 +936,7 @@ int launch_attn(const char* who, AttnParams& p, int sms, void* workspace, cudaSt
   using S = Shape<D, NT>;
   // few units: one CTA per SM leaves the fewest partial rows to join; many: small CTAs, whose unit changes overlap
   const long long units = static_cast<long long>(p.c.batch) * p.c.hkv * ((p.tokens * p.group + S::kRows - 1) / S::kRows);
-  if (KV8_FEW && units <= sms) return launch_with<D, E4M3, NT, S::kWarpsPerSm>(who, p, sms, workspace, s);
+  if (KV8_FEW && units * 4 <= sms) return launch_with<D, E4M3, NT, S::kWarpsPerSm>(who, p, sms, workspace, s);
   return launch_with<D, E4M3, NT, kSmallWarps>(who, p, sms, workspace, s);
 }
 
@@ -963,7 +998,8 @@ extern "C" int tokmix_kv8_attention(const void* q, long long q_batch_stride, lon
   if (p.c.batch > kMaxBatch) return fail(TOKMIX_ERR_UNSUPPORTED, "%s: at most %d sequences (got %d)", who, kMaxBatch, p.c.batch);
   const long long most_tiles = (static_cast<long long>(p.c.max_pages) * p.c.page + 15) / 16 * p.c.hkv *
                                ((static_cast<long long>(tokens) * (heads_q / p.c.hkv) + 7) / 8) * p.c.batch;
-  if (heads_q > 65536 || most_tiles > 0x7fffffffLL) return fail(TOKMIX_ERR_UNSUPPORTED, "%s: problem too large", who);
+  if (heads_q > 65536 || most_tiles > 0x7fffffffLL || static_cast<long long>(p.c.batch) * tokens * heads_q > 0x3fffffffLL)
+    return fail(TOKMIX_ERR_UNSUPPORTED, "%s: problem too large", who);
   if (const int rc = check_device()) return rc;
   const long long need = tokmix_kv8_attention_workspace_bytes(tokens, heads_q, cache->heads_kv, cache->head_dim);
   if (workspace_bytes < need)

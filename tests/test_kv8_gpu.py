@@ -282,6 +282,40 @@ def test_attention_many_ragged_sequences(cuda_device):
     assert bool((buf[0] == 7).all()) and bool((buf[301] == 7).all())
 
 
+@pytest.mark.parametrize("cache_dtype,b,most,t,hq,hkv,d,page", [
+    (E4M3, 40, 3000, 1, 8, 8, 64, 32), (INT8, 24, 2500, 1, 32, 8, 128, 64), (E4M3, 30, 2000, 3, 16, 4, 128, 16),
+    (INT8, 9, 9000, 1, 16, 2, 256, 128), (E4M3, 5, 9000, 2, 24, 2, 256, 64), (E4M3, 2, 120000, 1, 8, 1, 64, 128)])
+def test_attention_large_calls(cuda_device, cache_dtype, b, most, t, hq, hkv, d, page):
+    """Calls that give every CTA many tiles and several units: every row, the same bits every time
+    (also captured and replayed)."""
+    rng = np.random.default_rng(b)
+    lens = [most] + [int(x) for x in rng.integers(most // 2, most, b - 1)]
+    lens[b // 2] = 0 if b > 3 else lens[b // 2]
+    cache = _filled_cache(b, lens, hkv, d, page, cache_dtype, cuda_device, rng)
+    q = _queries(b, b, t, hq, d, torch.bfloat16, cuda_device)
+    seq, new = _i32(lens, cuda_device), _i32([min(t, n) for n in lens], cuda_device)
+    out, lse = attention.kernel_fn(q, *cache, seq, new, return_lse=True)
+    attention.check_device_status(cuda_device)
+    _assert_attention(out, lse, q, cache, seq, new)
+    for _ in range(5):
+        assert torch.equal(out, attention.kernel_fn(q, *cache, seq, new))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = attention.kernel_fn(q, *cache, seq, new)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cap = attention.kernel_fn(q, *cache, seq, new)
+    for _ in range(3):
+        cap.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(cap, out)
+    assert torch.equal(other, out)
+
+
+
+
 @pytest.mark.parametrize("sm_scale", [1e-6, 0.05, 30.0])
 def test_attention_flat_and_sharp_softmax(cuda_device, sm_scale):
     lens = [700, 64]
