@@ -25,10 +25,10 @@ struct AppendParams {
   const void* k;
   const void* v;
   long long k_sb, k_st, k_sh, v_sb, v_st, v_sh;  // element strides of the new keys and values
-  int rows;     // new tokens per sequence at most
-  int touched;  // pages a sequence can touch
+  int rows;          // new tokens per sequence at most
+  uint32_t touched;  // pages a sequence can touch
   int d, d_shift;
-  long long units;
+  uint32_t units;
   uint32_t* status;
 };
 
@@ -48,6 +48,11 @@ struct Half16;
 template <>
 struct Half16<__nv_bfloat16> {
   static constexpr uint32_t kInf = 0x7f80u;
+  // larger magnitude of each half (its sign is of no use), NaN if either is
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 m = __hmax2_nan(__habs2(*reinterpret_cast<const __nv_bfloat162*>(&a)), __habs2(*reinterpret_cast<const __nv_bfloat162*>(&b)));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
   static __device__ __forceinline__ float widen(uint32_t b) { return __uint_as_float(b << 16); }
   static __device__ __forceinline__ float2 widen2(uint32_t w) {
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
@@ -56,25 +61,29 @@ struct Half16<__nv_bfloat16> {
 template <>
 struct Half16<__half> {
   static constexpr uint32_t kInf = 0x7c00u;
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    const __half2 m = __hmax2_nan(__habs2(*reinterpret_cast<const __half2*>(&a)), __habs2(*reinterpret_cast<const __half2*>(&b)));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
   static __device__ __forceinline__ float widen(uint32_t b) { return __half2float(__ushort_as_half(static_cast<uint16_t>(b))); }
   static __device__ __forceinline__ float2 widen2(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
   }
 };
 
-// GT threads work on a unit (32: eight units per CTA; 256: one), NV vectors of 8 values each.
+// GT threads work on a unit (a warp: eight units per CTA; more: one), NV vectors of 8 values each.
 template <typename T, bool E4M3, int NV, int GT>
-__global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(GT == 32 ? 256 : GT) append_kernel(const AppendParams p) {
+  constexpr int kUnits = GT == 32 ? 8 : 1;
   const View& c = p.c;
-  const long long unit = static_cast<long long>(blockIdx.x) * (256 / GT) + threadIdx.x / GT;
-  if (unit >= p.units) return;  // warp-uniform (GT 32), never (GT 256)
+  const uint32_t unit = blockIdx.x * kUnits + threadIdx.x / GT;
+  if (unit >= p.units) return;  // warp-uniform (a warp per unit), never (a CTA per unit)
   const int lane = threadIdx.x & (GT - 1);
   const bool is_v = (unit & 1) != 0;
-  long long rest = unit >> 1;
-  const int h = static_cast<int>(rest % c.hkv);
-  rest /= c.hkv;
-  const int j = static_cast<int>(rest % p.touched);
-  const int b = static_cast<int>(rest / p.touched);
+  const uint32_t page_of = (unit >> 1) / p.c.hkv;  // 32-bit divisions: 64-bit ones cost more than the page's values do
+  const int h = static_cast<int>((unit >> 1) - page_of * p.c.hkv);
+  const int b = static_cast<int>(page_of / p.touched);
+  const int j = static_cast<int>(page_of - b * p.touched);
 
   const Seq s = load_seq(c, b, p.rows);
   if (!s.ok) {
@@ -85,31 +94,34 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
   const int page0 = pj << c.page_shift;  // position of the page's first slot
   const int lo = max(s.start, page0), hi = min(s.end, page0 + c.page);
   if (lo >= hi) return;  // a page the sequence does not reach
-  const int pid = __ldg(c.table + static_cast<long long>(b) * c.table_stride + pj);
-  if (pid < 0 || pid >= c.num_pages) {
-    if (lane == 0) report_bad(p.status);
-    return;
-  }
+  const int pid = __ldg(c.table + static_cast<long long>(b) * c.table_stride + pj);  // used behind the tokens' loads
   const T* src = is_v ? static_cast<const T*>(p.v) + b * p.v_sb + h * p.v_sh : static_cast<const T*>(p.k) + b * p.k_sb + h * p.k_sh;
   const long long st = is_v ? p.v_st : p.k_st;
   src += (lo - s.start) * st;
-  uint8_t* tile = is_v ? c.v + pid * c.v_page_stride + h * c.v_head_stride : c.k + pid * c.k_page_stride + h * c.k_head_stride;
-  float* scale = (is_v ? c.v_scale : c.k_scale) + static_cast<long long>(pid) * c.hkv + h;
-  const bool has_old = lo > page0;
-  const float s_old = has_old ? *scale : 0.0f;
 
   const int vshift = p.d_shift - 3;  // vectors per token: 1 << vshift
   const int nvec = (hi - lo) << vshift;
   uint4 x[NV];
-  uint32_t amax2 = 0;  // packed 16-bit magnitudes: as integers they order like the values, NaN above infinity
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int vi = lane + i * GT;
     x[i] = make_uint4(0u, 0u, 0u, 0u);
     if (vi < nvec) x[i] = __ldcs(reinterpret_cast<const uint4*>(src + (vi >> vshift) * st) + (vi & ((1 << vshift) - 1)));
-    amax2 = __vmaxu2(amax2, __vmaxu2(__vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu),
-                                     __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu)));
   }
+  if (pid < 0 || pid >= c.num_pages) {
+    if (lane == 0) report_bad(p.status);
+    return;  // the whole unit
+  }
+  uint8_t* tile = is_v ? c.v + pid * c.v_page_stride + h * c.v_head_stride : c.k + pid * c.k_page_stride + h * c.k_head_stride;
+  float* scale = (is_v ? c.v_scale : c.k_scale) + static_cast<long long>(pid) * c.hkv + h;
+  const bool has_old = lo > page0;
+  const float s_old = has_old ? *scale : 0.0f;
+
+  uint32_t amax2 = 0;  // packed magnitudes; a NaN stays one
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    amax2 = Half16<T>::max2(Half16<T>::max2(Half16<T>::max2(amax2, x[i].x), Half16<T>::max2(x[i].y, x[i].z)), x[i].w);
+  amax2 &= 0x7fff7fffu;  // as integers, magnitudes order like the values, NaN above infinity
   uint32_t amax = __reduce_max_sync(0xffffffffu, max(amax2 & 0xffffu, amax2 >> 16));
   if constexpr (GT > 32) {
     __shared__ uint32_t part[GT / 32];
@@ -162,13 +174,16 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
 template <typename T, bool E4M3>
 void launch_append(const AppendParams& p, cudaStream_t s) {
   const int most = std::min(p.rows, p.c.page) << (p.d_shift - 3);  // vectors of the largest unit
-  const unsigned ctas = static_cast<unsigned>(p.units);
+  // 8 vectors a thread keep enough loads in flight and few enough threads busy with the unit's pointers (4 prompts of
+  // 8192 tokens, Hkv 8, D 128, pages of 64: 128 threads x 8 23.4 us, 256 x 4 30.2 us, 64 x 16 28.5 us)
   if (most <= 4 * 32)
-    append_kernel<T, E4M3, 4, 32><<<static_cast<unsigned>((p.units + 7) / 8), 256, 0, s>>>(p);
-  else if (most <= 4 * 256)
-    append_kernel<T, E4M3, 4, 256><<<ctas, 256, 0, s>>>(p);
+    append_kernel<T, E4M3, 4, 32><<<(p.units + 7) / 8, 256, 0, s>>>(p);
+  else if (most <= 8 * 128)
+    append_kernel<T, E4M3, 8, 128><<<p.units, 128, 0, s>>>(p);
+  else if (most <= 8 * 256)
+    append_kernel<T, E4M3, 8, 256><<<p.units, 256, 0, s>>>(p);
   else
-    append_kernel<T, E4M3, 16, 256><<<ctas, 256, 0, s>>>(p);
+    append_kernel<T, E4M3, 16, 256><<<p.units, 256, 0, s>>>(p);
 }
 
 int make_view(const char* who, const tokmix_kv8_cache* c, View& out) {
@@ -248,8 +263,9 @@ extern "C" int tokmix_kv8_append(const void* k, long long k_batch_stride, long l
   p.touched = (tokens + p.c.page - 2) / p.c.page + 1;  // one token: 1; a page may be entered at any slot
   p.d = cache->head_dim;
   p.d_shift = p.d == 64 ? 6 : p.d == 128 ? 7 : 8;
-  p.units = 2LL * p.c.batch * p.touched * p.c.hkv;
-  if (p.units > 0x7FFFFFFFLL) return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_kv8_append: problem too large");
+  const long long units = 2LL * p.c.batch * p.touched * p.c.hkv;
+  if (units > 0x7FFFFFFFLL) return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_kv8_append: problem too large");
+  p.units = static_cast<uint32_t>(units);
   p.status = status;
   if (const int rc = check_device()) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
