@@ -202,6 +202,8 @@ int make_view(const char* who, const tokmix_kv8_cache* c, View& out) {
   for (const long long st : {c->k_page_stride, c->k_head_stride, c->v_page_stride, c->v_head_stride})
     if (st % 16 != 0 || st < tile)
       return fail(TOKMIX_ERR_INVALID_ARGUMENT, "%s: page and head strides must be multiples of 16 and at least a tile", who);
+  if (c->k_page_stride > 0xffffffffLL || c->v_page_stride > 0xffffffffLL)
+    return fail(TOKMIX_ERR_UNSUPPORTED, "%s: pages more than 4 GB apart", who);
   if (c->table_stride < c->max_pages) return fail(TOKMIX_ERR_INVALID_ARGUMENT, "%s: bad table stride", who);
   if (c->batch > 0) {
     if (!c->k || !c->v || !c->k_scale || !c->v_scale || !c->seq_lens || (c->max_pages > 0 && !c->block_table))

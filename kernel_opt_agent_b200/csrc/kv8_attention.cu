@@ -290,6 +290,17 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
     if (prefix[mid] <= walk.pos) walk.b = mid; else hi = mid;
   }
 
+  // byte offsets inside a tile: this lane's share of a copy, its keys, its values
+  constexpr int kCopies = D == 64 ? 1 : D == 128 ? 2 : 4;
+  uint32_t cp_off[kCopies], k_off[2], v_off[2];
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) cp_off[i] = tile_chunk<D>((i * 32 + lane) / (D / 16), lane % (D / 16)) - i * 512;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    k_off[i] = tile_chunk<D>(g, D == 64 ? cq : 2 * cq + i);
+    v_off[i] = D == 64 ? tile_chunk<D>(2 * cq + i, g >> 1) + (g & 1) * 8 : tile_chunk<D>(2 * cq + i, g);
+  }
+
   // ---- the loads run ahead of the products by up to STAGES tiles, across units; table entries by one more
   Walk<TOK, ROWS> ahead = walk;
   Segment ld{};         // unit of the next tile to load
@@ -297,10 +308,15 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
   bool ld_live;         // false: no tile is left
   int pid[MT];          // its pages
   int ld_stage = 0;
+  const uint8_t *ld_k = nullptr, *ld_v = nullptr;  // its head in page 0, this lane's 16 bytes
   auto find_tile = [&]() {
     while (ld_live && ld_t >= ld.t1) {
       ld_live = ahead.next(p, prefix, ld);
-      if (ld_live) ld_t = ld.t0 + warp;
+      if (ld_live) {
+        ld_t = ld.t0 + warp;
+        ld_k = c.k + ld.kvh * c.k_head_stride + lane * 16;
+        ld_v = c.v + ld.kvh * c.v_head_stride + lane * 16;
+      }
     }
     if (ld_live) {
 #pragma unroll
@@ -315,15 +331,15 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
       for (int mt = 0; mt < MT; ++mt) {
         const int tok = ld_t * TOK + mt * 16;
         const bool good = static_cast<unsigned>(pid[mt]) < static_cast<unsigned>(c.num_pages);
-        const long long pg = good ? pid[mt] : 0;
-        const int slot = (tok & (c.page - 1)) * D + lane * 16;
-        const uint8_t* ksrc = c.k + pg * c.k_page_stride + ld.kvh * c.k_head_stride + slot;
-        const uint8_t* vsrc = c.v + pg * c.v_page_stride + ld.kvh * c.v_head_stride + slot;
+        const uint32_t pg = good ? pid[mt] : 0;
+        const int slot = (tok & (c.page - 1)) * D;
+        const uint8_t* ksrc = ld_k + static_cast<unsigned long long>(pg) * static_cast<uint32_t>(c.k_page_stride) + slot;
+        const uint8_t* vsrc = ld_v + static_cast<unsigned long long>(pg) * static_cast<uint32_t>(c.v_page_stride) + slot;
         const int rows = good ? ld.s.end - tok : 0;  // token rows to read; zeros behind them
         if (rows >= 16) {
 #pragma unroll
           for (int i = 0; i < D / 32; ++i) {
-            const uint32_t dst = dst0 + mt * 16 * D + tile_chunk<D>((i * 32 + lane) / (D / 16), lane % (D / 16));
+            const uint32_t dst = dst0 + mt * 16 * D + i * 512 + cp_off[i % kCopies];
             copy16(dst, ksrc + i * 512);
             copy16(dst + TOK * D, vsrc + i * 512);
           }
@@ -331,14 +347,14 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
 #pragma unroll
           for (int i = 0; i < D / 32; ++i) {
             const int r = (i * 32 + lane) / (D / 16);
-            const uint32_t dst = dst0 + mt * 16 * D + tile_chunk<D>(r, lane % (D / 16));
+            const uint32_t dst = dst0 + mt * 16 * D + i * 512 + cp_off[i % kCopies];
             copy16_or_zero(dst, ksrc + i * 512, r < rows);
             copy16_or_zero(dst + TOK * D, vsrc + i * 512, r < rows);
           }
         }
         float* sc = scales + ld_stage * 2 * MT + mt;
         if (good) {
-          if (lane < 2) copy4(smem_addr(sc + lane * MT), (lane == 0 ? c.k_scale : c.v_scale) + pg * c.hkv + ld.kvh);
+          if (lane < 2) copy4(smem_addr(sc + lane * MT), (lane == 0 ? c.k_scale : c.v_scale) + static_cast<unsigned long long>(pg) * static_cast<uint32_t>(c.hkv) + ld.kvh);
         } else if (lane < 2) {  // NaN scores for the rows that see it
           sc[lane * MT] = lane == 0 && tok < ld.s.end ? nan_f() : 0.0f;
           if (lane == 0 && tok < ld.s.end) report_bad(p.status);
@@ -350,8 +366,8 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
     ld_stage = ld_stage == STAGES - 1 ? 0 : ld_stage + 1;
     find_tile();
   };
-  ld_live = ahead.next(p, prefix, ld);
-  ld_t = ld.t0 + warp;
+  ld_live = true;
+  ld_t = ld.t1;  // none yet
   find_tile();
 
   uint4 qraw[kQv];
@@ -470,11 +486,11 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
           qf[nt][0] = a.x; qf[nt][1] = a.y; qf[nt][2] = a.z; qf[nt][3] = a.w;
           qf[nt][4] = d.x; qf[nt][5] = d.y; qf[nt][6] = d.z; qf[nt][7] = d.w;
         }
-        const int ch = D == 64 ? cq : 8 * (j >> 1) + 2 * cq + (j & 1);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          const uint4 lo = *reinterpret_cast<const uint4*>(kt + mt * 16 * D + tile_chunk<D>(g, ch));
-          const uint4 hi = *reinterpret_cast<const uint4*>(kt + mt * 16 * D + tile_chunk<D>(g + 8, ch));
+          const uint8_t* kp = kt + mt * 16 * D + (j >> 1) * 128 + k_off[j & 1];
+          const uint4 lo = *reinterpret_cast<const uint4*>(kp);
+          const uint4 hi = *reinterpret_cast<const uint4*>(kp + 8 * D);
           const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
@@ -589,13 +605,13 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
           uint32_t w[4][X];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int r = 2 * cq + (i & 1) + (i >> 1) * 8;
+            const uint8_t* vp = vm + (i >> 1) * 8 * D + v_off[i & 1];  // token 2 cq + {0, 1, 8, 9}[i]
             if constexpr (D == 64) {
-              const uint2 v = *reinterpret_cast<const uint2*>(vm + tile_chunk<D>(r, g >> 1) + (g & 1) * 8);
+              const uint2 v = *reinterpret_cast<const uint2*>(vp);
               w[i][0] = v.x;
               w[i][1] = v.y;
             } else {
-              const uint4 v = *reinterpret_cast<const uint4*>(vm + tile_chunk<D>(r, 8 * jj + g));
+              const uint4 v = *reinterpret_cast<const uint4*>(vp + 128 * jj);
               w[i][0] = v.x;
               w[i][1] = v.y;
               w[i][2] = v.z;
