@@ -66,6 +66,7 @@ constexpr float kTiny = 7.888609052210118e-31f;  // 2^-100
 // GL lanes of 8 columns make a group (4: 32 columns, 16: 128 columns; 0: the whole row).
 template <typename T, int VPT, int GL, int MAXT>
 __global__ void __launch_bounds__(MAXT) kernel(const Params p) {
+  wait_previous_kernels();
   const int row = blockIdx.x * blockDim.y + threadIdx.y;
   const bool act = row < p.rows;
   const int t = threadIdx.x, tpr = blockDim.x;
@@ -173,17 +174,17 @@ void launch(const Params& p, cudaStream_t s) {
   const dim3 block(static_cast<unsigned>(tpr), static_cast<unsigned>(per));
   const unsigned grid = static_cast<unsigned>((p.rows + per - 1) / per);
   if (vpt == 1)
-    kernel<T, 1, GL, 256><<<grid, block, 0, s>>>(p);
+    launch_overlapped(kernel<T, 1, GL, 256>, grid, block, 0, s, p);
   else if (vpt == 2)
-    kernel<T, 2, GL, 256><<<grid, block, 0, s>>>(p);
+    launch_overlapped(kernel<T, 2, GL, 256>, grid, block, 0, s, p);
   else if (nvec <= 1024)
-    kernel<T, 4, GL, 256><<<grid, block, 0, s>>>(p);
+    launch_overlapped(kernel<T, 4, GL, 256>, grid, block, 0, s, p);
   else if (nvec <= 2048)
-    kernel<T, 4, GL, 512><<<grid, block, 0, s>>>(p);
+    launch_overlapped(kernel<T, 4, GL, 512>, grid, block, 0, s, p);
   else if (nvec <= 4096)
-    kernel<T, 8, GL, 512><<<grid, block, 0, s>>>(p);
+    launch_overlapped(kernel<T, 8, GL, 512>, grid, block, 0, s, p);
   else
-    kernel<T, 8, GL, 1024><<<grid, block, 0, s>>>(p);
+    launch_overlapped(kernel<T, 8, GL, 1024>, grid, block, 0, s, p);
 }
 
 template <typename T>

@@ -40,6 +40,31 @@ bool ensure_smem_attr(const void* func, int bytes);
 // TOKMIX_OK if the current device is a compute capability 10.0 part, else sets the error.
 int check_device();
 
+// Launches a kernel that may start while its predecessor in the stream drains (programmatic dependent
+// launch): its blocks are resident and past their set-up when the predecessor's last block ends, which
+// takes about a microsecond off a short kernel.  The kernel must call wait_previous_kernels() in every
+// thread before it reads or writes global memory.
+template <typename... P, typename... A>
+cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                              A&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+#ifdef __CUDACC__
+// Everything earlier in the stream has completed and its writes are visible.
+__device__ __forceinline__ void wait_previous_kernels() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+#endif
+
 // The GDN stage-1 options (tokmix_gdn_stage1): whether gates / q-k normalisation are requested,
 // and their checks -- gates need a, b, a_log, dt_bias and a bf16 or fp32 dtype; normalisation a
 // positive finite eps and, for the schedules that need it, the normalised-key buffer.

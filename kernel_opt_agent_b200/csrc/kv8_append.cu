@@ -75,6 +75,7 @@ struct Half16<__half> {
 template <typename T, bool E4M3, int NV, int GT>
 __global__ void __launch_bounds__(GT == 32 ? 256 : GT) append_kernel(const AppendParams p) {
   constexpr int kUnits = GT == 32 ? 8 : 1;
+  wait_previous_kernels();
   const View& c = p.c;
   const uint32_t unit = blockIdx.x * kUnits + threadIdx.x / GT;
   if (unit >= p.units) return;  // warp-uniform (a warp per unit), never (a CTA per unit)
@@ -177,13 +178,13 @@ void launch_append(const AppendParams& p, cudaStream_t s) {
   // 8 vectors a thread keep enough loads in flight and few enough threads busy with the unit's pointers (4 prompts of
   // 8192 tokens, Hkv 8, D 128, pages of 64: 128 threads x 8 23.4 us, 256 x 4 30.2 us, 64 x 16 28.5 us)
   if (most <= 4 * 32)
-    append_kernel<T, E4M3, 4, 32><<<(p.units + 7) / 8, 256, 0, s>>>(p);
+    launch_overlapped(append_kernel<T, E4M3, 4, 32>, dim3((p.units + 7) / 8), dim3(256), 0, s, p);
   else if (most <= 8 * 128)
-    append_kernel<T, E4M3, 8, 128><<<p.units, 128, 0, s>>>(p);
+    launch_overlapped(append_kernel<T, E4M3, 8, 128>, dim3(p.units), dim3(128), 0, s, p);
   else if (most <= 8 * 256)
-    append_kernel<T, E4M3, 8, 256><<<p.units, 256, 0, s>>>(p);
+    launch_overlapped(append_kernel<T, E4M3, 8, 256>, dim3(p.units), dim3(256), 0, s, p);
   else
-    append_kernel<T, E4M3, 16, 256><<<p.units, 256, 0, s>>>(p);
+    launch_overlapped(append_kernel<T, E4M3, 16, 256>, dim3(p.units), dim3(256), 0, s, p);
 }
 
 int make_view(const char* who, const tokmix_kv8_cache* c, View& out) {

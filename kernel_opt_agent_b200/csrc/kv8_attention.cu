@@ -39,7 +39,7 @@ constexpr int kMaxTokens = 16;
 constexpr int kMaxBatch = 8192;  // the plan keeps batch + 1 words in shared memory
 constexpr float kShift = 14.0f;  // weights are held times 2^14
 constexpr int kJoinThreads = 256;
-constexpr int kMaxCtas = 148 * 8;
+constexpr int kMaxCtas = 512;  // at most 3 per SM
 
 template <int D, int NT>
 struct Shape {
@@ -67,6 +67,7 @@ struct AttnParams {
   float scale_log2;  // sm_scale * log2(e)
   int grid;          // CTAs of the attention kernel
   int min_tiles;     // a CTA's range is at least this long
+  int row_lines, table_lines;  // 128-byte lines of a table row, of the table
   uint32_t* status;
 };
 
@@ -267,7 +268,7 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
   float* scales = reinterpret_cast<float*>(smem + W * STAGES * S::kStageBytes) + (threadIdx.x >> 5) * STAGES * 2 * MT;
   __half* qs = reinterpret_cast<__half*>(smem + W * STAGES * (S::kStageBytes + 8 * MT));  // [row][kQStride]
   uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + S::smem_bytes(W));
-  __shared__ float row_factor[ROWS], warp_m[W][ROWS], warp_l[W][ROWS], warp_v[W];
+  __shared__ float row_factor[ROWS], row_top[ROWS], row_sum[ROWS], warp_m[W][ROWS], warp_l[W][ROWS], warp_v[W];
   __shared__ int warp_at[W];  // where in `smem` a warp's partial rows lie
   __shared__ uint32_t scratch[W];
 
@@ -275,7 +276,12 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, cq = lane & 3;
 
-  asm volatile("griddepcontrol.launch_dependents;");
+  wait_previous_kernels();
+  asm volatile("griddepcontrol.launch_dependents;");  // the join kernel, which reads the lengths before it waits
+  if (blockIdx.x * kThreads + threadIdx.x < p.table_lines) {  // the table, read behind the plan, on its way to L2
+    const int line = blockIdx.x * kThreads + threadIdx.x, row = line / p.row_lines;
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(c.table + row * c.table_stride + (line - row * p.row_lines) * 32));
+  }
   make_plan<TOK, ROWS, kThreads>(p, prefix, scratch);
   const uint32_t total = prefix[c.batch];
   if (total == 0) return;
@@ -671,6 +677,18 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
       __syncthreads();
       const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (first ? 0 : 1);
       const int nw = min(W, t1 - cur.t0);  // warps that had a tile
+      if (threadIdx.x < 8) {  // a row's maximum and sum; warp_m becomes what a warp's rows are multiplied by
+        const int r = nt * 8 + threadIdx.x;
+        float top = warp_m[0][r], sum = 0.0f;
+        for (int i = 1; i < nw; ++i) top = fmaxf(top, warp_m[i][r]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        for (int i = 0; i < nw; ++i) sum += ex2(warp_m[i][r] - ref) * warp_l[i][r];
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        for (int i = 0; i < nw; ++i) warp_m[i][r] = ex2(warp_m[i][r] - ref) * inv * warp_v[i];
+        row_top[r] = top;
+        row_sum[r] = sum;
+      }
+      __syncthreads();
       constexpr int kOut = 8 * (D / 4);
 #pragma unroll
       for (int k = 0; k < (kOut + kThreads - 1) / kThreads; ++k) {
@@ -678,29 +696,22 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
         const int r8 = v / (D / 4), x = v % (D / 4);
         const int r = nt * 8 + r8, row = row0 + r;
         if (v >= kOut || row >= rows_valid) break;
-        float top = warp_m[0][r], sum = 0.0f;
-        for (int i = 1; i < nw; ++i) top = fmaxf(top, warp_m[i][r]);
-        const float ref = top == -INFINITY ? 0.0f : top;
         float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
         for (int i = 0; i < nw; ++i) {
           const float4 a = *reinterpret_cast<const float4*>(smem + warp_at[i] + r8 * D * 4 + 16 * merge_chunk<D>(r8, x));
-          const float w = ex2(warp_m[i][r] - ref);
-          sum += w * warp_l[i][r];
-          const float wv = w * warp_v[i];
-          o[0] += a.x * wv;
-          o[1] += a.y * wv;
-          o[2] += a.z * wv;
-          o[3] += a.w * wv;
+          const float w = warp_m[i][r];
+          o[0] += a.x * w;
+          o[1] += a.y * w;
+          o[2] += a.z * w;
+          o[3] += a.w * w;
         }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] *= inv;
+        const float top = row_top[r], sum = row_sum[r];
         if (cur.whole) {
           const int i = row / p.group, h = cur.kvh * p.group + row - i * p.group;
           const size_t orow = (static_cast<size_t>(cur.b) * p.tokens + i) * p.hq + h;
           store_out4(p, orow * D + 4 * x, o);
-          if (p.lse != nullptr && x == 0) p.lse[orow] = lse_of(ref, sum);
+          if (p.lse != nullptr && x == 0) p.lse[orow] = lse_of(top == -INFINITY ? 0.0f : top, sum);
         } else {
           *reinterpret_cast<float4*>(p.part_o + (slot * ROWS + r) * D + 4 * x) = make_float4(o[0], o[1], o[2], o[3]);
           if (x == 0) p.part_ml[slot * ROWS + r] = make_float2(top, sum);
@@ -779,7 +790,18 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
           const uint32_t slot0 = 2 * c0 + (range_begin(c0, total, ctas) >= first ? 0 : 1);
           const size_t slot = lane == 0 ? slot0 : 2 * (c0 + min(static_cast<uint32_t>(lane), c1 - c0));
           wait_partials();
-          const float2 ml = lane <= static_cast<int>(c1 - c0) ? __ldcg(&p.part_ml[slot * ROWS + rr]) : make_float2(-INFINITY, 0.0f);
+          const int n = static_cast<int>(c1 - c0) + 1;
+          const float2 ml = lane < n ? __ldcg(&p.part_ml[slot * ROWS + rr]) : make_float2(-INFINITY, 0.0f);
+          constexpr int X = (TPR + 31) / 32;
+          float4 part[kShort][X];
+#pragma unroll
+          for (int k = 0; k < kShort; ++k) {
+            const size_t sk = k == 0 ? slot0 : 2 * (c0 + k);
+            const float4* src = reinterpret_cast<const float4*>(p.part_o + (sk * ROWS + rr) * D);
+#pragma unroll
+            for (int x = 0; x < X; ++x)
+              part[k][x] = k < n && lane + 32 * x < TPR ? __ldcg(src + lane + 32 * x) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          }
           float top = ml.x;
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -789,7 +811,6 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
           const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-          constexpr int X = (TPR + 31) / 32;
           float acc[X][4];
 #pragma unroll
           for (int x = 0; x < X; ++x)
@@ -797,18 +818,14 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
             for (int e = 0; e < 4; ++e) acc[x][e] = 0.0f;
 #pragma unroll
           for (int k = 0; k < kShort; ++k) {
-            if (k > static_cast<int>(c1 - c0)) break;
             const float wk = __shfl_sync(0xffffffffu, w, k) * inv;
-            const size_t sk = k == 0 ? slot0 : 2 * (c0 + k);
-            const float4* src = reinterpret_cast<const float4*>(p.part_o + (sk * ROWS + rr) * D);
+            if (k < n) {
 #pragma unroll
-            for (int x = 0; x < X; ++x) {
-              if (lane + 32 * x < TPR) {
-                const float4 a = __ldcg(src + lane + 32 * x);
-                acc[x][0] += wk * a.x;
-                acc[x][1] += wk * a.y;
-                acc[x][2] += wk * a.z;
-                acc[x][3] += wk * a.w;
+              for (int x = 0; x < X; ++x) {
+                acc[x][0] += wk * part[k][x].x;
+                acc[x][1] += wk * part[k][x].y;
+                acc[x][2] += wk * part[k][x].z;
+                acc[x][3] += wk * part[k][x].w;
               }
             }
           }
@@ -829,13 +846,23 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
       // only the first CTA's partial may lie in its second slot
       const size_t slot0 = 2 * static_cast<size_t>(c0) + (range_begin(c0, total, ctas) >= first ? 0 : 1);
       auto slot_of = [&](int x) { return x == 0 ? slot0 : 2 * static_cast<size_t>(c0 + x); };
+      const int x = threadIdx.x % tpr, pg = threadIdx.x / tpr;
+      const int col = (blockIdx.y * tpr + x) * 4;
+      auto load_part = [&](int y) {
+        return __ldcg(reinterpret_cast<const float4*>(p.part_o + (slot_of(y) * ROWS + rr) * D + col));
+      };
+      constexpr int kEarly = 8;  // partials on their way while the weights are formed
+      float4 early[kEarly];
+#pragma unroll
+      for (int i = 0; i < kEarly; ++i)
+        early[i] = pg + i * pg_n < n ? load_part(pg + i * pg_n) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       constexpr int M = (kMaxCtas + kJoinThreads - 1) / kJoinThreads;
       float2 ml[M];
       float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < M; ++i) {
-        const int x = threadIdx.x + i * kJoinThreads;
-        ml[i] = x < n ? __ldcg(&p.part_ml[slot_of(x) * ROWS + rr]) : make_float2(-INFINITY, 0.0f);
+        const int y = threadIdx.x + i * kJoinThreads;
+        ml[i] = y < n ? __ldcg(&p.part_ml[slot_of(y) * ROWS + rr]) : make_float2(-INFINITY, 0.0f);
         top = fmaxf(top, ml[i].x);
       }
 #pragma unroll
@@ -848,9 +875,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
       float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < M; ++i) {
-        const int x = threadIdx.x + i * kJoinThreads;
+        const int y = threadIdx.x + i * kJoinThreads;
         const float w = ex2(ml[i].x - ref) * ml[i].y;
-        if (x < n) weight[x] = w;
+        if (y < n) weight[y] = w;
         sum += w;
       }
 #pragma unroll
@@ -861,18 +888,18 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
 #pragma unroll
       for (int w = 0; w < kJoinThreads / 32; ++w) sum += red[1][w];
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      const int x = threadIdx.x % tpr, pg = threadIdx.x / tpr;
-      const int col = (blockIdx.y * tpr + x) * 4;
       float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-      for (int y = pg; y < n; y += pg_n) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + (slot_of(y) * ROWS + rr) * D + col));
-        const float w = weight[y] * inv;
+      auto add = [&](float w, const float4& v) {
         a.x += w * v.x;
         a.y += w * v.y;
         a.z += w * v.z;
         a.w += w * v.w;
-      }
+      };
+#pragma unroll
+      for (int i = 0; i < kEarly; ++i)
+        if (pg + i * pg_n < n) add(weight[pg + i * pg_n] * inv, early[i]);
+#pragma unroll 4
+      for (int y = pg + kEarly * pg_n; y < n; y += pg_n) add(weight[y] * inv, load_part(y));
       sums[pg * tpr + x] = a;
       __syncthreads();
       if (pg == 0) {
@@ -927,23 +954,16 @@ int launch_with(const char* who, AttnParams& p, int sms, void* workspace, cudaSt
   if (!ensure_smem_attr(reinterpret_cast<const void*>(attn), S::smem_bytes(W) + attn_plan_max) ||
       !ensure_smem_attr(reinterpret_cast<const void*>(join), kMaxCtas * 4 + kJoinThreads * 16 + plan_max))
     return fail(TOKMIX_ERR_LAUNCH, "%s: cannot set the shared memory size", who);
-  attn<<<p.grid, 32 * W, S::smem_bytes(W) + plan, s>>>(p);
+  p.row_lines = (p.c.max_pages + 31) / 32;
+  p.table_lines = static_cast<int>(std::min<long long>(static_cast<long long>(p.row_lines) * p.c.batch, 32LL * W * p.grid));
+  launch_overlapped(attn, dim3(p.grid), dim3(32 * W), S::smem_bytes(W) + plan, s, p);
   if (const int rc = check_launch(who)) return rc;
   const long long rows = static_cast<long long>(p.c.batch) * p.tokens * p.hq;
   const int per = static_cast<int>(std::min<long long>(8, (rows + 2 * sms - 1) / (2 * sms)));
   const long long want = (rows + per - 1) / per;
-  cudaLaunchConfig_t cfg{};
   // with a row per CTA, rows of long sequences are shared by CTAs of 64 columns
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(want, 4LL * sms)), per == 1 ? D / 64 : 1);
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(join_smem);
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, join, static_cast<const AttnParams>(p), per) != cudaSuccess) return check_launch(who);
+  const dim3 join_grid(static_cast<unsigned>(std::min<long long>(want, 4LL * sms)), per == 1 ? D / 64 : 1);
+  launch_overlapped(join, join_grid, dim3(kJoinThreads), static_cast<size_t>(join_smem), s, p, per);
   return check_launch(who);
 }
 
