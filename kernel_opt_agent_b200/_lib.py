@@ -10,7 +10,6 @@ reference's plugin modules report them: bad shapes / dtypes / devices raise ``Va
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import pathlib
@@ -280,12 +279,17 @@ def after_host_status_launch(device: torch.device, what: str) -> None:
         take_host_status(device, what)
 
 
-_HERE = contextlib.nullcontext()
+def call_on(device: torch.device, fn, *args):
+    """fn(*args) with `device` current."""
+    if device.index == torch._C._cuda_getDevice():
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
 
 
-def on_device(device: torch.device):
-    """Context in which `device` is current (free when it already is)."""
-    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+def empty(shape: tuple, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """A contiguous tensor of at most two dimensions (torch.empty takes 0.8 us more to read its arguments)."""
+    return torch.empty_strided(shape, (shape[1], 1) if len(shape) == 2 else (1,), dtype=dtype, device=device)
 
 
 def aligned(x: torch.Tensor) -> torch.Tensor:

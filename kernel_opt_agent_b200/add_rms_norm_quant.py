@@ -50,16 +50,15 @@ def kernel_fn(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tens
     x, w = _lib.aligned(x), _lib.aligned(weight)
     rows = x.numel() // n
     y = torch.empty_like(x, dtype=torch.float8_e4m3fn)
-    y_scale = torch.empty((n // group, rows) if group else (rows,), dtype=torch.float32, device=dev)
+    y_scale = _lib.empty((n // group, rows) if group else (rows,), torch.float32, dev)
     if residual is None:
         res, res_out = None, x
     else:
         res = residual if inplace else _lib.aligned(residual)
         res_out = res if inplace else torch.empty_like(x)
-    with _lib.on_device(dev):
-        rc = _lib.load().tokmix_add_rms_norm_quant(
-            x.data_ptr(), res.data_ptr() if res is not None else None, w.data_ptr(), res_out.data_ptr(), y.data_ptr(),
-            y_scale.data_ptr(), rows, n, group or 0, _DTYPES[dtype], eps, _lib.stream_ptr(dev))
+    rc = _lib.call_on(dev, _lib.load().tokmix_add_rms_norm_quant,
+                      x.data_ptr(), res.data_ptr() if res is not None else None, w.data_ptr(), res_out.data_ptr(),
+                      y.data_ptr(), y_scale.data_ptr(), rows, n, group or 0, _DTYPES[dtype], eps, _lib.stream_ptr(dev))
     if rc:
         _lib.check(rc, "add_rms_norm_quant")
     return y, y_scale, res_out

@@ -44,13 +44,12 @@ def kernel_fn(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     dev = k.device
     k, ks = _kv8.token_strides(k)
     v, vs = _kv8.token_strides(v)
-    with _lib.on_device(dev):
-        status = _lib.host_status_ptr(dev, "kv8")
-        rc = _lib.load().tokmix_kv8_append(k.data_ptr(), *ks, v.data_ptr(), *vs, k.shape[1], _kv8.IO_DTYPES[k.dtype],
-                                           _kv8.byref(cache), status, _lib.stream_ptr(dev))
-        if rc:
-            _lib.check(rc, "kv8_append")
-        _lib.after_host_status_launch(dev, "kv8")
+    status = _lib.host_status_ptr(dev, "kv8")
+    rc = _lib.call_on(dev, _lib.load().tokmix_kv8_append, k.data_ptr(), *ks, v.data_ptr(), *vs, k.shape[1],
+                      _kv8.IO_DTYPES[k.dtype], _kv8.byref(cache), status, _lib.stream_ptr(dev))
+    if rc:
+        _lib.check(rc, "kv8_append")
+    _lib.after_host_status_launch(dev, "kv8")
     return [k_cache, v_cache, k_scale, v_scale]
 
 

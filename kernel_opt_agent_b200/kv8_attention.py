@@ -38,8 +38,9 @@ MAX_TOKENS = 16
 
 @functools.cache
 def _workspace_bytes(tokens: int, hq: int, hkv: int, d: int, device: int) -> int:
-    """The workspace of a shape on a device (which is current)."""
-    return _lib.load().tokmix_kv8_attention_workspace_bytes(tokens, hq, hkv, d)
+    """The workspace of a shape on a device."""
+    with torch.cuda.device(device):
+        return _lib.load().tokmix_kv8_attention_workspace_bytes(tokens, hq, hkv, d)
 
 
 def kernel_fn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -57,24 +58,22 @@ def kernel_fn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_s
         sm_scale = 1.0 / math.sqrt(d)
     dev = q.device
     if out is None:
-        out = torch.empty((batch, tokens, hq, d), dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
         raise ValueError("out must be a contiguous tensor shaped and typed like q")
     elif out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
         raise ValueError("out must not share memory with q")
     lse = torch.empty((batch, tokens, hq), dtype=torch.float32, device=dev) if return_lse else None
     q, qs = _kv8.token_strides(q)
-    lib = _lib.load()
-    with _lib.on_device(dev):
-        status = _lib.host_status_ptr(dev, "kv8")
-        need = _workspace_bytes(max(tokens, 1), hq, cache.heads_kv, d, dev.index)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)  # per call: calls may overlap on other streams
-        rc = lib.tokmix_kv8_attention(q.data_ptr(), *qs, out.data_ptr(), lse.data_ptr() if return_lse else None, tokens,
-                                      hq, _kv8.IO_DTYPES[q.dtype], sm_scale, _kv8.byref(cache), ws.data_ptr(), need,
-                                      status, _lib.stream_ptr(dev))
-        if rc:
-            _lib.check(rc, "kv8_attention")
-        _lib.after_host_status_launch(dev, "kv8")
+    status = _lib.host_status_ptr(dev, "kv8")
+    need = _workspace_bytes(max(tokens, 1), hq, cache.heads_kv, d, dev.index)
+    ws = _lib.empty((need,), torch.uint8, dev)  # per call: calls may overlap on other streams
+    rc = _lib.call_on(dev, _lib.load().tokmix_kv8_attention, q.data_ptr(), *qs, out.data_ptr(),
+                      lse.data_ptr() if return_lse else None, tokens, hq, _kv8.IO_DTYPES[q.dtype], sm_scale,
+                      _kv8.byref(cache), ws.data_ptr(), need, status, _lib.stream_ptr(dev))
+    if rc:
+        _lib.check(rc, "kv8_attention")
+    _lib.after_host_status_launch(dev, "kv8")
     return (out, lse) if return_lse else out
 
 
