@@ -68,6 +68,7 @@ struct AttnParams {
   int grid;          // CTAs of the attention kernel
   int min_tiles;     // a CTA's range is at least this long
   int row_lines, table_lines;  // 128-byte lines of a table row, of the table
+  int single;                  // a CTA per unit: none is cut
   uint32_t* status;
 };
 
@@ -208,19 +209,30 @@ template <int TOK, int ROWS>
 struct Walk {
   uint32_t pos, stop;
   int b;
+  int kvh, row0;  // single: the CTA's one unit, as a range of one
   __device__ __forceinline__ bool next(const AttnParams& p, const uint32_t* prefix, Segment& n) {
     if (pos >= stop) return false;
-    while (prefix[b + 1] <= pos) ++b;
+    if (!p.single)
+      while (prefix[b + 1] <= pos) ++b;
     n.b = b;
     n.s = load_seq(p.c, b, p.tokens);
+    n.rows_valid = (n.s.end - n.s.start) * p.group;
     const Unit u = unit_of<TOK, ROWS>(p, n.s);
+    if (p.single) {
+      n.t0 = 0;
+      n.t1 = u.tiles;
+      n.kvh = kvh;
+      n.row0 = row0;
+      n.whole = true;
+      pos = stop;
+      return true;
+    }
     const int off = static_cast<int>(pos - prefix[b]);
     const int ui = off / u.tiles;
     n.t0 = off - ui * u.tiles;
     n.t1 = min(u.tiles, n.t0 + static_cast<int>(stop - pos));
     n.kvh = ui / u.row_tiles;
     n.row0 = (ui - n.kvh * u.row_tiles) * ROWS;
-    n.rows_valid = (n.s.end - n.s.start) * p.group;
     n.whole = n.t0 == 0 && n.t1 == u.tiles;
     pos += n.t1 - n.t0;
     return true;
@@ -282,18 +294,41 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
     const int line = blockIdx.x * kThreads + threadIdx.x, row = line / p.row_lines;
     asm volatile("prefetch.global.L2 [%0];" ::"l"(c.table + row * c.table_stride + (line - row * p.row_lines) * 32));
   }
-  make_plan<TOK, ROWS, kThreads>(p, prefix, scratch);
-  const uint32_t total = prefix[c.batch];
-  if (total == 0) return;
-  const uint32_t ctas = active_ctas(p, total);
-  if (blockIdx.x >= ctas) return;
   Walk<TOK, ROWS> walk;
-  walk.pos = range_begin(blockIdx.x, total, ctas);
-  walk.stop = range_begin(blockIdx.x + 1, total, ctas);
-  walk.b = 0;
-  for (int hi = c.batch; hi - walk.b > 1;) {  // the last sequence with prefix <= pos
-    const int mid = (walk.b + hi) >> 1;
-    if (prefix[mid] <= walk.pos) walk.b = mid; else hi = mid;
+  if (p.single) {  // short sequences: a CTA per unit, no plan and nothing to join
+    const int row_tiles = (p.tokens * p.group + ROWS - 1) / ROWS;
+    walk.b = blockIdx.x / (row_tiles * c.hkv);
+    const int ui = blockIdx.x - walk.b * row_tiles * c.hkv;
+    walk.kvh = ui / row_tiles;
+    walk.row0 = (ui - walk.kvh * row_tiles) * ROWS;
+    walk.pos = 0;
+    walk.stop = 1;
+    const Seq s = load_seq(c, walk.b, p.tokens);
+    if (!s.ok && threadIdx.x == 0) report_bad(p.status);
+    const int seen = max(walk.row0, (s.end - s.start) * p.group), last = min(walk.row0 + ROWS, p.tokens * p.group);
+    const float f = s.ok ? 0.0f : nan_f();  // rows that see nothing
+    const float o[4] = {f, f, f, f};
+    for (int v = threadIdx.x; v < (last - seen) * (D / 4); v += kThreads) {
+      const int row = seen + v / (D / 4), x = v % (D / 4);
+      const int i = row / p.group, h = walk.kvh * p.group + row - i * p.group;
+      const size_t orow = (static_cast<size_t>(walk.b) * p.tokens + i) * p.hq + h;
+      store_out4(p, orow * D + 4 * x, o);
+      if (p.lse != nullptr && x == 0) p.lse[orow] = s.ok ? -INFINITY : f;
+    }
+    if (seen == walk.row0) return;
+  } else {
+    make_plan<TOK, ROWS, kThreads>(p, prefix, scratch);
+    const uint32_t total = prefix[c.batch];
+    if (total == 0) return;
+    const uint32_t ctas = active_ctas(p, total);
+    if (blockIdx.x >= ctas) return;
+    walk.pos = range_begin(blockIdx.x, total, ctas);
+    walk.stop = range_begin(blockIdx.x + 1, total, ctas);
+    walk.b = 0;
+    for (int hi = c.batch; hi - walk.b > 1;) {  // the last sequence with prefix <= pos
+      const int mid = (walk.b + hi) >> 1;
+      if (prefix[mid] <= walk.pos) walk.b = mid; else hi = mid;
+    }
   }
 
   // byte offsets inside a tile: this lane's share of a copy, its keys, its values
@@ -921,8 +956,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
   wait_partials();
 }
 
-#ifndef KV8_FEW
-#define KV8_FEW 1
+#ifndef KV8_ROUNDS
+#define KV8_ROUNDS 4
 #endif
 #ifndef KV8_MIN_FEW
 #define KV8_MIN_FEW 8
@@ -937,9 +972,10 @@ size_t workspace_bytes(int sms) {
 }
 
 template <int D, bool E4M3, int NT, int W>
-int launch_with(const char* who, AttnParams& p, int sms, void* workspace, cudaStream_t s) {
+int launch_with(const char* who, AttnParams& p, int sms, int single_units, void* workspace, cudaStream_t s) {
   using S = Shape<D, NT>;
-  p.grid = sms * (S::kWarpsPerSm / W);
+  p.single = single_units > 0;
+  p.grid = p.single ? single_units : sms * (S::kWarpsPerSm / W);
   p.min_tiles = W == kSmallWarps ? kSmallWarps : KV8_MIN_FEW;
   if (p.grid > kMaxCtas) return fail(TOKMIX_ERR_UNSUPPORTED, "%s: more SMs than the kernel is planned for", who);
   const size_t slots = 2 * static_cast<size_t>(p.grid);
@@ -958,6 +994,7 @@ int launch_with(const char* who, AttnParams& p, int sms, void* workspace, cudaSt
   p.table_lines = static_cast<int>(std::min<long long>(static_cast<long long>(p.row_lines) * p.c.batch, 32LL * W * p.grid));
   launch_overlapped(attn, dim3(p.grid), dim3(32 * W), S::smem_bytes(W) + plan, s, p);
   if (const int rc = check_launch(who)) return rc;
+  if (p.single) return TOKMIX_OK;
   const long long rows = static_cast<long long>(p.c.batch) * p.tokens * p.hq;
   const int per = static_cast<int>(std::min<long long>(8, (rows + 2 * sms - 1) / (2 * sms)));
   const long long want = (rows + per - 1) / per;
@@ -970,10 +1007,18 @@ int launch_with(const char* who, AttnParams& p, int sms, void* workspace, cudaSt
 template <int D, bool E4M3, int NT>
 int launch_attn(const char* who, AttnParams& p, int sms, void* workspace, cudaStream_t s) {
   using S = Shape<D, NT>;
-  // few units: one CTA per SM leaves the fewest partial rows to join; many: small CTAs, whose unit changes overlap
+  constexpr int kLarge = S::kWarpsPerSm;
   const long long units = static_cast<long long>(p.c.batch) * p.c.hkv * ((p.tokens * p.group + S::kRows - 1) / S::kRows);
-  if (KV8_FEW && units * 4 <= sms) return launch_with<D, E4M3, NT, S::kWarpsPerSm>(who, p, sms, workspace, s);
-  return launch_with<D, E4M3, NT, kSmallWarps>(who, p, sms, workspace, s);
+  // Tables with room for few tiles per warp, and no more units than CTAs the GPU holds: a CTA per unit, without a plan
+  // before it and a join behind it (which take about 4 us).
+  const long long most = (static_cast<long long>(p.c.max_pages) * p.c.page + S::kTok - 1) / S::kTok;
+  if (units <= sms && most <= KV8_ROUNDS * kLarge)
+    return launch_with<D, E4M3, NT, kLarge>(who, p, sms, static_cast<int>(units), workspace, s);
+  if (units <= sms * (kLarge / kSmallWarps) && most <= KV8_ROUNDS * kSmallWarps)
+    return launch_with<D, E4M3, NT, kSmallWarps>(who, p, sms, static_cast<int>(units), workspace, s);
+  // few units: one CTA per SM leaves the fewest partial rows to join; many: small CTAs, whose unit changes overlap
+  if (units * 4 <= sms) return launch_with<D, E4M3, NT, kLarge>(who, p, sms, 0, workspace, s);
+  return launch_with<D, E4M3, NT, kSmallWarps>(who, p, sms, 0, workspace, s);
 }
 
 template <int D>

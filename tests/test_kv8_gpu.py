@@ -264,6 +264,12 @@ def test_attention_matches_definition(cuda_device, cache_dtype, lens, t, hq, hkv
     assert torch.equal(out, attention.kernel_fn(q, *cache, seq, new))      # the same bits again
     if min(lens) >= t:
         assert torch.equal(out, attention.kernel_fn(q, *cache, seq))
+    # a table with room for much longer sequences takes the path that cuts sequences up
+    wide = torch.cat([cache[4], torch.full((len(lens), 4096), GARBAGE_PAGE, dtype=torch.int32, device=cuda_device)], 1)
+    out, lse = attention.kernel_fn(q, *cache[:4], wide, seq, new, return_lse=True)
+    attention.check_device_status(cuda_device)
+    _assert_attention(out, lse, q, cache, seq, new)
+    assert torch.equal(out, attention.kernel_fn(q, *cache[:4], wide, seq, new))
 
 
 def test_attention_many_ragged_sequences(cuda_device):
@@ -279,6 +285,10 @@ def test_attention_many_ragged_sequences(cuda_device):
     attention.check_device_status(cuda_device)
     assert out.data_ptr() == buf[1:].data_ptr()
     _assert_attention(out, lse, q, cache, seq, new)
+    # fewer sequences, so that each unit has a CTA of its own
+    some = slice(0, 60)
+    part, lse = attention.kernel_fn(q[some], *cache[:4], cache[4][some, :13], seq[some], new[some], return_lse=True)
+    _assert_attention(part, lse, q[some], cache[:4] + [cache[4][some]], seq[some], new[some])
     assert bool((buf[0] == 7).all()) and bool((buf[301] == 7).all())
 
 
