@@ -320,8 +320,8 @@ typedef struct tokmix_kv8_cache {
  * smallest power of two, at least 2^-100, with max |x| <= qmax * scale over the page's tokens (qmax 448
  * for e4m3, 127 for int8); values are rounded to nearest, ties to even; where new tokens raise the scale,
  * the page's older tokens are rounded again to it.  A page whose first slot is written starts afresh.  A
- * value that is not finite makes its block's scale NaN until the page is started afresh.  No two
- * sequences of a call may append to one page.
+ * value that is not finite makes its block's scale NaN until the page is started afresh.  A call
+ * must append to each page for one sequence only, at one place of its table.
  * Lengths that do not fit the call or the table, and table entries outside the pool, write nothing for
  * that sequence (page) and set TOKMIX_DEV_BAD_ARGS in *status (device memory or mapped host memory). */
 int tokmix_kv8_append(const void* k, long long k_batch_stride, long long k_token_stride, long long k_head_stride,
@@ -334,7 +334,7 @@ int tokmix_kv8_append(const void* k, long long k_batch_stride, long long k_token
  * softmax(q k^T * sm_scale) v in fp32, k and v as the cache holds them; query head h reads key/value
  * head h / (heads_q / heads_kv).  lse (NULL or fp32 [batch, tokens, heads_q]): the natural logarithm of the
  * row's sum of exponentials.  Rows i >= new_lens[b] give zeros and lse -infinity.
- * 1 <= tokens <= 16.  workspace: tokmix_kv8_attention_workspace_bytes(...) bytes of device memory, 16-byte
+ * 1 <= tokens <= 16, batch <= 8192.  workspace: tokmix_kv8_attention_workspace_bytes(...) bytes of device memory, 16-byte
  * aligned, no initialisation, not shared by calls that may overlap.
  * Lengths that do not fit give NaN for the sequence's rows, a table entry outside the pool NaN for the
  * rows that see it; both set TOKMIX_DEV_BAD_ARGS in *status (device memory or mapped host memory). */

@@ -258,7 +258,8 @@ def host_status_ptr(device: torch.device, what: str) -> int | None:
     if h is None:
         if torch.cuda.is_current_stream_capturing():
             return None
-        h = _host_status[device.index] = _HostStatus()
+        with _lock:
+            h = _host_status.setdefault(device.index, _HostStatus())
     if h.word.value:
         take_host_status(device, what)
     return h.ptr

@@ -7,20 +7,25 @@
 // Bound: HBM, the cache's bytes (4 heads_q / heads_kv flops per byte).  So the rows that read the same keys
 // and values -- the tokens and heads of a group -- share one pass over them, and the work is cut along the
 // sequences so that every SM streams until the end:
-//   * a unit is (sequence, key/value head, tile of 8 or 16 rows); its tokens come in tiles of 4 KB of keys and
-//     4 KB of values (16, 32 or 64 tokens).  All units' tiles laid end to end are cut into equal ranges, one
-//     per CTA of a grid that fills the GPU once; lengths are read on the device, so the launch does not depend
-//     on them.  A unit inside one range is written directly; a unit cut by range borders leaves normalised
-//     partial rows with their maximum and sum, and a second kernel joins them in the order of the CTAs
-//     (launched to start as the first drains; results do not depend on timing).
-//   * a warp takes every fourth tile of its CTA's range, loads it straight into registers with 16-byte loads
-//     (the order of the head dimension inside a product is free, so a lane's 16 bytes are its fragments), and
-//     loads the next tile's keys as soon as this tile's scores stand and its values as soon as they are
-//     used up: 8 KB in flight per warp, 12 warps per SM.  No shared memory, barrier or wait is on that path.
+//   * a unit is (sequence, key/value head, tile of 8 or 16 rows); its tokens come in tiles of 16 (head_dim 256) or
+//     32.  All units' tiles laid end to end are cut into equal ranges, one per CTA of a grid that fills the GPU once;
+//     lengths are read on the device, so the launch does not depend on them.  A unit inside one range is written
+//     directly; a unit cut by range borders leaves normalised partial rows with their maximum and sum, and a second
+//     kernel joins them in the order of the CTAs (launched to start as the first drains).  Results do not depend on
+//     timing.  Where the table has room for short sequences only, each unit has a CTA of its own instead and the
+//     second kernel falls away (129 tokens: 8.7 -> 7.2 us).
+//   * a warp takes every fourth (twelfth) tile of its CTA's range and copies tiles into a ring of its own in shared
+//     memory (cp.async, 16 KB per warp and twelve warps per SM in flight), running ahead over unit borders, so that a
+//     change of unit costs no memory latency.  Only changes of unit have barriers; there is no wait on another CTA.
 //   * scores S^T = K Q^T and outputs O^T = V^T P^T are m16n8k16 products with the cache's bytes as the 16-row
-//     operand: e4m3 and int8 values are exact in fp16, accumulation is fp32.  The tensor core's newer path
-//     (tcgen05) would want the bytes in shared memory and 128-row tiles of them for 8 to 16 query rows; the
-//     products take a tenth of the time the bytes do, so registers are the shorter way.
+//     operand, widened to fp16 in registers (exact) -- the order of the head dimension inside a product is free, so a
+//     lane's 16 bytes of a key are its fragments as they lie.  Accumulation is fp32.  tcgen05 products would take
+//     128 rows of bytes for 8 to 16 query rows and need the bytes in one 8-bit type with the weights, which 8 bits do
+//     not hold; the e4m3 form of this product runs on the same pipe with the same widening inside (it measured 5 % slower).
+// What it measured (B200, device time): Hq 32 Hkv 8 D 128, 64 sequences of 1024 to 4096 tokens 64 us, 5.3 TB/s (the same
+// copies without the products 59 us); Hq 16 Hkv 2 D 256, 16 sequences of up to 65536 tokens 113 to 117 us, 5.6 TB/s (105 us);
+// one of 65536 21 us.  The SMs' shares of the bandwidth differ (equal ranges end after 86 to 110 us of the 113), but short
+// ranges drawn as SMs got done cost more in changes of unit than they evened out.
 //
 // Number formats.  q rows enter fp16 after scaling by a power of two that brings their largest element to
 // [2^14, 2^15): exact for elements down to 2^-28 of it (bf16 has 8 bits, fp16 11).  Weights enter as
@@ -48,7 +53,7 @@ struct Shape {
   static constexpr int kRows = 8 * NT;        // query rows per unit
   static constexpr int kQStride = D + 8;      // halves between rows of q in shared memory (conflict-free 16-byte reads)
   static constexpr int kStageBytes = 2 * kTok * D;              // a tile's keys and values
-  static constexpr int kWarpsPerSm = NT == 1 ? 12 : 8;          // 168 or 255 registers a thread
+  static constexpr int kWarpsPerSm = NT == 1 ? 12 : 8;                       // 168 or 255 registers a thread
   static constexpr int kStages = (NT == 1 ? 16384 : 24576) / kStageBytes;  // 192 KB of tiles per SM
   __host__ __device__ static constexpr int smem_bytes(int warps) { return warps * kStages * (kStageBytes + 8 * kMt) + kRows * kQStride * 2; }
   static_assert(8 * D * 4 <= kStageBytes, "eight partial rows fit a stage");
@@ -956,13 +961,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
   wait_partials();
 }
 
-#ifndef KV8_ROUNDS
-#define KV8_ROUNDS 4
-#endif
-#ifndef KV8_MIN_FEW
-#define KV8_MIN_FEW 8
-#endif
-constexpr int kSmallWarps = 4;
+constexpr int kSmallWarps = 4;  // warps of a CTA where there are many units
+constexpr int kRounds = 4;      // tiles per warp up to which a CTA takes a whole unit
 
 template <int D, int NT>
 size_t workspace_bytes(int sms) {
@@ -976,7 +976,7 @@ int launch_with(const char* who, AttnParams& p, int sms, int single_units, void*
   using S = Shape<D, NT>;
   p.single = single_units > 0;
   p.grid = p.single ? single_units : sms * (S::kWarpsPerSm / W);
-  p.min_tiles = W == kSmallWarps ? kSmallWarps : KV8_MIN_FEW;
+  p.min_tiles = W == kSmallWarps ? kSmallWarps : 8;
   if (p.grid > kMaxCtas) return fail(TOKMIX_ERR_UNSUPPORTED, "%s: more SMs than the kernel is planned for", who);
   const size_t slots = 2 * static_cast<size_t>(p.grid);
   p.part_o = static_cast<float*>(workspace);
@@ -1012,9 +1012,9 @@ int launch_attn(const char* who, AttnParams& p, int sms, void* workspace, cudaSt
   // Tables with room for few tiles per warp, and no more units than CTAs the GPU holds: a CTA per unit, without a plan
   // before it and a join behind it (which take about 4 us).
   const long long most = (static_cast<long long>(p.c.max_pages) * p.c.page + S::kTok - 1) / S::kTok;
-  if (units <= sms && most <= KV8_ROUNDS * kLarge)
+  if (units <= sms && most <= kRounds * kLarge)
     return launch_with<D, E4M3, NT, kLarge>(who, p, sms, static_cast<int>(units), workspace, s);
-  if (units <= sms * (kLarge / kSmallWarps) && most <= KV8_ROUNDS * kSmallWarps)
+  if (units <= sms * (kLarge / kSmallWarps) && most <= kRounds * kSmallWarps)
     return launch_with<D, E4M3, NT, kSmallWarps>(who, p, sms, static_cast<int>(units), workspace, s);
   // few units: one CTA per SM leaves the fewest partial rows to join; many: small CTAs, whose unit changes overlap
   if (units * 4 <= sms) return launch_with<D, E4M3, NT, kLarge>(who, p, sms, 0, workspace, s);

@@ -16,8 +16,8 @@ a page's scale its older tokens are rounded again; a page whose first slot is wr
 so pages are reused without clearing.  A value that is not finite makes its block's scale NaN: the whole
 block reads as NaN until the page starts afresh.
 
-The caller keeps pages apart: no two sequences of a call append to one page (a page shared by several
-sequences is full, or copied first).  Lengths that do not fit the call or the table and table entries
+The caller keeps pages apart: a call appends to each page for one sequence, and at one place of its table (a
+page shared by several sequences is full, or copied first).  Lengths that do not fit the call or the table and table entries
 outside the pool write nothing for that sequence (page) and are reported as ``TokmixDeviceError`` by a
 later call or by ``check_device_status``.
 
@@ -55,9 +55,9 @@ def kernel_fn(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
 
 def check_device_status(device: torch.device | None = None) -> None:
     """Synchronise and raise if a kernel of the 8-bit cache met bad lengths or table entries on `device`."""
-    dev = device or torch.device("cuda", torch.cuda.current_device())
-    torch.cuda.synchronize(dev)
-    _lib.take_host_status(dev, "kv8")
+    idx = device.index if device is not None and device.index is not None else torch.cuda.current_device()
+    torch.cuda.synchronize(idx)
+    _lib.take_host_status(torch.device("cuda", idx), "kv8")
 
 
 def get_inputs(batch: int = 64, tokens: int = 1, seq_len: int = 4096, head_num_kv: int = 2, head_dim: int = 256,
