@@ -429,11 +429,14 @@ def test_cache_beyond_two_gigabytes(cuda_device):
 
 
 # ------------------------------------------------------------------------------------ errors
-def test_bad_pages_and_lengths_are_reported(cuda_device):
+@pytest.mark.parametrize("room", [0, 4096])
+def test_bad_pages_and_lengths_are_reported(cuda_device, room):
     """Table entries outside the pool and lengths that do not fit: nothing is read or written there, the other
-    sequences are right, the error arrives at the next look and is gone after it."""
+    sequences are right, the error arrives at the next look and is gone after it.  (With and without room for long
+    sequences in the table.)"""
     dev, lens, page = cuda_device, [40, 50, 60], 16
     cache = _filled_cache(13, lens, 2, 64, page, E4M3, dev)
+    cache[4] = torch.cat([cache[4], torch.full((3, room), GARBAGE_PAGE, dtype=torch.int32, device=dev)], 1)
     q = _queries(13, 3, 1, 4, 64, torch.bfloat16, dev)
     seq = _i32(lens, dev)
     want = attention.kernel_fn(q, *cache, seq)
@@ -509,6 +512,63 @@ def test_empty_batches(cuda_device):
     attention.check_device_status(cuda_device)
     assert bool((out == 0).all()) and bool((lse == -math.inf).all())
     assert attention.kernel_fn(q[:, :0], *cache, _i32([[0], [1]], cuda_device), zero).shape == (2, 0, 4, 64)
+
+
+@pytest.mark.parametrize("room", [0, 4096])
+def test_query_rows_do_not_touch_each_other(cuda_device, room):
+    """A NaN or infinite query spoils its own row, an empty sequence's rows are zero, all else keeps its bits."""
+    lens = [100, 0, 37]
+    cache = _filled_cache(40, lens, 2, 128, 32, E4M3, cuda_device)
+    cache[4] = torch.cat([cache[4], torch.full((3, room), GARBAGE_PAGE, dtype=torch.int32, device=cuda_device)], 1)
+    q = _queries(40, 3, 2, 8, 128, torch.bfloat16, cuda_device)
+    seq, new = _i32(lens, cuda_device), _i32([2, 0, 2], cuda_device)
+    want, want_lse = attention.kernel_fn(q, *cache, seq, new, return_lse=True)
+    assert bool((want[1] == 0).all()) and bool((want_lse[1] == -math.inf).all())
+    q[0, 1, 3, 5] = math.nan
+    q[2, 0, 6, 0] = math.inf
+    out, lse = attention.kernel_fn(q, *cache, seq, new, return_lse=True)
+    attention.check_device_status(cuda_device)
+    bad = torch.zeros(3, 2, 8, dtype=torch.bool, device=cuda_device)
+    bad[0, 1, 3] = bad[2, 0, 6] = True
+    assert bool(out[bad].isnan().all()) and torch.equal(out[~bad], want[~bad]) and torch.equal(lse[~bad], want_lse[~bad])
+
+
+def test_largest_batch(cuda_device):
+    """8192 sequences that share pages: every one has what a call of few sequences gives; more are refused."""
+    lens = [0, 70, 33, 128]
+    cache = _filled_cache(41, lens, 1, 64, 64, INT8, cuda_device)
+    q = _queries(41, 4, 1, 4, 64, torch.bfloat16, cuda_device)
+    seq = _i32(lens, cuda_device)
+    new = _i32([0, 1, 1, 1], cuda_device)
+    want = attention.kernel_fn(q, *cache, seq, new)
+    big = [q.repeat(2048, 1, 1, 1), *cache[:4], cache[4].repeat(2048, 1), seq.repeat(2048), new.repeat(2048)]
+    out = attention.kernel_fn(*big)
+    attention.check_device_status(cuda_device)
+    # where a range border cuts a sequence: both outputs rounded (2 * 2^-8), both sets of weights rounded to fp16
+    # (2 * 2^-11 of the largest value, 127 * 2^3)
+    tol = 2.0 ** -7 * want.float().abs() + 2.0 ** -10 * 127 * 8
+    assert bool(((out.view(2048, 4, 1, 4, 64).float() - want.float()).abs() <= tol).all())
+    assert bool((out[::4] == 0).all())
+    for i in (0, 5, 6, 8191):  # sequences whole inside a range are computed alike
+        _assert_attention(out[i:i + 1], None, big[0][i:i + 1], cache[:4] + [big[5][i:i + 1]], big[6][i:i + 1], big[7][i:i + 1])
+    more = [torch.cat([t, t[:1]]) for t in (big[0], big[5], big[6], big[7])]
+    with pytest.raises(RuntimeError, match="8192"):
+        attention.kernel_fn(more[0], *cache[:4], *more[1:])
+
+
+def test_append_extreme_magnitudes(cuda_device):
+    """Scales at both ends: the largest bf16 values, and values under 2^-100 of a byte's reach, which become zeros."""
+    table, seq = _i32([[0]], cuda_device), _i32([3], cuda_device)
+    for dtype in (E4M3, INT8):
+        for value in (3.3e38, 1e-36, 2.0 ** -95):
+            k = torch.full((1, 3, 1, 64), value, dtype=torch.bfloat16, device=cuda_device)
+            k[0, 1] = -k[0, 1]
+            cache = append.make_cache(1, 1, 16, 64, dtype, cuda_device)
+            want = references.kv8_append_ref(k, k, *cache, table, seq)
+            append.kernel_fn(k, k, *cache, table, seq)
+            assert all(_bits_equal(a, b) for a, b in zip(cache, want))
+            assert bool(torch.isfinite(cache[2]).all()) and float(cache[2]) >= 2.0 ** -100
+    append.check_device_status(cuda_device)
 
 
 # ------------------------------------------------------------------------------------ streams, graphs
