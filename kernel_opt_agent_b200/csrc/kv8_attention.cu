@@ -57,6 +57,7 @@ struct Shape {
   static constexpr int kStages = (NT == 1 ? 16384 : 24576) / kStageBytes;  // 192 KB of tiles per SM
   __host__ __device__ static constexpr int smem_bytes(int warps) { return warps * kStages * (kStageBytes + 8 * kMt) + kRows * kQStride * 2; }
   static_assert(8 * D * 4 <= kStageBytes, "eight partial rows fit a stage");
+  static_assert(kWarpsPerSm <= 16, "a row's warps are joined by 16 lanes");
 };
 
 struct AttnParams {
@@ -717,16 +718,21 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
       __syncthreads();
       const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (first ? 0 : 1);
       const int nw = min(W, t1 - cur.t0);  // warps that had a tile
-      if (threadIdx.x < 8) {  // a row's maximum and sum; warp_m becomes what a warp's rows are multiplied by
-        const int r = nt * 8 + threadIdx.x;
-        float top = warp_m[0][r], sum = 0.0f;
-        for (int i = 1; i < nw; ++i) top = fmaxf(top, warp_m[i][r]);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        for (int i = 0; i < nw; ++i) sum += ex2(warp_m[i][r] - ref) * warp_l[i][r];
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        for (int i = 0; i < nw; ++i) warp_m[i][r] = ex2(warp_m[i][r] - ref) * inv * warp_v[i];
-        row_top[r] = top;
-        row_sum[r] = sum;
+      if (threadIdx.x < 128) {  // a row's maximum and sum, 16 lanes each; warp_m becomes what a warp's rows are multiplied by
+        const int r = nt * 8 + (threadIdx.x >> 4), i = threadIdx.x & 15;
+        const float mi = i < nw ? warp_m[i][r] : -INFINITY;
+        float top = mi;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float w = ex2(mi - (top == -INFINITY ? 0.0f : top));
+        float sum = i < nw ? w * warp_l[i][r] : 0.0f;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (i < nw) warp_m[i][r] = w * (sum == 0.0f ? 0.0f : 1.0f / sum) * warp_v[i];
+        if (i == 0) {
+          row_top[r] = top;
+          row_sum[r] = sum;
+        }
       }
       __syncthreads();
       constexpr int kOut = 8 * (D / 4);
