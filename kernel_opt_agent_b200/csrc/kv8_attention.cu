@@ -53,8 +53,8 @@ struct Shape {
   static constexpr int kRows = 8 * NT;        // query rows per unit
   static constexpr int kQStride = D + 8;      // halves between rows of q in shared memory (conflict-free 16-byte reads)
   static constexpr int kStageBytes = 2 * kTok * D;              // a tile's keys and values
-  static constexpr int kWarpsPerSm = NT == 1 ? 12 : 8;                       // 168 or 255 registers a thread
-  static constexpr int kStages = (NT == 1 ? 16384 : 24576) / kStageBytes;  // 192 KB of tiles per SM
+  static constexpr int kWarpsPerSm = NT == 1 ? 12 : 8;  // 168 or 255 registers a thread
+  static constexpr int kStages = 196608 / kWarpsPerSm / kStageBytes;  // 192 KB of tiles per SM
   __host__ __device__ static constexpr int smem_bytes(int warps) { return warps * kStages * (kStageBytes + 8 * kMt) + kRows * kQStride * 2; }
   static_assert(8 * D * 4 <= kStageBytes, "eight partial rows fit a stage");
   static_assert(kWarpsPerSm <= 16, "a row's warps are joined by 16 lanes");
@@ -979,7 +979,6 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
 }
 
 constexpr int kSmallWarps = 4;  // warps of a CTA where there are many units
-constexpr int kRounds = 4;      // tiles per warp up to which a CTA takes a whole unit
 
 template <int D, int NT>
 size_t workspace_bytes(int sms) {
@@ -994,11 +993,11 @@ int launch_with(const char* who, AttnParams& p, int sms, int single_units, void*
   p.single = single_units > 0;
   p.grid = p.single ? single_units : sms * (S::kWarpsPerSm / W);
   p.min_tiles = W == kSmallWarps ? kSmallWarps : 8;
-  if (p.grid > kMaxCtas) return fail(TOKMIX_ERR_UNSUPPORTED, "%s: more SMs than the kernel is planned for", who);
+  if (!p.single && p.grid > kMaxCtas) return fail(TOKMIX_ERR_UNSUPPORTED, "%s: more SMs than the kernel is planned for", who);
   const size_t slots = 2 * static_cast<size_t>(p.grid);
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + slots * S::kRows * D);
-  const int plan = (p.c.batch + 1) * 4;
+  const int plan = p.single ? 0 : (p.c.batch + 1) * 4;
   const int join_smem = kMaxCtas * 4 + kJoinThreads * 16 + plan;
   const int plan_max = (kMaxBatch + 1) * 4;  // the limit is set once, for the largest batch
   const int attn_plan_max = W == kSmallWarps ? plan_max : (kMaxCtas + 1) * 4;  // large CTAs: at most a unit per SM
@@ -1015,8 +1014,9 @@ int launch_with(const char* who, AttnParams& p, int sms, int single_units, void*
   const long long rows = static_cast<long long>(p.c.batch) * p.tokens * p.hq;
   const int per = static_cast<int>(std::min<long long>(8, (rows + 2 * sms - 1) / (2 * sms)));
   const long long want = (rows + per - 1) / per;
-  // with a row per CTA, rows of long sequences are shared by CTAs of 64 columns
-  const dim3 join_grid(static_cast<unsigned>(std::min<long long>(want, 4LL * sms)), per == 1 ? D / 64 : 1);
+  // few rows of long sequences are shared by CTAs of 64 columns; more CTAs than run at once would cost more (256 rows of 14
+  // partials, D 256: 11.7 us, shared 18.8)
+  const dim3 join_grid(static_cast<unsigned>(std::min<long long>(want, 4LL * sms)), rows * (D / 64) <= 2 * sms ? D / 64 : 1);
   launch_overlapped(join, join_grid, dim3(kJoinThreads), static_cast<size_t>(join_smem), s, p, per);
   return check_launch(who);
 }
@@ -1026,15 +1026,23 @@ int launch_attn(const char* who, AttnParams& p, int sms, void* workspace, cudaSt
   using S = Shape<D, NT>;
   constexpr int kLarge = S::kWarpsPerSm;
   const long long units = static_cast<long long>(p.c.batch) * p.c.hkv * ((p.tokens * p.group + S::kRows - 1) / S::kRows);
-  // Tables with room for few tiles per warp, and no more units than CTAs the GPU holds: a CTA per unit, without a plan
-  // before it and a join behind it (which take about 4 us).
-  const long long most = (static_cast<long long>(p.c.max_pages) * p.c.page + S::kTok - 1) / S::kTok;
-  if (units <= sms && most <= kRounds * kLarge)
+  // A CTA per unit, without a plan before it and a join behind it, where the table has room for short sequences only.  Up to
+  // a unit per SM a unit's warps are all that read for it: 2 tiles a warp while most SMs have no unit, then 4, then 8 (planned
+  // -> a CTA per unit; Hkv 8, D 128, 8 units of 1024 tokens, 3 tiles: 8.0 -> 9.3 us; 48 units, 3 tiles: 9.2 -> 9.3; 96 units:
+  // 12.7 -> 10.7; D 256, 32 units of 1000 tokens, 6 tiles: 11.7 -> 14.4; D 128, 128 units of 2000, 6 tiles: 17.2 -> 16.2).
+  // More units: a change of unit costs a range more than a CTA of its own, as long as no unit is long (D 128, 400 units of up to
+  // 640 tokens: 20.0 -> 15.2 us; 800 units: 29.4 -> 24.7; of up to 1900: 49.5 -> 48.7; of up to 3800: 85 -> 94; 2400 units
+  // of up to 1024: 89 -> 80; D 256, 800 units of up to 1024: 65 -> 57; 600 of up to 1900: 75 -> 76).
+  const long long room = static_cast<long long>(p.c.max_pages) * p.c.page, most = (room + S::kTok - 1) / S::kTok;
+  const int rounds = units * 4 <= sms ? 2 : units * 2 <= sms ? 4 : 8;
+  if (units <= sms && most <= rounds * kLarge)
     return launch_with<D, E4M3, NT, kLarge>(who, p, sms, static_cast<int>(units), workspace, s);
-  if (units <= sms * (kLarge / kSmallWarps) && most <= kRounds * kSmallWarps)
+  if (units > sms && units <= 1 << 20 && room <= (D == 256 ? 1024 : 2048))  // (indexes of threads in 32 bits)
     return launch_with<D, E4M3, NT, kSmallWarps>(who, p, sms, static_cast<int>(units), workspace, s);
-  // few units: one CTA per SM leaves the fewest partial rows to join; many: small CTAs, whose unit changes overlap
-  if (units * 4 <= sms) return launch_with<D, E4M3, NT, kLarge>(who, p, sms, 0, workspace, s);
+  // Few units: a CTA per SM leaves the fewest partial rows to join (8-row units, 1 unit of 64000 tokens, D 128: 14.8 to 14.8 us;
+  // 2: 16.6 to 18.5; 4: 20.3 to 21.3; 16-row units, D 256, 8: 37 to 39; 32: 48 to 53).  Many: small CTAs, whose changes of unit
+  // overlap (8-row units, D 64, 8: 13.3 to 14.6 us; D 128, 32: 28.5 to 30.3; 16-row units, D 128, 64: 30.3 to 31.4).
+  if (units * (NT == 1 ? 32 : 4) <= sms) return launch_with<D, E4M3, NT, kLarge>(who, p, sms, 0, workspace, s);
   return launch_with<D, E4M3, NT, kSmallWarps>(who, p, sms, 0, workspace, s);
 }
 

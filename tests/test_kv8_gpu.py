@@ -556,6 +556,73 @@ def test_largest_batch(cuda_device):
         attention.kernel_fn(more[0], *cache[:4], *more[1:])
 
 
+@pytest.mark.parametrize("cache_dtype,b,t,hq,hkv,d,page,room", [
+    (E4M3, 37, 1, 8, 1, 128, 32, 768), (E4M3, 38, 1, 8, 1, 128, 32, 1536), (INT8, 74, 1, 4, 1, 128, 64, 1536),
+    (E4M3, 75, 1, 4, 1, 256, 16, 1536), (INT8, 148, 1, 4, 1, 64, 64, 6144), (E4M3, 149, 1, 4, 1, 64, 64, 2048),
+    (E4M3, 149, 1, 4, 1, 64, 16, 2064), (INT8, 111, 1, 16, 4, 128, 128, 2048), (E4M3, 112, 1, 16, 4, 256, 32, 1024),
+    (E4M3, 112, 1, 16, 4, 256, 32, 1056), (INT8, 90, 3, 20, 2, 128, 16, 2048), (E4M3, 300, 2, 16, 2, 64, 32, 2048),
+    (E4M3, 9, 2, 16, 4, 64, 64, 2048), (E4M3, 10, 16, 3, 1, 256, 64, 512)])
+def test_attention_where_the_layout_changes(cuda_device, cache_dtype, b, t, hq, hkv, d, page, room):
+    """Units (sequences times heads times row tiles) and room in the table on both sides of each border between the ways to lay
+    the work out: one sequence fills its table, others are short or empty, one has nothing new."""
+    rng = np.random.default_rng(b + d)
+    lens = [int(x) for x in rng.integers(t, 150, b)]
+    lens[b // 2], lens[1], lens[b - 1] = room, 0, t
+    cache = _filled_cache(b, lens, hkv, d, page, cache_dtype, cuda_device, rng)
+    table = torch.full((b, room // page), GARBAGE_PAGE, dtype=torch.int32, device=cuda_device)
+    table[:] = cache[4][:, :room // page]
+    cache[4] = table
+    q = _queries(b, b, t, hq, d, torch.bfloat16, cuda_device)
+    seq, new = _i32(lens, cuda_device), _i32([min(t, n) for n in lens[:2]] + [0] + [t] * (b - 3), cuda_device)
+    out, lse = attention.kernel_fn(q, *cache, seq, new, return_lse=True)
+    attention.check_device_status(cuda_device)
+    _assert_attention(out, lse, q, cache, seq, new)
+    assert torch.equal(out, attention.kernel_fn(q, *cache, seq, new))
+    bad = seq.clone()
+    bad[0] = room + 1
+    out2, lse2 = attention.kernel_fn(q, *cache, bad, new, return_lse=True)
+    with pytest.raises(_lib.TokmixDeviceError):
+        attention.check_device_status(cuda_device)
+    assert bool(out2[0].isnan().all()) and bool(lse2[0].isnan().all())
+    _assert_attention(out2[1:], lse2[1:], q[1:], cache[:4] + [cache[4][1:]], seq[1:], new[1:])
+
+
+@pytest.mark.parametrize("room", [0, 40])
+def test_a_batch_of_thousands_of_units(cuda_device, room):
+    """3000 sequences with 8 heads that share pages, as a CTA each or as ranges (room for 40 more pages): all have the bits or,
+    where a range border cuts a sequence, nearly what a call of few sequences gives."""
+    lens = [70, 33, 128]
+    cache = _filled_cache(43, lens, 8, 64, 64, E4M3, cuda_device)
+    q = _queries(43, 3, 1, 8, 64, torch.float16, cuda_device)
+    seq = _i32(lens, cuda_device)
+    want = attention.kernel_fn(q, *cache, seq)
+    table = torch.cat([cache[4], torch.full((3, room), GARBAGE_PAGE, dtype=torch.int32, device=cuda_device)], 1)
+    out = attention.kernel_fn(q.repeat(1000, 1, 1, 1), *cache[:4], table.repeat(1000, 1), seq.repeat(1000))
+    attention.check_device_status(cuda_device)
+    # both outputs rounded (2 * 2^-11 of it), both sets of weights rounded to fp16 (2 * 2^-11 of the largest value, 448 * 2^3)
+    tol = 2.0 ** -10 * want.float().abs() + 2.0 ** -10 * 448 * 8
+    assert bool(((out.view(1000, 3, 1, 8, 64).float() - want.float()).abs() <= tol).all())
+    for i in (0, 1, 2, 1499, 2998, 2999):
+        _assert_attention(out[i:i + 1], None, q[i % 3:i % 3 + 1], cache[:4] + [cache[4][i % 3:i % 3 + 1]], seq[i % 3:i % 3 + 1])
+
+
+def test_largest_batch_in_ranges(cuda_device):
+    """8192 sequences with room for long ones, so that the call is cut into ranges."""
+    lens = [1, 70, 33, 128]
+    cache = _filled_cache(42, lens, 1, 64, 64, INT8, cuda_device)
+    q = _queries(42, 4, 1, 4, 64, torch.bfloat16, cuda_device)
+    seq = _i32(lens, cuda_device)
+    want = attention.kernel_fn(q, *cache, seq)
+    table = torch.cat([cache[4], torch.full((4, 40), GARBAGE_PAGE, dtype=torch.int32, device=cuda_device)], 1)
+    out = attention.kernel_fn(q.repeat(2048, 1, 1, 1), *cache[:4], table.repeat(2048, 1), seq.repeat(2048))
+    attention.check_device_status(cuda_device)
+    # both outputs rounded (2 * 2^-8), both sets of weights rounded to fp16 (2 * 2^-11 of the largest value, 127 * 2^3)
+    tol = 2.0 ** -7 * want.float().abs() + 2.0 ** -10 * 127 * 8
+    assert bool(((out.view(2048, 4, 1, 4, 64).float() - want.float()).abs() <= tol).all())
+    for i in (0, 1, 2, 3, 4000, 8190, 8191):
+        _assert_attention(out[i:i + 1], None, q[i % 4:i % 4 + 1], cache[:4] + [cache[4][i % 4:i % 4 + 1]], seq[i % 4:i % 4 + 1])
+
+
 def test_append_extreme_magnitudes(cuda_device):
     """Scales at both ends: the largest bf16 values, and values under 2^-100 of a byte's reach, which become zeros."""
     table, seq = _i32([[0]], cuda_device), _i32([3], cuda_device)
