@@ -48,12 +48,12 @@ constexpr int kMaxCtas = 512;  // at most 3 per SM
 
 template <int D, int NT>
 struct Shape {
-  static constexpr int kTok = D == 256 ? 16 : 32;  // tokens per tile
+  static constexpr int kTok = D == 256 ? 16 : D == 64 && NT == 1 ? 64 : 32;  // tokens per tile: 8 KB, 4 KB (D 64, 16 rows)
   static constexpr int kMt = kTok / 16;       // 16-token subtiles (a page holds whole ones)
   static constexpr int kRows = 8 * NT;        // query rows per unit
   static constexpr int kQStride = D + 8;      // halves between rows of q in shared memory (conflict-free 16-byte reads)
   static constexpr int kStageBytes = 2 * kTok * D;              // a tile's keys and values
-  static constexpr int kWarpsPerSm = NT == 1 ? 12 : 8;  // 168 or 255 registers a thread
+  static constexpr int kWarpsPerSm = NT == 1 || D == 64 ? 12 : 8;  // 168 or 255 registers a thread
   static constexpr int kStages = 196608 / kWarpsPerSm / kStageBytes;  // 192 KB of tiles per SM
   __host__ __device__ static constexpr int smem_bytes(int warps) { return warps * kStages * (kStageBytes + 8 * kMt) + kRows * kQStride * 2; }
   static_assert(8 * D * 4 <= kStageBytes, "eight partial rows fit a stage");
@@ -81,7 +81,8 @@ struct AttnParams {
 // ------------------------------------------------------------------------------------ the plan
 // What a change of unit costs a CTA, in tiles (its warps end at different times, join, and start anew): ranges that count it
 // end together (128 sequences of up to 1024 tokens, Hq 32 Hkv 8 D 128: 0 53.3 us, 4 47.8, 8 45.3, 12 44.0, 16 43.7, 24 43.9).
-constexpr int kUnitCost = 12;
+template <int TOK>
+constexpr int kUnitCost = TOK == 64 ? 8 : 12;
 
 struct Unit {
   int tiles;      // token tiles of each of the sequence's units
@@ -94,7 +95,7 @@ __device__ __forceinline__ Unit unit_of(const AttnParams& p, const Seq& s) {
   Unit u;
   u.tiles = (s.end + TOK - 1) / TOK;
   u.row_tiles = ((s.end - s.start) * p.group + ROWS - 1) / ROWS;
-  u.length = u.tiles + kUnitCost;
+  u.length = u.tiles + kUnitCost<TOK>;
   return u;
 }
 
@@ -243,9 +244,9 @@ struct Walk {
       const int ui = off / u.length;
       const int from = off - ui * u.length, to = min(u.length, from + static_cast<int>(stop - pos));
       pos += to - from;
-      if (to <= kUnitCost) continue;  // the range ends before the unit's first tile
-      n.t0 = max(from - kUnitCost, 0);
-      n.t1 = to - kUnitCost;
+      if (to <= kUnitCost<TOK>) continue;  // the range ends before the unit's first tile
+      n.t0 = max(from - kUnitCost<TOK>, 0);
+      n.t1 = to - kUnitCost<TOK>;
       n.kvh = ui / u.row_tiles;
       n.row0 = (ui - n.kvh * u.row_tiles) * ROWS;
       n.whole = n.t0 == 0 && n.t1 == u.tiles;
@@ -832,7 +833,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
         const Unit u = unit_of<TOK, ROWS>(p, s);
         const int kvh = h / p.group, r = i * p.group + h - kvh * p.group;
         const uint32_t first = prefix[b] + static_cast<uint32_t>(kvh * u.row_tiles + r / ROWS) * u.length;
-        const uint32_t c0 = cta_of(first + kUnitCost, total, ctas), c1 = cta_of(first + u.length - 1, total, ctas);
+        const uint32_t c0 = cta_of(first + kUnitCost<TOK>, total, ctas), c1 = cta_of(first + u.length - 1, total, ctas);
         const int rr = r % ROWS;
         if (c1 - c0 >= kShort) {
           if (lane == 0) {
@@ -1102,7 +1103,7 @@ extern "C" int tokmix_kv8_attention(const void* q, long long q_batch_stride, lon
     if (st % 8 != 0 || st < 0)
       return fail(TOKMIX_ERR_INVALID_ARGUMENT, "%s: strides of q must be multiples of 8 elements", who);
   if (p.c.batch > kMaxBatch) return fail(TOKMIX_ERR_UNSUPPORTED, "%s: at most %d sequences (got %d)", who, kMaxBatch, p.c.batch);
-  const long long most_tiles = ((static_cast<long long>(p.c.max_pages) * p.c.page + 15) / 16 + kUnitCost) * p.c.hkv *
+  const long long most_tiles = ((static_cast<long long>(p.c.max_pages) * p.c.page + 15) / 16 + kUnitCost<32>) * p.c.hkv *
                                ((static_cast<long long>(tokens) * (heads_q / p.c.hkv) + 7) / 8) * p.c.batch;
   if (heads_q > 65536 || most_tiles > 0x7fffffffLL || static_cast<long long>(p.c.batch) * tokens * heads_q > 0x3fffffffLL)
     return fail(TOKMIX_ERR_UNSUPPORTED, "%s: problem too large", who);
