@@ -7,25 +7,26 @@
 // Bound: HBM, the cache's bytes (4 heads_q / heads_kv flops per byte).  So the rows that read the same keys
 // and values -- the tokens and heads of a group -- share one pass over them, and the work is cut along the
 // sequences so that every SM streams until the end:
-//   * a unit is (sequence, key/value head, tile of 8 or 16 rows); its tokens come in tiles of 16 (head_dim 256) or
-//     32.  All units' tiles laid end to end are cut into equal ranges, one per CTA of a grid that fills the GPU once;
+//   * a unit is (sequence, key/value head, tile of 8 or 16 rows); its tokens come in tiles of 16 (D 256), 32 or
+//     64 (D 64, 8 rows).  All units' tiles laid end to end are cut into equal ranges, one per CTA of a grid that fills the GPU once;
 //     lengths are read on the device, so the launch does not depend on them.  A unit inside one range is written
 //     directly; a unit cut by range borders leaves normalised partial rows with their maximum and sum, and a second
 //     kernel joins them in the order of the CTAs (launched to start as the first drains).  Results do not depend on
 //     timing.  Where the table has room for short sequences only, each unit has a CTA of its own instead and the
-//     second kernel falls away (129 tokens: 8.7 -> 7.2 us).
-//   * a warp takes every fourth (twelfth) tile of its CTA's range and copies tiles into a ring of its own in shared
-//     memory (cp.async, 16 KB per warp and twelve warps per SM in flight), running ahead over unit borders, so that a
-//     change of unit costs no memory latency.  Only changes of unit have barriers; there is no wait on another CTA.
+//     second kernel falls away (one sequence of 129 tokens: 6.7 us; 2400 units of up to 1024: 89 -> 80).
+//   * a CTA's 4, 8 or 12 warps take its range's tiles in turn, each with a ring of its own in shared memory (cp.async,
+//     192 KB per SM in flight) that is filled ahead over unit borders, so that a change of unit costs no memory latency.  Only changes of unit have barriers; there is no wait on another CTA.
 //   * scores S^T = K Q^T and outputs O^T = V^T P^T are m16n8k16 products with the cache's bytes as the 16-row
 //     operand, widened to fp16 in registers (exact) -- the order of the head dimension inside a product is free, so a
 //     lane's 16 bytes of a key are its fragments as they lie.  Accumulation is fp32.  tcgen05 products would take
 //     128 rows of bytes for 8 to 16 query rows and need the bytes in one 8-bit type with the weights, which 8 bits do
 //     not hold; the e4m3 form of this product runs on the same pipe with the same widening inside (it measured 5 % slower).
-// What it measured (B200, device time): Hq 32 Hkv 8 D 128, 64 sequences of 1024 to 4096 tokens 64 us, 5.3 TB/s (the same
-// copies without the products 59 us); Hq 16 Hkv 2 D 256, 16 sequences of up to 65536 tokens 113 to 117 us, 5.6 TB/s (105 us);
-// one of 65536 21 us.  The SMs' shares of the bandwidth differ (equal ranges end after 86 to 110 us of the 113), but short
-// ranges drawn as SMs got done cost more in changes of unit than they evened out.
+// What it measured (B200, device time): Hq 32 Hkv 8 D 128, 64 sequences of 1024 to 4096 tokens 61 us, 5.5 TB/s (the same
+// copies without the products 59 us at a time when the whole took 64); Hq 16 Hkv 2 D 256, 16 sequences of up to 65536 tokens
+// 111 to 112 us, 5.8 TB/s; one of 65536 21 us.  The SMs' shares of the bandwidth differ (equal ranges end after 86 to 110 us
+// of those), but short ranges drawn as SMs got done cost more in changes of unit than they evened out.  16 rows and D >= 128
+// are bound by eight warps' latency instead: 20 sequences of up to 9000 tokens, Hq 32 Hkv 4, two queries, 33 us, 3.0 TB/s
+// (twelve warps of 168 registers 39 to 43).
 //
 // Number formats.  q rows enter fp16 after scaling by a power of two that brings their largest element to
 // [2^14, 2^15): exact for elements down to 2^-28 of it (bf16 has 8 bits, fp16 11).  Weights enter as
@@ -53,7 +54,8 @@ struct Shape {
   static constexpr int kRows = 8 * NT;        // query rows per unit
   static constexpr int kQStride = D + 8;      // halves between rows of q in shared memory (conflict-free 16-byte reads)
   static constexpr int kStageBytes = 2 * kTok * D;              // a tile's keys and values
-  static constexpr int kWarpsPerSm = NT == 1 || D == 64 ? 12 : 8;  // 168 or 255 registers a thread
+  // 168 or 255 registers a thread: 16 rows of D 64 fit 168 (64 sequences of up to 2000 tokens 44.9 -> 41.9 us), of D 128 do not
+  static constexpr int kWarpsPerSm = NT == 1 || D == 64 ? 12 : 8;
   static constexpr int kStages = 196608 / kWarpsPerSm / kStageBytes;  // 192 KB of tiles per SM
   __host__ __device__ static constexpr int smem_bytes(int warps) { return warps * kStages * (kStageBytes + 8 * kMt) + kRows * kQStride * 2; }
   static_assert(8 * D * 4 <= kStageBytes, "eight partial rows fit a stage");
@@ -80,7 +82,8 @@ struct AttnParams {
 
 // ------------------------------------------------------------------------------------ the plan
 // What a change of unit costs a CTA, in tiles (its warps end at different times, join, and start anew): ranges that count it
-// end together (128 sequences of up to 1024 tokens, Hq 32 Hkv 8 D 128: 0 53.3 us, 4 47.8, 8 45.3, 12 44.0, 16 43.7, 24 43.9).
+// end together (128 sequences of up to 1024 tokens, Hq 32 Hkv 8 D 128: 0 53.3 us, 4 47.8, 8 45.3, 12 44.0, 16 43.7, 24 43.9;
+// with tiles of 64 tokens, 32 sequences of up to 2500, Hq 32 Hkv 8 D 64: 4 24.0 us, 8 23.0, 12 24.3).
 template <int TOK>
 constexpr int kUnitCost = TOK == 64 ? 8 : 12;
 
@@ -99,7 +102,7 @@ __device__ __forceinline__ Unit unit_of(const AttnParams& p, const Seq& s) {
   return u;
 }
 
-// prefix[b] = tiles of the sequences before b (exclusive), prefix[batch] = all; every thread calls.
+// prefix[b] = places on the line of the sequences before b, prefix[batch] = all; every thread calls.
 template <int TOK, int ROWS, int THREADS>
 __device__ __forceinline__ void make_plan(const AttnParams& p, uint32_t* prefix, uint32_t* scratch) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -134,7 +137,7 @@ __device__ __forceinline__ void make_plan(const AttnParams& p, uint32_t* prefix,
   __syncthreads();
 }
 
-// CTAs that take part: none is empty
+// CTAs that take part: none has an empty range (it may lie in a unit's places without a tile)
 __device__ __forceinline__ uint32_t active_ctas(const AttnParams& p, uint32_t total) {
   return min(static_cast<uint32_t>(p.grid), max(1u, total / p.min_tiles));
 }
