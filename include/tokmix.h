@@ -286,7 +286,7 @@ int tokmix_qkv_part_rope(const void* qkv, const float* cos, const float* sin, vo
  * so y_fp8 * y_scale is the normalised row.  group 32 or 128 (n a multiple of it): y_scale is
  * [n / group, rows] as tokmix_swiglu_input_quant lays its scales out; group 0: one scale per row,
  * y_scale [rows].  residual NULL: h = x, and residual_out is not used.  residual_out may equal
- * residual or x.  n a multiple of 8, at most 65536; 16-byte aligned. */
+ * residual or x.  n a multiple of 8, at most 65536; rows at most 2^31 - 256; 16-byte aligned. */
 int tokmix_add_rms_norm_quant(const void* x, const void* residual, const void* weight, void* residual_out, void* y_fp8,
                               float* y_scale, int rows, int n, int group, int dtype, float eps, void* stream);
 

@@ -14,7 +14,8 @@ out (the first layer; residual_out is then x itself).
 ``group`` columns share a scale: 128 or 32 (N a multiple of it; y_scale is [N / group, M], M the number
 of rows, as ``swiglu_input_quant`` lays its scales out) or None, one scale per row (y_scale [M]).
 y_fp8 is e4m3, shaped like x; the largest magnitude of a group is held as 448.  ``inplace=True`` writes
-residual_out over ``residual``, so that a decode loop keeps one residual buffer.
+residual_out over ``residual``, so that a decode loop keeps one residual buffer (x may be the residual
+itself; it must not overlap it otherwise).
 
 ``kernel_fn`` runs ``tokmix_add_rms_norm_quant`` (``csrc/add_rms_norm_quant.cu``), no fallback."""
 
@@ -27,6 +28,7 @@ from . import _lib
 KERNEL_TYPE = "add_rms_norm_quant"
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 MAX_N = 65536
+MAX_ROWS = 2 ** 31 - 256
 
 
 def kernel_fn(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float = 1e-6, *,
@@ -47,8 +49,12 @@ def kernel_fn(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tens
         raise ValueError("weight must be [N], N the last dimension of x")
     if inplace and (residual is None or not residual.is_contiguous() or residual.data_ptr() % 16):
         raise ValueError("inplace=True needs a contiguous, 16-byte aligned residual")
-    x, w = _lib.aligned(x), _lib.aligned(weight)
     rows = x.numel() // n
+    if rows > MAX_ROWS:
+        raise ValueError(f"at most {MAX_ROWS} rows (got {rows})")
+    x, w = _lib.aligned(x), _lib.aligned(weight)
+    if inplace and 0 < abs(x.data_ptr() - residual.data_ptr()) < 2 * rows * n:
+        raise ValueError("inplace=True: x must be the residual itself or share no memory with it")
     y = torch.empty_like(x, dtype=torch.float8_e4m3fn)
     y_scale = _lib.empty((n // group, rows) if group else (rows,), torch.float32, dev)
     if residual is None:

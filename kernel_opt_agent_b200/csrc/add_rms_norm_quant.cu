@@ -215,6 +215,7 @@ extern "C" int tokmix_add_rms_norm_quant(const void* x, const void* residual, co
   if (dtype != TOKMIX_DTYPE_BF16 && dtype != TOKMIX_DTYPE_FP16)
     return fail(TOKMIX_ERR_UNSUPPORTED, "%s: bf16 or fp16 only (dtype %d)", who, dtype);
   if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(TOKMIX_ERR_INVALID_ARGUMENT, "%s: bad eps", who);
+  if (rows > 0x7fffff00) return fail(TOKMIX_ERR_UNSUPPORTED, "%s: at most 2^31 - 256 rows (got %d)", who, rows);  // int row indexes
   if (rows == 0) return TOKMIX_OK;
   if (!x || !weight || !y_fp8 || !y_scale || (residual && !residual_out))
     return fail(TOKMIX_ERR_INVALID_ARGUMENT, "%s: null pointer argument", who);

@@ -129,6 +129,26 @@ def test_refusals(cuda_device):
             bad()
 
 
+def test_refuses_more_rows_than_int_and_overlaps(cuda_device):
+    w = torch.ones(8, dtype=torch.bfloat16, device=cuda_device)
+    for rows in (2 ** 31 - 255, 2 ** 32 + 4):  # one row of memory
+        with pytest.raises(ValueError, match="rows"):
+            norm.kernel_fn(w.expand(rows, 8), None, w, group=None)
+    buf = torch.randn(9, 256, device=cuda_device).to(torch.bfloat16)
+    w = torch.ones(256, dtype=torch.bfloat16, device=cuda_device)
+    for x, r in ((buf[1:], buf[:-1]), (buf[:-1], buf[1:])):
+        with pytest.raises(ValueError, match="share no memory"):
+            norm.kernel_fn(x, r, w, inplace=True)
+    keep = buf.clone()
+    got = norm.kernel_fn(buf[4:8], buf[:4], w, inplace=True)  # neighbours
+    want = norm.kernel_fn(keep[4:8], keep[:4], w)
+    assert torch.equal(buf[4:], keep[4:]) and torch.equal(got[2], want[2]) and torch.equal(got[1], want[1])
+    same = keep[:4].clone()
+    got = norm.kernel_fn(same, same, w, inplace=True)
+    want = norm.kernel_fn(keep[:4], keep[:4], w)
+    assert torch.equal(same, want[2]) and torch.equal(got[1], want[1])
+
+
 def test_other_stream_and_graph(cuda_device):
     x, r, w = _inputs(cuda_device, 64, 4096, torch.bfloat16)
     want = norm.kernel_fn(x, r, w)

@@ -29,6 +29,11 @@ def test_norm_rejects_bad_arguments(changes, code):
     assert _lib.load().tokmix_add_rms_norm_quant(*args.values()) == code
 
 
+@pytest.mark.parametrize("rows,code", [(2 ** 31 - 1, UNSUPPORTED), (2 ** 31 - 255, UNSUPPORTED)])
+def test_norm_rejects_rows_its_indexes_do_not_hold(rows, code):
+    assert _lib.load().tokmix_add_rms_norm_quant(P, P, P, P, P, P, rows, 256, 128, 0, 1e-6, None) == code
+
+
 def _cache(**changes):
     c = dict(k=16, v=16, k_scale=16, v_scale=16, k_page_stride=16384, k_head_stride=8192, v_page_stride=16384,
              v_head_stride=8192, block_table=16, table_stride=4, seq_lens=16, new_lens=None, num_pages=8, page_size=64,
