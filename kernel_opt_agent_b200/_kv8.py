@@ -60,7 +60,9 @@ def cache_args(x: torch.Tensor, k_cache, v_cache, k_scale, v_scale, block_table,
     if x.ndim != 4 or len(shape) != 4 or v_cache.shape != shape:
         raise ValueError("new tokens must be [B, T, heads, D], k_cache and v_cache [num_pages, Hkv, page, D]")
     num_pages, heads, page, d = shape
-    batch = x.shape[0]
+    batch, tokens = x.shape[:2]
+    if batch >= 1 << 31 or tokens >= 1 << 31:
+        raise ValueError("fewer than 2^31 sequences and new tokens per sequence")
     dtype = CACHE_DTYPES.get(k_cache.dtype)
     if dtype is None or v_cache.dtype != k_cache.dtype:
         raise ValueError("k_cache and v_cache must both be float8_e4m3fn or both int8")

@@ -500,6 +500,17 @@ def test_refusals(cuda_device):
     attention.check_device_status(cuda_device)
 
 
+def test_refuses_more_sequences_or_tokens_than_int(cuda_device):
+    cache = append.make_cache(2, 2, 16, 64, E4M3, cuda_device)
+    one = torch.ones(1, 1, 2, 64, dtype=torch.bfloat16, device=cuda_device)
+    table, seq = _i32([[0, 1]], cuda_device), _i32([1], cuda_device)
+    for k in (one.expand(2 ** 32 + 1, 1, 2, 64), one.expand(1, 2 ** 32 + 1, 2, 64)):  # one row of memory
+        with pytest.raises(ValueError, match="2.31"):
+            append.kernel_fn(k, k, *cache, table, seq)
+        with pytest.raises(ValueError, match="2.31"):
+            attention.kernel_fn(k, *cache, table, seq)
+
+
 def test_empty_batches(cuda_device):
     cache = append.make_cache(2, 2, 16, 64, E4M3, cuda_device)
     q = torch.empty(0, 1, 4, 64, dtype=torch.bfloat16, device=cuda_device)
