@@ -334,8 +334,8 @@ int tokmix_kv8_append(const void* k, long long k_batch_stride, long long k_token
  * softmax(q k^T * sm_scale) v in fp32, k and v as the cache holds them; query head h reads key/value
  * head h / (heads_q / heads_kv).  lse (NULL or fp32 [batch, tokens, heads_q]): the natural logarithm of the
  * row's sum of exponentials.  Rows i >= new_lens[b] give zeros and lse -infinity.
- * 1 <= tokens <= 16, batch <= 8192.  workspace: tokmix_kv8_attention_workspace_bytes(...) bytes of device memory, 16-byte
- * aligned, no initialisation, not shared by calls that may overlap.
+ * 1 <= tokens <= 16, batch <= 8192.  workspace: tokmix_kv8_attention_workspace_bytes_for(...) bytes of device memory, 16-byte
+ * aligned, no initialisation, not shared by calls that may overlap (NULL where that is 0).
  * Lengths that do not fit give NaN for the sequence's rows, a table entry outside the pool NaN for the
  * rows that see it; both set TOKMIX_DEV_BAD_ARGS in *status (device memory or mapped host memory). */
 int tokmix_kv8_attention(const void* q, long long q_batch_stride, long long q_token_stride, long long q_head_stride,
@@ -343,8 +343,11 @@ int tokmix_kv8_attention(const void* q, long long q_batch_stride, long long q_to
                          const tokmix_kv8_cache* cache, void* workspace, long long workspace_bytes, uint32_t* status,
                          void* stream);
 
-/* Workspace size of tokmix_kv8_attention in bytes on the current device (-1 for bad arguments). */
+/* Workspace size of tokmix_kv8_attention in bytes on the current device (-1 for bad arguments): enough for any batch and table,
+ * and what a call with this batch and table needs (0 where the table holds short sequences only). */
 long long tokmix_kv8_attention_workspace_bytes(int tokens, int heads_q, int heads_kv, int head_dim);
+long long tokmix_kv8_attention_workspace_bytes_for(int tokens, int heads_q, int heads_kv, int head_dim, int batch, int max_pages,
+                                                   int page_size);
 
 /* Self-test of the bounded waits every pipelined kernel relies on: one small kernel waits on an
  * event that never happens -- which = 0: a transaction barrier whose bytes never land (a TMA load

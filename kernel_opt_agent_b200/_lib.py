@@ -70,6 +70,7 @@ SIGNATURES = {
     "tokmix_kv8_append": (_I, [_VP, _LL, _LL, _LL, _VP, _LL, _LL, _LL, _I, _I, _VP, _VP, _VP]),
     "tokmix_kv8_attention": (_I, [_VP, _LL, _LL, _LL, _VP, _VP, _I, _I, _I, _F, _VP, _VP, _LL, _VP, _VP]),
     "tokmix_kv8_attention_workspace_bytes": (_LL, [_I, _I, _I, _I]),
+    "tokmix_kv8_attention_workspace_bytes_for": (_LL, [_I, _I, _I, _I, _I, _I, _I]),
     "tokmix_selftest_wait_timeout": (_I, [_I, ctypes.c_longlong, _VP, _VP, _VP, _VP]),
     "tokmix_last_error": (ctypes.c_char_p, []),
     "tokmix_version": (ctypes.c_char_p, []),

@@ -985,6 +985,11 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, 
 constexpr int kSmallWarps = 4;  // warps of a CTA where there are many units
 
 template <int D, int NT>
+struct Tag {
+  static constexpr int kD = D, kNt = NT;
+};
+
+template <int D, int NT>
 size_t workspace_bytes(int sms) {
   using S = Shape<D, NT>;
   const size_t slots = 2 * static_cast<size_t>(sms) * (S::kWarpsPerSm / kSmallWarps);
@@ -1025,10 +1030,14 @@ int launch_with(const char* who, AttnParams& p, int sms, int single_units, void*
   return check_launch(who);
 }
 
-template <int D, bool E4M3, int NT>
-int launch_attn(const char* who, AttnParams& p, int sms, void* workspace, cudaStream_t s) {
+struct Layout {
+  int single_units;  // a CTA per unit; 0: ranges of the line
+  bool large;        // CTAs that have the SM to themselves
+};
+
+template <int D, int NT>
+Layout layout_of(const AttnParams& p, int sms) {
   using S = Shape<D, NT>;
-  constexpr int kLarge = S::kWarpsPerSm;
   const long long units = static_cast<long long>(p.c.batch) * p.c.hkv * ((p.tokens * p.group + S::kRows - 1) / S::kRows);
   // A CTA per unit, without a plan before it and a join behind it, where the table has room for short sequences only.  Up to
   // a unit per SM a unit's warps are all that read for it: 2 tiles a warp while most SMs have no unit, then 4, then 8 (planned
@@ -1039,15 +1048,20 @@ int launch_attn(const char* who, AttnParams& p, int sms, void* workspace, cudaSt
   // of up to 1024: 89 -> 80; D 256, 800 units of up to 1024: 65 -> 57; 600 of up to 1900: 75 -> 76).
   const long long room = static_cast<long long>(p.c.max_pages) * p.c.page, most = (room + S::kTok - 1) / S::kTok;
   const int rounds = units * 4 <= sms ? 2 : units * 2 <= sms ? 4 : 8;
-  if (units <= sms && most <= rounds * kLarge)
-    return launch_with<D, E4M3, NT, kLarge>(who, p, sms, static_cast<int>(units), workspace, s);
+  if (units <= sms && most <= rounds * S::kWarpsPerSm) return {static_cast<int>(units), true};
   if (units > sms && units <= 1 << 20 && room <= (D == 256 ? 1024 : 2048))  // (indexes of threads in 32 bits)
-    return launch_with<D, E4M3, NT, kSmallWarps>(who, p, sms, static_cast<int>(units), workspace, s);
+    return {static_cast<int>(units), false};
   // Few units: a CTA per SM leaves the fewest partial rows to join (8-row units, 1 unit of 64000 tokens, D 128: 14.8 to 14.8 us;
   // 2: 16.6 to 18.5; 4: 20.3 to 21.3; 16-row units, D 256, 8: 37 to 39; 32: 48 to 53).  Many: small CTAs, whose changes of unit
   // overlap (8-row units, D 64, 8: 13.3 to 14.6 us; D 128, 32: 28.5 to 30.3; 16-row units, D 128, 64: 30.3 to 31.4).
-  if (units * (NT == 1 ? 32 : 4) <= sms) return launch_with<D, E4M3, NT, kLarge>(who, p, sms, 0, workspace, s);
-  return launch_with<D, E4M3, NT, kSmallWarps>(who, p, sms, 0, workspace, s);
+  return {0, units * (NT == 1 ? 32 : 4) <= sms};
+}
+
+template <int D, bool E4M3, int NT>
+int launch_attn(const char* who, AttnParams& p, int sms, void* workspace, cudaStream_t s) {
+  const Layout l = layout_of<D, NT>(p, sms);
+  return l.large ? launch_with<D, E4M3, NT, Shape<D, NT>::kWarpsPerSm>(who, p, sms, l.single_units, workspace, s)
+                 : launch_with<D, E4M3, NT, kSmallWarps>(who, p, sms, l.single_units, workspace, s);
 }
 
 template <int D>
@@ -1056,6 +1070,23 @@ int dispatch_attn(const char* who, AttnParams& p, bool e4m3, int sms, void* ws, 
   if (p.tokens * p.group <= 8)
     return e4m3 ? launch_attn<D, true, 1>(who, p, sms, ws, s) : launch_attn<D, false, 1>(who, p, sms, ws, s);
   return e4m3 ? launch_attn<D, true, 2>(who, p, sms, ws, s) : launch_attn<D, false, 2>(who, p, sms, ws, s);
+}
+
+// f(Tag<D, NT>) of a call's shape: up to 8 query rows share a pass (8 columns of the product), else 16
+template <typename F>
+long long of_shape(int head_dim, long long rows_per_head, F f) {
+  const bool one = rows_per_head <= 8;
+  if (head_dim == 64) return one ? f(Tag<64, 1>{}) : f(Tag<64, 2>{});
+  if (head_dim == 128) return one ? f(Tag<128, 1>{}) : f(Tag<128, 2>{});
+  return one ? f(Tag<256, 1>{}) : f(Tag<256, 2>{});
+}
+
+// Bytes of workspace that a call needs: none where each unit has a CTA of its own
+long long workspace_of(const AttnParams& p, int head_dim, int sms) {
+  return of_shape(head_dim, static_cast<long long>(p.tokens) * p.group, [&](auto t) -> long long {
+    constexpr int D = decltype(t)::kD, NT = decltype(t)::kNt;
+    return layout_of<D, NT>(p, sms).single_units > 0 ? 0 : workspace_bytes<D, NT>(sms);
+  });
 }
 
 }  // namespace kv8
@@ -1068,15 +1099,27 @@ extern "C" long long tokmix_kv8_attention_workspace_bytes(int tokens, int heads_
       (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return -1;
   const int sms = device_sm_count();
-  const bool one = static_cast<long long>(tokens) * (heads_q / heads_kv) <= 8;
-  size_t n = 0;
-  if (head_dim == 64)
-    n = one ? workspace_bytes<64, 1>(sms) : workspace_bytes<64, 2>(sms);
-  else if (head_dim == 128)
-    n = one ? workspace_bytes<128, 1>(sms) : workspace_bytes<128, 2>(sms);
-  else
-    n = one ? workspace_bytes<256, 1>(sms) : workspace_bytes<256, 2>(sms);
-  return static_cast<long long>(n);
+  return of_shape(head_dim, static_cast<long long>(tokens) * (heads_q / heads_kv), [&](auto t) -> long long {
+    return workspace_bytes<decltype(t)::kD, decltype(t)::kNt>(sms);
+  });
+}
+
+extern "C" long long tokmix_kv8_attention_workspace_bytes_for(int tokens, int heads_q, int heads_kv, int head_dim, int batch,
+                                                              int max_pages, int page_size) {
+  using namespace tokmix;
+  using namespace tokmix::kv8;
+  const long long most = tokmix_kv8_attention_workspace_bytes(tokens, heads_q, heads_kv, head_dim);
+  if (most < 0 || batch < 0 || max_pages < 0 || page_size <= 0) return -1;
+  if (batch == 0) return 0;
+  if (batch > kMaxBatch || heads_q > 65536) return most;  // the call itself refuses them
+  AttnParams p{};
+  p.tokens = tokens;
+  p.group = heads_q / heads_kv;
+  p.c.batch = batch;
+  p.c.hkv = heads_kv;
+  p.c.max_pages = max_pages;
+  p.c.page = page_size;
+  return workspace_of(p, head_dim, device_sm_count());
 }
 
 extern "C" int tokmix_kv8_attention(const void* q, long long q_batch_stride, long long q_token_stride,
@@ -1098,7 +1141,7 @@ extern "C" int tokmix_kv8_attention(const void* q, long long q_batch_stride, lon
   if (!(sm_scale > 0.0f) || !std::isfinite(sm_scale))
     return fail(TOKMIX_ERR_INVALID_ARGUMENT, "%s: sm_scale must be positive and finite", who);
   if (tokens == 0 || p.c.batch == 0) return TOKMIX_OK;
-  if (!q || !out || !workspace) return fail(TOKMIX_ERR_INVALID_ARGUMENT, "%s: null pointer argument", who);
+  if (!q || !out) return fail(TOKMIX_ERR_INVALID_ARGUMENT, "%s: null pointer argument", who);
   if (reinterpret_cast<uintptr_t>(q) % 16 != 0 || reinterpret_cast<uintptr_t>(out) % 16 != 0 ||
       reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
     return fail(TOKMIX_ERR_INVALID_ARGUMENT, "%s: tensors must be 16-byte aligned", who);
@@ -1111,9 +1154,6 @@ extern "C" int tokmix_kv8_attention(const void* q, long long q_batch_stride, lon
   if (heads_q > 65536 || most_tiles > 0x7fffffffLL || static_cast<long long>(p.c.batch) * tokens * heads_q > 0x3fffffffLL)
     return fail(TOKMIX_ERR_UNSUPPORTED, "%s: problem too large", who);
   if (const int rc = check_device()) return rc;
-  const long long need = tokmix_kv8_attention_workspace_bytes(tokens, heads_q, cache->heads_kv, cache->head_dim);
-  if (workspace_bytes < need)
-    return fail(TOKMIX_ERR_INVALID_ARGUMENT, "%s: workspace of %lld bytes, %lld needed", who, workspace_bytes, need);
   p.q = q;
   p.q_sb = q_batch_stride;
   p.q_st = q_token_stride;
@@ -1129,6 +1169,9 @@ extern "C" int tokmix_kv8_attention(const void* q, long long q_batch_stride, lon
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool e4m3 = cache->dtype == TOKMIX_DTYPE_E4M3;
   const int sms = device_sm_count();
+  const long long need = workspace_of(p, cache->head_dim, sms);
+  if (workspace_bytes < need || (need > 0 && !workspace))
+    return fail(TOKMIX_ERR_INVALID_ARGUMENT, "%s: workspace of %lld bytes, %lld needed", who, workspace ? workspace_bytes : 0, need);
   if (cache->head_dim == 64) return dispatch_attn<64>(who, p, e4m3, sms, workspace, s);
   if (cache->head_dim == 128) return dispatch_attn<128>(who, p, e4m3, sms, workspace, s);
   return dispatch_attn<256>(who, p, e4m3, sms, workspace, s);

@@ -36,11 +36,11 @@ KERNEL_TYPE = "kv8_attention"
 MAX_TOKENS = 16
 
 
-@functools.cache
-def _workspace_bytes(tokens: int, hq: int, hkv: int, d: int, device: int) -> int:
-    """The workspace of a shape on a device."""
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(tokens: int, hq: int, hkv: int, d: int, batch: int, max_pages: int, page: int, device: int) -> int:
+    """The workspace of a call's sizes on a device."""
     with torch.cuda.device(device):
-        return _lib.load().tokmix_kv8_attention_workspace_bytes(tokens, hq, hkv, d)
+        return _lib.load().tokmix_kv8_attention_workspace_bytes_for(tokens, hq, hkv, d, batch, max_pages, page)
 
 
 def kernel_fn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -66,11 +66,11 @@ def kernel_fn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_s
     lse = torch.empty((batch, tokens, hq), dtype=torch.float32, device=dev) if return_lse else None
     q, qs = _kv8.token_strides(q)
     status = _lib.host_status_ptr(dev, "kv8")
-    need = _workspace_bytes(max(tokens, 1), hq, cache.heads_kv, d, dev.index)
-    ws = _lib.empty((need,), torch.uint8, dev)  # per call: calls may overlap on other streams
+    need = _workspace_bytes(max(tokens, 1), hq, cache.heads_kv, d, batch, cache.max_pages, cache.page_size, dev.index)
+    ws = _lib.empty((need,), torch.uint8, dev) if need else None  # per call: calls may overlap on other streams
     rc = _lib.call_on(dev, _lib.load().tokmix_kv8_attention, q.data_ptr(), *qs, out.data_ptr(),
                       lse.data_ptr() if return_lse else None, tokens, hq, _kv8.IO_DTYPES[q.dtype], sm_scale,
-                      _kv8.byref(cache), ws.data_ptr(), need, status, _lib.stream_ptr(dev))
+                      _kv8.byref(cache), ws.data_ptr() if need else None, need, status, _lib.stream_ptr(dev))
     if rc:
         _lib.check(rc, "kv8_attention")
     _lib.after_host_status_launch(dev, "kv8")

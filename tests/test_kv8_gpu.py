@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from kernel_opt_agent_b200 import _lib, add_rms_norm_quant, references
+from kernel_opt_agent_b200 import _kv8, _lib, add_rms_norm_quant, references
 from kernel_opt_agent_b200 import flash_attention_2 as fa2
 from kernel_opt_agent_b200 import kv8_append as append
 from kernel_opt_agent_b200 import kv8_attention as attention
@@ -498,6 +498,34 @@ def test_refusals(cuda_device):
         with pytest.raises(ValueError):
             append.kernel_fn(**{**args, **bad})
     attention.check_device_status(cuda_device)
+
+
+def test_workspace_sizes(cuda_device):
+    """A call needs no workspace with a short table; with room for long sequences it refuses less than it needs."""
+    lib, lens = _lib.load(), [40, 50]
+    cache = _filled_cache(15, lens, 2, 128, 16, E4M3, cuda_device)
+    q, seq = _queries(15, 2, 1, 8, 128, torch.bfloat16, cuda_device), _i32(lens, cuda_device)
+    want = attention.kernel_fn(q, *cache, seq)
+    for room in (0, 4096):
+        table = torch.cat([cache[4], torch.full((2, room), GARBAGE_PAGE, dtype=torch.int32, device=cuda_device)], 1)
+        need = lib.tokmix_kv8_attention_workspace_bytes_for(1, 8, 2, 128, 2, table.shape[1], 16)
+        most = lib.tokmix_kv8_attention_workspace_bytes(1, 8, 2, 128)
+        assert need == (most if room else 0) and most > 0
+        out = torch.zeros_like(q)
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=cuda_device)
+        desc = _kv8.cache_args(q, *cache[:4], table, seq, None)
+
+        def call(ptr, size):
+            return lib.tokmix_kv8_attention(q.data_ptr(), *q.stride()[:3], out.data_ptr(), None, 1, 8, 0, 128 ** -0.5,
+                                            _kv8.byref(desc), ptr, size, None, _lib.stream_ptr(cuda_device))
+        if room:
+            assert call(None, need) == call(ws.data_ptr(), need - 1) == _lib.TOKMIX_ERR_INVALID_ARGUMENT
+            assert call(ws.data_ptr(), need) == 0
+        else:
+            assert call(None, 0) == 0
+            assert torch.equal(out, want)
+        torch.cuda.synchronize()
+        _assert_attention(out, None, q, cache, seq)
 
 
 def test_refuses_more_sequences_or_tokens_than_int(cuda_device):

@@ -83,6 +83,13 @@ def test_null_cache_and_workspace_sizes():
         assert lib.tokmix_kv8_attention_workspace_bytes(*bad) == -1
 
 
+@pytest.mark.parametrize("bad", [(0, 8, 2, 128, 3, 4, 64), (1, 7, 2, 128, 3, 4, 64), (1, 8, 2, 96, 3, 4, 64), (1, 8, 2, 128, -1, 4, 64),
+                                 (1, 8, 2, 128, 3, -1, 64), (1, 8, 2, 128, 3, 4, 0)])
+def test_workspace_of_bad_sizes(bad):
+    assert _lib.load().tokmix_kv8_attention_workspace_bytes_for(*bad) == -1
+    assert _lib.load().tokmix_kv8_attention_workspace_bytes_for(1, 8, 2, 128, 0, 4, 64) == 0
+
+
 def test_modules_refuse_cpu_tensors():
     x = torch.zeros(2, 128, dtype=torch.bfloat16)
     with pytest.raises(ValueError):
