@@ -1046,6 +1046,7 @@ Layout layout_of(const AttnParams& p, int sms) {
   // More units: a change of unit costs a range more than a CTA of its own, as long as no unit is long (D 128, 400 units of up to
   // 640 tokens: 20.0 -> 15.2 us; 800 units: 29.4 -> 24.7; of up to 1900: 49.5 -> 48.7; of up to 3800: 85 -> 94; 2400 units
   // of up to 1024: 89 -> 80; D 256, 800 units of up to 1024: 65 -> 57; 600 of up to 1900: 75 -> 76).
+  // One long sequence among short ones loses: 128 units, D 128, of 50 tokens 9.7 -> 5.7 us, 8 of them of 2000 12.0 -> 13.8.
   const long long room = static_cast<long long>(p.c.max_pages) * p.c.page, most = (room + S::kTok - 1) / S::kTok;
   const int rounds = units * 4 <= sms ? 2 : units * 2 <= sms ? 4 : 8;
   if (units <= sms && most <= rounds * S::kWarpsPerSm) return {static_cast<int>(units), true};
