@@ -1043,14 +1043,20 @@ Layout layout_of(const AttnParams& p, int sms) {
   // a unit per SM a unit's warps are all that read for it: 2 tiles a warp while most SMs have no unit, then 4, then 8 (planned
   // -> a CTA per unit; Hkv 8, D 128, 8 units of 1024 tokens, 3 tiles: 8.0 -> 9.3 us; 48 units, 3 tiles: 9.2 -> 9.3; 96 units:
   // 12.7 -> 10.7; D 256, 32 units of 1000 tokens, 6 tiles: 11.7 -> 14.4; D 128, 128 units of 2000, 6 tiles: 17.2 -> 16.2).
-  // More units: a change of unit costs a range more than a CTA of its own, as long as no unit is long (D 128, 400 units of up to
-  // 640 tokens: 20.0 -> 15.2 us; 800 units: 29.4 -> 24.7; of up to 1900: 49.5 -> 48.7; of up to 3800: 85 -> 94; 2400 units
-  // of up to 1024: 89 -> 80; D 256, 800 units of up to 1024: 65 -> 57; 600 of up to 1900: 75 -> 76).
-  // One long sequence among short ones loses: 128 units, D 128, of 50 tokens 9.7 -> 5.7 us, 8 of them of 2000 12.0 -> 13.8.
+  // More units: a change of unit costs a range more than a CTA of its own, as long as no unit is long: up to 256 KB, or 512 KB
+  // where there are enough units to even out the ends.  Ranges -> a CTA per unit, with lengths uniform up to the table's (u), a
+  // tenth filling it and the others short (t), all filling it (f):
+  //   D 128, 800 units,  256 KB:  u 32.0 -> 30.7 us, t 21.0 -> 20.5, f 44.0 -> 39.9
+  //           240 units,  512 KB:  u 18.4 -> 27.0,    t 13.9 -> 23.2, f 30.3 -> 32.2
+  //          1760 units,  512 KB:  u 88.1 -> 82.7,    t 51.9 -> 54.5, f 150 -> 142
+  //   D 256, 160 units,  512 KB:  u 18.8 -> 21.7,    t 19.0 -> 22.3, f 23.3 -> 24.7
+  //           400 units,  512 KB:  u 34.8 -> 30.2,    t 23.0 -> 26.4, f 49.3 -> 39.8
   const long long room = static_cast<long long>(p.c.max_pages) * p.c.page, most = (room + S::kTok - 1) / S::kTok;
   const int rounds = units * 4 <= sms ? 2 : units * 2 <= sms ? 4 : 8;
   if (units <= sms && most <= rounds * S::kWarpsPerSm) return {static_cast<int>(units), true};
-  if (units > sms && units <= 1 << 20 && room <= (D == 256 ? 1024 : 2048))  // (indexes of threads in 32 bits)
+  const long long slots = static_cast<long long>(sms) * (S::kWarpsPerSm / kSmallWarps);
+  const long long bytes = (units * 4 >= (D == 256 ? 3 : 12) * slots ? 512 : 256) << 10;
+  if (units > sms && units <= 1 << 20 && room * 2 * D <= bytes)  // (indexes of threads in 32 bits)
     return {static_cast<int>(units), false};
   // Few units: a CTA per SM leaves the fewest partial rows to join (8-row units, 1 unit of 64000 tokens, D 128: 14.8 to 14.8 us;
   // 2: 16.6 to 18.5; 4: 20.3 to 21.3; 16-row units, D 256, 8: 37 to 39; 32: 48 to 53).  Many: small CTAs, whose changes of unit

@@ -600,7 +600,9 @@ def test_largest_batch(cuda_device):
     (E4M3, 75, 1, 4, 1, 256, 16, 1536), (INT8, 148, 1, 4, 1, 64, 64, 6144), (E4M3, 149, 1, 4, 1, 64, 64, 2048),
     (E4M3, 149, 1, 4, 1, 64, 16, 2064), (INT8, 111, 1, 16, 4, 128, 128, 2048), (E4M3, 112, 1, 16, 4, 256, 32, 1024),
     (E4M3, 112, 1, 16, 4, 256, 32, 1056), (INT8, 90, 3, 20, 2, 128, 16, 2048), (E4M3, 300, 2, 16, 2, 64, 32, 2048),
-    (E4M3, 9, 2, 16, 4, 64, 64, 2048), (E4M3, 10, 16, 3, 1, 256, 64, 512)])
+    (E4M3, 9, 2, 16, 4, 64, 64, 2048), (E4M3, 10, 16, 3, 1, 256, 64, 512), (INT8, 150, 1, 4, 1, 128, 16, 1024),
+    (E4M3, 150, 1, 4, 1, 128, 16, 1040), (E4M3, 333, 1, 8, 4, 128, 64, 2048), (INT8, 167, 1, 8, 2, 256, 16, 1024),
+    (E4M3, 166, 1, 8, 2, 256, 16, 1024), (E4M3, 166, 1, 8, 2, 256, 16, 512)])
 def test_attention_where_the_layout_changes(cuda_device, cache_dtype, b, t, hq, hkv, d, page, room):
     """Units (sequences times heads times row tiles) and room in the table on both sides of each border between the ways to lay
     the work out: one sequence fills its table, others are short or empty, one has nothing new."""
