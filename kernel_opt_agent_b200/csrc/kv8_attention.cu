@@ -23,7 +23,7 @@
 //     not hold; the e4m3 form of this product runs on the same pipe with the same widening inside (it measured 5 % slower).
 // What it measured (B200, device time): Hq 32 Hkv 8 D 128, 64 sequences of 1024 to 4096 tokens 61 us, 5.5 TB/s (the same
 // copies without the products 59 us at a time when the whole took 64); Hq 16 Hkv 2 D 256, 16 sequences of up to 65536 tokens
-// 111 to 112 us, 5.8 TB/s; one of 65536 21 us.  The SMs' shares of the bandwidth differ (equal ranges end after 86 to 110 us
+// 110 to 112 us, 5.8 TB/s; one of 65536 21 us.  The SMs' shares of the bandwidth differ (equal ranges end after 86 to 110 us
 // of those), but short ranges drawn as SMs got done cost more in changes of unit than they evened out.  16 rows and D >= 128
 // are bound by eight warps' latency instead: 20 sequences of up to 9000 tokens, Hq 32 Hkv 4, two queries, 33 us, 3.0 TB/s
 // (twelve warps of 168 registers 39 to 43).
