@@ -320,7 +320,7 @@ typedef struct tokmix_kv8_cache {
  * smallest power of two, at least 2^-100, with max |x| <= qmax * scale over the page's tokens (qmax 448
  * for e4m3, 127 for int8); values are rounded to nearest, ties to even; where new tokens raise the scale,
  * the page's older tokens are rounded again to it.  A page whose first slot is written starts afresh.  A
- * value that is not finite makes its block's scale NaN until the page is started afresh.  A call
+ * value that is not finite makes its block's scale NaN (its call's bytes there are zeros) until the page is started afresh.  A call
  * must append to each page for one sequence only, at one place of its table.
  * Lengths that do not fit the call or the table, and table entries outside the pool, write nothing for
  * that sequence (page) and set TOKMIX_DEV_BAD_ARGS in *status (device memory or mapped host memory). */

@@ -138,6 +138,7 @@ __global__ void __launch_bounds__(GT == 32 ? 256 : GT) append_kernel(const Appen
   if (lane == 0) *scale = s_new;
 
   const float inv = 1.0f / s_new;  // exact
+  const bool marked = isnan(s_new);  // zeros then: the scale alone marks the block, a NaN byte would reach rows that do not see it (0 * NaN)
   uint8_t* dst = tile + ((lo - page0) << p.d_shift);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -152,7 +153,8 @@ __global__ void __launch_bounds__(GT == 32 ? 256 : GT) append_kernel(const Appen
         f[2 * e + 1] = t.y * inv;
       }
       *reinterpret_cast<uint2*>(dst + (static_cast<size_t>(vi) << 3)) =
-          make_uint2(float4_to_bytes<E4M3>(f[0], f[1], f[2], f[3]), float4_to_bytes<E4M3>(f[4], f[5], f[6], f[7]));
+          marked ? make_uint2(0u, 0u)
+                 : make_uint2(float4_to_bytes<E4M3>(f[0], f[1], f[2], f[3]), float4_to_bytes<E4M3>(f[4], f[5], f[6], f[7]));
     }
   }
   if (has_old && s_old < s_new) {  // (false for a NaN scale)

@@ -13,8 +13,8 @@ The cache's layout and the sequence tensors: ``_kv8``; ``make_cache`` allocates 
 Scales: per (page, head), for keys and values apart, the smallest power of two (at least 2^-100) with
 max |x| <= qmax * scale over the page's tokens (qmax 448 for e4m3, 127 for int8).  When new tokens raise
 a page's scale its older tokens are rounded again; a page whose first slot is written starts afresh,
-so pages are reused without clearing.  A value that is not finite makes its block's scale NaN: the whole
-block reads as NaN until the page starts afresh.
+so pages are reused without clearing.  A value that is not finite makes its block's scale NaN (the bytes
+it brings are zeros): the whole block reads as NaN until the page starts afresh.
 
 The caller keeps pages apart: a call appends to each page for one sequence, and at one place of its table (a
 page shared by several sequences is full, or copied first).  Lengths that do not fit the call or the table and table entries

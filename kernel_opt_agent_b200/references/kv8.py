@@ -28,7 +28,9 @@ def _append_page(cache, scale, pid, h, lo, hi, x):
     s = _scale_of(float(x.float().abs().amax()), QMAX[cache.dtype])
     s = math.nan if math.isnan(s) or math.isnan(s_old) else max(s, s_old)
     tile = cache[pid, h]
-    if not math.isnan(s):
+    if math.isnan(s):
+        tile[lo:hi] = torch.zeros_like(x, dtype=torch.float32).to(cache.dtype)
+    else:
         if s_old < s:
             tile[:lo] = _round(tile[:lo].float() * (s_old / s), cache.dtype)
         tile[lo:hi] = _round(x.float() / s, cache.dtype)
@@ -36,7 +38,7 @@ def _append_page(cache, scale, pid, h, lo, hi, x):
 
 
 def kv8_append_ref(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, new_lens=None):
-    """Updated copies of the cache and its scales.  (Bytes of a block whose scale is NaN mean nothing.)"""
+    """Updated copies of the cache and its scales.  (A block whose scale is NaN reads as NaN; its new bytes are zeros.)"""
     out = [t.clone() for t in (k_cache, v_cache, k_scale, v_scale)]
     page = k_cache.shape[2]
     ends = seq_lens.tolist()
