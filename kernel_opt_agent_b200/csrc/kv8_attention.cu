@@ -194,6 +194,9 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 
 __device__ __forceinline__ float nan_f() { return __uint_as_float(0x7fc00000u); }
 
+// 0x80 in every byte of four e4m3 ones that is NaN (0x7f, 0xff)
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
 __device__ __forceinline__ void store_out4(const AttnParams& p, size_t at, const float (&o)[4]) {
   uint2 w;
   if (p.bf16) {
@@ -654,6 +657,47 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
               w1 = tok >= lim[nt][1] ? 0.0f : w1;
             }
             pb[mt][nt][half] = transpose8x8(half2_bits(w0, w1));
+          }
+        }
+      }
+      // Tokens that some rows see and others do not: 0 * NaN would stay in the others' products, so a NaN byte among their values
+      // becomes zero here and NaN in that dimension of the rows that see it.  (Tokens that all rows see need no such care.)
+      if constexpr (E4M3) {
+        if (tail && min_lim < s.end) {
+          uint8_t* vw = ring + stage * S::kStageBytes + TOK * D;
+          const int lo = max(min_lim - t * TOK, 0), hi = min(s.end - t * TOK, TOK);
+          bool found = false;
+          for (int v = lane; v < (hi - lo) * (D / 16); v += 32) {
+            const uint4 w = *reinterpret_cast<const uint4*>(vw + tile_chunk<D>(lo + v / (D / 16), v % (D / 16)));
+            found |= (nan_bytes(w.x) | nan_bytes(w.y) | nan_bytes(w.z) | nan_bytes(w.w)) != 0;
+          }
+          if (__any_sync(0xffffffffu, found)) {
+            constexpr int X = D == 64 ? 2 : 4;  // words of this lane's dims, as in the products below
+            for (int r = lo; r < hi; ++r) {
+#pragma unroll
+              for (int jj = 0; jj < (D + 127) / 128; ++jj) {
+                uint32_t* src = reinterpret_cast<uint32_t*>(
+                    vw + (D == 64 ? tile_chunk<D>(r, g >> 1) + (g & 1) * 8 : tile_chunk<D>(r, 8 * jj + g)));
+                uint32_t nan[X];
+#pragma unroll
+                for (int x = 0; x < X; ++x) {
+                  nan[x] = nan_bytes(src[x]);
+#pragma unroll
+                  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+#pragma unroll
+                      for (int e = 0; e < 2; ++e)
+                        if ((nan[x] >> (8 * y + 7) & 1) != 0 && t * TOK + r < lim[nt][e]) acc[nt][2 * (4 * jj + x) + (y >> 1)][2 * (y & 1) + e] = nan_f();
+                }
+                __syncwarp();
+                if (cq == 0) {
+#pragma unroll
+                  for (int x = 0; x < X; ++x) src[x] &= ~((nan[x] >> 7) * 0xffu);
+                }
+              }
+            }
+            __syncwarp();
           }
         }
       }

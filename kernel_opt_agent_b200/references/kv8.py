@@ -80,10 +80,10 @@ def kv8_attention_ref(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_le
             continue
         k = kv8_values(k_cache, k_scale, block_table, b, end, dtype).repeat_interleave(hq // hkv, 0)
         v = kv8_values(v_cache, v_scale, block_table, b, end, dtype).repeat_interleave(hq // hkv, 0)
-        s = torch.einsum("thd,hld->htl", q[b, :n].to(dtype), k) * scale
-        pos = torch.arange(end, device=q.device)
-        s = s.masked_fill(pos > (end - n + torch.arange(n, device=q.device))[:, None], -math.inf)
-        lse[b, :n] = torch.logsumexp(s, -1).t()
-        out[b, :n] = torch.einsum("htl,hld->thd", torch.softmax(s, -1), v)
+        for i in range(n):  # a row at a time: what it does not see stays out of its sums (0 * NaN would not)
+            seen = end - n + i + 1
+            s = torch.einsum("hd,hld->hl", q[b, i].to(dtype), k[:, :seen]) * scale
+            lse[b, i] = torch.logsumexp(s, -1)
+            out[b, i] = torch.einsum("hl,hld->hd", torch.softmax(s, -1), v[:, :seen])
     out = out if dtype == torch.float64 else out.to(q.dtype)
     return (out, lse) if return_lse else out
