@@ -331,9 +331,10 @@ int tokmix_kv8_append(const void* k, long long k_batch_stride, long long k_token
 /* Attention of the newest tokens over the cache: row i < new_lens[b] of q [batch, tokens, heads_q,
  * head_dim] (bf16 or fp16, element strides given) is the query at position p = seq_lens[b] - new_lens[b] + i
  * and sees positions 0 .. p; out [batch, tokens, heads_q, head_dim] (contiguous, q's type) =
- * softmax(q k^T * sm_scale) v in fp32, k and v as the cache holds them; query head h reads key/value
- * head h / (heads_q / heads_kv).  lse (NULL or fp32 [batch, tokens, heads_q]): the natural logarithm of the
- * row's sum of exponentials.  Rows i >= new_lens[b] give zeros and lse -infinity.
+ * softmax(q k^T * sm_scale) v, k and v as the cache holds them (maxima, sums and accumulation in fp32; q, scaled by a
+ * power of two per row, and the weights times the value scales are rounded to fp16, where what is under 2^-39 of a
+ * row's largest such product is lost); query head h reads key/value head h / (heads_q / heads_kv).  lse (NULL or fp32
+ * [batch, tokens, heads_q]): the natural logarithm of the row's sum of exponentials.  Rows i >= new_lens[b] give zeros and lse -infinity.
  * 1 <= tokens <= 16, batch <= 8192.  workspace: tokmix_kv8_attention_workspace_bytes_for(...) bytes of device memory, 16-byte
  * aligned, no initialisation, not shared by calls that may overlap (NULL where that is 0).
  * Lengths that do not fit give NaN for the sequence's rows, a table entry outside the pool NaN for the

@@ -29,10 +29,12 @@
 // (twelve warps of 168 registers 39 to 43).
 //
 // Number formats.  q rows enter fp16 after scaling by a power of two that brings their largest element to
-// [2^14, 2^15): exact for elements down to 2^-28 of it (bf16 has 8 bits, fp16 11).  Weights enter as
-// 2^14 e^{s_j - m} rounded to fp16 (half a step is 2^-11; under 2^-38 of the largest they vanish), times
-// vs_j / vref, vref the largest value scale a warp has met -- powers of two, so exact; a block whose scale is under
-// 2^-28 of vref loses bits that are 2^-39 of the largest block's values.  Maxima, sums and outputs are fp32.
+// [2^14, 2^15): exact for elements down to 2^-28 of it (bf16 has 8 bits, fp16 11).  A weight enters with its scale, as
+// 2^14 e^{s_j} vs_j / 2^mv rounded to fp16 (half a step is 2^-11), mv the largest s_j + log2 vs_j (s in base 2) the row has met:
+// the products fill fp16's range whatever the scales are, and only what is under 2^-39 of the row's largest e^{s_j} vs_j
+// vanishes.  (One reference for all rows, the largest vs_j loaded, would let a block of little or no weight take the
+// others' bits; a reference per row costs 8 rows up to 2 %, 16 rows 3 to 11 %: 20 sequences of up to 9000 tokens, Hq 32 Hkv 4
+// D 128, two queries, 33.0 -> 35.1 us.)  Maxima, sums and outputs are fp32; weights under 2^-140 of the largest are zero.
 #include "kv8_common.cuh"
 
 #include <algorithm>
@@ -44,6 +46,7 @@ namespace kv8 {
 constexpr int kMaxTokens = 16;
 constexpr int kMaxBatch = 8192;  // the plan keeps batch + 1 words in shared memory
 constexpr float kShift = 14.0f;  // weights are held times 2^14
+constexpr float kSpan = 112.0f;  // a row's accumulators are held times 2^112 / (its largest weight) at most
 constexpr int kJoinThreads = 256;
 constexpr int kMaxCtas = 512;  // at most 3 per SM
 
@@ -187,6 +190,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// log2 |x|; -infinity for 0 and subnormals
+__device__ __forceinline__ float lg2_abs(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fabsf(x)));
+  return y;
+}
+
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -303,7 +313,7 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
   float* scales = reinterpret_cast<float*>(smem + W * STAGES * S::kStageBytes) + (threadIdx.x >> 5) * STAGES * 2 * MT;
   __half* qs = reinterpret_cast<__half*>(smem + W * STAGES * (S::kStageBytes + 8 * MT));  // [row][kQStride]
   uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + S::smem_bytes(W));
-  __shared__ float row_factor[ROWS], row_top[ROWS], row_sum[ROWS], warp_m[W][ROWS], warp_l[W][ROWS], warp_v[W];
+  __shared__ float row_factor[ROWS], row_top[ROWS], row_sum[ROWS], row_up[ROWS], warp_m[W][ROWS], warp_l[W][ROWS], warp_mv[W][ROWS];
   __shared__ int warp_at[W];  // where in `smem` a warp's partial rows lie
   __shared__ uint32_t scratch[W];
 
@@ -495,7 +505,10 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
     __syncthreads();
 
     // this lane's rows (columns of the products): 8 nt + 2 cq + {0, 1}
-    float factor[NT][2], m[NT][2], l[NT][2];
+    // m is the largest score s_j so far, the sum's reference; mv the largest s_j + log2 vs_j, the accumulators': a block counts by
+    // its softmax weight times its scale, so one of little weight cannot take the others' bits (kept within m - kSpan and
+    // m + 126: the factor between the two is a normal number)
+    float factor[NT][2], m[NT][2], mv[NT][2], l[NT][2];
     int lim[NT][2];
     int min_lim = s.end;
 #pragma unroll
@@ -506,7 +519,7 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
         factor[nt][e] = row_factor[r];
         lim[nt][e] = row0 + r < rows_valid ? s.start + (row0 + r) / p.group + 1 : s.end;
         min_lim = min(min_lim, lim[nt][e]);
-        m[nt][e] = -INFINITY;
+        m[nt][e] = mv[nt][e] = -INFINITY;
         l[nt][e] = 0.0f;
       }
     }
@@ -518,7 +531,6 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
       for (int x = 0; x < D / 16; ++x)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[nt][x][e] = 0.0f;
-    float vref = 0.0f;
 
     int t = cur.t0 + warp;
     const bool any = t < t1;
@@ -527,11 +539,12 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
       __syncwarp();
       const uint8_t* kt = ring + stage * S::kStageBytes;
       const uint8_t* vt = kt + TOK * D;
-      float ks[MT], vs[MT];
+      float ks[MT], vs[MT], lv[MT];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         ks[mt] = scales[stage * 2 * MT + mt];
         vs[mt] = scales[stage * 2 * MT + MT + mt];
+        lv[mt] = lg2_abs(vs[mt]);
       }
       // scores: two accumulators per product shorten the dependent chain
       float sc[MT][NT][2][4];
@@ -568,7 +581,7 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
         }
       }
       // softmax: a lane has tokens g and g + 8 of each subtile for its rows
-      float top[NT][2];
+      float top[NT][2], topv[NT][2];
       const bool tail = t * TOK + TOK > min_lim;  // some token is hidden from some row
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -591,36 +604,47 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           top[nt][e] = fmaxf(sc[0][nt][0][e], sc[0][nt][0][2 + e]);
+          topv[nt][e] = top[nt][e] + lv[0];
 #pragma unroll
-          for (int mt = 1; mt < MT; ++mt) top[nt][e] = fmaxf(top[nt][e], fmaxf(sc[mt][nt][0][e], sc[mt][nt][0][2 + e]));
+          for (int mt = 1; mt < MT; ++mt) {
+            const float a = fmaxf(sc[mt][nt][0][e], sc[mt][nt][0][2 + e]);
+            top[nt][e] = fmaxf(top[nt][e], a);
+            topv[nt][e] = fmaxf(topv[nt][e], a + lv[mt]);
+          }
         }
       }
       bool grew = false;
-      float ref[NT][2];
+      float ref[NT][2], down[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) top[nt][e] = fmaxf(top[nt][e], __shfl_xor_sync(0xffffffffu, top[nt][e], o));
+          if constexpr (MT == 1) {
+            topv[nt][e] = top[nt][e] + lv[0];
+          } else {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) topv[nt][e] = fmaxf(topv[nt][e], __shfl_xor_sync(0xffffffffu, topv[nt][e], o));
+          }
           top[nt][e] = fmaxf(top[nt][e], m[nt][e]);
-          grew |= top[nt][e] > m[nt][e];
+          topv[nt][e] = fminf(fmaxf(fmaxf(topv[nt][e], mv[nt][e]), top[nt][e] - kSpan), top[nt][e] + 126.0f);
+          grew |= top[nt][e] > m[nt][e] || topv[nt][e] > mv[nt][e];
           ref[nt][e] = top[nt][e] == -INFINITY ? 0.0f : top[nt][e];  // a row that has seen nothing yet
+          down[nt][e] = ex2(ref[nt][e] - (topv[nt][e] == -INFINITY ? 0.0f : topv[nt][e]));
         }
       }
-      float vnew = vref;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) vnew = fmaxf(vnew, vs[mt]);
-      if (__any_sync(0xffffffffu, grew) || vnew > vref) {
-        const float vcorr = vnew > vref ? vref / vnew : 1.0f;
+      if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float c0 = ex2(m[nt][0] - ref[nt][0]), c1 = ex2(m[nt][1] - ref[nt][1]);
-          l[nt][0] *= c0;
-          l[nt][1] *= c1;
+          l[nt][0] *= ex2(m[nt][0] - ref[nt][0]);
+          l[nt][1] *= ex2(m[nt][1] - ref[nt][1]);
           m[nt][0] = top[nt][0];
           m[nt][1] = top[nt][1];
-          const float a0 = c0 * vcorr, a1 = c1 * vcorr;
+          const float a0 = topv[nt][0] == -INFINITY ? 0.0f : ex2(mv[nt][0] - topv[nt][0]);
+          const float a1 = topv[nt][1] == -INFINITY ? 0.0f : ex2(mv[nt][1] - topv[nt][1]);
+          mv[nt][0] = topv[nt][0];
+          mv[nt][1] = topv[nt][1];
 #pragma unroll
           for (int x = 0; x < D / 16; ++x) {
             acc[nt][x][0] *= a0;
@@ -629,7 +653,6 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
             acc[nt][x][3] *= a1;
           }
         }
-        vref = vnew;
       }
       uint32_t pb[MT][NT][2];
 #pragma unroll
@@ -645,12 +668,12 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
       }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        const float rv = vref > 0.0f ? __fdividef(vs[mt], vref) : vs[mt] * 0.0f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            float w0 = sc[mt][nt][0][half * 2] * rv, w1 = sc[mt][nt][0][half * 2 + 1] * rv;
+            // (in this order: a weight is at most 2^14, so times 2^kSpan finite)
+            float w0 = sc[mt][nt][0][half * 2] * down[nt][0] * vs[mt], w1 = sc[mt][nt][0][half * 2 + 1] * down[nt][1] * vs[mt];
             if (tail) {  // a hidden token weighs nothing even where its block's scale is NaN
               const int tok = t * TOK + mt * 16 + half * 8 + g;
               w0 = tok >= lim[nt][0] ? 0.0f : w0;
@@ -759,6 +782,7 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
         if (g == 0) {
           warp_m[warp][nt * 8 + r] = m[nt][e];
           warp_l[warp][nt * 8 + r] = l[nt][e];
+          warp_mv[warp][nt * 8 + r] = mv[nt][e];
         }
         if (any) {
           // dims of acc[2x], acc[2x + 1]: D 64: 8 g + 4 x; else 128 (x / 4) + 16 g + 4 (x % 4), four in a row
@@ -770,27 +794,30 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
           }
         }
       }
-      if (lane == 0) {
-        warp_v[warp] = vref;
-        warp_at[warp] = static_cast<int>(reinterpret_cast<uint8_t*>(dst) - smem);
-      }
+      if (lane == 0) warp_at[warp] = static_cast<int>(reinterpret_cast<uint8_t*>(dst) - smem);
       __syncthreads();
       const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (first ? 0 : 1);
       const int nw = min(W, t1 - cur.t0);  // warps that had a tile
       if (threadIdx.x < 128) {  // a row's maximum and sum, 16 lanes each; warp_m becomes what a warp's rows are multiplied by
         const int r = nt * 8 + (threadIdx.x >> 4), i = threadIdx.x & 15;
-        const float mi = i < nw ? warp_m[i][r] : -INFINITY;
-        float top = mi;
+        const float mi = i < nw ? warp_m[i][r] : -INFINITY, mvi = i < nw ? warp_mv[i][r] : -INFINITY;
+        float top = mi, topv = mvi;
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int o = 8; o > 0; o >>= 1) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, o));
+        }
         const float w = ex2(mi - (top == -INFINITY ? 0.0f : top));
         float sum = i < nw ? w * warp_l[i][r] : 0.0f;
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (i < nw) warp_m[i][r] = w * (sum == 0.0f ? 0.0f : 1.0f / sum) * warp_v[i];
+        const float refv = topv == -INFINITY ? 0.0f : topv;
+        if (i < nw) warp_m[i][r] = ex2(mvi - refv) * (sum == 0.0f ? 0.0f : 1.0f / sum);
         if (i == 0) {
           row_top[r] = top;
           row_sum[r] = sum;
+          // what is left of the accumulators' reference, 2^(refv - top), in two halves: subnormal outputs keep their bits
+          row_up[r] = ex2(0.5f * (refv - (top == -INFINITY ? refv : top)));
         }
       }
       __syncthreads();
@@ -811,7 +838,9 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
           o[2] += a.z * w;
           o[3] += a.w * w;
         }
-        const float top = row_top[r], sum = row_sum[r];
+        const float top = row_top[r], sum = row_sum[r], up = row_up[r];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = o[e] * up * up;
         if (cur.whole) {
           const int i = row / p.group, h = cur.kvh * p.group + row - i * p.group;
           const size_t orow = (static_cast<size_t>(cur.b) * p.tokens + i) * p.hq + h;

@@ -9,8 +9,9 @@ prefill only.
 q [B, T, Hq, D] bf16 or fp16, 1 <= T <= 16: the queries of each sequence's newest tokens (one in a decode
 step, a few when drafted tokens are verified), already appended to the cache.  Row i < new_lens[b] stands at
 position seq_lens[b] - new_lens[b] + i and sees the positions up to its own; query head h reads key/value
-head h // (Hq // Hkv); default scale 1 / sqrt(D).  out [B, T, Hq, D] in q's type, arithmetic in fp32 on
-the values the cache stands for.  Rows that see nothing (padding behind new_lens[b], empty sequences) are
+head h // (Hq // Hkv); default scale 1 / sqrt(D).  out [B, T, Hq, D] in q's type, on the values the cache stands for:
+maxima, sums and accumulation in fp32; q (scaled by a power of two per row) and each softmax weight times its
+value scale enter the products as fp16, where what is under 2^-39 of a row's largest such product is lost.  Rows that see nothing (padding behind new_lens[b], empty sequences) are
 zero, their lse -inf.  ``lse`` [B, T, Hq] fp32 is the logarithm of the row's sum of exponentials, for
 joining with attention over other tokens.  q may be a slice of a packed tensor.  The cache's layout and the
 sequence tensors: ``_kv8``.
