@@ -252,16 +252,14 @@ _host_status: dict[int, _HostStatus] = {}
 def host_status_ptr(device: torch.device, what: str) -> int | None:
     """Raises if an earlier launch on `device` stored a bit in the host status word (and clears it), else
     its address for the next launch (None for a first call inside a graph capture, where it cannot be
-    allocated, and with TOKMIX_CHECK_STATUS=0)."""
-    if _STATUS_MODE == "off":
-        return None
+    allocated).  With TOKMIX_CHECK_STATUS=0 the launch gets it all the same and only explicit checks look at it."""
     h = _host_status.get(device.index)
     if h is None:
         if torch.cuda.is_current_stream_capturing():
             return None
         with _lock:
             h = _host_status.setdefault(device.index, _HostStatus())
-    if h.word.value:
+    if h.word.value and _STATUS_MODE != "off":
         take_host_status(device, what)
     return h.ptr
 
