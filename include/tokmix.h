@@ -323,7 +323,9 @@ typedef struct tokmix_kv8_cache {
  * value that is not finite makes its block's scale NaN (its call's bytes there are zeros) until the page is started afresh.  A call
  * must append to each page for one sequence only, at one place of its table.
  * Lengths that do not fit the call or the table, and table entries outside the pool, write nothing for
- * that sequence (page) and set TOKMIX_DEV_BAD_ARGS in *status (device memory or mapped host memory). */
+ * that sequence (page) and set TOKMIX_DEV_BAD_ARGS in *status (device memory or mapped host memory).  The bit is
+ * added to what the word holds, not atomically: calls of other kinds that may run at the same time, and a host that
+ * clears the word then, need a word of their own. */
 int tokmix_kv8_append(const void* k, long long k_batch_stride, long long k_token_stride, long long k_head_stride,
                       const void* v, long long v_batch_stride, long long v_token_stride, long long v_head_stride,
                       int tokens, int io_dtype, const tokmix_kv8_cache* cache, uint32_t* status, void* stream);
@@ -338,7 +340,7 @@ int tokmix_kv8_append(const void* k, long long k_batch_stride, long long k_token
  * 1 <= tokens <= 16, batch <= 8192.  workspace: tokmix_kv8_attention_workspace_bytes_for(...) bytes of device memory, 16-byte
  * aligned, no initialisation, not shared by calls that may overlap (NULL where that is 0).
  * Lengths that do not fit give NaN for the sequence's rows, a table entry outside the pool NaN for the
- * rows that see it; both set TOKMIX_DEV_BAD_ARGS in *status (device memory or mapped host memory). */
+ * rows that see it; both set TOKMIX_DEV_BAD_ARGS in *status, as tokmix_kv8_append does. */
 int tokmix_kv8_attention(const void* q, long long q_batch_stride, long long q_token_stride, long long q_head_stride,
                          void* out, float* lse, int tokens, int heads_q, int io_dtype, float sm_scale,
                          const tokmix_kv8_cache* cache, void* workspace, long long workspace_bytes, uint32_t* status,

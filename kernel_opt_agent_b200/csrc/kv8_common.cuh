@@ -40,9 +40,12 @@ struct View {
 // Checks a cache description on the host and makes the device view; head_dim is returned for dispatch.
 int make_view(const char* who, const tokmix_kv8_cache* c, View& out);
 
-// The word may be device memory or mapped host memory: a plain store, and only ever of this one bit.
+// Sets the bit and keeps the word's others.  The word may be device memory or mapped host memory, where an atomic is not to be
+// relied on: a load and a store, which calls of this file may do at once (they set the same bit).
 __device__ __forceinline__ void report_bad(uint32_t* status) {
-  if (status != nullptr) *reinterpret_cast<volatile uint32_t*>(status) = kStatusBadArgs;
+  if (status == nullptr) return;
+  volatile uint32_t* word = reinterpret_cast<volatile uint32_t*>(status);
+  *word = *word | kStatusBadArgs;
 }
 
 struct Seq {

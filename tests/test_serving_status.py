@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from kernel_opt_agent_b200 import _lib
+from kernel_opt_agent_b200 import _kv8, _lib
 from kernel_opt_agent_b200 import kv8_append as append
 from kernel_opt_agent_b200 import kv8_attention as attention
 
@@ -57,3 +57,23 @@ def test_an_explicit_look_finds_errors_without_checks(cuda_device, monkeypatch):
         with pytest.raises(_lib.TokmixDeviceError, match="argument"):
             append.check_device_status(dev)
         append.check_device_status(dev)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("before", [0, 0x1, 0x6])
+def test_a_status_word_keeps_its_other_bits(cuda_device, before):
+    """One device word for several kinds of call: a bad table entry adds its bit to those that are there."""
+    dev, lib = cuda_device, _lib.load()
+    cache = append.make_cache(2, 1, 16, 64, device=dev)
+    x, out = torch.ones(1, 1, 1, 64, dtype=torch.bfloat16, device=dev), torch.empty(1, 1, 1, 64, dtype=torch.bfloat16, device=dev)
+    ws = torch.empty(lib.tokmix_kv8_attention_workspace_bytes(1, 1, 1, 64), dtype=torch.uint8, device=dev)
+    seq = _i32([1], dev)  # (the description holds addresses only)
+    for table, want in ((_i32([[7, 0]], dev), before | 8), (_i32([[1, 0]], dev), before)):
+        desc = _kv8.cache_args(x, *cache, table, seq, None)
+        st, stream = x.stride()[:3], _lib.stream_ptr(dev)
+        for call in (lambda w: lib.tokmix_kv8_append(x.data_ptr(), *st, x.data_ptr(), *st, 1, 0, _kv8.byref(desc), w, stream),
+                     lambda w: lib.tokmix_kv8_attention(x.data_ptr(), *st, out.data_ptr(), None, 1, 1, 0, 0.125, _kv8.byref(desc),
+                                                        ws.data_ptr(), ws.numel(), w, stream)):
+            word = torch.tensor([before], dtype=torch.int32, device=dev)
+            assert call(word.data_ptr()) == 0
+            assert int(word) == want
