@@ -104,8 +104,11 @@ def token_strides(x: torch.Tensor) -> tuple[torch.Tensor, tuple[int, int, int]]:
     (a slice of a packed QKV tensor, say), else a contiguous copy and the copy's."""
     sb, st, sh, sd = x.stride()
     if sd != 1 or (sb | st | sh) % 8 or x.data_ptr() % 16:
-        x = x.contiguous() if not x.is_contiguous() else x.clone()
-        sb, st, sh, _ = x.stride()
+        # nothing is read along a dimension of size 1, whatever its stride
+        sb, st, sh = (s if n > 1 else x.shape[3] for s, n in zip((sb, st, sh), x.shape))
+        if sd != 1 or (sb | st | sh) % 8 or x.data_ptr() % 16:
+            x = x.clone(memory_format=torch.contiguous_format)
+            sb, st, sh, _ = x.stride()
     return x, (sb, st, sh)
 
 

@@ -1,0 +1,45 @@
+"""Views that the 8-bit cache's calls take: rows of packed tensors, buffers shared with the output."""
+
+import pytest
+import torch
+
+from kernel_opt_agent_b200 import _kv8
+from kernel_opt_agent_b200 import kv8_append as append
+from kernel_opt_agent_b200 import kv8_attention as attention
+
+
+def _i32(v, dev):
+    return torch.tensor(v, dtype=torch.int32, device=dev)
+
+
+# ------------------------------------------------------------------------------------ views
+def _packed_slices(dev="cpu"):
+    """One token (or head) of a packed tensor whose rows are no multiple of 8 long: the strides of dimensions of size 1
+    are odd, though nothing is read along them."""
+    flat = torch.arange(4 * 1 * 2 * 67, device=dev).to(torch.bfloat16)
+    return [flat.view(4, 1, 2, 67)[:1, :, :1, :64], flat.view(8, 67)[1:2].as_strided((1, 1, 1, 64), (67, 67, 67, 1), 0),
+            flat.view(8, 67)[:1].as_strided((1, 1, 2, 64), (131, 131, 64, 1), 0), flat[1:].view(-1)[:128].view(1, 1, 2, 64)]
+
+
+def test_token_strides_of_single_rows():
+    for x in _packed_slices():
+        y, strides = _kv8.token_strides(x)
+        assert torch.equal(x, y) and y.data_ptr() % 16 == 0
+        assert all(s % 8 == 0 and s >= 0 for s in strides), (x.stride(), strides)
+    both = torch.zeros(2, 3, 12, 64, dtype=torch.bfloat16)[:, :, 4:8]  # read in place
+    assert _kv8.token_strides(both)[0] is both and _kv8.token_strides(both)[1] == both.stride()[:3]
+
+
+@pytest.mark.gpu
+def test_single_rows_of_packed_tensors(cuda_device):
+    dev = cuda_device
+    table, seq = _i32([[1, 0]], dev), _i32([1], dev)
+    for x in _packed_slices(dev):
+        hkv = x.shape[2]
+        a, b = (append.make_cache(2, hkv, 16, 64, device=dev) for _ in range(2))
+        append.kernel_fn(x, x, *a, table, seq)
+        append.kernel_fn(x.flatten().clone().view(x.shape), x.flatten().clone().view(x.shape), *b, table, seq)
+        assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(a, b))
+        got = attention.kernel_fn(x, *a, table, seq)
+        assert torch.equal(got, attention.kernel_fn(x.flatten().clone().view(x.shape), *a, table, seq))
+    append.check_device_status(dev)
