@@ -44,6 +44,12 @@ def _workspace_bytes(tokens: int, hq: int, hkv: int, d: int, batch: int, max_pag
         return _lib.load().tokmix_kv8_attention_workspace_bytes_for(tokens, hq, hkv, d, batch, max_pages, page)
 
 
+def _overlap(out: torch.Tensor, q: torch.Tensor) -> bool:
+    """Whether out (contiguous) reaches into the memory between q's first and last element."""
+    last = sum((n - 1) * s for n, s in zip(q.shape, q.stride()))
+    return q.numel() > 0 and out.data_ptr() < q.data_ptr() + 2 * (last + 1) and q.data_ptr() < out.data_ptr() + 2 * out.numel()
+
+
 def kernel_fn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
               v_scale: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
               new_lens: torch.Tensor | None = None, sm_scale: float | None = None, *,
@@ -62,7 +68,7 @@ def kernel_fn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_s
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
         raise ValueError("out must be a contiguous tensor shaped and typed like q")
-    elif out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
+    elif out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr() and _overlap(out, q):
         raise ValueError("out must not share memory with q")
     lse = torch.empty((batch, tokens, hq), dtype=torch.float32, device=dev) if return_lse else None
     q, qs = _kv8.token_strides(q)

@@ -43,3 +43,38 @@ def test_single_rows_of_packed_tensors(cuda_device):
         got = attention.kernel_fn(x, *a, table, seq)
         assert torch.equal(got, attention.kernel_fn(x.flatten().clone().view(x.shape), *a, table, seq))
     append.check_device_status(dev)
+
+
+# ------------------------------------------------------------------------------------ the output's memory
+def test_overlap_of_output_and_queries():
+    buf = torch.zeros(4 * 512, dtype=torch.bfloat16)
+    q = buf[:512].view(1, 2, 4, 64)
+    for at, want in ((0, True), (8, True), (504, True), (512, False), (1024, False)):
+        assert attention._overlap(buf[at:at + 512].view(q.shape), q) == want
+        assert attention._overlap(q, buf[at:at + 512].view(q.shape)) == want
+    packed = torch.zeros(2, 2, 12, 64, dtype=torch.bfloat16)[:, :, 4:8]
+    assert not attention._overlap(buf[:1024].view(2, 2, 4, 64), packed) and attention._overlap(packed[:1, :1], packed)
+
+
+@pytest.mark.gpu
+def test_queries_and_output_in_one_buffer(cuda_device):
+    """A step's buffer that holds both: taken where they are apart, refused where they overlap."""
+    dev, shape = cuda_device, (2, 1, 4, 64)
+    gen = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(2, 9, 2, 64, generator=gen).to(torch.bfloat16).to(dev) for _ in range(2))
+    cache, table, seq = append.make_cache(2, 2, 16, 64, device=dev), _i32([[1], [0]], dev), _i32([9, 9], dev)
+    append.kernel_fn(k, v, *cache, table, seq)
+    q = torch.randn(shape, generator=gen).to(torch.bfloat16).to(dev)
+    want = attention.kernel_fn(q, *cache, table, seq)
+    n = q.numel()
+    buf = torch.full((3 * n,), 7.0, dtype=torch.bfloat16, device=dev)
+    for a, b in ((0, n), (2 * n, n), (0, 2 * n)):
+        buf.fill_(7.0)
+        one, two = buf[a:a + n].view(shape), buf[b:b + n].view(shape)
+        one.copy_(q)
+        assert attention.kernel_fn(one, *cache, table, seq, out=two) is two
+        assert torch.equal(two, want) and torch.equal(one, q) and int((buf == 7).sum()) >= n
+    for b in (0, 64, n - 64):
+        with pytest.raises(ValueError, match="share"):
+            attention.kernel_fn(buf[:n].view(shape), *cache, table, seq, out=buf[b:b + n].view(shape))
+    append.check_device_status(dev)
