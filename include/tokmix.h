@@ -321,7 +321,8 @@ typedef struct tokmix_kv8_cache {
  * for e4m3, 127 for int8); values are rounded to nearest, ties to even; where new tokens raise the scale,
  * the page's older tokens are rounded again to it.  A page whose first slot is written starts afresh.  A
  * value that is not finite makes its block's scale NaN (its call's bytes there are zeros) until the page is started afresh.  A call
- * must append to each page for one sequence only, at one place of its table.
+ * must append to each page for one sequence only, at one place of its table, and k and v (k_scale and v_scale) must
+ * not be the same memory.
  * Lengths that do not fit the call or the table, and table entries outside the pool, write nothing for
  * that sequence (page) and set TOKMIX_DEV_BAD_ARGS in *status (device memory or mapped host memory).  The bit is
  * added to what the word holds, not atomically: calls of other kinds that may run at the same time, and a host that

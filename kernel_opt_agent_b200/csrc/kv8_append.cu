@@ -256,6 +256,9 @@ extern "C" int tokmix_kv8_append(const void* k, long long k_batch_stride, long l
   for (const long long st : {k_batch_stride, k_token_stride, k_head_stride, v_batch_stride, v_token_stride, v_head_stride})
     if (st % 8 != 0 || st < 0)
       return fail(TOKMIX_ERR_INVALID_ARGUMENT, "tokmix_kv8_append: strides of k and v must be multiples of 8 elements");
+  // a key's unit and a value's would race for the same tile and scale
+  if (cache->k == cache->v || cache->k_scale == cache->v_scale)
+    return fail(TOKMIX_ERR_INVALID_ARGUMENT, "tokmix_kv8_append: keys and values need a cache and scales each");
   p.k = k;
   p.v = v;
   p.k_sb = k_batch_stride;

@@ -17,9 +17,10 @@ so pages are reused without clearing.  A value that is not finite makes its bloc
 it brings are zeros): the whole block reads as NaN until the page starts afresh.
 
 The caller keeps pages apart: a call appends to each page for one sequence, and at one place of its table (a
-page shared by several sequences is full, or copied first).  Lengths that do not fit the call or the table and table entries
-outside the pool write nothing for that sequence (page) and are reported as ``TokmixDeviceError`` by a
-later call or by ``check_device_status``.
+page shared by several sequences is full, or copied first), and k_cache and v_cache (k_scale and v_scale) are
+not the same memory.  Lengths that do not fit the call or the table and table entries outside the pool write
+nothing for that sequence (page) and are reported as ``TokmixDeviceError`` by a later call or by
+``check_device_status``.
 
 ``kernel_fn`` runs ``tokmix_kv8_append`` (``csrc/kv8_append.cu``), no fallback."""
 

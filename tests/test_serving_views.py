@@ -1,9 +1,11 @@
 """Views that the 8-bit cache's calls take: rows of packed tensors, buffers shared with the output."""
 
+import ctypes
+
 import pytest
 import torch
 
-from kernel_opt_agent_b200 import _kv8
+from kernel_opt_agent_b200 import _kv8, _lib
 from kernel_opt_agent_b200 import kv8_append as append
 from kernel_opt_agent_b200 import kv8_attention as attention
 
@@ -78,3 +80,20 @@ def test_queries_and_output_in_one_buffer(cuda_device):
         with pytest.raises(ValueError, match="share"):
             attention.kernel_fn(buf[:n].view(shape), *cache, table, seq, out=buf[b:b + n].view(shape))
     append.check_device_status(dev)
+
+
+# ------------------------------------------------------------------------------------ one cache for two
+@pytest.mark.parametrize("same", ["k", "k_scale"])
+def test_append_refuses_one_cache_for_keys_and_values(same):
+    """The kernel would write both to the same bytes at once (refused on the host: no GPU is touched)."""
+    sizes = dict(k_page_stride=2048, k_head_stride=1024, v_page_stride=2048, v_head_stride=1024, block_table=4096, table_stride=4,
+                 seq_lens=4096, new_lens=None, num_pages=8, page_size=16, heads_kv=2, head_dim=64, dtype=_lib.DTYPE_E4M3, batch=1,
+                 max_pages=4)
+    ptrs = dict(k=4096, v=8192, k_scale=12288, v_scale=16384)
+    ptrs["v" if same == "k" else "v_scale"] = ptrs[same]
+    cache = _lib.Kv8Cache(*ptrs.values(), *sizes.values())
+    x = ctypes.c_void_p(4096)
+    rc = _lib.load().tokmix_kv8_append(x, 128, 128, 64, x, 128, 128, 64, 1, 0, ctypes.byref(cache), None, None)
+    assert rc == _lib.TOKMIX_ERR_INVALID_ARGUMENT and "each" in _lib.last_error()
+    none = _lib.load().tokmix_kv8_append(x, 128, 128, 64, x, 128, 128, 64, 0, 0, ctypes.byref(cache), None, None)
+    assert none == _lib.TOKMIX_OK
