@@ -52,19 +52,19 @@ def kernel_fn(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tens
     rows = x.numel() // n
     if rows > MAX_ROWS:
         raise ValueError(f"at most {MAX_ROWS} rows (got {rows})")
-    x, w = _lib.aligned(x), _lib.aligned(weight)
+    given, x, w = x, _lib.aligned(x), _lib.aligned(weight)
     if inplace and 0 < abs(x.data_ptr() - residual.data_ptr()) < 2 * rows * n:
         raise ValueError("inplace=True: x must be the residual itself or share no memory with it")
     y = torch.empty_like(x, dtype=torch.float8_e4m3fn)
     y_scale = _lib.empty((n // group, rows) if group else (rows,), torch.float32, dev)
     if residual is None:
-        res, res_out = None, x
+        res_out, res_ptr, out_ptr = given, None, None
     else:
         res = residual if inplace else _lib.aligned(residual)
         res_out = res if inplace else torch.empty_like(x)
-    rc = _lib.call_on(dev, _lib.load().tokmix_add_rms_norm_quant,
-                      x.data_ptr(), res.data_ptr() if res is not None else None, w.data_ptr(), res_out.data_ptr(),
-                      y.data_ptr(), y_scale.data_ptr(), rows, n, group or 0, _DTYPES[dtype], eps, _lib.stream_ptr(dev))
+        res_ptr, out_ptr = res.data_ptr(), res_out.data_ptr()
+    rc = _lib.call_on(dev, _lib.load().tokmix_add_rms_norm_quant, x.data_ptr(), res_ptr, w.data_ptr(), out_ptr, y.data_ptr(),
+                      y_scale.data_ptr(), rows, n, group or 0, _DTYPES[dtype], eps, _lib.stream_ptr(dev))
     if rc:
         _lib.check(rc, "add_rms_norm_quant")
     return y, y_scale, res_out
