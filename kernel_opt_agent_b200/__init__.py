@@ -9,8 +9,8 @@ Beside them, the serving step's operators, modules of the same contract:
   * :mod:`kernel_opt_agent_b200.kv8_append`         -- new keys/values into a paged 8-bit cache
   * :mod:`kernel_opt_agent_b200.kv8_attention`      -- decode attention over that cache
 
-All call the hand-written tcgen05/TMA kernels in ``libtokmix.so`` through the C ABI in
-``include/tokmix.h``.  ``kernel_configs`` and ``references`` mirror the reference's registry and
+All call the hand-written kernels in ``libtokmix.so`` (the prefill mixers on tcgen05 and TMA, the serving step on
+``mma.sync``, ``cp.async`` and plain loads) through the C ABI in ``include/tokmix.h``.  ``kernel_configs`` and ``references`` mirror the reference's registry and
 checkers; ``sharding`` holds the multi-GPU work partition.
 """
 

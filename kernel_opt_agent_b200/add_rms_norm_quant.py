@@ -13,7 +13,8 @@ out (the first layer; residual_out is then x itself).
 
 ``group`` columns share a scale: 128 or 32 (N a multiple of it; y_scale is [N / group, M], M the number
 of rows, as ``swiglu_input_quant`` lays its scales out) or None, one scale per row (y_scale [M]).
-y_fp8 is e4m3, shaped like x; the largest magnitude of a group is held as 448.  ``inplace=True`` writes
+y_fp8 is e4m3, shaped like x; the largest magnitude of a group is held as 448.  Scales are fp32 and no powers of two in any
+grouping: they go to products that scale partial sums in fp32, not to block-scaled ones that want e8m0 scales.  ``inplace=True`` writes
 residual_out over ``residual``, so that a decode loop keeps one residual buffer (x may be the residual
 itself; it must not overlap it otherwise).
 

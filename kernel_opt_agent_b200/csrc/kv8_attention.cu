@@ -4,16 +4,19 @@
 //   s_j = sm_scale (q . k8_j) ks_j,   o = sum_j e^{s_j} vs_j v8_j / sum_j e^{s_j}
 // with k8, v8 the cached bytes' values and ks, vs the scales of token j's (page, head).
 //
-// Bound: HBM, the cache's bytes (4 heads_q / heads_kv flops per byte).  So the rows that read the same keys
-// and values -- the tokens and heads of a group -- share one pass over them, and the work is cut along the
-// sequences so that every SM streams until the end:
+// Bound: HBM, the cache's bytes (4 heads_q / heads_kv flops per byte).  So up to 16 rows that read the same keys
+// and values -- the tokens and heads of a group -- share one pass over them (more rows are units of their own, each with
+// its pass: 20 sequences of up to 9000 tokens, Hq 32 Hkv 4 D 128, 16 rows of two queries 35 us, 32 of four 61, 128 of
+// sixteen 212), and the work is cut along the sequences so that every SM streams until the end:
 //   * a unit is (sequence, key/value head, tile of 8 or 16 rows); its tokens come in tiles of 16 (D 256), 32 or
 //     64 (D 64, 8 rows).  All units' tiles laid end to end are cut into equal ranges, one per CTA of a grid that fills the GPU once;
 //     lengths are read on the device, so the launch does not depend on them.  A unit inside one range is written
 //     directly; a unit cut by range borders leaves normalised partial rows with their maximum and sum, and a second
 //     kernel joins them in the order of the CTAs (launched to start as the first drains).  Results do not depend on
 //     timing.  Where the table has room for short sequences only, each unit has a CTA of its own instead and the
-//     second kernel falls away (one sequence of 129 tokens: 6.7 us; 2400 units of up to 1024: 89 -> 80).
+//     second kernel falls away (one sequence of 129 tokens: 6.5 to 7.1 us; 2400 units of up to 1024: 89 -> 80).  The same
+//     sequences with a wide table pay for plan and join (129 tokens 9.7 us; 16 x 1031, four queries 8.8 -> 12), the more the
+//     larger the batch, since every CTA forms the plan (8192 sequences of 512, Hkv 1, D 128: 210 -> 430).
 //   * a CTA's 4, 8 or 12 warps take its range's tiles in turn, each with a ring of its own in shared memory (cp.async,
 //     192 KB per SM in flight) that is filled ahead over unit borders, so that a change of unit costs no memory latency.  Only changes of unit have barriers; there is no wait on another CTA.
 //   * scores S^T = K Q^T and outputs O^T = V^T P^T are m16n8k16 products with the cache's bytes as the 16-row
@@ -21,12 +24,13 @@
 //     lane's 16 bytes of a key are its fragments as they lie.  Accumulation is fp32.  tcgen05 products would take
 //     128 rows of bytes for 8 to 16 query rows and need the bytes in one 8-bit type with the weights, which 8 bits do
 //     not hold; the e4m3 form of this product runs on the same pipe with the same widening inside (it measured 5 % slower).
-// What it measured (B200, device time): Hq 32 Hkv 8 D 128, 64 sequences of 1024 to 4096 tokens 61 us, 5.5 TB/s (the same
+// What it measured (B200, device time): Hq 32 Hkv 8 D 128, 64 sequences of 1024 to 4096 tokens 61.5 us, 5.5 TB/s (the same
 // copies without the products 59 us at a time when the whole took 64); Hq 16 Hkv 2 D 256, 16 sequences of up to 65536 tokens
-// 110 to 112 us, 5.8 TB/s; one of 65536 21 us.  The SMs' shares of the bandwidth differ (equal ranges end after 86 to 110 us
-// of those), but short ranges drawn as SMs got done cost more in changes of unit than they evened out.  16 rows and D >= 128
-// are bound by eight warps' latency instead: 20 sequences of up to 9000 tokens, Hq 32 Hkv 4, two queries, 33 us, 3.0 TB/s
-// (twelve warps of 168 registers 39 to 43).
+// 112 to 114 us, 5.7 TB/s; one of 65536 20.5 to 20.8 us.  The SMs' shares of the bandwidth differ (equal ranges ended after
+// 86 to 110 us of those), but short ranges drawn as SMs got done cost more in changes of unit than they evened out.  16 rows and
+// D >= 128 are bound by eight warps' latency instead: 20 sequences of up to 9000 tokens, Hq 32 Hkv 4, two queries, 35 us,
+// 2.9 TB/s.  The figures beside the choices below (tiles, warps, layouts, joins) were taken before each row had its own
+// reference (last paragraph), which adds the same to both sides.
 //
 // Number formats.  q rows enter fp16 after scaling by a power of two that brings their largest element to
 // [2^14, 2^15): exact for elements down to 2^-28 of it (bf16 has 8 bits, fp16 11).  A weight enters with its scale, as
@@ -57,7 +61,8 @@ struct Shape {
   static constexpr int kRows = 8 * NT;        // query rows per unit
   static constexpr int kQStride = D + 8;      // halves between rows of q in shared memory (conflict-free 16-byte reads)
   static constexpr int kStageBytes = 2 * kTok * D;              // a tile's keys and values
-  // 168 or 255 registers a thread: 16 rows of D 64 fit 168 (64 sequences of up to 2000 tokens 44.9 -> 41.9 us), of D 128 do not
+  // 168 or 255 registers a thread: 16 rows of D 64 fit 168 (64 sequences of up to 2000 tokens 44.9 -> 41.9 us), of D 128 do
+  // not (20 sequences of up to 9000 tokens, two queries: 33 us, with twelve warps 39 to 43)
   static constexpr int kWarpsPerSm = NT == 1 || D == 64 ? 12 : 8;
   static constexpr int kStages = 196608 / kWarpsPerSm / kStageBytes;  // 192 KB of tiles per SM
   __host__ __device__ static constexpr int smem_bytes(int warps) { return warps * kStages * (kStageBytes + 8 * kMt) + kRows * kQStride * 2; }

@@ -11,14 +11,16 @@ step, a few when drafted tokens are verified), already appended to the cache.  R
 position seq_lens[b] - new_lens[b] + i and sees the positions up to its own; query head h reads key/value
 head h // (Hq // Hkv); default scale 1 / sqrt(D).  out [B, T, Hq, D] in q's type, on the values the cache stands for:
 maxima, sums and accumulation in fp32; q (scaled by a power of two per row) and each softmax weight times its
-value scale enter the products as fp16, where what is under 2^-39 of a row's largest such product is lost.  Rows that see nothing (padding behind new_lens[b], empty sequences) are
-zero, their lse -inf.  ``lse`` [B, T, Hq] fp32 is the logarithm of the row's sum of exponentials, for
-joining with attention over other tokens.  q may be a slice of a packed tensor.  The cache's layout and the
+value scale enter the products as fp16, where what is under 2^-39 of a row's largest such product is lost.
+Rows that see nothing (padding behind new_lens[b], empty sequences) are zero, their lse -inf.  ``lse``
+[B, T, Hq] fp32 is the logarithm of the row's sum of exponentials, for joining with attention over other
+tokens.  q may be a slice of a packed tensor.  The cache's layout and the
 sequence tensors: ``_kv8``.
 
 Lengths that do not fit the call or the table make the sequence's rows NaN, a table entry outside the pool
-the rows that see it; a later call or ``check_device_status`` reports them as ``TokmixDeviceError``.  Prompts
-go through ``flash_attention_2`` (their keys and values enter the cache with ``kv8_append``).
+the rows that see it; a later call or ``check_device_status`` reports them as ``TokmixDeviceError``.  A prompt
+goes through ``flash_attention_2`` (bf16, its own tokens only) and its keys and values into the cache with
+``kv8_append``; a chunk of more than 16 tokens behind a cached prefix has no attention here.
 
 ``kernel_fn`` runs ``tokmix_kv8_attention`` (``csrc/kv8_attention.cu``), no fallback."""
 
