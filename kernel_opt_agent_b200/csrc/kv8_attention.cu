@@ -50,6 +50,9 @@ namespace kv8 {
 constexpr int kMaxTokens = 16;
 constexpr int kMaxBatch = 8192;  // the plan keeps batch + 1 words in shared memory
 constexpr float kShift = 14.0f;  // weights are held times 2^14
+// a little under 126, so that 2^-kRise stays a normal number when the score it is added to rounds the sum up; a weight times a
+// scale of up to 2^127.9 is then within fp16
+constexpr float kRise = 125.9375f;
 constexpr float kSpan = 112.0f;  // a row's accumulators are held times 2^112 / (its largest weight) at most
 constexpr int kJoinThreads = 256;
 constexpr int kMaxCtas = 512;  // at most 3 per SM
@@ -512,7 +515,7 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
     // this lane's rows (columns of the products): 8 nt + 2 cq + {0, 1}
     // m is the largest score s_j so far, the sum's reference; mv the largest s_j + log2 vs_j, the accumulators': a block counts by
     // its softmax weight times its scale, so one of little weight cannot take the others' bits (kept within m - kSpan and
-    // m + 126: the factor between the two is a normal number)
+    // m + kRise: the factor between the two is a normal number)
     float factor[NT][2], m[NT][2], mv[NT][2], l[NT][2];
     int lim[NT][2];
     int min_lim = s.end;
@@ -633,7 +636,7 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
             for (int o = 4; o < 32; o <<= 1) topv[nt][e] = fmaxf(topv[nt][e], __shfl_xor_sync(0xffffffffu, topv[nt][e], o));
           }
           top[nt][e] = fmaxf(top[nt][e], m[nt][e]);
-          topv[nt][e] = fminf(fmaxf(fmaxf(topv[nt][e], mv[nt][e]), top[nt][e] - kSpan), top[nt][e] + 126.0f);
+          topv[nt][e] = fminf(fmaxf(fmaxf(topv[nt][e], mv[nt][e]), top[nt][e] - kSpan), top[nt][e] + kRise);
           grew |= top[nt][e] > m[nt][e] || topv[nt][e] > mv[nt][e];
           ref[nt][e] = top[nt][e] == -INFINITY ? 0.0f : top[nt][e];  // a row that has seen nothing yet
           down[nt][e] = ex2(ref[nt][e] - (topv[nt][e] == -INFINITY ? 0.0f : topv[nt][e]));

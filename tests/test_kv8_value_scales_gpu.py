@@ -157,3 +157,20 @@ def test_scales_of_every_kind(cuda_device, room):
     for b in (0, 2, 3, 4):
         s = slice(b, b + 1)
         _assert_near(out[s], q[s], cache[:4] + [cache[4][s]], seq[s], new[s])
+
+
+@pytest.mark.parametrize("room", [0, 4096])
+def test_scales_at_the_end_of_the_range(cuda_device, room):
+    """Bytes -1, 0 and 1 at scales up to 1.5 * 2^127 beside ordinary ones."""
+    dev, page, d, lens = cuda_device, 16, 64, [100, 300, 40]
+    cache = _wide(_filled_cache(78, lens, 1, d, page, INT8, dev), room)
+    cache[1].copy_(cache[1].sign())
+    q = _queries(78, 3, 1, 4, d, torch.bfloat16, dev)
+    rng = np.random.default_rng(6)
+    for b, kinds in enumerate(([2.0 ** 126, 1.0], [1.5 * 2.0 ** 127, 2.0 ** -100, 2.0 ** 20], [2.0 ** 127])):
+        for p in range(-(-lens[b] // page)):
+            cache[3][int(cache[4][b, p])] = float(rng.choice(kinds))
+    seq, new = _i32(lens, dev), _i32([1] * 3, dev)
+    out = attention.kernel_fn(q, *cache, seq, new)
+    assert bool(out.isfinite().all())
+    _assert_near(out, q, cache, seq, new)
