@@ -325,8 +325,8 @@ typedef struct tokmix_kv8_cache {
  * not be the same memory.
  * Lengths that do not fit the call or the table, and table entries outside the pool, write nothing for
  * that sequence (page) and set TOKMIX_DEV_BAD_ARGS in *status (device memory or mapped host memory).  The bit is
- * added to what the word holds, not atomically: calls of other kinds that may run at the same time, and a host that
- * clears the word then, need a word of their own. */
+ * added to what the word holds, as the other entry points do; in mapped host memory that is not atomic towards a host that
+ * changes the word at the same time. */
 int tokmix_kv8_append(const void* k, long long k_batch_stride, long long k_token_stride, long long k_head_stride,
                       const void* v, long long v_batch_stride, long long v_token_stride, long long v_head_stride,
                       int tokens, int io_dtype, const tokmix_kv8_cache* cache, uint32_t* status, void* stream);

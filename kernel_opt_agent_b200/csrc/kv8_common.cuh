@@ -40,12 +40,10 @@ struct View {
 // Checks a cache description on the host and makes the device view; head_dim is returned for dispatch.
 int make_view(const char* who, const tokmix_kv8_cache* c, View& out);
 
-// Sets the bit and keeps the word's others.  The word may be device memory or mapped host memory, where an atomic is not to be
-// relied on: a load and a store, which calls of this file may do at once (they set the same bit).
+// Sets the bit and keeps the word's others.  The word may be device memory or mapped host memory (where the operation is atomic
+// for this device's kernels, not towards the host).
 __device__ __forceinline__ void report_bad(uint32_t* status) {
-  if (status == nullptr) return;
-  volatile uint32_t* word = reinterpret_cast<volatile uint32_t*>(status);
-  *word = *word | kStatusBadArgs;
+  if (status != nullptr) atomicOr(status, kStatusBadArgs);
 }
 
 struct Seq {
