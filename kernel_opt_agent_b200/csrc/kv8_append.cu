@@ -134,11 +134,15 @@ __global__ void __launch_bounds__(GT == 32 ? 256 : GT) append_kernel(const Appen
     __syncwarp();  // every lane has read the old scale
   }
   float s_new = fmaxf(s_old, pow2_scale<E4M3>(Half16<T>::widen(amax)));
-  if (amax >= Half16<T>::kInf || isnan(s_old)) s_new = __uint_as_float(0x7fc00000u);  // the block reads as NaN from here on
+  if (amax >= Half16<T>::kInf || isnan(s_old)) {  // the block reads as NaN from here on
+    s_new = __uint_as_float(0x7fc00000u);
+    // the scale alone marks it: a NaN byte would reach rows that do not see it (0 * NaN)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) x[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
   if (lane == 0) *scale = s_new;
 
-  const float inv = 1.0f / s_new;  // exact
-  const bool marked = isnan(s_new);  // zeros then: the scale alone marks the block, a NaN byte would reach rows that do not see it (0 * NaN)
+  const float inv = isnan(s_new) ? 0.0f : 1.0f / s_new;  // exact
   uint8_t* dst = tile + ((lo - page0) << p.d_shift);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -153,8 +157,7 @@ __global__ void __launch_bounds__(GT == 32 ? 256 : GT) append_kernel(const Appen
         f[2 * e + 1] = t.y * inv;
       }
       *reinterpret_cast<uint2*>(dst + (static_cast<size_t>(vi) << 3)) =
-          marked ? make_uint2(0u, 0u)
-                 : make_uint2(float4_to_bytes<E4M3>(f[0], f[1], f[2], f[3]), float4_to_bytes<E4M3>(f[4], f[5], f[6], f[7]));
+          make_uint2(float4_to_bytes<E4M3>(f[0], f[1], f[2], f[3]), float4_to_bytes<E4M3>(f[4], f[5], f[6], f[7]));
     }
   }
   if (has_old && s_old < s_new) {  // (false for a NaN scale)
