@@ -323,7 +323,8 @@ __global__ void __launch_bounds__(32 * W, Shape<D, NT>::kWarpsPerSm / W) attn_ke
   uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + S::smem_bytes(W));
   __shared__ float row_factor[ROWS], row_top[ROWS], row_sum[ROWS], row_up[ROWS], warp_m[W][ROWS], warp_l[W][ROWS], warp_mv[W][ROWS];
   __shared__ int warp_at[W];  // where in `smem` a warp's partial rows lie
-  __shared__ int met_bad_page[W];  // each warp's lane 0 alone; reported at the end (beside the loads: 400 sequences of up to 640, Hkv 8, D 128: 78.2 -> 79.3 us)
+  // each warp's lane 0 alone; reported at the end (beside the loads: 400 sequences of up to 640, Hkv 8, D 128, 78.2 -> 79.3 us)
+  __shared__ int met_bad_page[W];
   __shared__ uint32_t scratch[W];
 
   const View& c = p.c;
