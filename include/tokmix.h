@@ -71,6 +71,27 @@ int tokmix_fa2_fwd(const void* q, const void* k, const void* v, void* o, int bat
                    int seqlen_q, int seqlen_kv, int head_dim, int layout, int causal, float sm_scale,
                    uint32_t* status, void* stream);
 
+/* The same, and in lse (NULL, or fp32 [batch, heads_q, seqlen_q] in either layout) the natural logarithm of each row's sum of
+ * exponentials, which the backward pass takes. */
+int tokmix_fa2_fwd_lse(const void* q, const void* k, const void* v, void* o, float* lse, int batch, int heads_q,
+                       int heads_kv, int seqlen_q, int seqlen_kv, int head_dim, int layout, int causal, float sm_scale,
+                       uint32_t* status, void* stream);
+
+/* Gradients of the attention forward (the reference has no backward pass).  dout, q, o, dq and k, v, dk, dv as tokmix_fa2_fwd's
+ * o, q and k (bf16, contiguous, 16-byte aligned); lse from tokmix_fa2_fwd_lse.  With P = exp(sm_scale q k^T - lse) under the
+ * mask and delta = sum(dout * o):
+ *   dv = P^T dout,  dS = P * (dout v^T - delta),  dq = sm_scale dS k,  dk = sm_scale dS^T q
+ * P and dS are rounded to bf16 as operands; sums are fp32 (dk and dv over the heads that share a key/value head too), in an order
+ * that sizes alone decide: the same bits every time.  workspace: tokmix_fa2_bwd_workspace_bytes(...) bytes of device memory, 16-byte
+ * aligned, no initialisation, not shared by calls that may overlap.  seqlen_q == 0 gives zeros in dk and dv. */
+int tokmix_fa2_bwd(const void* dout, const void* q, const void* k, const void* v, const void* o, const float* lse,
+                   void* dq, void* dk, void* dv, int batch, int heads_q, int heads_kv, int seqlen_q, int seqlen_kv,
+                   int head_dim, int layout, int causal, float sm_scale, void* workspace, long long workspace_bytes,
+                   uint32_t* status, void* stream);
+
+/* Workspace size of tokmix_fa2_bwd in bytes (-1 for bad arguments). */
+long long tokmix_fa2_bwd_workspace_bytes(int batch, int heads_q, int seqlen_q, int seqlen_kv, int head_dim);
+
 /* Steps before the recurrence that the GDN prefill entry points can do inside their first stage
  * (the `gates` argument; NULL = neither).  The reference takes normalised q, k and ready g, beta
  * (kernels/qwen35moe_gdn_prefill.py:107-136).

@@ -1,0 +1,843 @@
+// fa2_bwd.cu -- gradient of the attention forward (fa2_fwd.cu) for sm_100a (B200).
+//
+// With c = sm_scale and the forward's lse (natural logarithm), for every query head:
+//   P = exp(c q k^T - lse) under the mask,  delta = sum_d do * o  (a row each)
+//   dv = P^T do,   dS = P * (do v^T - delta),   dq = c dS k,   dk = c dS^T q
+// dk and dv are summed over the query heads that share a key/value head.  P is formed again from
+// q, k and lse, so the forward keeps one number per row instead of the S x S matrix.
+//
+// Two launches:
+//   fa2_bwd_prep    delta and lse * log2(e) in rows padded to whole query tiles (padding: +inf, 0,
+//                   so that a padded row's P is 0), the counters below set to 0.
+//   fa2_bwd_kernel  persistent, one CTA per SM.  A unit is a tile of 128 keys of one key/value head: K and V stay in
+//                   shared memory, the tiles of BQ queries of every query head of the group pass by
+//                   (last tile first), and dK and dV grow in TMEM.  Scores are held transposed, keys
+//                   along the 128 TMEM lanes:
+//     S^T  = K Q^T     (SS)            P^T = 2^(c log2e S^T - lse2), bf16, over S^T's own columns
+//     dV  += P^T dO    (A from TMEM)
+//     dP^T = V dO^T    (SS)            dS^T = P^T * (dP^T - delta), bf16, into shared memory
+//     dK  += dS^T Q    (SS)
+//     dQ   = dS K      (SS; A is the same dS^T tile read MN-major)
+//   A query tile's dQ is the sum over key tiles, that is, over CTAs.  It grows in fp32 in global
+//   memory by vector reductions, in the order of the key tiles: the CTA of key tile j waits for the
+//   turn counter of (query tile, warp) to read j, adds, and sets it to j + 1.  So the bits are the
+//   same every time; the first tile stores instead of adding (no clearing pass) and the last adds
+//   from registers, scales, rounds and writes dq (no closing pass).
+//   Units are taken from a counter in order of (batch, key/value head, key tile): a CTA waits only
+//   for units that were taken earlier, by CTAs that are running, so the waits end with any number
+//   of resident CTAs.  Under the causal mask this order is longest first.
+// Roles (512 threads): warps 0-7 softmax (two warpgroups, each half of a tile's query columns; thread =
+// key row), warps 8-11 dQ (TMEM to global), warp 12 TMA and unit counter, warp 13 TMEM owner and MMA
+// issuer, warps 14-15 idle (setmaxnreg works on whole warpgroups).
+// Order of the MMAs:  dP(t) dV(t) S(t+1) dQ(t) dK(t) | dP(t+1) ...: while the softmax warps form P
+// the tensor core has dQ and dK to do, and while they form dS it has dV and the next S.
+//
+// head_dim 256: dV and dK of 128 keys alone would fill TMEM (2 x 256 columns), so a unit takes half
+// of their columns (and of dQ's) and forms S and dP whole; queries come in tiles of 64, which
+// leaves K, V (64 KB each), Q, dO (32 KB each) and dS (16 KB) room in shared memory.  dQ is formed
+// transposed there (dQ^T = K^T dS^T), which keeps M at 128.
+//
+// Every wait is bounded (sm100.cuh): a stuck pipeline sets a status bit and the CTA drains.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "host_common.h"
+#include "sm100.cuh"
+
+namespace tokmix {
+namespace fa2b {
+
+constexpr int kBK = 128;             // keys per unit
+constexpr int kThreads = 512;
+constexpr int kSoftmaxWarps = 8, kDqWarps = 4;
+constexpr int kWarpTma = 12, kWarpMma = 13;
+constexpr int kUnitReaders = 1 + kSoftmaxWarps + kDqWarps;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int D>
+struct Cfg {
+  static constexpr int kBQ = D == 256 ? 64 : 128;      // queries per step
+  static constexpr int kDH = D < 128 ? D : 128;        // columns of dV, dK and dQ that a unit forms
+  static constexpr int kSplit = D / kDH;
+  static constexpr int kNQ = D == 256 ? 1 : 2;         // stages of Q, and of the row statistics
+  static constexpr int kNDO = D == 64 ? 2 : 1;         // stages of dO
+  static constexpr bool kAhead = kNQ > 1;              // S(t+1) before dQ(t): needs a second Q stage
+  static constexpr bool kAlias = D == 128;             // dQ in dP's columns
+  static constexpr bool kTransDq = D == 256;           // dQ^T: lanes are columns of dq, columns are queries
+  static constexpr int kDqCols = kTransDq ? kBQ : kDH; // TMEM columns of dQ
+  static constexpr int kHalfQ = kBQ / 2;               // query columns of a softmax warpgroup
+  static constexpr uint32_t kColS = 0;
+  static constexpr uint32_t kColDp = kBQ;
+  static constexpr uint32_t kColDq = kAlias ? kColDp : 2 * kBQ;
+  static constexpr uint32_t kColDv = kAlias ? 2 * kBQ : kColDq + kDqCols;
+  static constexpr uint32_t kColDk = kColDv + kDH;
+  static_assert(kColDk + kDH <= 512, "TMEM columns");
+  static constexpr int kKBox = kBK * 128;              // 128 keys x 64 columns
+  static constexpr int kQBox = kBQ * 128;              // kBQ queries x 64 columns
+  static constexpr int kKBytes = (D / 64) * kKBox;
+  static constexpr int kQBytes = (D / 64) * kQBox;
+  static constexpr int kDsBytes = kBK * kBQ * 2;       // boxes of 128 keys x 64 queries
+  static constexpr int kStatBytes = 2 * kBQ * 4;       // lse2 and delta of a query tile
+  static constexpr int kK = 0;
+  static constexpr int kV = kK + kKBytes;
+  static constexpr int kQ = kV + kKBytes;
+  static constexpr int kDO = kQ + kNQ * kQBytes;
+  static constexpr int kDs = kDO + kNDO * kQBytes;
+  static constexpr int kStat = kDs + kDsBytes;
+  static constexpr int kBytes = kStat + kNQ * kStatBytes;
+  static_assert(kBytes + 1024 + 512 <= 227 * 1024, "shared memory");
+};
+
+struct Params {
+  __nv_bfloat16 *dq, *dk, *dv;
+  long long q_sb, q_sh, q_ss;        // element strides of q, o, do, dq (batch, head, row)
+  long long k_sb, k_sh, k_ss;        // and of k, v, dk, dv
+  const float* stats;                // [batch * hq][nq][lse2, delta][kBQ]
+  float* acc;                        // [batch * hq][nq][split][kDqCols / 4][128][4]
+  uint32_t* turns;                   // [batch * hq][nq][split][4]
+  uint32_t* ticket;
+  int batch, hq, hkv, group, sq, skv, nq, nk;
+  int units;
+  int causal;
+  float scale, scale_log2;
+  uint32_t* status;
+};
+
+// One unit: key tile j of (b, kvh), column half `half`; its steps visit, for each query head of the
+// group, the query tiles nq-1 .. i_min.
+struct Unit {
+  int b, kvh, j, half, i_min, per_head, steps;
+};
+
+template <int D>
+__device__ __forceinline__ Unit decode_unit(const Params& p, int u) {
+  using C = Cfg<D>;
+  Unit x;
+  x.half = u % C::kSplit;
+  u /= C::kSplit;
+  x.j = u % p.nk;
+  u /= p.nk;
+  x.kvh = u % p.hkv;
+  x.b = u / p.hkv;
+  x.i_min = p.causal ? x.j * (kBK / C::kBQ) : 0;
+  x.per_head = max(0, p.nq - x.i_min);
+  x.steps = x.per_head * p.group;
+  return x;
+}
+
+// number of key tiles that add to query tile i
+template <int D>
+__device__ __forceinline__ int contributors(const Params& p, int i) {
+  if (!p.causal) return p.nk;
+  return min(p.nk, (min((i + 1) * Cfg<D>::kBQ, p.sq) - 1) / kBK + 1);
+}
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+__device__ __forceinline__ void red_add_v4(float* dst, float a, float b, float c, float d) {
+  asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(dst), "f"(a), "f"(b), "f"(c), "f"(d)
+               : "memory");
+}
+
+// Whole warp: waits (bounded) until the turn counter reads `want`; lane 0 polls.
+__device__ __forceinline__ bool wait_turn(const uint32_t* turn, uint32_t want, uint32_t* status) {
+  bool ok = true;
+  if (lane_id() == 0) {
+    const unsigned long long t0 = global_timer_ns();
+    while (true) {
+      uint32_t v;
+      asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(turn) : "memory");
+      if (v == want) break;
+      if (cta_abort_flag() != 0u) { ok = false; break; }
+      if (global_timer_ns() - t0 > kWaitTimeoutNs) {
+        record_status(status, kDevTimeoutPipe);
+        cta_abort_flag() = 1u;
+        ok = false;
+        break;
+      }
+      __nanosleep(64);
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[N]) {
+  static_assert(N == 32 || N == 64 || N == 128, "columns");
+  if constexpr (N == 32) {
+    tmem_ld32(addr, r);
+  } else if constexpr (N == 64) {
+    tmem_ld64(addr, r);
+  } else {
+    tmem_ld64(addr, *reinterpret_cast<uint32_t(*)[64]>(&r[0]));
+    tmem_ld64(addr + 64, *reinterpret_cast<uint32_t(*)[64]>(&r[64]));
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    fa2_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
+                   const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                   const Params p) {
+  using C = Cfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t bar_unit_full[2], bar_unit_empty[2], bar_kv_full, bar_kv_empty, bar_q_full[2], bar_q_empty[2],
+      bar_do_full[2], bar_do_empty[2], bar_s, bar_p, bar_dp, bar_ds, bar_dq, bar_dqfree, bar_acc, bar_accfree, bar_drain;
+  __shared__ int unit_ring[2];
+  __shared__ uint32_t tmem_base_shared;
+
+  const int warp = warp_id();
+  const int lane = lane_id();
+
+  if (threadIdx.x == 0) {
+    cta_abort_flag() = 0u;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar_unit_full[i], 1);
+      mbar_init(&bar_unit_empty[i], kUnitReaders);
+      mbar_init(&bar_q_full[i], 1);
+      mbar_init(&bar_q_empty[i], 1);
+      mbar_init(&bar_do_full[i], 1);
+      mbar_init(&bar_do_empty[i], 1);
+    }
+    mbar_init(&bar_kv_full, 1);
+    mbar_init(&bar_kv_empty, 1);
+    mbar_init(&bar_s, 1);
+    mbar_init(&bar_p, kSoftmaxWarps);
+    mbar_init(&bar_dp, 1);
+    mbar_init(&bar_ds, kSoftmaxWarps);
+    mbar_init(&bar_dq, 1);
+    mbar_init(&bar_dqfree, kDqWarps);
+    mbar_init(&bar_acc, 1);
+    mbar_init(&bar_accfree, kSoftmaxWarps);
+    mbar_init(&bar_drain, 1);
+    fence_barrier_init();
+  }
+  if (warp == kWarpMma) {
+    tmem_alloc(&tmem_base_shared, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = tmem_base_shared;
+  wait_previous_kernels();
+
+  // The r-th unit of this CTA (-1: no more), for the one thread or the warp that reads the ring.
+  auto next_unit = [&](int r, bool& ok) -> int {
+    if (!mbar_wait(&bar_unit_full[r & 1], (r >> 1) & 1, p.status, kDevTimeoutPipe)) {
+      ok = false;
+      return -1;
+    }
+    return *reinterpret_cast<volatile int*>(&unit_ring[r & 1]);
+  };
+
+  if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == kWarpTma) {
+      // ---------------------------------------------------------------- unit counter, TMA
+      if (lane == 0) {
+        tma_prefetch_desc(&map_q);
+        tma_prefetch_desc(&map_do);
+        tma_prefetch_desc(&map_k);
+        tma_prefetch_desc(&map_v);
+        asm volatile("fence.proxy.async.global;" ::: "memory");  // the statistics of the launch before
+        bool ok = true;
+        int g = 0;       // steps begun
+        int loads = 0;   // units whose K and V were loaded
+        int q_issued = 0, do_issued = 0;
+        for (int r = 0; ok; ++r) {
+          if (r >= 2 && !mbar_wait(&bar_unit_empty[r & 1], ((r >> 1) - 1) & 1, p.status, kDevTimeoutPipe)) break;
+          const uint32_t tk = atomicAdd(p.ticket, 1u);
+          const int u = tk < static_cast<uint32_t>(p.units) ? static_cast<int>(tk) : -1;
+          *reinterpret_cast<volatile int*>(&unit_ring[r & 1]) = u;
+          mbar_arrive(&bar_unit_full[r & 1]);
+          if (u < 0) break;
+          const Unit x = decode_unit<D>(p, u);
+          int t = 0;
+          for (int h = 0; ok && h < p.group; ++h) {
+            const int head = x.kvh * p.group + h;
+            const long long bh = static_cast<long long>(x.b) * p.hq + head;
+            for (int i = p.nq - 1; i >= x.i_min; --i, ++t, ++g) {
+              const int qs = g % C::kNQ, ds = g % C::kNDO;
+              if (g >= C::kNQ && !mbar_wait(&bar_q_empty[qs], (g / C::kNQ - 1) & 1, p.status, kDevTimeoutPipe)) {
+                ok = false;
+                break;
+              }
+              mbar_arrive_expect_tx(&bar_q_full[qs], C::kQBytes + C::kStatBytes);
+              for (int bx = 0; bx < D / 64; ++bx)
+                tma_load_4d(smem + C::kQ + qs * C::kQBytes + bx * C::kQBox, &map_q, &bar_q_full[qs], bx * 64, i * C::kBQ,
+                            head, x.b);
+              bulk_load(smem + C::kStat + qs * C::kStatBytes, p.stats + (bh * p.nq + i) * (2 * C::kBQ), C::kStatBytes,
+                        &bar_q_full[qs]);
+              q_issued = g + 1;
+              if (t == 0) {
+                if (loads > 0 && !mbar_wait(&bar_kv_empty, (loads - 1) & 1, p.status, kDevTimeoutPipe)) {
+                  ok = false;
+                  break;
+                }
+                mbar_arrive_expect_tx(&bar_kv_full, 2 * C::kKBytes);
+                for (int bx = 0; bx < D / 64; ++bx)
+                  tma_load_4d(smem + C::kK + bx * C::kKBox, &map_k, &bar_kv_full, bx * 64, x.j * kBK, x.kvh, x.b);
+                for (int bx = 0; bx < D / 64; ++bx)
+                  tma_load_4d(smem + C::kV + bx * C::kKBox, &map_v, &bar_kv_full, bx * 64, x.j * kBK, x.kvh, x.b);
+                ++loads;
+              }
+              if (g >= C::kNDO && !mbar_wait(&bar_do_empty[ds], (g / C::kNDO - 1) & 1, p.status, kDevTimeoutPipe)) {
+                ok = false;
+                break;
+              }
+              mbar_arrive_expect_tx(&bar_do_full[ds], C::kQBytes);
+              for (int bx = 0; bx < D / 64; ++bx)
+                tma_load_4d(smem + C::kDO + ds * C::kQBytes + bx * C::kQBox, &map_do, &bar_do_full[ds], bx * 64,
+                            i * C::kBQ, head, x.b);
+              do_issued = g + 1;
+            }
+          }
+        }
+        // before the CTA retires, let the last loads land (bounded; a no-op on the normal path)
+        if (loads > 0) mbar_drain(&bar_kv_full, (loads - 1) & 1);
+        for (int t = max(0, q_issued - C::kNQ); t < q_issued; ++t) mbar_drain(&bar_q_full[t % C::kNQ], (t / C::kNQ) & 1);
+        for (int t = max(0, do_issued - C::kNDO); t < do_issued; ++t)
+          mbar_drain(&bar_do_full[t % C::kNDO], (t / C::kNDO) & 1);
+      }
+      __syncwarp();
+    } else if (warp == kWarpMma) {
+      // ---------------------------------------------------------------- MMA issuer
+      if (lane == 0) {
+        constexpr uint32_t idesc_s = make_idesc(kBK, C::kBQ, 1, 0, 0);
+        constexpr uint32_t idesc_kv = make_idesc(kBK, C::kDH, 1, 0, 1);
+        constexpr uint32_t idesc_dq = C::kTransDq ? make_idesc(C::kDH, C::kBQ, 1, 1, 1) : make_idesc(C::kBQ, C::kDH, 1, 1, 1);
+        const uint32_t k_addr = smem_u32(smem + C::kK), v_addr = smem_u32(smem + C::kV), ds_addr = smem_u32(smem + C::kDs);
+        const uint32_t q_base = smem_u32(smem + C::kQ), do_base = smem_u32(smem + C::kDO);
+        // X^T = A B^T over head_dim: S^T = K Q^T, dP^T = V dO^T (all K-major)
+        auto issue_scores = [&](uint32_t a, uint32_t b, uint32_t col) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_bf16_ss(tbase + col, make_sdesc_sw128(a + (kk >> 2) * C::kKBox + (kk & 3) * 32, 16, 1024),
+                         make_sdesc_sw128(b + (kk >> 2) * C::kQBox + (kk & 3) * 32, 16, 1024), idesc_s, kk > 0 ? 1u : 0u);
+        };
+        bool ok = true;
+        int g = 0;          // steps of earlier units
+        int active = 0;     // earlier units with steps (K/V and accumulator phases)
+        for (int r = 0; ok; ++r) {
+          const int u = next_unit(r, ok);
+          if (!ok || u < 0) break;
+          mbar_arrive(&bar_unit_empty[r & 1]);
+          const Unit x = decode_unit<D>(p, u);
+          if (x.steps == 0) continue;
+          const uint32_t half_k = x.half * (C::kDH / 64) * C::kKBox, half_q = x.half * (C::kDH / 64) * C::kQBox;
+          auto issue_s = [&](int gs) -> bool {
+            const int st = gs % C::kNQ;
+            if (!mbar_wait(&bar_q_full[st], (gs / C::kNQ) & 1, p.status, kDevTimeoutTma)) return false;
+            tc_fence_after();
+            issue_scores(k_addr, q_base + st * C::kQBytes, C::kColS);
+            umma_commit(&bar_s);
+            return true;
+          };
+          ok = mbar_wait(&bar_kv_full, active & 1, p.status, kDevTimeoutTma) && issue_s(g);
+          for (int t = 0; ok && t < x.steps; ++t) {
+            const int gt = g + t, qs = gt % C::kNQ, dos = gt % C::kNDO;
+            const uint32_t q_addr = q_base + qs * C::kQBytes + half_q, do_addr = do_base + dos * C::kQBytes;
+            // dP(t); its columns hold dQ(t-1) until the dQ warps have read it
+            ok = mbar_wait(&bar_do_full[dos], (gt / C::kNDO) & 1, p.status, kDevTimeoutTma) &&
+                 (!C::kAlias || gt == 0 || mbar_wait(&bar_dqfree, (gt - 1) & 1, p.status, kDevTimeoutPipe));
+            if (!ok) break;
+            tc_fence_after();
+            issue_scores(v_addr, do_addr, C::kColDp);
+            umma_commit(&bar_dp);
+            // dV += P^T dO; the first overwrites an accumulator that the previous unit's epilogue has read
+            ok = mbar_wait(&bar_p, gt & 1, p.status, kDevTimeoutPipe) &&
+                 (t > 0 || active == 0 || mbar_wait(&bar_accfree, (active - 1) & 1, p.status, kDevTimeoutPipe));
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < C::kBQ / 16; ++kk) {
+              constexpr int per = C::kHalfQ / 16;  // steps in a warpgroup's part of P
+              const uint32_t a = tbase + C::kColS + (kk / per) * C::kHalfQ + (kk % per) * 8;
+              umma_bf16_ts(tbase + C::kColDv, a, make_sdesc_sw128(do_addr + half_q + kk * 2048, C::kQBox, 1024), idesc_kv,
+                           (t > 0 || kk > 0) ? 1u : 0u);
+            }
+            umma_commit(&bar_do_empty[dos]);
+            if (C::kAhead && t + 1 < x.steps) {
+              ok = issue_s(gt + 1);
+              if (!ok) break;
+            }
+            ok = mbar_wait(&bar_ds, gt & 1, p.status, kDevTimeoutPipe) &&
+                 (C::kAlias || gt == 0 || mbar_wait(&bar_dqfree, (gt - 1) & 1, p.status, kDevTimeoutPipe));
+            if (!ok) break;
+            tc_fence_after();
+            // dQ = dS K (or its transpose)
+#pragma unroll
+            for (int kk = 0; kk < kBK / 16; ++kk) {
+              const uint64_t dsd = make_sdesc_sw128(ds_addr + kk * 2048, C::kKBox, 1024);
+              const uint64_t kd = make_sdesc_sw128(k_addr + half_k + kk * 2048, C::kKBox, 1024);
+              umma_bf16_ss(tbase + C::kColDq, C::kTransDq ? kd : dsd, C::kTransDq ? dsd : kd, idesc_dq, kk > 0 ? 1u : 0u);
+            }
+            umma_commit(&bar_dq);
+            // dK += dS^T Q
+#pragma unroll
+            for (int kk = 0; kk < C::kBQ / 16; ++kk)
+              umma_bf16_ss(tbase + C::kColDk, make_sdesc_sw128(ds_addr + (kk >> 2) * C::kKBox + (kk & 3) * 32, 16, 1024),
+                           make_sdesc_sw128(q_addr + kk * 2048, C::kQBox, 1024), idesc_kv, (t > 0 || kk > 0) ? 1u : 0u);
+            umma_commit(&bar_q_empty[qs]);
+            if (!C::kAhead && t + 1 < x.steps) ok = issue_s(gt + 1);
+          }
+          if (!ok) break;
+          umma_commit(&bar_acc);
+          umma_commit(&bar_kv_empty);
+          g += x.steps;
+          ++active;
+        }
+        // every MMA issued by this thread completes before TMEM is released (bounded)
+        umma_commit(&bar_drain);
+        mbar_drain(&bar_drain, 0);
+      }
+      __syncwarp();
+    }
+  } else if (warp >= kSoftmaxWarps) {
+    // ------------------------------------------------------------------ dQ: TMEM -> global, in turn
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+    const int wq = warp & 3;
+    const int row = wq * 32 + lane;  // TMEM lane: a query of the tile, or (transposed) a column of dq
+    const uint32_t col = tmem_addr(tbase, wq * 32, C::kColDq);
+    bool ok = true;
+    int g = 0;
+    for (int r = 0; ok; ++r) {
+      const int u = __shfl_sync(0xffffffffu, lane == 0 ? next_unit(r, ok) : 0, 0);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok || u < 0) break;
+      if (lane == 0) mbar_arrive(&bar_unit_empty[r & 1]);
+      const Unit x = decode_unit<D>(p, u);
+      for (int h = 0; ok && h < p.group; ++h) {
+        const int head = x.kvh * p.group + h;
+        const long long bh = static_cast<long long>(x.b) * p.hq + head;
+        for (int i = p.nq - 1; i >= x.i_min; --i, ++g) {
+          const long long tile = (bh * p.nq + i) * C::kSplit + x.half;
+          uint32_t* turn = p.turns + tile * 4 + wq;
+          const int count = contributors<D>(p, i);
+          if (!__all_sync(0xffffffffu, mbar_wait(&bar_dq, g & 1, p.status, kDevTimeoutMma))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          uint32_t v[C::kDqCols];
+          tmem_load(col, v);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar_dqfree);
+          float* acc = p.acc + tile * (C::kDqCols * 128) + row * 4;
+          if (x.j > 0 && !wait_turn(turn, static_cast<uint32_t>(x.j), p.status)) {
+            ok = false;
+            break;
+          }
+          if (x.j + 1 < count) {
+            if (x.j == 0) {
+#pragma unroll
+              for (int c = 0; c < C::kDqCols / 4; ++c)
+                __stcg(reinterpret_cast<float4*>(acc + c * 512),
+                       make_float4(__uint_as_float(v[4 * c]), __uint_as_float(v[4 * c + 1]), __uint_as_float(v[4 * c + 2]),
+                                   __uint_as_float(v[4 * c + 3])));
+            } else {
+#pragma unroll
+              for (int c = 0; c < C::kDqCols / 4; ++c)
+                red_add_v4(acc + c * 512, __uint_as_float(v[4 * c]), __uint_as_float(v[4 * c + 1]),
+                           __uint_as_float(v[4 * c + 2]), __uint_as_float(v[4 * c + 3]));
+            }
+            __syncwarp();
+            if (lane == 0) {
+              __threadfence();
+              asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(turn), "r"(static_cast<uint32_t>(x.j + 1)) : "memory");
+            }
+          } else {
+            // the last key tile: the sum is complete
+            if (x.j > 0) {
+#pragma unroll
+              for (int c = 0; c < C::kDqCols / 4; ++c) {
+                const float4 a = __ldcg(reinterpret_cast<const float4*>(acc + c * 512));
+                v[4 * c] = __float_as_uint(a.x + __uint_as_float(v[4 * c]));
+                v[4 * c + 1] = __float_as_uint(a.y + __uint_as_float(v[4 * c + 1]));
+                v[4 * c + 2] = __float_as_uint(a.z + __uint_as_float(v[4 * c + 2]));
+                v[4 * c + 3] = __float_as_uint(a.w + __uint_as_float(v[4 * c + 3]));
+              }
+            }
+            __nv_bfloat16* out = p.dq + x.b * p.q_sb + head * p.q_sh + static_cast<long long>(i) * C::kBQ * p.q_ss +
+                                 x.half * C::kDH;
+            const int rows = min(C::kBQ, p.sq - i * C::kBQ);
+            if constexpr (C::kTransDq) {
+#pragma unroll
+              for (int q = 0; q < C::kDqCols; ++q)
+                if (q < rows) out[q * p.q_ss + row] = __float2bfloat16_rn(__uint_as_float(v[q]) * p.scale);
+            } else if (row < rows) {
+              uint4* dst = reinterpret_cast<uint4*>(out + row * p.q_ss);
+#pragma unroll
+              for (int c = 0; c < C::kDqCols / 8; ++c) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  w[e] = pack_bf16x2(__uint_as_float(v[8 * c + 2 * e]) * p.scale, __uint_as_float(v[8 * c + 2 * e + 1]) * p.scale);
+                dst[c] = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+            }
+          }
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax warps, epilogue of dV and dK
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+    const int wg = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;  // key of the tile
+    const uint32_t lanes = tmem_addr(tbase, (warp & 3) * 32, 0);
+    const uint32_t col_s = lanes + C::kColS + wg * C::kHalfQ;
+    const uint32_t col_dp = lanes + C::kColDp + wg * C::kHalfQ;
+    uint8_t* ds_row = smem + C::kDs + (C::kHalfQ == 64 ? wg * C::kKBox : 0);
+    constexpr int kChunk0 = 0;
+    const int chunk0 = C::kHalfQ == 64 ? kChunk0 : wg * 4;  // first 16-byte piece of this warpgroup's part of a dS row
+    const float c = p.scale_log2;
+    bool ok = true;
+    int g = 0, active = 0;
+    for (int r = 0; ok; ++r) {
+      const int u = __shfl_sync(0xffffffffu, lane == 0 ? next_unit(r, ok) : 0, 0);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok || u < 0) break;
+      if (lane == 0) mbar_arrive(&bar_unit_empty[r & 1]);
+      const Unit x = decode_unit<D>(p, u);
+      const int key = x.j * kBK + row;
+      const bool ragged = x.j * kBK + kBK > p.skv;  // keys behind the last one
+      for (int h = 0; ok && h < p.group; ++h) {
+        for (int i = p.nq - 1; i >= x.i_min; --i, ++g) {
+          const int qs = g % C::kNQ;
+          if (!__all_sync(0xffffffffu, mbar_wait(&bar_q_full[qs], (g / C::kNQ) & 1, p.status, kDevTimeoutTma) &&
+                                           mbar_wait(&bar_s, g & 1, p.status, kDevTimeoutMma))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const float4* lse2 = reinterpret_cast<const float4*>(smem + C::kStat + qs * C::kStatBytes) + wg * (C::kHalfQ / 4);
+          const float4* delta = lse2 + C::kBQ / 4;
+          const int q0 = i * C::kBQ + wg * C::kHalfQ;
+          // query columns before `first` are masked for this key
+          const bool masked = ragged || (p.causal && q0 < x.j * kBK + kBK - 1);
+          const int first = key >= p.skv ? C::kHalfQ : (p.causal ? key - q0 : 0);
+          float pr[C::kHalfQ];
+#pragma unroll
+          for (int ch = 0; ch < C::kHalfQ / 32; ++ch) {
+            uint32_t s[32];
+            tmem_ld32(col_s + ch * 32, s);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float4 l = lse2[ch * 8 + e];
+              const int n = ch * 32 + e * 4;
+              pr[n] = ex2_approx(fmaf(__uint_as_float(s[e * 4]), c, -l.x));
+              pr[n + 1] = ex2_approx(fmaf(__uint_as_float(s[e * 4 + 1]), c, -l.y));
+              pr[n + 2] = ex2_approx(fmaf(__uint_as_float(s[e * 4 + 2]), c, -l.z));
+              pr[n + 3] = ex2_approx(fmaf(__uint_as_float(s[e * 4 + 3]), c, -l.w));
+            }
+            if (masked) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (ch * 32 + e < first) pr[ch * 32 + e] = 0.0f;
+            }
+            uint32_t packed[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) packed[e] = pack_bf16x2(pr[ch * 32 + 2 * e], pr[ch * 32 + 2 * e + 1]);
+            tmem_st16(col_s + ch * 16, packed);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar_p);
+          if (!__all_sync(0xffffffffu, mbar_wait(&bar_dp, g & 1, p.status, kDevTimeoutMma))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int ch = 0; ch < C::kHalfQ / 32; ++ch) {
+            uint32_t dp[32];
+            tmem_ld32(col_dp + ch * 32, dp);
+            float ds[32];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float4 d = delta[ch * 8 + e];
+              const int n = ch * 32 + e * 4;
+              ds[e * 4] = pr[n] * (__uint_as_float(dp[e * 4]) - d.x);
+              ds[e * 4 + 1] = pr[n + 1] * (__uint_as_float(dp[e * 4 + 1]) - d.y);
+              ds[e * 4 + 2] = pr[n + 2] * (__uint_as_float(dp[e * 4 + 2]) - d.z);
+              ds[e * 4 + 3] = pr[n + 3] * (__uint_as_float(dp[e * 4 + 3]) - d.w);
+            }
+            if (masked) {  // dP may be infinite or NaN there
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (ch * 32 + e < first) ds[e] = 0.0f;
+            }
+#pragma unroll
+            for (int v4 = 0; v4 < 4; ++v4) {
+              uint4 w;
+              w.x = pack_bf16x2(ds[v4 * 8], ds[v4 * 8 + 1]);
+              w.y = pack_bf16x2(ds[v4 * 8 + 2], ds[v4 * 8 + 3]);
+              w.z = pack_bf16x2(ds[v4 * 8 + 4], ds[v4 * 8 + 5]);
+              w.w = pack_bf16x2(ds[v4 * 8 + 6], ds[v4 * 8 + 7]);
+              *reinterpret_cast<uint4*>(ds_row + sw128_offset(row, (chunk0 + ch * 4 + v4) * 16)) = w;
+            }
+          }
+          fence_async_smem();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar_ds);
+        }
+      }
+      if (!ok) break;
+      // epilogue: warpgroup 0 writes dV, warpgroup 1 dK; a tile that no query sees gets zeros
+      if (x.steps > 0) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&bar_acc, active & 1, p.status, kDevTimeoutMma))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+      }
+      const float mul = wg == 0 ? 1.0f : p.scale;
+      __nv_bfloat16* out = (wg == 0 ? p.dv : p.dk) + x.b * p.k_sb + x.kvh * p.k_sh + key * p.k_ss + x.half * C::kDH;
+#pragma unroll 1
+      for (int dc = 0; dc < C::kDH; dc += 32) {
+        uint32_t a[32];
+        if (x.steps > 0) {
+          tmem_ld32(lanes + (wg == 0 ? C::kColDv : C::kColDk) + dc, a);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) a[e] = 0u;
+        }
+        if (key < p.skv) {
+          uint4* dst = reinterpret_cast<uint4*>(out + dc);
+#pragma unroll
+          for (int v4 = 0; v4 < 4; ++v4) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = pack_bf16x2(__uint_as_float(a[v4 * 8 + 2 * e]) * mul, __uint_as_float(a[v4 * 8 + 2 * e + 1]) * mul);
+            dst[v4] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      if (x.steps > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar_accfree);
+        ++active;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kWarpMma) {
+    tc_fence_after();
+    tmem_dealloc(tbase, 512);
+  }
+}
+
+// delta = sum do * o and lse * log2(e) of every row, in rows padded to whole query tiles; D / 8
+// lanes a row, 16 bytes a lane.  Also sets the unit counter and the turn counters to 0.
+template <int D>
+__global__ void __launch_bounds__(256) fa2_bwd_prep(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ dout,
+                                                    const float* __restrict__ lse, float* __restrict__ stats,
+                                                    uint32_t* __restrict__ counters, long long n_counters, long long rows,
+                                                    int sq, int sq_pad, int hq, long long sb, long long sh, long long ss) {
+  using C = Cfg<D>;
+  constexpr int kLanes = D / 8;
+  wait_previous_kernels();
+  const long long t = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  for (long long i = t; i < n_counters; i += static_cast<long long>(gridDim.x) * 256) counters[i] = 0u;
+  const long long r = t / kLanes;  // padded row: (b * hq + h) * sq_pad + i
+  const int part = threadIdx.x % kLanes;
+  const bool in = r < rows;
+  const long long bh = in ? r / sq_pad : 0;
+  const int i = in ? static_cast<int>(r - bh * sq_pad) : sq;
+  float sum = 0.0f;
+  if (i < sq) {
+    const long long off = (bh / hq) * sb + (bh % hq) * sh + i * ss + part * 8;
+    const uint4 a = *reinterpret_cast<const uint4*>(o + off);
+    const uint4 b = *reinterpret_cast<const uint4*>(dout + off);
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      sum = fmaf(__uint_as_float(x[e] << 16), __uint_as_float(y[e] << 16), sum);
+      sum = fmaf(__uint_as_float(x[e] & 0xffff0000u), __uint_as_float(y[e] & 0xffff0000u), sum);
+    }
+  }
+#pragma unroll
+  for (int m = kLanes / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+  if (in && part == 0) {
+    const int tile = i / C::kBQ, in_tile = i - tile * C::kBQ;
+    float* s = stats + (bh * (sq_pad / C::kBQ) + tile) * (2 * C::kBQ) + in_tile;
+    s[0] = i < sq ? lse[bh * sq + i] * kLog2e : INFINITY;
+    s[C::kBQ] = sum;
+  }
+}
+
+struct Sizes {
+  long long counters, stats, acc, total;  // bytes
+};
+
+template <int D>
+Sizes sizes(long long batch, long long hq, long long sq, long long skv) {
+  using C = Cfg<D>;
+  const long long tiles = batch * hq * ((sq + C::kBQ - 1) / C::kBQ);
+  auto up = [](long long n) { return (n + 255) / 256 * 256; };
+  Sizes s{};
+  s.counters = up((1 + tiles * C::kSplit * 4) * 4);
+  s.stats = up(tiles * C::kStatBytes);
+  s.acc = skv > kBK ? tiles * C::kSplit * C::kDqCols * 128 * 4 : 0;  // one key tile: dq is written at once
+  s.total = s.counters + s.stats + s.acc;
+  return s;
+}
+
+template <int D>
+int launch(const void* dout, const void* q, const void* k, const void* v, const void* o, const float* lse, void* dq,
+           void* dk, void* dv, int batch, int hq, int hkv, int sq, int skv, int layout, int causal, float sm_scale,
+           void* workspace, long long workspace_bytes, uint32_t* status, cudaStream_t stream) {
+  using C = Cfg<D>;
+  const Sizes sz = sizes<D>(batch, hq, sq, skv);
+  if (workspace == nullptr || workspace_bytes < sz.total || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+    return fail(TOKMIX_ERR_INVALID_ARGUMENT, "tokmix_fa2_bwd: needs a 16-byte aligned workspace of %lld bytes", sz.total);
+  // 4-D tensor maps over (d, seq, head, batch); the layout only changes the strides.
+  auto make = [&](CUtensorMap* map, const void* base, int s, int h, uint32_t rows) {
+    uint64_t dims[4] = {static_cast<uint64_t>(D), static_cast<uint64_t>(s), static_cast<uint64_t>(h),
+                        static_cast<uint64_t>(batch)};
+    const uint64_t row = static_cast<uint64_t>(D) * 2;
+    uint64_t strides[3] = {layout == TOKMIX_LAYOUT_BHSD ? row : row * h, layout == TOKMIX_LAYOUT_BHSD ? row * s : row,
+                           row * s * h};
+    uint32_t box[4] = {64, rows, 1, 1};
+    return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  CUtensorMap mq, mdo, mk, mv;
+  if (!make(&mq, q, sq, hq, C::kBQ) || !make(&mdo, dout, sq, hq, C::kBQ) || !make(&mk, k, skv, hkv, kBK) ||
+      !make(&mv, v, skv, hkv, kBK))
+    return TOKMIX_ERR_INVALID_ARGUMENT;
+
+  Params p{};
+  p.dq = static_cast<__nv_bfloat16*>(dq);
+  p.dk = static_cast<__nv_bfloat16*>(dk);
+  p.dv = static_cast<__nv_bfloat16*>(dv);
+  const bool bhsd = layout == TOKMIX_LAYOUT_BHSD;
+  p.q_sb = static_cast<long long>(D) * sq * hq;
+  p.q_sh = bhsd ? static_cast<long long>(D) * sq : D;
+  p.q_ss = bhsd ? D : static_cast<long long>(D) * hq;
+  p.k_sb = static_cast<long long>(D) * skv * hkv;
+  p.k_sh = bhsd ? static_cast<long long>(D) * skv : D;
+  p.k_ss = bhsd ? D : static_cast<long long>(D) * hkv;
+  p.batch = batch;
+  p.hq = hq;
+  p.hkv = hkv;
+  p.group = hq / hkv;
+  p.sq = sq;
+  p.skv = skv;
+  p.nq = (sq + C::kBQ - 1) / C::kBQ;
+  p.nk = (skv + kBK - 1) / kBK;
+  p.causal = causal ? 1 : 0;
+  p.scale = sm_scale;
+  p.scale_log2 = sm_scale * kLog2e;
+  p.status = status;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.ticket = reinterpret_cast<uint32_t*>(ws);
+  p.turns = p.ticket + 1;
+  p.stats = reinterpret_cast<const float*>(ws + sz.counters);
+  p.acc = reinterpret_cast<float*>(ws + sz.counters + sz.stats);
+  const long long units = static_cast<long long>(batch) * hkv * p.nk * C::kSplit;
+  const long long steps = static_cast<long long>(p.nq) * p.group;
+  if (units > 0x3FFFFFFFll || steps > 0x3FFFFFFFll)
+    return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_fa2_bwd: too many tiles (%lld x %lld)", units, steps);
+  p.units = static_cast<int>(units);
+
+  const long long rows = static_cast<long long>(batch) * hq * p.nq * C::kBQ;
+  const long long blocks = (rows * (D / 8) + 255) / 256;
+  if (blocks > 0x7FFFFFFFll) return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_fa2_bwd: too many rows (%lld)", rows);
+  const int smem_bytes = C::kBytes + 1024;
+  if (!ensure_smem_attr(reinterpret_cast<const void*>(&fa2_bwd_kernel<D>), smem_bytes))
+    return check_launch("tokmix_fa2_bwd: cudaFuncSetAttribute");
+  cudaError_t e = launch_overlapped(&fa2_bwd_prep<D>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream,
+                                    static_cast<const __nv_bfloat16*>(o), static_cast<const __nv_bfloat16*>(dout), lse,
+                                    const_cast<float*>(p.stats), p.ticket, sz.counters / 4, rows, sq, p.nq * C::kBQ, hq,
+                                    p.q_sb, p.q_sh, p.q_ss);
+  if (e == cudaSuccess) {
+    const int grid = static_cast<int>(std::min<long long>(units, std::max(1, device_sm_count())));
+    e = launch_overlapped(&fa2_bwd_kernel<D>, dim3(static_cast<unsigned>(grid)), dim3(kThreads),
+                          static_cast<size_t>(smem_bytes), stream, mq, mdo, mk, mv, p);
+  }
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(TOKMIX_ERR_LAUNCH, "tokmix_fa2_bwd: %s", cudaGetErrorString(e));
+  }
+  return check_launch("tokmix_fa2_bwd");
+}
+
+// Checks shared by the entry points; 0 for a head_dim without a kernel
+template <typename F64, typename F128, typename F256>
+auto by_head_dim(int head_dim, F64 f64, F128 f128, F256 f256, decltype(f64()) otherwise) {
+  return head_dim == 64 ? f64() : head_dim == 128 ? f128() : head_dim == 256 ? f256() : otherwise;
+}
+
+}  // namespace fa2b
+}  // namespace tokmix
+
+extern "C" long long tokmix_fa2_bwd_workspace_bytes(int batch, int heads_q, int seqlen_q, int seqlen_kv, int head_dim) {
+  using namespace tokmix::fa2b;
+  if (batch < 0 || heads_q <= 0 || seqlen_q < 0 || seqlen_kv < 0) return -1;
+  return by_head_dim(
+      head_dim, [&] { return sizes<64>(batch, heads_q, seqlen_q, seqlen_kv).total; },
+      [&] { return sizes<128>(batch, heads_q, seqlen_q, seqlen_kv).total; },
+      [&] { return sizes<256>(batch, heads_q, seqlen_q, seqlen_kv).total; }, -1LL);
+}
+
+extern "C" int tokmix_fa2_bwd(const void* dout, const void* q, const void* k, const void* v, const void* o,
+                              const float* lse, void* dq, void* dk, void* dv, int batch, int heads_q, int heads_kv,
+                              int seqlen_q, int seqlen_kv, int head_dim, int layout, int causal, float sm_scale,
+                              void* workspace, long long workspace_bytes, uint32_t* status, void* stream) {
+  using namespace tokmix;
+  if (batch < 0 || heads_q <= 0 || heads_kv <= 0 || seqlen_q < 0 || seqlen_kv < 0)
+    return fail(TOKMIX_ERR_INVALID_ARGUMENT, "tokmix_fa2_bwd: negative or zero size");
+  if (heads_q % heads_kv != 0)
+    return fail(TOKMIX_ERR_INVALID_ARGUMENT, "tokmix_fa2_bwd: heads_q (%d) must be a multiple of heads_kv (%d)", heads_q,
+                heads_kv);
+  if (layout != TOKMIX_LAYOUT_BHSD && layout != TOKMIX_LAYOUT_BSHD)
+    return fail(TOKMIX_ERR_INVALID_ARGUMENT, "tokmix_fa2_bwd: unknown layout %d", layout);
+  if (!(sm_scale > 0.0f) || !std::isfinite(sm_scale))
+    return fail(TOKMIX_ERR_INVALID_ARGUMENT, "tokmix_fa2_bwd: sm_scale must be finite and positive");
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_fa2_bwd: head_dim %d not supported (64, 128 or 256)", head_dim);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (batch == 0 || (seqlen_q == 0 && seqlen_kv == 0)) return TOKMIX_OK;
+  if (seqlen_kv == 0)
+    return fail(TOKMIX_ERR_INVALID_ARGUMENT, "tokmix_fa2_bwd: seqlen_kv must be positive when seqlen_q is");
+  for (const void* ptr : {k, v, static_cast<const void*>(dk), static_cast<const void*>(dv)})
+    if (ptr == nullptr || reinterpret_cast<uintptr_t>(ptr) % 16 != 0)
+      return fail(TOKMIX_ERR_INVALID_ARGUMENT, "tokmix_fa2_bwd: tensors must be non-null and 16-byte aligned");
+  if (seqlen_q > 0) {
+    for (const void* ptr : {dout, q, o, static_cast<const void*>(dq)})
+      if (ptr == nullptr || reinterpret_cast<uintptr_t>(ptr) % 16 != 0)
+        return fail(TOKMIX_ERR_INVALID_ARGUMENT, "tokmix_fa2_bwd: tensors must be non-null and 16-byte aligned");
+    if (lse == nullptr) return fail(TOKMIX_ERR_INVALID_ARGUMENT, "tokmix_fa2_bwd: null lse");
+  }
+  if (const int rc = check_device()) return rc;
+  if (seqlen_q == 0) {  // no query: no gradient reaches the keys and values
+    const size_t bytes = static_cast<size_t>(batch) * heads_kv * seqlen_kv * head_dim * 2;
+    if (cudaMemsetAsync(dk, 0, bytes, s) != cudaSuccess || cudaMemsetAsync(dv, 0, bytes, s) != cudaSuccess)
+      return check_launch("tokmix_fa2_bwd");
+    return TOKMIX_OK;
+  }
+  auto run = [&](auto d) {
+    return fa2b::launch<decltype(d)::value>(dout, q, k, v, o, lse, dq, dk, dv, batch, heads_q, heads_kv, seqlen_q,
+                                            seqlen_kv, layout, causal, sm_scale, workspace, workspace_bytes, status, s);
+  };
+  return fa2b::by_head_dim(
+      head_dim, [&] { return run(std::integral_constant<int, 64>()); }, [&] { return run(std::integral_constant<int, 128>()); },
+      [&] { return run(std::integral_constant<int, 256>()); }, static_cast<int>(TOKMIX_ERR_UNSUPPORTED));
+}

@@ -65,8 +65,15 @@ struct Params {
   int n_qtiles;                // ceil(sq / 128)
   int head_units;              // pairs of heads (pair_heads) or heads
   int units;                   // work units (tile pairs), heaviest first
+  float* lse;                  // [batch, hq, sq] natural-log sums of the rows' exponentials, or null
   uint32_t* status;
 };
+
+// The row's log-sum-exp (natural logarithm) from its base-2 reference m and sum l
+__device__ __forceinline__ void store_lse(const Params& p, int b, int head, int qrow, float m, float l) {
+  if (p.lse != nullptr && qrow < p.sq)
+    p.lse[(static_cast<long long>(b) * p.hq + head) * p.sq + qrow] = (m + log2f(l)) * 0.6931471805599453f;
+}
 
 struct TileInfo {
   int head;     // query head
@@ -406,6 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       {
         tc_fence_after();
+        store_lse(p, b, tile[i].head, qrow, m, l);
         const float inv_l = 1.0f / l;
         __nv_bfloat16* orow = p.o + static_cast<long long>(b) * p.o_sb + static_cast<long long>(tile[i].head) * p.o_sh +
                               static_cast<long long>(qrow) * p.o_ss;
@@ -443,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 template <int D>
 int launch(const void* q, const void* k, const void* v, void* o, int batch, int hq, int hkv, int sq, int skv,
-           int layout, int causal, float sm_scale, uint32_t* status, cudaStream_t stream) {
+           int layout, int causal, float sm_scale, float* lse, uint32_t* status, cudaStream_t stream) {
   using L = Layout<D>;
   // 4-D tensor maps over (d, seq, head, batch); the layout only changes the strides.
   auto make = [&](CUtensorMap* map, const void* base, int s, int h) {
@@ -489,6 +497,7 @@ int launch(const void* q, const void* k, const void* v, void* o, int batch, int 
   p.pair_heads = (group % 2 == 0) ? 1 : 0;
   p.n_qtiles = (sq + kBM - 1) / kBM;
   p.head_units = p.pair_heads ? hq / 2 : hq;
+  p.lse = lse;
   p.status = status;
   const long long rows = p.pair_heads ? p.n_qtiles : (p.n_qtiles + 1) / 2;
   const long long units = rows * batch * p.head_units;
@@ -794,6 +803,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       {
         tc_fence_after();
+        store_lse(p, b, head, qrow, m, l);
         const float inv_l = 1.0f / l;
         __nv_bfloat16* orow = p.o + static_cast<long long>(b) * p.o_sb + static_cast<long long>(head) * p.o_sh +
                               static_cast<long long>(qrow) * p.o_ss;
@@ -829,7 +839,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 int launch(const void* q, const void* k, const void* v, void* o, int batch, int hq, int hkv, int sq, int skv,
-           int layout, int causal, float sm_scale, uint32_t* status, cudaStream_t stream) {
+           int layout, int causal, float sm_scale, float* lse, uint32_t* status, cudaStream_t stream) {
   auto make = [&](CUtensorMap* map, const void* base, int s, int h, uint32_t rows) {
     uint64_t dims[4] = {static_cast<uint64_t>(kD), static_cast<uint64_t>(s), static_cast<uint64_t>(h),
                         static_cast<uint64_t>(batch)};
@@ -870,6 +880,7 @@ int launch(const void* q, const void* k, const void* v, void* o, int batch, int 
   p.causal = causal ? 1 : 0;
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.n_qtiles = (sq + kBM - 1) / kBM;
+  p.lse = lse;
   p.status = status;
   const long long units = static_cast<long long>(p.n_qtiles) * batch * hq;
   if (units <= 0) return TOKMIX_OK;
@@ -888,9 +899,9 @@ int launch(const void* q, const void* k, const void* v, void* o, int batch, int 
 }  // namespace fa2
 }  // namespace tokmix
 
-extern "C" int tokmix_fa2_fwd(const void* q, const void* k, const void* v, void* o, int batch, int heads_q,
-                              int heads_kv, int seqlen_q, int seqlen_kv, int head_dim, int layout, int causal,
-                              float sm_scale, uint32_t* status, void* stream) {
+extern "C" int tokmix_fa2_fwd_lse(const void* q, const void* k, const void* v, void* o, float* lse, int batch,
+                                  int heads_q, int heads_kv, int seqlen_q, int seqlen_kv, int head_dim, int layout,
+                                  int causal, float sm_scale, uint32_t* status, void* stream) {
   using namespace tokmix;
   if (batch < 0 || heads_q <= 0 || heads_kv <= 0 || seqlen_q < 0 || seqlen_kv < 0)
     return fail(TOKMIX_ERR_INVALID_ARGUMENT, "tokmix_fa2_fwd: negative or zero size");
@@ -913,14 +924,21 @@ extern "C" int tokmix_fa2_fwd(const void* q, const void* k, const void* v, void*
   switch (head_dim) {
     case 64:
       return fa2::launch<64>(q, k, v, o, batch, heads_q, heads_kv, seqlen_q, seqlen_kv, layout, causal, sm_scale,
-                             status, s);
+                             lse, status, s);
     case 128:
       return fa2::launch<128>(q, k, v, o, batch, heads_q, heads_kv, seqlen_q, seqlen_kv, layout, causal, sm_scale,
-                              status, s);
+                              lse, status, s);
     case 256:
       return fa2::d256::launch(q, k, v, o, batch, heads_q, heads_kv, seqlen_q, seqlen_kv, layout, causal, sm_scale,
-                               status, s);
+                               lse, status, s);
     default:
       return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_fa2_fwd: head_dim %d not supported (64, 128 or 256)", head_dim);
   }
+}
+
+extern "C" int tokmix_fa2_fwd(const void* q, const void* k, const void* v, void* o, int batch, int heads_q,
+                              int heads_kv, int seqlen_q, int seqlen_kv, int head_dim, int layout, int causal,
+                              float sm_scale, uint32_t* status, void* stream) {
+  return tokmix_fa2_fwd_lse(q, k, v, o, nullptr, batch, heads_q, heads_kv, seqlen_q, seqlen_kv, head_dim, layout, causal,
+                            sm_scale, status, stream);
 }

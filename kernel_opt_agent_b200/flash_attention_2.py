@@ -8,6 +8,8 @@ Compared with the reference module (``kernels_optimized/flash_attention_2.py:110
 accepts grouped-query attention (k/v with fewer heads), head_dim 64 and 256 and a ``layout="bshd"``
 keyword; with the reference's arguments it behaves the same: q, k, v bf16 CUDA tensors
 [batch, heads, seq, head_dim], default scale 1/sqrt(head_dim), returns a new bf16 tensor.
+``return_lse=True`` returns (out, lse), lse fp32 [batch, heads, seq] (in both layouts): the natural
+logarithm of each row's sum of exponentials, for ``flash_attention_2_bwd``.
 """
 
 from __future__ import annotations
@@ -57,7 +59,8 @@ def kernel_fn(
     *,
     layout: str = "bhsd",
     out: torch.Tensor | None = None,
-) -> torch.Tensor:
+    return_lse: bool = False,
+):
     q, k, v, hd, sd = _validate_inputs(q, k, v, layout)
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(q.shape[-1])
@@ -67,16 +70,17 @@ def kernel_fn(
         raise ValueError("out must be a contiguous bf16 tensor shaped like q")
     lib = _lib.load()
     dev = q.device
+    lse = torch.empty((q.shape[0], q.shape[hd], q.shape[sd]), dtype=torch.float32, device=dev) if return_lse else None
     word = _lib.status_word(dev)
     with torch.cuda.device(dev):
-        rc = lib.tokmix_fa2_fwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+        rc = lib.tokmix_fa2_fwd_lse(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None,
             q.shape[0], q.shape[hd], k.shape[hd], q.shape[sd], k.shape[sd], q.shape[3],
             _lib.LAYOUT_BHSD if layout == "bhsd" else _lib.LAYOUT_BSHD, 1 if causal else 0, float(sm_scale),
             word.data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "flash_attention_2")
     _lib.after_launch(dev, "flash_attention_2")
-    return out
+    return (out, lse) if return_lse else out
 
 
 def check_device_status(device: torch.device | None = None) -> None:

@@ -1,0 +1,81 @@
+"""flash_attention_2_bwd plugin module: the gradients of ``flash_attention_2``, with the module contract
+of the reference's plugins (``kernels/__init__.py:3-8``).  The reference has no backward pass.
+
+    kernel_fn(do, q, k, v, o, lse, causal=True, sm_scale=None, *, layout="bhsd") -> (dq, dk, dv)
+
+q, k, v, causal, sm_scale and layout as the forward took them; o and lse what it returned with
+``return_lse=True``; do the gradient of o, shaped like it.  All bf16, lse fp32 [batch, heads, seq] (in
+both layouts).  With P = exp(sm_scale q k^T - lse) under the mask and delta = sum(do * o) per row:
+
+    dv = P^T do,   dS = P * (do v^T - delta),   dq = sm_scale dS k,   dk = sm_scale dS^T q
+
+dk and dv are summed over the query heads that share a key/value head.  P and dS enter their products in
+bf16, sums are fp32, and every sum has an order that sizes alone decide: the same bits every time.
+A key or value that no query sees gets zeros.  Tensors that are not contiguous (a gradient that autograd
+expanded, say) are copied first.
+
+``kernel_fn`` runs ``tokmix_fa2_bwd`` (``csrc/fa2_bwd.cu``), no fallback.  ``training.attention`` is the forward
+and this in one differentiable call."""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+from . import flash_attention_2 as _forward
+from .flash_attention_2 import check_device_status  # noqa: F401  (one status word for both directions)
+
+KERNEL_TYPE = "flash_attention_2_bwd"
+
+
+def kernel_fn(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
+              causal: bool = True, sm_scale: float | None = None, *, layout: str = "bhsd"):
+    q, k, v, hd, sd = _forward._validate_inputs(q, k, v, layout)
+    for name, t in (("do", do), ("o", o)):
+        if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:
+            raise ValueError(f"{name} must be a bfloat16 tensor shaped like q on its device")
+    batch, heads, heads_kv, sq, skv, d = q.shape[0], q.shape[hd], k.shape[hd], q.shape[sd], k.shape[sd], q.shape[3]
+    if lse.shape != (batch, heads, sq) or lse.dtype != torch.float32 or lse.device != q.device:
+        raise ValueError("lse must be float32 [batch, heads, seq_len] on the device of q")
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(d)
+    do, q, k, v, o, lse = (_lib.aligned(t) for t in (do, q, k, v, o, lse))
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    lib, dev = _lib.load(), q.device
+    need = lib.tokmix_fa2_bwd_workspace_bytes(batch, heads, sq, skv, d) if q.numel() else 0
+    # from the allocator on every call: calls on several streams and captured graphs do not share it
+    workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    word = _lib.status_word(dev)
+    rc = _lib.call_on(dev, lib.tokmix_fa2_bwd, do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                      lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), batch, heads, heads_kv, sq, skv, d,
+                      _lib.LAYOUT_BHSD if layout == "bhsd" else _lib.LAYOUT_BSHD, 1 if causal else 0, float(sm_scale),
+                      workspace.data_ptr(), need, word.data_ptr(), _lib.stream_ptr(dev))
+    _lib.check(rc, "flash_attention_2_bwd")
+    _lib.after_launch(dev, "flash_attention_2_bwd")
+    return dq, dk, dv
+
+
+def get_inputs(batch: int = 8, head_num: int = 8, seq_len: int = 2048, head_dim: int = 128,
+               dtype: torch.dtype = torch.bfloat16, causal: bool = True, seed: int = 42, *,
+               head_num_kv: int | None = None, layout: str = "bhsd", device: str = "cuda") -> dict:
+    """The forward's inputs and its outputs, and an N(0,1) gradient of the output."""
+    inp = _forward.get_inputs(batch, head_num, seq_len, head_dim, dtype, causal, seed, head_num_kv=head_num_kv,
+                              layout=layout, device=device)
+    inp["o"], inp["lse"] = _forward.kernel_fn(**inp, return_lse=True)
+    gen = torch.Generator().manual_seed(seed + 1)
+    inp["do"] = torch.randn(inp["q"].shape, generator=gen).to(dtype).to(device)
+    return inp
+
+
+def get_flops(batch: int = 8, head_num: int = 8, seq_len: int = 2048, head_dim: int = 128, causal: bool = True) -> int:
+    """Five products over the visible pairs (the forward has two)."""
+    return _forward.get_flops(batch, head_num, seq_len, head_dim, causal) * 5 // 2
+
+
+def get_bytes(batch: int = 8, head_num: int = 8, seq_len: int = 2048, head_dim: int = 128, element_size: int = 2, *,
+              head_num_kv: int | None = None) -> int:
+    """q, k, v, o, do and lse read once, dq, dk and dv written once."""
+    hkv = head_num if head_num_kv is None else head_num_kv
+    return batch * seq_len * (4 * (head_num + hkv) * head_dim * element_size + 4 * head_num)
