@@ -54,6 +54,7 @@ constexpr int kThreads = 512;
 constexpr int kSoftmaxWarps = 8, kDqWarps = 4;
 constexpr int kWarpTma = 12, kWarpMma = 13;
 constexpr int kUnitReaders = 1 + kSoftmaxWarps + kDqWarps;
+constexpr int kWaveCtas = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D>
@@ -62,7 +63,7 @@ struct Cfg {
   static constexpr int kDH = D < 128 ? D : 128;        // columns of dV, dK and dQ that a unit forms
   static constexpr int kSplit = D / kDH;
   static constexpr int kNQ = D == 256 ? 1 : 2;         // stages of Q, and of the row statistics
-  static constexpr int kNDO = D == 64 ? 2 : 1;         // stages of dO
+  static constexpr int kNDO = D == 256 ? 1 : 2;        // stages of dO
   static constexpr bool kAhead = kNQ > 1;              // S(t+1) before dQ(t): needs a second Q stage
   static constexpr bool kAlias = D == 128;             // dQ in dP's columns
   static constexpr bool kTransDq = D == 256;           // dQ^T: lanes are columns of dq, columns are queries
@@ -87,7 +88,7 @@ struct Cfg {
   static constexpr int kDs = kDO + kNDO * kQBytes;
   static constexpr int kStat = kDs + kDsBytes;
   static constexpr int kBytes = kStat + kNQ * kStatBytes;
-  static_assert(kBytes + 1024 + 512 <= 227 * 1024, "shared memory");
+  static_assert(kBytes + 1024 <= 227 * 1024, "shared memory");  // 1024: the barriers, rounded up to the tiles' alignment
 };
 
 struct Params {
@@ -100,13 +101,15 @@ struct Params {
   uint32_t* ticket;
   int batch, hq, hkv, group, sq, skv, nq, nk;
   int units;
+  int wave;                          // (batch, key/value head, half) rows whose key tiles are interleaved
   int causal;
   float scale, scale_log2;
   uint32_t* status;
 };
 
 // One unit: key tile j of (b, kvh), column half `half`; its steps visit, for each query head of the
-// group, the query tiles nq-1 .. i_min.
+// group, the query tiles nq-1 .. i_min.  Units are numbered wave by wave: within a wave of p.wave
+// (b, kvh, half) rows, all their first key tiles, then all their second ones, and so on.
 struct Unit {
   int b, kvh, j, half, i_min, per_head, steps;
 };
@@ -115,12 +118,16 @@ template <int D>
 __device__ __forceinline__ Unit decode_unit(const Params& p, int u) {
   using C = Cfg<D>;
   Unit x;
-  x.half = u % C::kSplit;
-  u /= C::kSplit;
-  x.j = u % p.nk;
-  u /= p.nk;
-  x.kvh = u % p.hkv;
-  x.b = u / p.hkv;
+  const int rows = p.batch * p.hkv * C::kSplit;
+  const int first = u / (p.wave * p.nk) * p.wave;  // first row of the wave
+  const int in_wave = min(p.wave, rows - first);
+  u -= first * p.nk;
+  x.j = u / in_wave;
+  int row = first + u - x.j * in_wave;
+  x.half = row % C::kSplit;
+  row /= C::kSplit;
+  x.kvh = row % p.hkv;
+  x.b = row / p.hkv;
   x.i_min = p.causal ? x.j * (kBK / C::kBQ) : 0;
   x.per_head = max(0, p.nq - x.i_min);
   x.steps = x.per_head * p.group;
@@ -162,10 +169,64 @@ __device__ __forceinline__ bool wait_turn(const uint32_t* turn, uint32_t want, u
         ok = false;
         break;
       }
-      __nanosleep(64);
+      __nanosleep(20);
     }
   }
   return __all_sync(0xffffffffu, ok);
+}
+
+// 16 lanes x 8 N columns of TMEM, dealt out like an mma accumulator: thread l gets, of every 8 columns i,
+// r[4i], r[4i+1] = columns 2 (l % 4), + 1 of lane l / 4 and r[4i+2], r[4i+3] the same of lane l / 4 + 8.
+// No wait.
+template <int N>
+__device__ __forceinline__ void tmem_ld_frag(uint32_t a, uint32_t* r) {
+  static_assert(N == 4 || N == 8, "groups of columns");
+  if constexpr (N == 8) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(a)
+        : "memory");
+  } else {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(a)
+        : "memory");
+  }
+}
+
+// The counterpart for values packed in pairs: 16 lanes x 4 N 32-bit columns, r[2i] of lane l / 4, r[2i+1] of
+// lane l / 4 + 8, column 4 i + l % 4.
+template <int N>
+__device__ __forceinline__ void tmem_st_frag(uint32_t a, const uint32_t* r) {
+  static_assert(N == 4 || N == 8, "groups of columns");
+  if constexpr (N == 8) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(a),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+  } else {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"r"(a), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+  }
+}
+
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// Four 8 x 8 matrices of 16-bit values from such a layout to shared memory; lane l gives the address
+// of row l % 8 of matrix l / 8.
+__device__ __forceinline__ void st_matrix_x4(uint32_t addr, const uint32_t* r) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3])
+               : "memory");
 }
 
 template <int N>
@@ -187,8 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                    const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                    const Params p) {
   using C = Cfg<D>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];  // no room is left to round its start up
   __shared__ uint64_t bar_unit_full[2], bar_unit_empty[2], bar_kv_full, bar_kv_empty, bar_q_full[2], bar_q_empty[2],
       bar_do_full[2], bar_do_empty[2], bar_s, bar_p, bar_dp, bar_ds, bar_dq, bar_dqfree, bar_acc, bar_accfree, bar_drain;
   __shared__ int unit_ring[2];
@@ -196,6 +256,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int warp = warp_id();
   const int lane = lane_id();
+  if ((smem_u32(smem) & 1023u) != 0u) {  // the swizzled tiles would lie wrong
+    if (threadIdx.x == 0) record_status(p.status, kDevBadArgs);
+    return;
+  }
 
   if (threadIdx.x == 0) {
     cta_abort_flag() = 0u;
@@ -454,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) {
               __threadfence();
-              asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(turn), "r"(static_cast<uint32_t>(x.j + 1)) : "memory");
+              asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(turn), "r"(static_cast<uint32_t>(x.j + 1)) : "memory");
             }
           } else {
             // the last key tile: the sum is complete
@@ -494,13 +558,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------------ softmax warps, epilogue of dV and dK
     asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     const int wg = warp >> 2;
-    const int row = (warp & 3) * 32 + lane;  // key of the tile
+    const int row = (warp & 3) * 32 + lane;  // key of the tile (epilogue)
     const uint32_t lanes = tmem_addr(tbase, (warp & 3) * 32, 0);
     const uint32_t col_s = lanes + C::kColS + wg * C::kHalfQ;
     const uint32_t col_dp = lanes + C::kColDp + wg * C::kHalfQ;
-    uint8_t* ds_row = smem + C::kDs + (C::kHalfQ == 64 ? wg * C::kKBox : 0);
-    constexpr int kChunk0 = 0;
-    const int chunk0 = C::kHalfQ == 64 ? kChunk0 : wg * 4;  // first 16-byte piece of this warpgroup's part of a dS row
+    constexpr int kGroups = C::kHalfQ / 8;  // groups of 8 query columns
+    // this lane's row and first piece in the matrices it stores: matrix l / 8 is the lower (upper) 8 keys of 16
+    // in an even (odd) group of 8 queries
+    const uint32_t ds_base = smem_u32(smem + C::kDs + (C::kHalfQ == 64 ? wg * C::kKBox : 0));
+    const int st_row = (warp & 3) * 32 + ((lane >> 3) & 1) * 8 + (lane & 7);
+    const int st_piece = (lane >> 4) + (C::kHalfQ == 64 ? 0 : wg * 4);
     const float c = p.scale_log2;
     bool ok = true;
     int g = 0, active = 0;
@@ -521,72 +588,95 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
           tc_fence_after();
-          const float4* lse2 = reinterpret_cast<const float4*>(smem + C::kStat + qs * C::kStatBytes) + wg * (C::kHalfQ / 4);
-          const float4* delta = lse2 + C::kBQ / 4;
+          // this lane's two query columns of every group of 8
+          const float2* lse2 = reinterpret_cast<const float2*>(smem + C::kStat + qs * C::kStatBytes) + wg * (C::kHalfQ / 2) +
+                               (lane & 3);
+          const float2* delta = lse2 + C::kBQ / 2;
           const int q0 = i * C::kBQ + wg * C::kHalfQ;
-          // query columns before `first` are masked for this key
           const bool masked = ragged || (p.causal && q0 < x.j * kBK + kBK - 1);
-          const int first = key >= p.skv ? C::kHalfQ : (p.causal ? key - q0 : 0);
-          float pr[C::kHalfQ];
+          // fragment (h16, rg): key (warp & 3) * 32 + h16 * 16 + rg * 8 + lane / 4
+          const int key0 = x.j * kBK + (warp & 3) * 32 + (lane >> 2);
+          uint32_t raw[2][4 * kGroups];
+          tmem_ld_frag<kGroups>(col_s, raw[0]);
+          tmem_ld_frag<kGroups>(col_s + (16u << 16), raw[1]);
+          float pr[2][4 * kGroups];
+          float2 st[kGroups];
 #pragma unroll
-          for (int ch = 0; ch < C::kHalfQ / 32; ++ch) {
-            uint32_t s[32];
-            tmem_ld32(col_s + ch * 32, s);
+          for (int n = 0; n < kGroups; ++n) st[n] = lse2[4 * n];
+          tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float4 l = lse2[ch * 8 + e];
-              const int n = ch * 32 + e * 4;
-              pr[n] = ex2_approx(fmaf(__uint_as_float(s[e * 4]), c, -l.x));
-              pr[n + 1] = ex2_approx(fmaf(__uint_as_float(s[e * 4 + 1]), c, -l.y));
-              pr[n + 2] = ex2_approx(fmaf(__uint_as_float(s[e * 4 + 2]), c, -l.z));
-              pr[n + 3] = ex2_approx(fmaf(__uint_as_float(s[e * 4 + 3]), c, -l.w));
+          for (int h16 = 0; h16 < 2; ++h16) {
+#pragma unroll
+            for (int n = 0; n < kGroups; ++n) {
+#pragma unroll
+              for (int rg = 0; rg < 2; ++rg) {
+                const int e = 4 * n + 2 * rg;
+                pr[h16][e] = ex2_approx(fmaf(__uint_as_float(raw[h16][e]), c, -st[n].x));
+                pr[h16][e + 1] = ex2_approx(fmaf(__uint_as_float(raw[h16][e + 1]), c, -st[n].y));
+              }
             }
             if (masked) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (ch * 32 + e < first) pr[ch * 32 + e] = 0.0f;
-            }
-            uint32_t packed[16];
+              for (int rg = 0; rg < 2; ++rg) {
+                const int key = key0 + h16 * 16 + rg * 8;
+                // query columns before `first` are masked for this key
+                const int first = (key >= p.skv ? C::kHalfQ : (p.causal ? key - q0 : 0)) - 2 * (lane & 3);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) packed[e] = pack_bf16x2(pr[ch * 32 + 2 * e], pr[ch * 32 + 2 * e + 1]);
-            tmem_st16(col_s + ch * 16, packed);
+                for (int n = 0; n < kGroups; ++n) {
+                  if (8 * n < first) pr[h16][4 * n + 2 * rg] = 0.0f;
+                  if (8 * n + 1 < first) pr[h16][4 * n + 2 * rg + 1] = 0.0f;
+                }
+              }
+            }
+            uint32_t packed[2 * kGroups];
+#pragma unroll
+            for (int e = 0; e < 2 * kGroups; ++e) packed[e] = pack_bf16x2(pr[h16][2 * e], pr[h16][2 * e + 1]);
+            tmem_st_frag<kGroups>(col_s + (static_cast<uint32_t>(h16 * 16) << 16), packed);
           }
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bar_p);
+#pragma unroll
+          for (int n = 0; n < kGroups; ++n) st[n] = delta[4 * n];
           if (!__all_sync(0xffffffffu, mbar_wait(&bar_dp, g & 1, p.status, kDevTimeoutMma))) {
             ok = false;
             break;
           }
           tc_fence_after();
+          tmem_ld_frag<kGroups>(col_dp, raw[0]);
+          tmem_ld_frag<kGroups>(col_dp + (16u << 16), raw[1]);
+          tmem_wait_ld();
 #pragma unroll
-          for (int ch = 0; ch < C::kHalfQ / 32; ++ch) {
-            uint32_t dp[32];
-            tmem_ld32(col_dp + ch * 32, dp);
-            float ds[32];
+          for (int h16 = 0; h16 < 2; ++h16) {
+            float ds[4 * kGroups];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float4 d = delta[ch * 8 + e];
-              const int n = ch * 32 + e * 4;
-              ds[e * 4] = pr[n] * (__uint_as_float(dp[e * 4]) - d.x);
-              ds[e * 4 + 1] = pr[n + 1] * (__uint_as_float(dp[e * 4 + 1]) - d.y);
-              ds[e * 4 + 2] = pr[n + 2] * (__uint_as_float(dp[e * 4 + 2]) - d.z);
-              ds[e * 4 + 3] = pr[n + 3] * (__uint_as_float(dp[e * 4 + 3]) - d.w);
+            for (int n = 0; n < kGroups; ++n) {
+#pragma unroll
+              for (int rg = 0; rg < 2; ++rg) {
+                const int e = 4 * n + 2 * rg;
+                ds[e] = pr[h16][e] * (__uint_as_float(raw[h16][e]) - st[n].x);
+                ds[e + 1] = pr[h16][e + 1] * (__uint_as_float(raw[h16][e + 1]) - st[n].y);
+              }
             }
             if (masked) {  // dP may be infinite or NaN there
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (ch * 32 + e < first) ds[e] = 0.0f;
+              for (int rg = 0; rg < 2; ++rg) {
+                const int key = key0 + h16 * 16 + rg * 8;
+                const int first = (key >= p.skv ? C::kHalfQ : (p.causal ? key - q0 : 0)) - 2 * (lane & 3);
+#pragma unroll
+                for (int n = 0; n < kGroups; ++n) {
+                  if (8 * n < first) ds[4 * n + 2 * rg] = 0.0f;
+                  if (8 * n + 1 < first) ds[4 * n + 2 * rg + 1] = 0.0f;
+                }
+              }
             }
 #pragma unroll
-            for (int v4 = 0; v4 < 4; ++v4) {
-              uint4 w;
-              w.x = pack_bf16x2(ds[v4 * 8], ds[v4 * 8 + 1]);
-              w.y = pack_bf16x2(ds[v4 * 8 + 2], ds[v4 * 8 + 3]);
-              w.z = pack_bf16x2(ds[v4 * 8 + 4], ds[v4 * 8 + 5]);
-              w.w = pack_bf16x2(ds[v4 * 8 + 6], ds[v4 * 8 + 7]);
-              *reinterpret_cast<uint4*>(ds_row + sw128_offset(row, (chunk0 + ch * 4 + v4) * 16)) = w;
+            for (int n = 0; n < kGroups; n += 2) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(ds[4 * n + 2 * e], ds[4 * n + 2 * e + 1]);
+              st_matrix_x4(ds_base + sw128_offset(st_row + h16 * 16, (st_piece + n) * 16), w);
             }
           }
           fence_async_smem();
@@ -756,11 +846,12 @@ int launch(const void* dout, const void* q, const void* k, const void* v, const 
   if (units > 0x3FFFFFFFll || steps > 0x3FFFFFFFll)
     return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_fa2_bwd: too many tiles (%lld x %lld)", units, steps);
   p.units = static_cast<int>(units);
+  p.wave = (std::max(1, device_sm_count()) + kWaveCtas - 1) / kWaveCtas;
 
   const long long rows = static_cast<long long>(batch) * hq * p.nq * C::kBQ;
   const long long blocks = (rows * (D / 8) + 255) / 256;
   if (blocks > 0x7FFFFFFFll) return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_fa2_bwd: too many rows (%lld)", rows);
-  const int smem_bytes = C::kBytes + 1024;
+  const int smem_bytes = C::kBytes;
   if (!ensure_smem_attr(reinterpret_cast<const void*>(&fa2_bwd_kernel<D>), smem_bytes))
     return check_launch("tokmix_fa2_bwd: cudaFuncSetAttribute");
   cudaError_t e = launch_overlapped(&fa2_bwd_prep<D>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream,
