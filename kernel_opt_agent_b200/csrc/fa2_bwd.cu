@@ -141,6 +141,17 @@ __device__ __forceinline__ int contributors(const Params& p, int i) {
   return min(p.nk, (min((i + 1) * Cfg<D>::kBQ, p.sq) - 1) / kBK + 1);
 }
 
+// One lane of the (whole) warp, the same on every call.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(is));
+  return is != 0;
+}
+
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
                    smem_u32(dst)),
@@ -375,92 +386,120 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
     } else if (warp == kWarpMma) {
       // ---------------------------------------------------------------- MMA issuer
-      if (lane == 0) {
-        constexpr uint32_t idesc_s = make_idesc(kBK, C::kBQ, 1, 0, 0);
-        constexpr uint32_t idesc_kv = make_idesc(kBK, C::kDH, 1, 0, 1);
-        constexpr uint32_t idesc_dq = C::kTransDq ? make_idesc(C::kDH, C::kBQ, 1, 1, 1) : make_idesc(C::kBQ, C::kDH, 1, 1, 1);
-        const uint32_t k_addr = smem_u32(smem + C::kK), v_addr = smem_u32(smem + C::kV), ds_addr = smem_u32(smem + C::kDs);
-        const uint32_t q_base = smem_u32(smem + C::kQ), do_base = smem_u32(smem + C::kDO);
-        // X^T = A B^T over head_dim: S^T = K Q^T, dP^T = V dO^T (all K-major)
-        auto issue_scores = [&](uint32_t a, uint32_t b, uint32_t col) {
+      // The whole warp walks the steps and waits, one elected lane issues: so addresses and
+      // descriptors are warp-uniform (issued from a branch of one lane, an MMA took 75 to 135 cycles
+      // instead of the tensor core's 64, D 128).
+      constexpr uint32_t idesc_s = make_idesc(kBK, C::kBQ, 1, 0, 0);
+      constexpr uint32_t idesc_kv = make_idesc(kBK, C::kDH, 1, 0, 1);
+      constexpr uint32_t idesc_dq = C::kTransDq ? make_idesc(C::kDH, C::kBQ, 1, 1, 1) : make_idesc(C::kBQ, C::kDH, 1, 1, 1);
+      const uint32_t tb = __shfl_sync(0xffffffffu, tbase, 0);
+      const uint32_t base = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
+      const bool leader = elect_one();
+      const uint32_t k_addr = base + C::kK, v_addr = base + C::kV, ds_addr = base + C::kDs;
+      const uint32_t q_base = base + C::kQ, do_base = base + C::kDO;
+      // X^T = A B^T over head_dim: S^T = K Q^T, dP^T = V dO^T (all K-major)
+      auto issue_scores = [&](uint32_t a, uint32_t b, uint32_t col) {
+        const uint64_t ad = make_sdesc_sw128(a, 16, 1024), bd = make_sdesc_sw128(b, 16, 1024);
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            umma_bf16_ss(tbase + col, make_sdesc_sw128(a + (kk >> 2) * C::kKBox + (kk & 3) * 32, 16, 1024),
-                         make_sdesc_sw128(b + (kk >> 2) * C::kQBox + (kk & 3) * 32, 16, 1024), idesc_s, kk > 0 ? 1u : 0u);
-        };
-        bool ok = true;
-        int g = 0;          // steps of earlier units
-        int active = 0;     // earlier units with steps (K/V and accumulator phases)
-        for (int r = 0; ok; ++r) {
-          const int u = next_unit(r, ok);
-          if (!ok || u < 0) break;
-          mbar_arrive(&bar_unit_empty[r & 1]);
-          const Unit x = decode_unit<D>(p, u);
-          if (x.steps == 0) continue;
-          const uint32_t half_k = x.half * (C::kDH / 64) * C::kKBox, half_q = x.half * (C::kDH / 64) * C::kQBox;
-          auto issue_s = [&](int gs) -> bool {
-            const int st = gs % C::kNQ;
-            if (!mbar_wait(&bar_q_full[st], (gs / C::kNQ) & 1, p.status, kDevTimeoutTma)) return false;
-            tc_fence_after();
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_bf16_ss(tb + col, ad + (((kk >> 2) * C::kKBox + (kk & 3) * 32) >> 4), bd + (((kk >> 2) * C::kQBox + (kk & 3) * 32) >> 4),
+                       idesc_s, kk > 0 ? 1u : 0u);
+      };
+      bool ok = true;
+      int g = 0;          // steps of earlier units
+      int active = 0;     // earlier units with steps (K/V and accumulator phases)
+      auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
+        return static_cast<bool>(__all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, code)));
+      };
+      for (int r = 0; ok; ++r) {
+        const int u = __shfl_sync(0xffffffffu, next_unit(r, ok), 0);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok || u < 0) break;
+        if (leader) mbar_arrive(&bar_unit_empty[r & 1]);
+        const Unit x = decode_unit<D>(p, u);
+        if (x.steps == 0) continue;
+        const uint32_t half_k = x.half * (C::kDH / 64) * C::kKBox, half_q = x.half * (C::kDH / 64) * C::kQBox;
+        auto issue_s = [&](int gs) -> bool {
+          const int st = gs % C::kNQ;
+          if (!wait(&bar_q_full[st], (gs / C::kNQ) & 1, kDevTimeoutTma)) return false;
+          tc_fence_after();
+          if (leader) {
             issue_scores(k_addr, q_base + st * C::kQBytes, C::kColS);
             umma_commit(&bar_s);
-            return true;
-          };
-          ok = mbar_wait(&bar_kv_full, active & 1, p.status, kDevTimeoutTma) && issue_s(g);
-          for (int t = 0; ok && t < x.steps; ++t) {
-            const int gt = g + t, qs = gt % C::kNQ, dos = gt % C::kNDO;
-            const uint32_t q_addr = q_base + qs * C::kQBytes + half_q, do_addr = do_base + dos * C::kQBytes;
-            // dP(t); its columns hold dQ(t-1) until the dQ warps have read it
-            ok = mbar_wait(&bar_do_full[dos], (gt / C::kNDO) & 1, p.status, kDevTimeoutTma) &&
-                 (!C::kAlias || gt == 0 || mbar_wait(&bar_dqfree, (gt - 1) & 1, p.status, kDevTimeoutPipe));
-            if (!ok) break;
-            tc_fence_after();
+          }
+          __syncwarp();
+          return true;
+        };
+        ok = wait(&bar_kv_full, active & 1, kDevTimeoutTma) && issue_s(g);
+        for (int t = 0; ok && t < x.steps; ++t) {
+          const int gt = g + t, qs = gt % C::kNQ, dos = gt % C::kNDO;
+          const uint32_t q_addr = q_base + qs * C::kQBytes, do_addr = do_base + dos * C::kQBytes;
+          // dP(t); its columns hold dQ(t-1) until the dQ warps have read it
+          ok = wait(&bar_do_full[dos], (gt / C::kNDO) & 1, kDevTimeoutTma) &&
+               (!C::kAlias || gt == 0 || wait(&bar_dqfree, (gt - 1) & 1, kDevTimeoutPipe));
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
             issue_scores(v_addr, do_addr, C::kColDp);
             umma_commit(&bar_dp);
-            // dV += P^T dO; the first overwrites an accumulator that the previous unit's epilogue has read
-            ok = mbar_wait(&bar_p, gt & 1, p.status, kDevTimeoutPipe) &&
-                 (t > 0 || active == 0 || mbar_wait(&bar_accfree, (active - 1) & 1, p.status, kDevTimeoutPipe));
-            if (!ok) break;
-            tc_fence_after();
+          }
+          __syncwarp();
+          // dV += P^T dO; the first overwrites an accumulator that the previous unit's epilogue has read
+          ok = wait(&bar_p, gt & 1, kDevTimeoutPipe) &&
+               (t > 0 || active == 0 || wait(&bar_accfree, (active - 1) & 1, kDevTimeoutPipe));
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
+            const uint64_t bd = make_sdesc_sw128(do_addr + half_q, C::kQBox, 1024);
 #pragma unroll
             for (int kk = 0; kk < C::kBQ / 16; ++kk) {
               constexpr int per = C::kHalfQ / 16;  // steps in a warpgroup's part of P
-              const uint32_t a = tbase + C::kColS + (kk / per) * C::kHalfQ + (kk % per) * 8;
-              umma_bf16_ts(tbase + C::kColDv, a, make_sdesc_sw128(do_addr + half_q + kk * 2048, C::kQBox, 1024), idesc_kv,
-                           (t > 0 || kk > 0) ? 1u : 0u);
+              umma_bf16_ts(tb + C::kColDv, tb + C::kColS + (kk / per) * C::kHalfQ + (kk % per) * 8, bd + ((kk * 2048) >> 4),
+                           idesc_kv, (t > 0 || kk > 0) ? 1u : 0u);
             }
             umma_commit(&bar_do_empty[dos]);
-            if (C::kAhead && t + 1 < x.steps) {
-              ok = issue_s(gt + 1);
-              if (!ok) break;
-            }
-            ok = mbar_wait(&bar_ds, gt & 1, p.status, kDevTimeoutPipe) &&
-                 (C::kAlias || gt == 0 || mbar_wait(&bar_dqfree, (gt - 1) & 1, p.status, kDevTimeoutPipe));
+          }
+          __syncwarp();
+          if (C::kAhead && t + 1 < x.steps) {
+            ok = issue_s(gt + 1);
             if (!ok) break;
-            tc_fence_after();
+          }
+          ok = wait(&bar_ds, gt & 1, kDevTimeoutPipe) &&
+               (C::kAlias || gt == 0 || wait(&bar_dqfree, (gt - 1) & 1, kDevTimeoutPipe));
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
             // dQ = dS K (or its transpose)
+            const uint64_t dsd = make_sdesc_sw128(ds_addr, C::kKBox, 1024);
+            const uint64_t kd = make_sdesc_sw128(k_addr + half_k, C::kKBox, 1024);
 #pragma unroll
-            for (int kk = 0; kk < kBK / 16; ++kk) {
-              const uint64_t dsd = make_sdesc_sw128(ds_addr + kk * 2048, C::kKBox, 1024);
-              const uint64_t kd = make_sdesc_sw128(k_addr + half_k + kk * 2048, C::kKBox, 1024);
-              umma_bf16_ss(tbase + C::kColDq, C::kTransDq ? kd : dsd, C::kTransDq ? dsd : kd, idesc_dq, kk > 0 ? 1u : 0u);
-            }
+            for (int kk = 0; kk < kBK / 16; ++kk)
+              umma_bf16_ss(tb + C::kColDq, (C::kTransDq ? kd : dsd) + ((kk * 2048) >> 4),
+                           (C::kTransDq ? dsd : kd) + ((kk * 2048) >> 4), idesc_dq, kk > 0 ? 1u : 0u);
             umma_commit(&bar_dq);
             // dK += dS^T Q
+            const uint64_t dsk = make_sdesc_sw128(ds_addr, 16, 1024);
+            const uint64_t qd = make_sdesc_sw128(q_addr + half_q, C::kQBox, 1024);
 #pragma unroll
             for (int kk = 0; kk < C::kBQ / 16; ++kk)
-              umma_bf16_ss(tbase + C::kColDk, make_sdesc_sw128(ds_addr + (kk >> 2) * C::kKBox + (kk & 3) * 32, 16, 1024),
-                           make_sdesc_sw128(q_addr + kk * 2048, C::kQBox, 1024), idesc_kv, (t > 0 || kk > 0) ? 1u : 0u);
+              umma_bf16_ss(tb + C::kColDk, dsk + (((kk >> 2) * C::kKBox + (kk & 3) * 32) >> 4), qd + ((kk * 2048) >> 4), idesc_kv,
+                           (t > 0 || kk > 0) ? 1u : 0u);
             umma_commit(&bar_q_empty[qs]);
-            if (!C::kAhead && t + 1 < x.steps) ok = issue_s(gt + 1);
           }
-          if (!ok) break;
+          __syncwarp();
+          if (!C::kAhead && t + 1 < x.steps) ok = issue_s(gt + 1);
+        }
+        if (!ok) break;
+        if (leader) {
           umma_commit(&bar_acc);
           umma_commit(&bar_kv_empty);
-          g += x.steps;
-          ++active;
         }
-        // every MMA issued by this thread completes before TMEM is released (bounded)
+        __syncwarp();
+        g += x.steps;
+        ++active;
+      }
+      // every MMA issued completes before TMEM is released (bounded)
+      if (leader) {
         umma_commit(&bar_drain);
         mbar_drain(&bar_drain, 0);
       }
