@@ -107,8 +107,9 @@ struct Params {
   uint32_t* status;
 };
 
-// One unit: key tile j of (b, kvh), column half `half`; its steps visit, for each query head of the
-// group, the query tiles nq-1 .. i_min.  Units are numbered wave by wave: within a wave of p.wave
+// One unit: key tile j of (b, kvh), column half `half`; its steps visit the query tiles nq-1 .. i_min, each for
+// every query head of the group (heads inside tiles: head by head, a later and shorter unit could not
+// pass the earlier one into the next head, B2 Hq16 Hkv2 S4096 D256 took 2490 us).  Units are numbered wave by wave: within a wave of p.wave
 // (b, kvh, half) rows, all their first key tiles, then all their second ones, and so on.
 struct Unit {
   int b, kvh, j, half, i_min, per_head, steps;
@@ -337,10 +338,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (u < 0) break;
           const Unit x = decode_unit<D>(p, u);
           int t = 0;
-          for (int h = 0; ok && h < p.group; ++h) {
-            const int head = x.kvh * p.group + h;
-            const long long bh = static_cast<long long>(x.b) * p.hq + head;
-            for (int i = p.nq - 1; i >= x.i_min; --i, ++t, ++g) {
+          for (int i = p.nq - 1; ok && i >= x.i_min; --i) {
+            for (int h = 0; h < p.group; ++h, ++t, ++g) {
+              const int head = x.kvh * p.group + h;
+              const long long bh = static_cast<long long>(x.b) * p.hq + head;
               const int qs = g % C::kNQ, ds = g % C::kNDO;
               if (g >= C::kNQ && !mbar_wait(&bar_q_empty[qs], (g / C::kNQ - 1) & 1, p.status, kDevTimeoutPipe)) {
                 ok = false;
@@ -519,10 +520,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok || u < 0) break;
       if (lane == 0) mbar_arrive(&bar_unit_empty[r & 1]);
       const Unit x = decode_unit<D>(p, u);
-      for (int h = 0; ok && h < p.group; ++h) {
-        const int head = x.kvh * p.group + h;
-        const long long bh = static_cast<long long>(x.b) * p.hq + head;
-        for (int i = p.nq - 1; i >= x.i_min; --i, ++g) {
+      for (int i = p.nq - 1; ok && i >= x.i_min; --i) {
+        for (int h = 0; h < p.group; ++h, ++g) {
+          const int head = x.kvh * p.group + h;
+          const long long bh = static_cast<long long>(x.b) * p.hq + head;
           const long long tile = (bh * p.nq + i) * C::kSplit + x.half;
           uint32_t* turn = p.turns + tile * 4 + wq;
           const int count = contributors<D>(p, i);
@@ -618,8 +619,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Unit x = decode_unit<D>(p, u);
       const int key = x.j * kBK + row;
       const bool ragged = x.j * kBK + kBK > p.skv;  // keys behind the last one
-      for (int h = 0; ok && h < p.group; ++h) {
-        for (int i = p.nq - 1; i >= x.i_min; --i, ++g) {
+      for (int i = p.nq - 1; ok && i >= x.i_min; --i) {
+        for (int h = 0; h < p.group; ++h, ++g) {
           const int qs = g % C::kNQ;
           if (!__all_sync(0xffffffffu, mbar_wait(&bar_q_full[qs], (g / C::kNQ) & 1, p.status, kDevTimeoutTma) &&
                                            mbar_wait(&bar_s, g & 1, p.status, kDevTimeoutMma))) {
