@@ -311,6 +311,48 @@ int tokmix_qkv_part_rope(const void* qkv, const float* cos, const float* sin, vo
 int tokmix_add_rms_norm_quant(const void* x, const void* residual, const void* weight, void* residual_out, void* y_fp8,
                               float* y_scale, int rows, int n, int group, int dtype, float eps, void* stream);
 
+/* ---- RMS norm of each query and key head with the position rotation, and its gradient (the reference rotates without a norm:
+ * qkv_part_rope) ---- */
+
+/* One call.  q [batch, seqlen, heads_q, head_dim] and k [..., heads_k, ...] in `dtype` (bf16 or fp16): element strides given, multiples
+ * of 8, head_dim contiguous, 16-byte aligned.  For every head row x with its weight w [head_dim] (`weight_dtype`: dtype or fp32):
+ *   n = x / sqrt(mean x^2 + eps) * w;  y = n with the pairs (j, j + half) of the 2 half columns behind `nope` rotated:
+ *   y_j = n_j cos - n_{j+half} sin,  y_{j+half} = n_j sin + n_{j+half} cos
+ * in fp32, rounded once.  cos, sin: fp32 [table_rows, half].  positions: the table row of every token, int32 [axes, batch, seqlen], or
+ * NULL: the token's index in its sequence (axes 1).  axes 2 to 4: pair j takes its row from axis pair_axis[j] (host memory,
+ * half entries, read during the call).  head_dim 64, 128 or 256; half and nope multiples of 8, half > 0.
+ * Forward: q_out, k_out contiguous [batch, seqlen, heads, head_dim].  Backward: dq, dk are the gradients of those outputs (strides
+ * like q's), and q_out, k_out receive the gradients of q and k.
+ * A position outside the tables is not followed: it gives NaN in the token's rotated columns (backward: its rows and the weights'
+ * gradients) and sets TOKMIX_DEV_BAD_ARGS in *status (device memory or mapped host memory). */
+typedef struct tokmix_qk_norm_rope {
+  const void* q;
+  const void* k;
+  const void* q_weight;
+  const void* k_weight;
+  const float* cos;
+  const float* sin;
+  const int32_t* positions;
+  const uint8_t* pair_axis;
+  const void* dq;
+  const void* dk;
+  void* q_out;
+  void* k_out;
+  long long q_batch_stride, q_token_stride, q_head_stride, k_batch_stride, k_token_stride, k_head_stride;
+  long long dq_batch_stride, dq_token_stride, dq_head_stride, dk_batch_stride, dk_token_stride, dk_head_stride;
+  int batch, seqlen, heads_q, heads_k, head_dim, half, nope, axes, table_rows, dtype, weight_dtype;
+  float eps;
+} tokmix_qk_norm_rope;
+
+int tokmix_qk_norm_rope_fwd(const tokmix_qk_norm_rope* args, uint32_t* status, void* stream);
+
+/* The gradients; dq_weight, dk_weight [head_dim] in weight_dtype are summed over all tokens and heads in fp32, in an order that
+ * sizes alone decide.  workspace: tokmix_qk_norm_rope_bwd_workspace_bytes(batch * seqlen, ...) bytes of device memory, 16-byte aligned,
+ * not shared by calls that may overlap. */
+int tokmix_qk_norm_rope_bwd(const tokmix_qk_norm_rope* args, void* dq_weight, void* dk_weight, void* workspace,
+                            long long workspace_bytes, uint32_t* status, void* stream);
+long long tokmix_qk_norm_rope_bwd_workspace_bytes(long long tokens, int heads_q, int heads_k, int head_dim);
+
 /* ---- a paged key/value cache held in 8 bits, and the decode attention that reads it (no counterpart
  * in the reference, whose attention is prefill only) ---- */
 

@@ -70,6 +70,9 @@ SIGNATURES = {
     "tokmix_swiglu_input_quant": (_I, [_VP, _VP, _VP, _VP, _I, _I, _F, _VP]),
     "tokmix_qkv_part_rope": (_I, [_VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _I, _VP]),
     "tokmix_add_rms_norm_quant": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _F, _VP]),
+    "tokmix_qk_norm_rope_fwd": (_I, [_VP, _VP, _VP]),
+    "tokmix_qk_norm_rope_bwd": (_I, [_VP, _VP, _VP, _VP, _LL, _VP, _VP]),
+    "tokmix_qk_norm_rope_bwd_workspace_bytes": (_LL, [_LL, _I, _I, _I]),
     "tokmix_kv8_append": (_I, [_VP, _LL, _LL, _LL, _VP, _LL, _LL, _LL, _I, _I, _VP, _VP, _VP]),
     "tokmix_kv8_attention": (_I, [_VP, _LL, _LL, _LL, _VP, _VP, _I, _I, _I, _F, _VP, _VP, _LL, _VP, _VP]),
     "tokmix_kv8_attention_workspace_bytes": (_LL, [_I, _I, _I, _I]),
@@ -95,6 +98,17 @@ class Kv8Cache(ctypes.Structure):
                 ("block_table", _VP), ("table_stride", _LL), ("seq_lens", _VP), ("new_lens", _VP),
                 ("num_pages", _I), ("page_size", _I), ("heads_kv", _I), ("head_dim", _I), ("dtype", _I),
                 ("batch", _I), ("max_pages", _I)]
+
+
+class QkNormRope(ctypes.Structure):
+    """tokmix_qk_norm_rope: one call of the head norm with rotation, or of its gradient."""
+
+    _fields_ = [(n, _VP) for n in ("q", "k", "q_weight", "k_weight", "cos", "sin", "positions", "pair_axis", "dq", "dk",
+                                   "q_out", "k_out")]
+    _fields_ += [(f"{t}_{d}_stride", _LL) for t in ("q", "k", "dq", "dk") for d in ("batch", "token", "head")]
+    _fields_ += [(n, _I) for n in ("batch", "seqlen", "heads_q", "heads_k", "head_dim", "half", "nope", "axes", "table_rows",
+                                   "dtype", "weight_dtype")]
+    _fields_ += [("eps", _F)]
 
 
 _lib = None

@@ -54,7 +54,6 @@ constexpr int kThreads = 512;
 constexpr int kSoftmaxWarps = 8, kDqWarps = 4;
 constexpr int kWarpTma = 12, kWarpMma = 13;
 constexpr int kUnitReaders = 1 + kSoftmaxWarps + kDqWarps;
-constexpr int kWaveCtas = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D>
@@ -112,7 +111,7 @@ struct Params {
 // pass the earlier one into the next head, B2 Hq16 Hkv2 S4096 D256 took 2490 us).  Units are numbered wave by wave: within a wave of p.wave
 // (b, kvh, half) rows, all their first key tiles, then all their second ones, and so on.
 struct Unit {
-  int b, kvh, j, half, i_min, per_head, steps;
+  int b, kvh, j, half, i_min, steps;
 };
 
 template <int D>
@@ -130,8 +129,7 @@ __device__ __forceinline__ Unit decode_unit(const Params& p, int u) {
   x.kvh = row % p.hkv;
   x.b = row / p.hkv;
   x.i_min = p.causal ? x.j * (kBK / C::kBQ) : 0;
-  x.per_head = max(0, p.nq - x.i_min);
-  x.steps = x.per_head * p.group;
+  x.steps = max(0, p.nq - x.i_min) * p.group;
   return x;
 }
 
@@ -886,7 +884,11 @@ int launch(const void* dout, const void* q, const void* k, const void* v, const 
   if (units > 0x3FFFFFFFll || steps > 0x3FFFFFFFll)
     return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_fa2_bwd: too many tiles (%lld x %lld)", units, steps);
   p.units = static_cast<int>(units);
-  p.wave = (std::max(1, device_sm_count()) + kWaveCtas - 1) / kWaveCtas;
+  // CTAs of a row run side by side and share its tiles of Q, dO and dQ in L2, each a turn behind the one before:
+  // 4 to a row, 8 where several heads give the turns more time (B4 Hq32 Hkv8 S8192 D128: 6970 us at 4, 6759 at 8,
+  // 6900 at 16; B8 H8 S2048 D128: 298 at 4, 358 at 8, 466 at 16).
+  const int side_by_side = p.group > 1 ? 8 : 4;
+  p.wave = (std::max(1, device_sm_count()) + side_by_side - 1) / side_by_side;
 
   const long long rows = static_cast<long long>(batch) * hq * p.nq * C::kBQ;
   const long long blocks = (rows * (D / 8) + 255) / 256;

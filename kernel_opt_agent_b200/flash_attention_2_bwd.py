@@ -25,7 +25,6 @@ import torch
 
 from . import _lib
 from . import flash_attention_2 as _forward
-from .flash_attention_2 import check_device_status  # noqa: F401  (one status word for both directions)
 
 KERNEL_TYPE = "flash_attention_2_bwd"
 
@@ -47,14 +46,23 @@ def kernel_fn(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
     need = lib.tokmix_fa2_bwd_workspace_bytes(batch, heads, sq, skv, d) if q.numel() else 0
     # from the allocator on every call: calls on several streams and captured graphs do not share it
     workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
-    word = _lib.status_word(dev)
+    status = _lib.host_status_ptr(dev, "flash_attention_2_bwd")
     rc = _lib.call_on(dev, lib.tokmix_fa2_bwd, do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
                       lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), batch, heads, heads_kv, sq, skv, d,
                       _lib.LAYOUT_BHSD if layout == "bhsd" else _lib.LAYOUT_BSHD, 1 if causal else 0, float(sm_scale),
-                      workspace.data_ptr(), need, word.data_ptr(), _lib.stream_ptr(dev))
-    _lib.check(rc, "flash_attention_2_bwd")
-    _lib.after_launch(dev, "flash_attention_2_bwd")
+                      workspace.data_ptr(), need, status, _lib.stream_ptr(dev))
+    if rc:
+        _lib.check(rc, "flash_attention_2_bwd")
+    _lib.after_host_status_launch(dev, "flash_attention_2_bwd")
     return dq, dk, dv
+
+
+def check_device_status(device: torch.device | None = None) -> None:
+    """Synchronise and raise if a call on `device` reported a device-side timeout."""
+    dev = torch.device(device) if device is not None else torch.device("cuda")
+    dev = torch.device("cuda", dev.index if dev.index is not None else torch.cuda.current_device())
+    torch.cuda.synchronize(dev)
+    _lib.take_host_status(dev, "flash_attention_2_bwd")
 
 
 def get_inputs(batch: int = 8, head_num: int = 8, seq_len: int = 2048, head_dim: int = 128,

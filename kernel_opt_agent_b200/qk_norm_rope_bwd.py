@@ -1,0 +1,76 @@
+"""qk_norm_rope_bwd plugin module: the gradients of ``qk_norm_rope``, with the module contract of the reference's
+plugins (``kernels/__init__.py:3-8``).  The reference has no backward pass.
+
+    kernel_fn(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, positions=None, *, eps=1e-6, nope_dim=None,
+              sections=None, interleaved=False) -> (dq, dk, dq_weight, dk_weight)
+
+dq_out, dk_out are the gradients of the forward's outputs, shaped and typed like q and k; everything else as the forward
+took it (nothing needs to be kept from it).  With r = 1 / sqrt(mean(x^2) + eps) and g the gradient turned back by the
+position's angles:
+
+    dweight = sum over rows of g x r,    dx = r (g weight - x r^2 mean(g weight x))
+
+fp32 arithmetic.  dq, dk are contiguous in the type of q; the weights' gradients are summed over all tokens and heads in fp32 in
+an order that sizes alone decide (the same bits every time) and rounded to the weights' type.
+
+``kernel_fn`` runs ``tokmix_qk_norm_rope_bwd`` (``csrc/qk_norm_rope.cu``), no fallback."""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _kv8, _lib
+from . import qk_norm_rope as _forward
+from .qk_norm_rope import check_device_status  # noqa: F401
+
+KERNEL_TYPE = "qk_norm_rope_bwd"
+
+
+def kernel_fn(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
+              k_weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None = None, *,
+              eps: float = 1e-6, nope_dim: int | None = None, sections: tuple | None = None, interleaved: bool = False):
+    args, keep = _forward.describe(q, k, q_weight, k_weight, cos, sin, positions, eps, nope_dim, sections, interleaved)
+    for name, t, x in (("dq_out", dq_out, q), ("dk_out", dk_out, k)):
+        if t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
+            raise ValueError(f"{name} must have the shape, type and device of {name[1]}")
+    dev = q.device
+    dq_out, (args.dq_batch_stride, args.dq_token_stride, args.dq_head_stride) = _kv8.token_strides(dq_out)
+    dk_out, (args.dk_batch_stride, args.dk_token_stride, args.dk_head_stride) = _kv8.token_strides(dk_out)
+    args.dq, args.dk = dq_out.data_ptr(), dk_out.data_ptr()
+    dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    dk = torch.empty(k.shape, dtype=q.dtype, device=dev)
+    args.q_out, args.k_out = dq.data_ptr(), dk.data_ptr()
+    dqw, dkw = torch.empty_like(keep[2]), torch.empty_like(keep[3])
+    lib = _lib.load()
+    need = _lib.call_on(dev, lib.tokmix_qk_norm_rope_bwd_workspace_bytes, q.shape[0] * q.shape[1], q.shape[2], k.shape[2],
+                        q.shape[3])
+    ws = _lib.empty((max(need, 1),), torch.uint8, dev)  # per call: calls may overlap on other streams
+    status = _lib.host_status_ptr(dev, "qk_norm_rope")
+    rc = _lib.call_on(dev, lib.tokmix_qk_norm_rope_bwd, ctypes.byref(args), dqw.data_ptr(), dkw.data_ptr(), ws.data_ptr(),
+                      need, status, _lib.stream_ptr(dev))
+    del keep
+    if rc:
+        _lib.check(rc, "qk_norm_rope_bwd")
+    _lib.after_host_status_launch(dev, "qk_norm_rope")
+    return dq, dk, dqw, dkw
+
+
+def get_inputs(batch: int = 4, seq_len: int = 2048, q_heads: int = 16, kv_heads: int = 2, head_dim: int = 256,
+               pairs: int = 32, dtype: torch.dtype = torch.bfloat16, seed: int = 42, device: str = "cuda") -> dict:
+    inp = _forward.get_inputs(batch, seq_len, q_heads, kv_heads, head_dim, pairs, dtype, seed, device)
+    gen = torch.Generator().manual_seed(seed + 1)
+    return {"dq_out": torch.randn(inp["q"].shape, generator=gen).to(dtype).to(device),
+            "dk_out": torch.randn(inp["k"].shape, generator=gen).to(dtype).to(device), **inp}
+
+
+def get_flops(batch: int = 4, seq_len: int = 2048, q_heads: int = 16, kv_heads: int = 2, head_dim: int = 256) -> int:
+    return 16 * batch * seq_len * (q_heads + kv_heads) * head_dim
+
+
+def get_bytes(batch: int = 4, seq_len: int = 2048, q_heads: int = 16, kv_heads: int = 2, head_dim: int = 256,
+              pairs: int = 32, element_size: int = 2) -> int:
+    """q, k and the outputs' gradients read, dq and dk written once; tables, weights and their gradients once."""
+    return (batch * seq_len * (q_heads + kv_heads) * head_dim * element_size * 3 + seq_len * pairs * 8
+            + 4 * head_dim * element_size)
