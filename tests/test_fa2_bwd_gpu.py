@@ -118,3 +118,160 @@ CASES = [
 @pytest.mark.parametrize("b,hq,hkv,sq,skv,d,causal,layout", CASES)
 def test_gradients_match_the_formula(cuda_device, b, hq, hkv, sq, skv, d, causal, layout):
     check(b, hq, hkv, sq, skv, d, causal, layout, seed=sq + skv + hq)
+
+
+@pytest.mark.parametrize("d,group", [(64, 3), (128, 4), (256, 8)])
+def test_many_tiles_and_waves(cuda_device, d, group):
+    """More units than SMs: every CTA takes several, rows of several waves."""
+    check(3, 4 * group, 4, 1700, 1700, d, True, "bhsd", seed=d)
+
+
+def test_custom_scale_and_sharp_rows(cuda_device):
+    check(1, 4, 2, 300, 300, 128, True, "bhsd", seed=3, scale=0.3)
+    check(1, 2, 1, 300, 333, 64, False, "bshd", seed=4, q_scale=6.0)   # weights of nearly one key
+    check(1, 2, 1, 200, 200, 256, True, "bshd", seed=5, q_scale=0.01)  # nearly flat
+
+
+def test_gradient_against_differences(cuda_device):
+    """The formula that the kernel is tested against is the forward's derivative (float64, central differences)."""
+    q, k, v, do = (t.double() for t in make(1, 2, 1, 9, 9, 64, "bhsd", seed=1))
+
+    def forward(q, k, v):
+        s = q @ k.repeat_interleave(2, 1).transpose(2, 3) * 0.1
+        s = s.masked_fill(~torch.ones(9, 9, dtype=torch.bool, device=s.device).tril(), -math.inf)
+        return torch.softmax(s, -1) @ v.repeat_interleave(2, 1), torch.logsumexp(s, -1)
+
+    o, lse = forward(q, k, v)
+    grads = [x for x, _ in formula(do, q, k, v, o, lse, True, 0.1, "bhsd")]
+    h = 2.0 ** -14
+    for n, at in [(0, (0, 0, 0, 0)), (0, (0, 1, 8, 63)), (1, (0, 0, 0, 5)), (1, (0, 0, 8, 1)), (2, (0, 0, 3, 7))]:
+        args = [q, k, v]
+        step = torch.zeros_like(args[n])
+        step[at] = h
+        up, down = ([a + f * step if i == n else a for i, a in enumerate(args)] for f in (1, -1))
+        diff = ((forward(*up)[0] - forward(*down)[0]) * do).sum() / (2 * h)
+        assert abs(diff - grads[n][at]).item() < 1e-6
+
+
+@pytest.mark.parametrize("d,s,hq,hkv,causal,layout", [(64, 200, 4, 2, True, "bshd"), (128, 333, 2, 2, False, "bhsd"),
+                                                      (128, 1, 2, 1, True, "bhsd"), (256, 130, 4, 1, True, "bhsd"),
+                                                      (128, 300, 3, 1, True, "bhsd")])
+def test_forward_lse(cuda_device, d, s, hq, hkv, causal, layout):
+    """lse against 64 bits: the exponents are fp32 (their parts' 2^-24, d / 16 + 8 roundings), each exponential and sum adds
+    at most (s + 8) 2^-23; the output is the one of the call without lse."""
+    q, k, v, _ = make(2, hq, hkv, s, s, d, layout, seed=s)
+    o, lse = fa2.kernel_fn(q, k, v, causal, layout=layout, return_lse=True)
+    assert lse.shape == (2, hq, s) and lse.dtype == torch.float32
+    assert torch.equal(o, fa2.kernel_fn(q, k, v, causal, layout=layout))
+    if layout == "bshd":
+        q, k = q.transpose(1, 2), k.transpose(1, 2)
+    kx = k.double().repeat_interleave(hq // hkv, 1).transpose(2, 3)
+    x = q.double() @ kx * d ** -0.5
+    size = (q.double().abs() @ kx.abs() * d ** -0.5).amax(-1)
+    if causal:
+        x = x.masked_fill(~torch.ones(s, s, dtype=torch.bool, device=x.device).tril(), -math.inf)
+    ref = torch.logsumexp(x, -1)
+    assert ((lse.double() - ref).abs() <= (size + ref.abs()) * (d / 16 + 8) * 2.0 ** -24 + (s + 8) * 2.0 ** -23).all()
+
+
+def test_same_bits_every_time(cuda_device):
+    for b, hq, hkv, s, d, causal in [(2, 8, 2, 1500, 128, True), (1, 8, 8, 1000, 64, False), (1, 8, 2, 700, 256, True)]:
+        q, k, v, do = make(b, hq, hkv, s, s, d, "bhsd", seed=d)
+        o, lse = fa2.kernel_fn(q, k, v, causal, return_lse=True)
+        first = bwd.kernel_fn(do, q, k, v, o, lse, causal)
+        for _ in range(4):
+            assert all(torch.equal(x, y) for x, y in zip(first, bwd.kernel_fn(do, q, k, v, o, lse, causal)))
+
+
+def test_heads_that_share_keys_are_summed(cuda_device):
+    """dk and dv of a shared key head are those of the heads apart, added; dq is each head's own."""
+    q, k, v, do = make(1, 4, 1, 260, 260, 128, "bhsd", seed=2)
+    kx, vx = k.expand(1, 4, 260, 128).contiguous(), v.expand(1, 4, 260, 128).contiguous()
+    o, lse = fa2.kernel_fn(q, k, v, return_lse=True)
+    dq, dk, dv = bwd.kernel_fn(do, q, k, v, o, lse)
+    dq4, dk4, dv4 = bwd.kernel_fn(do, q, kx, vx, o, lse)
+    assert torch.equal(dq, dq4)
+    for a, b in ((dk, dk4), (dv, dv4)):
+        b = b.double()
+        # four values rounded to bf16 and their sum rounded once; and the fp32 sums' order
+        assert ((a.double() - b.sum(1, keepdim=True)).abs() <= 2.0 ** -8 * (b.abs().sum(1, keepdim=True) + a.double().abs())
+                + 2.0 ** -16 * b.abs().sum(1, keepdim=True) + 2.0 ** -12).all()
+
+
+@pytest.mark.parametrize("sq,skv,b", [(0, 5, 2), (5, 5, 0), (0, 0, 1)])
+def test_empty(cuda_device, sq, skv, b):
+    q, k, v, do = make(b, 4, 2, sq, skv, 64, "bhsd")
+    dq, dk, dv = bwd.kernel_fn(do, q, k, v, q.clone(), torch.zeros(b, 4, sq, device=q.device))
+    assert dq.shape == q.shape and dk.shape == k.shape and dk.eq(0).all() and dv.eq(0).all()
+
+
+def test_refusals(cuda_device):
+    q, k, v, do = make(1, 4, 2, 20, 20, 64, "bhsd")
+    o, lse = fa2.kernel_fn(q, k, v, return_lse=True)
+    ok = dict(do=do, q=q, k=k, v=v, o=o, lse=lse)
+    for bad in (dict(do=do[:, :2]), dict(do=do.float()), dict(o=o[:, :, :3]), dict(lse=lse[..., :3]), dict(lse=lse.double()),
+                dict(lse=lse.cpu()), dict(do=do.cpu()), dict(sm_scale=-1.0), dict(sm_scale=float("nan")),
+                dict(k=k[:, :, :0], v=v[:, :, :0]), dict(layout="bshd")):
+        with pytest.raises(ValueError):
+            bwd.kernel_fn(**{**ok, **bad})
+
+
+def test_views_and_expanded_gradients(cuda_device):
+    q, k, v, do = make(2, 4, 2, 150, 150, 128, "bhsd", seed=7)
+    o, lse = fa2.kernel_fn(q, k, v, return_lse=True)
+    want = bwd.kernel_fn(do, q, k, v, o, lse)
+    t = lambda x: x.transpose(1, 2).contiguous().transpose(1, 2)  # noqa: E731
+    odd = torch.zeros(do.numel() + 1, dtype=do.dtype, device=do.device)[1:].view(do.shape).copy_(do)
+    for args in ((t(do), t(q), t(k), t(v), t(o), lse), (odd, q, k, v, o, lse), (do, q, k, v, o, lse.double().float())):
+        assert all(torch.equal(a, b) for a, b in zip(bwd.kernel_fn(*args), want))
+    one = torch.ones((), dtype=do.dtype, device=do.device).expand(do.shape)
+    assert all(torch.equal(a, b) for a, b in zip(bwd.kernel_fn(one, q, k, v, o, lse), bwd.kernel_fn(one.contiguous(), q, k, v, o, lse)))
+
+
+def test_calls_on_two_streams_and_in_graphs(cuda_device):
+    """Two calls at once, and two graphs replayed at once: neither shares the other's sums."""
+    cases = [make(2, 8, 2, 900, 900, 128, "bhsd", seed=1), make(2, 8, 2, 900, 900, 128, "bhsd", seed=2)]
+    states = []
+    for q, k, v, do in cases:
+        states.append((do, q, k, v, *fa2.kernel_fn(q, k, v, return_lse=True)))
+    want = [bwd.kernel_fn(*s) for s in states]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in states]
+    for _ in range(3):
+        got = []
+        for s, st in zip(states, streams):
+            with torch.cuda.stream(st):
+                got.append([bwd.kernel_fn(*s) for _ in range(3)])
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert all(torch.equal(a, b) for r in g for a, b in zip(r, w))
+    graphs, outs = [], []
+    held = [tuple(t.clone() for t in s) for s in states]
+    for s in held:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(bwd.kernel_fn(*s))
+        graphs.append(g)
+    for pick in ((0, 1), (1, 0)):
+        for h, i in zip(held, pick):
+            for a, b in zip(h, states[i]):
+                a.copy_(b)
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, i in zip(outs, pick):
+            assert all(torch.equal(a, b) for a, b in zip(o, want[i]))
+
+
+def test_masked_infinities_stay_out(cuda_device):
+    """A value row of infinities that no query up to some row sees: those rows' dq are what they were."""
+    q, k, v, do = make(1, 1, 1, 256, 256, 128, "bhsd", seed=9)
+    o, lse = fa2.kernel_fn(q, k, v, return_lse=True)
+    want = bwd.kernel_fn(do, q, k, v, o, lse)
+    v2 = v.clone()
+    v2[0, 0, 200] = float("inf")
+    got = bwd.kernel_fn(do, q, k, v2, o, lse)
+    assert torch.equal(got[0][0, 0, :200], want[0][0, 0, :200])   # dS is replaced, not multiplied, where masked
+    assert not torch.isfinite(got[0][0, 0, 200:].float()).all()
