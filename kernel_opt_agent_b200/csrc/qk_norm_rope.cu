@@ -11,10 +11,11 @@
 //
 // Both are streams: a few flops per byte, bound by HBM (forward 4 bytes an element, backward 6) or, for
 // few rows, by latency.  A row lies in D / 8 lanes, 8 columns (16 bytes) each, so a warp holds 32 / (D / 8) heads
-// of a token; sums are butterflies over a row's lanes, and the other half of a pair comes from the lane half / 8
-// away.  A warp takes a token (or, when tokens are few, a part of its heads): the cos and sin of its
-// columns are read once and serve all heads, and the loads of `U` rows are issued before the first
-// is used.
+// of a token at a time (an iteration); sums are butterflies over a row's lanes.  Every warp takes an equal share of all
+// iterations, token by token: the cos and sin of its columns are read once per token and serve its heads.
+// The rows come through a ring of kDepth iterations per warp in shared memory (cp.async, each lane its own 16
+// bytes), which runs ahead across tokens: what is in flight costs no registers (with loads into registers, 16 warps of 100
+// registers, B4 S8192 Hq32 Hkv8 D128 ran at 4.4 TB/s), and the other half of a pair is read from the ring.
 // The weights' gradients: a lane adds up its columns in registers over all its rows, a CTA adds its
 // warps' sums in order and writes them to its row of a workspace, and a second launch adds those rows in
 // order: the same bits every time, no atomics.
@@ -50,8 +51,9 @@ struct Params {
   const float *cos, *sin;    // [table_rows, half]
   const int32_t* positions;  // [axes, tokens], or null: the token's index in its sequence
   float* partial;            // backward: [CTAs, 2, D]
-  long long tokens, units;
-  int seq, parts;            // a unit is one of `parts` parts of a token's heads
+  long long tokens, iters;   // tokens fit 32 bits
+  int seq;
+  int q_iters, k_iters;      // iterations of a token: 256 / D heads each
   int half, nope, axes, table_rows;
   int w_fp32;
   float eps;
@@ -81,25 +83,49 @@ __device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
+// Two fp32 values in a register pair, and Blackwell's arithmetic on them (half the instructions; the kernels
+// are issue-bound before they are HBM-bound).
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pair2(float a, float b) {
+  F2 v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ float2 split2(F2 v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 template <typename T>
-__device__ __forceinline__ void widen(const uint4& v, float (&x)[8]) {
+__device__ __forceinline__ void widen(const uint4& v, F2 (&x)[4]) {
   const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const float2 f = unpack<T>(u[e]);
-    x[2 * e] = f.x;
-    x[2 * e + 1] = f.y;
+    x[e] = pair2(f.x, f.y);
   }
 }
 
 template <typename T>
-__device__ __forceinline__ uint4 narrow(const float (&x)[8]) {
-  return make_uint4(pack<T>(x[0], x[1]), pack<T>(x[2], x[3]), pack<T>(x[4], x[5]), pack<T>(x[6], x[7]));
-}
-
-__device__ __forceinline__ uint4 shfl4(const uint4& v, int src) {
-  return make_uint4(__shfl_sync(0xffffffffu, v.x, src), __shfl_sync(0xffffffffu, v.y, src),
-                    __shfl_sync(0xffffffffu, v.z, src), __shfl_sync(0xffffffffu, v.w, src));
+__device__ __forceinline__ uint4 narrow(const F2 (&x)[4]) {
+  uint32_t u[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 f = split2(x[e]);
+    u[e] = pack<T>(f.x, f.y);
+  }
+  return make_uint4(u[0], u[1], u[2], u[3]);
 }
 
 // A lane's place in its row: columns 8 part .. 8 part + 7, rotated or not, in the first or the second half of
@@ -108,7 +134,7 @@ struct Place {
   int part, row;       // piece of the row, row of the warp
   bool rot, first;
   int pair0;           // first pair of the 8
-  int partner;
+  int partner;         // the lane itself where nothing is rotated
 };
 
 template <int D>
@@ -188,176 +214,269 @@ __device__ __forceinline__ void stage_weights(const Params& p, int d, float* w) 
   __syncthreads();
 }
 
-// The rows [lo, hi) of iterations of a unit, one iteration being 32 / (D / 8) heads; the queries' come first.
-struct Range {
-  long long token;
-  int q_lo, q_hi, k_lo, k_hi;
+// A place in the sequence of all iterations, token by token, the queries' of a token before its keys'.
+// Every warp takes an equal share of the sequence, which may begin and end inside a token.
+struct Spot {
+  unsigned token, b, s;
+  int it;            // iteration of the token
+  long long left;    // iterations to the end of the warp's share
+
+  __device__ __forceinline__ void begin(const Params& p) {
+    const long long warps = static_cast<long long>(gridDim.x) * kWarps, w = static_cast<long long>(blockIdx.x) * kWarps + warp_id();
+    const int per = p.q_iters + p.k_iters;
+    const long long lo = p.iters / warps * w + min(w, p.iters % warps);
+    left = p.iters / warps + (w < p.iters % warps ? 1 : 0);
+    token = static_cast<unsigned>(lo / per);
+    it = static_cast<int>(lo - static_cast<long long>(token) * per);
+    b = token / static_cast<unsigned>(p.seq);
+    s = token - b * static_cast<unsigned>(p.seq);
+  }
+  __device__ __forceinline__ void next_token(const Params& p) {
+    it = 0;
+    ++token;
+    if (++s == static_cast<unsigned>(p.seq)) {
+      s = 0;
+      ++b;
+    }
+  }
 };
 
-template <int D>
-__device__ __forceinline__ Range unit_range(const Params& p, long long u) {
-  constexpr int kRows = 256 / D;
-  const int nq = (p.q.heads + kRows - 1) / kRows, nk = (p.k.heads + kRows - 1) / kRows;
-  Range r;
-  r.token = u / p.parts;
-  const int part = static_cast<int>(u - r.token * p.parts);
-  const int lo = static_cast<int>(static_cast<long long>(nq + nk) * part / p.parts);
-  const int hi = static_cast<int>(static_cast<long long>(nq + nk) * (part + 1) / p.parts);
-  r.q_lo = min(lo, nq);
-  r.q_hi = min(hi, nq);
-  r.k_lo = max(lo, nq) - nq;
-  r.k_hi = max(hi, nq) - nq;
-  return r;
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-template <int D, typename T, int U>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_constant__ Params p) {
+// The warp ahead of its work: copies iteration after iteration into the ring.
+template <int D, typename T, bool kBackward>
+struct Ahead {
+  static constexpr int kRows = 256 / D;
+  Spot at;
+  int until;                  // iterations of this kind left in the token
+  int h, heads;               // this lane's head in the iteration, heads of the kind
+  const T *x, *g;             // its 16 bytes
+  long long x_step, g_step;   // to the next iteration's
+
+  __device__ __forceinline__ void point(const Params& p, const Place& a) {
+    const bool is_q = at.it < p.q_iters;
+    const Rows& r = is_q ? p.q : p.k;
+    const int first = is_q ? at.it : at.it - p.q_iters;
+    until = (is_q ? p.q_iters : p.k_iters) - first;
+    h = first * kRows + a.row;
+    heads = r.heads;
+    x = static_cast<const T*>(r.x) + at.b * r.sb + at.s * r.ss + h * r.sh + a.part * 8;
+    x_step = r.sh * kRows;
+    if (kBackward) {
+      g = static_cast<const T*>(r.dy) + at.b * r.gb + at.s * r.gs + h * r.gh + a.part * 8;
+      g_step = r.gh * kRows;
+    }
+  }
+  __device__ __forceinline__ void begin(const Params& p, const Place& a) {
+    at.begin(p);
+    if (at.left > 0) point(p, a);
+  }
+  __device__ __forceinline__ void fetch(const Params& p, const Place& a, uint32_t slot) {
+    if (at.left > 0) {
+      copy16(slot, x, h < heads);
+      if (kBackward) copy16(slot + 512, g, h < heads);
+      x += x_step;
+      if (kBackward) g += g_step;
+      h += kRows;
+      ++at.it;
+      --at.left;
+      if (--until == 0 && at.left > 0) {
+        if (at.it == p.q_iters + p.k_iters) at.next_token(p);
+        point(p, a);
+      }
+    }
+    copy_commit();
+  }
+};
+
+__device__ __forceinline__ uint4 ring_read(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+constexpr int kFwdDepth = 8, kBwdDepth = 10;
+constexpr int kFwdPerSm = 3, kBwdPerSm = 2;  // CTAs
+
+template <int D, typename T>
+__global__ void __launch_bounds__(kThreads, kFwdPerSm) qk_norm_rope_kernel(const __grid_constant__ Params p) {
   constexpr int kLanes = D / 8, kRows = 32 / kLanes;
   __shared__ __align__(16) float w[2 * D];
+  __shared__ __align__(16) uint8_t ring_mem[kWarps][kFwdDepth * 512];
   wait_previous_kernels();
   stage_weights<T>(p, D, w);
   const Place a = place<D>(p.half, p.nope);
   const int partner_part = a.partner % kLanes;
-  const long long stride = static_cast<long long>(gridDim.x) * kWarps;
-  for (long long u = static_cast<long long>(blockIdx.x) * kWarps + warp_id(); u < p.units; u += stride) {
-    const Range rg = unit_range<D>(p, u);
-    const long long b = rg.token / p.seq, s = rg.token - b * p.seq;
-    float c[8], sn[8];
-    load_turn(p, a, rg.token, c, sn);
-    auto rows = [&](const Rows& r, const float* wr, int lo, int hi) {
-      if (lo >= hi) return;
-      const T* src = static_cast<const T*>(r.x) + b * r.sb + s * r.ss + a.part * 8;
-      T* dst = static_cast<T*>(r.out) + rg.token * r.heads * D + a.part * 8;
-      // own weights times cos, the partner's times sin: y = r (x (w cos) + x_partner (w_partner sin))
-      float wc[8], ws[8];
+  const uint32_t ring = smem_u32(ring_mem[warp_id()]);
+  const uint32_t own = lane_id() * 16, other = a.partner * 16;
+  Ahead<D, T, false> ahead;
+  ahead.begin(p, a);
+  Spot c = ahead.at;
+#pragma unroll 1
+  for (int i = 0; i < kFwdDepth; ++i) ahead.fetch(p, a, ring + i * 512 + own);
+  uint32_t slot = ring;
+  for (; c.left > 0; c.next_token(p)) {
+    const int end = static_cast<int>(min(static_cast<long long>(p.q_iters + p.k_iters), c.it + c.left));
+    c.left -= end - c.it;
+    float cs[8], sn[8];
+    load_turn(p, a, c.token, cs, sn);
+#pragma unroll 1
+    for (int kind = 0; kind < 2; ++kind) {
+      const Rows& r = kind ? p.k : p.q;
+      const int lo = kind ? max(c.it - p.q_iters, 0) : c.it;
+      const int hi = kind ? end - p.q_iters : min(end, p.q_iters);
+      if (lo >= hi) continue;
+      int h = lo * kRows + a.row;
+      T* dst = static_cast<T*>(r.out) + (static_cast<long long>(c.token) * r.heads + h) * D + a.part * 8;
+      // own weights times cos, the partner's times sin: y = r (x (w cos) + x_partner (w_partner sin)); where nothing is
+      // rotated the partner is the lane itself and sin 0
+      const float *wo = w + kind * D + a.part * 8, *wp = w + kind * D + partner_part * 8;
+      F2 wc[4], ws[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        wc[e] = wr[a.part * 8 + e] * c[e];
-        ws[e] = wr[partner_part * 8 + e] * sn[e];
+      for (int e = 0; e < 4; ++e) {
+        wc[e] = pair2(wo[2 * e] * cs[2 * e], wo[2 * e + 1] * cs[2 * e + 1]);
+        ws[e] = pair2(wp[2 * e] * sn[2 * e], wp[2 * e + 1] * sn[2 * e + 1]);
       }
-      for (int it = lo; it < hi; it += U) {
-        uint4 v[U];
+#pragma unroll 1
+      for (int left = hi - lo; left > 0; --left, h += kRows, dst += kRows * D) {
+        copy_wait<kFwdDepth - 1>();
+        __syncwarp();
+        F2 x[4], o[4];
+        widen<T>(ring_read(slot + own), x);
+        widen<T>(ring_read(slot + other), o);
+        __syncwarp();
+        ahead.fetch(p, a, slot + own);
+        slot = slot == ring + (kFwdDepth - 1) * 512 ? ring : slot + 512;
+        F2 sq = mul2(x[0], x[0]);
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-          const int h = (it + k) * kRows + a.row;
-          v[k] = it + k < hi && h < r.heads ? __ldcs(reinterpret_cast<const uint4*>(src + h * r.sh)) : make_uint4(0u, 0u, 0u, 0u);
-        }
+        for (int e = 1; e < 4; ++e) sq = fma2(x[e], x[e], sq);
+        float sum = split2(sq).x + split2(sq).y;
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-          if (it + k >= hi) break;  // warp-uniform
-          const int h = (it + k) * kRows + a.row;
-          float x[8], o[8];
-          widen<T>(v[k], x);
-          widen<T>(shfl4(v[k], a.partner), o);
-          float sum = 0.0f;
+        for (int m = kLanes / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+        const float inv = rsqrtf(sum * (1.0f / D) + p.eps);
+        const F2 inv2 = pair2(inv, inv);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
-#pragma unroll
-          for (int m = kLanes / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-          const float inv = rsqrtf(sum * (1.0f / D) + p.eps);
-          // an unrotated lane has no second term (0 times an infinite x would be NaN)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = inv * (a.rot ? fmaf(o[e], ws[e], x[e] * wc[e]) : x[e] * wc[e]);
-          if (h < r.heads) *reinterpret_cast<uint4*>(dst + h * D) = narrow<T>(x);
-        }
+        for (int e = 0; e < 4; ++e) x[e] = mul2(inv2, fma2(o[e], ws[e], mul2(x[e], wc[e])));
+        if (h < r.heads) *reinterpret_cast<uint4*>(dst) = narrow<T>(x);
       }
-    };
-    rows(p.q, w, rg.q_lo, rg.q_hi);
-    rows(p.k, w + D, rg.k_lo, rg.k_hi);
+    }
   }
 }
 
-template <int D, typename T, int U>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_bwd_kernel(const __grid_constant__ Params p) {
+template <int D, typename T>
+__global__ void __launch_bounds__(kThreads, kBwdPerSm) qk_norm_rope_bwd_kernel(const __grid_constant__ Params p) {
   constexpr int kLanes = D / 8, kRows = 32 / kLanes;
+  extern __shared__ __align__(16) uint8_t dyn[];  // the rings: [kWarps][kBwdDepth][x, dy][512]
   __shared__ __align__(16) float w[2 * D];
-  __shared__ float sums[kWarps][2 * D];
   wait_previous_kernels();
   stage_weights<T>(p, D, w);
   const Place a = place<D>(p.half, p.nope);
-  float acc[2][8];
+  F2 acc[2][4];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[i][e] = 0.0f;
-  const long long stride = static_cast<long long>(gridDim.x) * kWarps;
-  for (long long u = static_cast<long long>(blockIdx.x) * kWarps + warp_id(); u < p.units; u += stride) {
-    const Range rg = unit_range<D>(p, u);
-    const long long b = rg.token / p.seq, s = rg.token - b * p.seq;
-    float c[8], sn[8];
-    load_turn(p, a, rg.token, c, sn);
-    auto rows = [&](const Rows& r, const float* wr, float (&dw)[8], int lo, int hi) {
-      if (lo >= hi) return;
-      const T* src = static_cast<const T*>(r.x) + b * r.sb + s * r.ss + a.part * 8;
-      const T* grad = static_cast<const T*>(r.dy) + b * r.gb + s * r.gs + a.part * 8;
-      T* dst = static_cast<T*>(r.out) + rg.token * r.heads * D + a.part * 8;
-      float wl[8];
+    for (int e = 0; e < 4; ++e) acc[i][e] = 0ull;
+  const uint32_t ring = smem_u32(dyn) + warp_id() * (kBwdDepth * 1024);
+  const uint32_t own = lane_id() * 16, other = a.partner * 16;
+  Ahead<D, T, true> ahead;
+  ahead.begin(p, a);
+  Spot c = ahead.at;
+#pragma unroll 1
+  for (int i = 0; i < kBwdDepth; ++i) ahead.fetch(p, a, ring + i * 1024 + own);
+  uint32_t slot = ring;
+  for (; c.left > 0; c.next_token(p)) {
+    const int end = static_cast<int>(min(static_cast<long long>(p.q_iters + p.k_iters), c.it + c.left));
+    c.left -= end - c.it;
+    F2 c2[4], s2[4];
+    {
+      float cs[8], sn[8];
+      load_turn(p, a, c.token, cs, sn);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) wl[e] = wr[a.part * 8 + e];
-      for (int it = lo; it < hi; it += U) {
-        uint4 v[U], dv[U];
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-          const int h = (it + k) * kRows + a.row;
-          const bool in = it + k < hi && h < r.heads;
-          v[k] = in ? __ldcs(reinterpret_cast<const uint4*>(src + h * r.sh)) : make_uint4(0u, 0u, 0u, 0u);
-          dv[k] = in ? __ldcs(reinterpret_cast<const uint4*>(grad + h * r.gh)) : make_uint4(0u, 0u, 0u, 0u);
-        }
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-          if (it + k >= hi) break;  // warp-uniform
-          const int h = (it + k) * kRows + a.row;
-          float x[8], g[8], o[8];
-          widen<T>(v[k], x);
-          widen<T>(dv[k], g);
-          widen<T>(shfl4(dv[k], a.partner), o);
-          if (a.rot) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) g[e] = fmaf(o[e], -sn[e], g[e] * c[e]);  // turned back
-          }
-          float sum = 0.0f, dot = 0.0f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            sum = fmaf(x[e], x[e], sum);
-            dot = fmaf(g[e] * wl[e], x[e], dot);
-          }
-#pragma unroll
-          for (int m = kLanes / 2; m > 0; m >>= 1) {
-            sum += __shfl_xor_sync(0xffffffffu, sum, m);
-            dot += __shfl_xor_sync(0xffffffffu, dot, m);
-          }
-          const float inv = rsqrtf(sum * (1.0f / D) + p.eps);
-          const float back = inv * inv * (dot * (1.0f / D));
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            dw[e] = fmaf(g[e], x[e] * inv, dw[e]);
-            x[e] = inv * fmaf(-back, x[e], g[e] * wl[e]);
-          }
-          if (h < r.heads) *reinterpret_cast<uint4*>(dst + h * D) = narrow<T>(x);
-        }
+      for (int e = 0; e < 4; ++e) {
+        c2[e] = pair2(cs[2 * e], cs[2 * e + 1]);
+        s2[e] = pair2(-sn[2 * e], -sn[2 * e + 1]);
       }
-    };
-    rows(p.q, w, acc[0], rg.q_lo, rg.q_hi);
-    rows(p.k, w + D, acc[1], rg.k_lo, rg.k_hi);
+    }
+#pragma unroll
+    for (int kind = 0; kind < 2; ++kind) {
+      const Rows& r = kind ? p.k : p.q;
+      const int lo = kind ? max(c.it - p.q_iters, 0) : c.it;
+      const int hi = kind ? end - p.q_iters : min(end, p.q_iters);
+      if (lo >= hi) continue;
+      int h = lo * kRows + a.row;
+      T* dst = static_cast<T*>(r.out) + (static_cast<long long>(c.token) * r.heads + h) * D + a.part * 8;
+      const F2* wo = reinterpret_cast<const F2*>(w + kind * D + a.part * 8);
+      F2 wl[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) wl[e] = wo[e];
+#pragma unroll 1
+      for (int left = hi - lo; left > 0; --left, h += kRows, dst += kRows * D) {
+        copy_wait<kBwdDepth - 1>();
+        __syncwarp();
+        F2 x[4], g[4], o[4];
+        widen<T>(ring_read(slot + own), x);
+        widen<T>(ring_read(slot + 512 + own), g);
+        widen<T>(ring_read(slot + 512 + other), o);
+        __syncwarp();
+        ahead.fetch(p, a, slot + own);
+        slot = slot == ring + (kBwdDepth - 1) * 1024 ? ring : slot + 1024;
+        F2 sq = 0ull, gx = 0ull;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          g[e] = fma2(o[e], s2[e], mul2(g[e], c2[e]));  // turned back
+          o[e] = mul2(g[e], wl[e]);
+          sq = fma2(x[e], x[e], sq);
+          gx = fma2(o[e], x[e], gx);
+        }
+        float sum = split2(sq).x + split2(sq).y, dot = split2(gx).x + split2(gx).y;
+#pragma unroll
+        for (int m = kLanes / 2; m > 0; m >>= 1) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, m);
+          dot += __shfl_xor_sync(0xffffffffu, dot, m);
+        }
+        const float inv = rsqrtf(sum * (1.0f / D) + p.eps);
+        const float back = -inv * inv * (dot * (1.0f / D));
+        const F2 inv2 = pair2(inv, inv), back2 = pair2(back, back);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          acc[kind][e] = fma2(g[e], mul2(x[e], inv2), acc[kind][e]);
+          x[e] = mul2(inv2, fma2(back2, x[e], o[e]));
+        }
+        if (h < r.heads) *reinterpret_cast<uint4*>(dst) = narrow<T>(x);
+      }
+    }
   }
-  // the warp's rows, then the CTA's warps in order
+  // the warp's rows, then the CTA's warps in order (over the rings)
+  copy_wait<0>();
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(dyn);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
+      float t = e % 2 ? split2(acc[i][e / 2]).y : split2(acc[i][e / 2]).x;
 #pragma unroll
-      for (int m = kLanes; m < 32; m <<= 1) acc[i][e] += __shfl_xor_sync(0xffffffffu, acc[i][e], m);
-      if (a.row == 0) sums[warp_id()][i * D + a.part * 8 + e] = acc[i][e];
+      for (int m = kLanes; m < 32; m <<= 1) t += __shfl_xor_sync(0xffffffffu, t, m);
+      if (a.row == 0) sums[warp_id() * 2 * D + i * D + a.part * 8 + e] = t;
     }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * D; i += kThreads) {
     float t = 0.0f;
 #pragma unroll
-    for (int v = 0; v < kWarps; ++v) t += sums[v][i];
+    for (int v = 0; v < kWarps; ++v) t += sums[v * 2 * D + i];
     p.partial[static_cast<long long>(blockIdx.x) * 2 * D + i] = t;
   }
 }
+constexpr int kBwdSmem = kWarps * kBwdDepth * 1024;
+static_assert(kBwdSmem >= kWarps * 2 * 256 * 4, "the warps' sums fit where the rings were");
 
 // dw[i] = the sum of the CTAs' rows in order: 32 columns a block, each by 32 threads that take every
 // 32nd row, joined in order.  Rounded to the weights' type.
@@ -382,39 +501,31 @@ __global__ void __launch_bounds__(1024) weight_grad_kernel(const float* __restri
   }
 }
 
-// CTAs of a backward call: four to an SM (its registers), fewer where warps would have no unit.
-int bwd_ctas(long long units) {
-  return static_cast<int>(std::min<long long>((units + kWarps - 1) / kWarps, 4LL * std::max(1, device_sm_count())));
+// CTAs of a call: `per_sm` to an SM (its registers), fewer where warps would have no iteration.
+int ctas(long long iters, int per_sm) {
+  return static_cast<int>(std::min<long long>((iters + kWarps - 1) / kWarps, static_cast<long long>(per_sm) * std::max(1, device_sm_count())));
 }
 
-// Parts of a token's heads: as many as it takes to give every SM 32 warps, at most one per iteration.
-int head_parts(long long tokens, int heads_q, int heads_k, int d) {
-  const int rows = 256 / d;
-  const int iters = (heads_q + rows - 1) / rows + (heads_k + rows - 1) / rows;
-  const long long want = 32LL * std::max(1, device_sm_count());
-  return static_cast<int>(std::max<long long>(1, std::min<long long>(iters, (want + tokens - 1) / std::max<long long>(1, tokens))));
-}
+int iterations(int heads, int d) { return (heads + 256 / d - 1) / (256 / d); }
 
 template <int D, typename T>
 cudaError_t run_fwd(const Params& p, cudaStream_t stream) {
-  const long long ctas = std::min<long long>((p.units + kWarps - 1) / kWarps, 8LL * std::max(1, device_sm_count()));
-  const dim3 grid(static_cast<unsigned>(ctas));
-  if (p.parts > 1) return launch_overlapped(&qk_norm_rope_kernel<D, T, 1>, grid, dim3(kThreads), 0, stream, p);
-  return launch_overlapped(&qk_norm_rope_kernel<D, T, 4>, grid, dim3(kThreads), 0, stream, p);
+  return launch_overlapped(&qk_norm_rope_kernel<D, T>, dim3(static_cast<unsigned>(ctas(p.iters, kFwdPerSm))), dim3(kThreads), 0, stream,
+                           p);
 }
 
 template <int D, typename T>
 cudaError_t run_bwd(const Params& p, void* dwq, void* dwk, cudaStream_t stream) {
-  const int ctas = bwd_ctas(p.units);
-  const dim3 grid(static_cast<unsigned>(ctas));
-  cudaError_t e = p.parts > 1 ? launch_overlapped(&qk_norm_rope_bwd_kernel<D, T, 1>, grid, dim3(kThreads), 0, stream, p)
-                              : launch_overlapped(&qk_norm_rope_bwd_kernel<D, T, 2>, grid, dim3(kThreads), 0, stream, p);
+  const int rows = ctas(p.iters, kBwdPerSm);
+  if (!ensure_smem_attr(reinterpret_cast<const void*>(&qk_norm_rope_bwd_kernel<D, T>), kBwdSmem)) return cudaGetLastError();
+  const cudaError_t e = launch_overlapped(&qk_norm_rope_bwd_kernel<D, T>, dim3(static_cast<unsigned>(rows)), dim3(kThreads),
+                                          static_cast<size_t>(kBwdSmem), stream, p);
   if (e != cudaSuccess) return e;
   const dim3 blocks(2 * D / 32), threads(32, 32);
   if (p.w_fp32)
-    return launch_overlapped(&weight_grad_kernel<float>, blocks, threads, 0, stream, p.partial, ctas, D, static_cast<float*>(dwq),
+    return launch_overlapped(&weight_grad_kernel<float>, blocks, threads, 0, stream, p.partial, rows, D, static_cast<float*>(dwq),
                              static_cast<float*>(dwk));
-  return launch_overlapped(&weight_grad_kernel<T>, blocks, threads, 0, stream, p.partial, ctas, D, static_cast<T*>(dwq),
+  return launch_overlapped(&weight_grad_kernel<T>, blocks, threads, 0, stream, p.partial, rows, D, static_cast<T*>(dwq),
                            static_cast<T*>(dwk));
 }
 
@@ -445,6 +556,8 @@ int prepare(const char* who, const tokmix_qk_norm_rope* a, bool backward, Params
                               a->dk_head_stride})
       if (s % 8 != 0) return fail(TOKMIX_ERR_INVALID_ARGUMENT, "%s: strides must be multiples of 8 elements", who);
   p.tokens = static_cast<long long>(a->batch) * a->seqlen;
+  if (p.tokens > 0x7FFFFFFFll) return fail(TOKMIX_ERR_UNSUPPORTED, "%s: too many tokens (%lld)", who, p.tokens);
+  if (a->heads_q > 65536 || a->heads_k > 65536) return fail(TOKMIX_ERR_UNSUPPORTED, "%s: more than 65536 heads", who);
   if (p.tokens == 0 && !backward) return TOKMIX_OK;
   if (a->q_weight == nullptr || a->k_weight == nullptr)
     return fail(TOKMIX_ERR_INVALID_ARGUMENT, "%s: null weight", who);
@@ -464,6 +577,9 @@ int prepare(const char* who, const tokmix_qk_norm_rope* a, bool backward, Params
   p.sin = a->sin;
   p.positions = a->positions;
   p.seq = std::max(1, a->seqlen);
+  p.q_iters = iterations(a->heads_q, a->head_dim);
+  p.k_iters = iterations(a->heads_k, a->head_dim);
+  p.iters = p.tokens * (p.q_iters + p.k_iters);
   p.half = a->half;
   p.nope = a->nope;
   p.axes = a->axes;
@@ -478,11 +594,6 @@ int prepare(const char* who, const tokmix_qk_norm_rope* a, bool backward, Params
   return TOKMIX_OK;
 }
 
-void split_units(Params& p, const tokmix_qk_norm_rope* a) {
-  p.parts = head_parts(p.tokens, a->heads_q, a->heads_k, a->head_dim);
-  p.units = p.tokens * p.parts;
-}
-
 }  // namespace qkr
 }  // namespace tokmix
 
@@ -492,7 +603,6 @@ extern "C" int tokmix_qk_norm_rope_fwd(const tokmix_qk_norm_rope* a, uint32_t* s
   if (const int rc = qkr::prepare("tokmix_qk_norm_rope_fwd", a, false, p)) return rc;
   if (p.tokens == 0) return TOKMIX_OK;
   if (const int rc = check_device()) return rc;
-  qkr::split_units(p, a);
   p.status = status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = a->dtype == TOKMIX_DTYPE_BF16;
@@ -513,8 +623,8 @@ extern "C" int tokmix_qk_norm_rope_fwd(const tokmix_qk_norm_rope* a, uint32_t* s
 extern "C" long long tokmix_qk_norm_rope_bwd_workspace_bytes(long long tokens, int heads_q, int heads_k, int head_dim) {
   using namespace tokmix;
   if (tokens < 0 || heads_q <= 0 || heads_k <= 0 || (head_dim != 64 && head_dim != 128 && head_dim != 256)) return -1;
-  const long long units = tokens * qkr::head_parts(tokens, heads_q, heads_k, head_dim);
-  return static_cast<long long>(qkr::bwd_ctas(units)) * 2 * head_dim * 4;
+  const long long iters = tokens * (qkr::iterations(heads_q, head_dim) + qkr::iterations(heads_k, head_dim));
+  return static_cast<long long>(qkr::ctas(iters, qkr::kBwdPerSm)) * 2 * head_dim * 4;
 }
 
 extern "C" int tokmix_qk_norm_rope_bwd(const tokmix_qk_norm_rope* a, void* dq_weight, void* dk_weight, void* workspace,
@@ -535,7 +645,6 @@ extern "C" int tokmix_qk_norm_rope_bwd(const tokmix_qk_norm_rope* a, void* dq_we
   const long long need = tokmix_qk_norm_rope_bwd_workspace_bytes(p.tokens, a->heads_q, a->heads_k, a->head_dim);
   if (workspace == nullptr || workspace_bytes < need || !qkr::aligned16(workspace))
     return fail(TOKMIX_ERR_INVALID_ARGUMENT, "tokmix_qk_norm_rope_bwd: needs a 16-byte aligned workspace of %lld bytes", need);
-  qkr::split_units(p, a);
   p.partial = static_cast<float*>(workspace);
   p.status = status;
   const bool bf16 = a->dtype == TOKMIX_DTYPE_BF16;
