@@ -58,7 +58,7 @@ struct Params {
   int w_fp32;
   float eps;
   uint32_t* status;
-  uint8_t axis[kMaxPairs];   // the axis of each pair (axes > 1)
+  uint16_t axis[kMaxPairs / 8];  // the axes of each 8 pairs, two bits a pair (axes > 1)
 };
 
 template <typename T>
@@ -135,10 +135,12 @@ struct Place {
   bool rot, first;
   int pair0;           // first pair of the 8
   int partner;         // the lane itself where nothing is rotated
+  uint32_t axes;       // of the 8 pairs, two bits each
 };
 
 template <int D>
-__device__ __forceinline__ Place place(int half, int nope) {
+__device__ __forceinline__ Place place(const Params& p) {
+  const int half = p.half, nope = p.nope;
   constexpr int kLanes = D / 8;
   const int lane = static_cast<int>(lane_id());
   Place a;
@@ -149,54 +151,58 @@ __device__ __forceinline__ Place place(int half, int nope) {
   a.first = v < hv;
   a.pair0 = a.rot ? 8 * (a.first ? v : v - hv) : 0;
   a.partner = a.rot ? (a.first ? lane + hv : lane - hv) : lane;
+  a.axes = p.axis[a.pair0 / 8];
   return a;
 }
 
-// cos and sin of the lane's 8 pairs at token t; 1 and 0 where nothing is rotated, NaN (and a status
-// bit) where a position lies outside the tables.  sin is negated for the first half, so that
-// y = n cos + n_partner sin in both.
-__device__ __forceinline__ void load_turn(const Params& p, const Place& a, long long t, float (&c)[8], float (&s)[8]) {
+// The table rows of a token's axes (its index s in its sequence without positions).  Asked for a token ahead: the
+// tables wait for them.
+__device__ __forceinline__ int4 load_rows(const Params& p, unsigned token, unsigned s) {
+  int4 r = make_int4(static_cast<int>(s), 0, 0, 0);
+  if (p.positions != nullptr && token < p.tokens) {
+    const int32_t* at = p.positions + token;
+    r.x = __ldg(at);
+    if (p.axes > 1) r.y = __ldg(at + p.tokens);
+    if (p.axes > 2) r.z = __ldg(at + 2 * p.tokens);
+    if (p.axes > 3) r.w = __ldg(at + 3 * p.tokens);
+  }
+  return r;
+}
+
+// cos and sin of the lane's 8 pairs; 1 and 0 where nothing is rotated, NaN (and a status bit) where a
+// position lies outside the tables.  sin is negated for the first half, so that y = n cos + n_partner sin
+// in both.
+__device__ __forceinline__ void load_turn(const Params& p, const Place& a, const int4& row, float (&c)[8], float (&s)[8]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     c[e] = 1.0f;
     s[e] = 0.0f;
   }
   if (!a.rot) return;
-  bool bad = false;
-  if (p.axes <= 1) {
-    const long long row = p.positions != nullptr ? p.positions[t] : t % p.seq;
-    bad = row < 0 || row >= p.table_rows;
-    if (!bad) {
-      const float4* cp = reinterpret_cast<const float4*>(p.cos + row * p.half + a.pair0);
-      const float4* sp = reinterpret_cast<const float4*>(p.sin + row * p.half + a.pair0);
-#pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        const float4 cv = __ldg(cp + v), sv = __ldg(sp + v);
-        c[4 * v] = cv.x; c[4 * v + 1] = cv.y; c[4 * v + 2] = cv.z; c[4 * v + 3] = cv.w;
-        s[4 * v] = sv.x; s[4 * v + 1] = sv.y; s[4 * v + 2] = sv.z; s[4 * v + 3] = sv.w;
-      }
-    }
-  } else {
-    long long row[4];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      row[x] = x < p.axes ? p.positions[x * p.tokens + t] : 0;
-      bad = bad || row[x] < 0 || row[x] >= p.table_rows;
-    }
-    if (!bad) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int x = p.axis[a.pair0 + e];
-        const long long at = (x == 0 ? row[0] : x == 1 ? row[1] : x == 2 ? row[2] : row[3]) * p.half + a.pair0 + e;
-        c[e] = __ldg(p.cos + at);
-        s[e] = __ldg(p.sin + at);
-      }
-    }
-  }
-  if (bad) {
+  const unsigned rows = static_cast<unsigned>(p.table_rows);
+  if (static_cast<unsigned>(row.x) >= rows || static_cast<unsigned>(row.y) >= rows || static_cast<unsigned>(row.z) >= rows ||
+      static_cast<unsigned>(row.w) >= rows) {
     record_status(p.status, kDevBadArgs);
 #pragma unroll
     for (int e = 0; e < 8; ++e) c[e] = s[e] = __int_as_float(0x7fffffff);
+  } else if (p.axes <= 1) {
+    const long long at = static_cast<long long>(row.x) * p.half + a.pair0;
+    const float4* cp = reinterpret_cast<const float4*>(p.cos + at);
+    const float4* sp = reinterpret_cast<const float4*>(p.sin + at);
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      const float4 cv = __ldg(cp + v), sv = __ldg(sp + v);
+      c[4 * v] = cv.x; c[4 * v + 1] = cv.y; c[4 * v + 2] = cv.z; c[4 * v + 3] = cv.w;
+      s[4 * v] = sv.x; s[4 * v + 1] = sv.y; s[4 * v + 2] = sv.z; s[4 * v + 3] = sv.w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t x = a.axes >> (2 * e) & 3u;
+      const long long at = static_cast<long long>(x == 0 ? row.x : x == 1 ? row.y : x == 2 ? row.z : row.w) * p.half + a.pair0 + e;
+      c[e] = __ldg(p.cos + at);
+      s[e] = __ldg(p.sin + at);
+    }
   }
   if (a.first) {
 #pragma unroll
@@ -302,8 +308,8 @@ __device__ __forceinline__ uint4 ring_read(uint32_t addr) {
   return v;
 }
 
-constexpr int kFwdDepth = 8, kBwdDepth = 10;
-constexpr int kFwdPerSm = 3, kBwdPerSm = 2;  // CTAs
+constexpr int kFwdDepth = 10, kBwdDepth = 10;
+constexpr int kFwdPerSm = 2, kBwdPerSm = 2;  // CTAs
 
 template <int D, typename T>
 __global__ void __launch_bounds__(kThreads, kFwdPerSm) qk_norm_rope_kernel(const __grid_constant__ Params p) {
@@ -312,13 +318,14 @@ __global__ void __launch_bounds__(kThreads, kFwdPerSm) qk_norm_rope_kernel(const
   __shared__ __align__(16) uint8_t ring_mem[kWarps][kFwdDepth * 512];
   wait_previous_kernels();
   stage_weights<T>(p, D, w);
-  const Place a = place<D>(p.half, p.nope);
+  const Place a = place<D>(p);
   const int partner_part = a.partner % kLanes;
   const uint32_t ring = smem_u32(ring_mem[warp_id()]);
   const uint32_t own = lane_id() * 16, other = a.partner * 16;
   Ahead<D, T, false> ahead;
   ahead.begin(p, a);
   Spot c = ahead.at;
+  int4 rows = load_rows(p, c.token, c.s);
 #pragma unroll 1
   for (int i = 0; i < kFwdDepth; ++i) ahead.fetch(p, a, ring + i * 512 + own);
   uint32_t slot = ring;
@@ -326,7 +333,8 @@ __global__ void __launch_bounds__(kThreads, kFwdPerSm) qk_norm_rope_kernel(const
     const int end = static_cast<int>(min(static_cast<long long>(p.q_iters + p.k_iters), c.it + c.left));
     c.left -= end - c.it;
     float cs[8], sn[8];
-    load_turn(p, a, c.token, cs, sn);
+    load_turn(p, a, rows, cs, sn);
+    rows = load_rows(p, c.token + 1, c.s + 1 == static_cast<unsigned>(p.seq) ? 0u : c.s + 1);
 #pragma unroll 1
     for (int kind = 0; kind < 2; ++kind) {
       const Rows& r = kind ? p.k : p.q;
@@ -377,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, kBwdPerSm) qk_norm_rope_bwd_kernel(c
   __shared__ __align__(16) float w[2 * D];
   wait_previous_kernels();
   stage_weights<T>(p, D, w);
-  const Place a = place<D>(p.half, p.nope);
+  const Place a = place<D>(p);
   F2 acc[2][4];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -388,6 +396,7 @@ __global__ void __launch_bounds__(kThreads, kBwdPerSm) qk_norm_rope_bwd_kernel(c
   Ahead<D, T, true> ahead;
   ahead.begin(p, a);
   Spot c = ahead.at;
+  int4 rows = load_rows(p, c.token, c.s);
 #pragma unroll 1
   for (int i = 0; i < kBwdDepth; ++i) ahead.fetch(p, a, ring + i * 1024 + own);
   uint32_t slot = ring;
@@ -397,7 +406,8 @@ __global__ void __launch_bounds__(kThreads, kBwdPerSm) qk_norm_rope_bwd_kernel(c
     F2 c2[4], s2[4];
     {
       float cs[8], sn[8];
-      load_turn(p, a, c.token, cs, sn);
+      load_turn(p, a, rows, cs, sn);
+      rows = load_rows(p, c.token + 1, c.s + 1 == static_cast<unsigned>(p.seq) ? 0u : c.s + 1);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         c2[e] = pair2(cs[2 * e], cs[2 * e + 1]);
@@ -589,7 +599,7 @@ int prepare(const char* who, const tokmix_qk_norm_rope* a, bool backward, Params
   for (int i = 0; i < a->half; ++i) {
     const int x = a->axes > 1 ? a->pair_axis[i] : 0;
     if (x >= a->axes) return fail(TOKMIX_ERR_INVALID_ARGUMENT, "%s: pair %d names axis %d of %d", who, i, x, a->axes);
-    p.axis[i] = static_cast<uint8_t>(x);
+    p.axis[i / 8] = static_cast<uint16_t>(p.axis[i / 8] | x << (2 * (i % 8)));
   }
   return TOKMIX_OK;
 }
