@@ -33,9 +33,11 @@
 // the tensor core has dQ and dK to do, and while they form dS it has dV and the next S.
 //
 // head_dim 256: dV and dK of 128 keys alone would fill TMEM (2 x 256 columns), so a unit takes half
-// of their columns (and of dQ's) and forms S and dP whole; queries come in tiles of 64, which
-// leaves K, V (64 KB each), Q, dO (32 KB each) and dS (16 KB) room in shared memory.  dQ is formed
-// transposed there (dQ^T = K^T dS^T), which keeps M at 128.
+// of their columns (and of dQ's) and forms S and dP whole; queries come in tiles of 64.  V stays in
+// TMEM as the A operand of dP (128 columns), which leaves shared memory room for two stages of Q and dO (32 KB
+// each) beside K (64 KB), and takes V's rows out of what the tensor core reads there: at N = 64 an MMA
+// with both operands in shared memory reads its full width, 128 bytes a cycle.  dQ is formed transposed
+// (dQ^T = K^T dS^T), which keeps M at 128.
 //
 // Every wait is bounded (sm100.cuh): a stuck pipeline sets a status bit and the CTA drains.
 #include <cuda_runtime.h>
@@ -61,10 +63,10 @@ struct Cfg {
   static constexpr int kBQ = D == 256 ? 64 : 128;      // queries per step
   static constexpr int kDH = D < 128 ? D : 128;        // columns of dV, dK and dQ that a unit forms
   static constexpr int kSplit = D / kDH;
-  static constexpr int kNQ = D == 256 ? 1 : 2;         // stages of Q, and of the row statistics
-  static constexpr int kNDO = D == 256 ? 1 : 2;        // stages of dO
-  static constexpr bool kAhead = kNQ > 1;              // S(t+1) before dQ(t): needs a second Q stage
-  static constexpr bool kAlias = D == 128;             // dQ in dP's columns
+  static constexpr int kNQ = 2;                        // stages of Q, and of the row statistics
+  static constexpr int kNDO = 2;                       // stages of dO
+  static constexpr bool kAlias = D >= 128;             // dQ in dP's columns
+  static constexpr bool kVTmem = D == 256;             // V in TMEM, as the A operand of dP
   static constexpr bool kTransDq = D == 256;           // dQ^T: lanes are columns of dq, columns are queries
   static constexpr int kDqCols = kTransDq ? kBQ : kDH; // TMEM columns of dQ
   static constexpr int kHalfQ = kBQ / 2;               // query columns of a softmax warpgroup
@@ -73,7 +75,8 @@ struct Cfg {
   static constexpr uint32_t kColDq = kAlias ? kColDp : 2 * kBQ;
   static constexpr uint32_t kColDv = kAlias ? 2 * kBQ : kColDq + kDqCols;
   static constexpr uint32_t kColDk = kColDv + kDH;
-  static_assert(kColDk + kDH <= 512, "TMEM columns");
+  static constexpr uint32_t kColV = kColDk + kDH;
+  static_assert(kColV + (kVTmem ? D / 2 : 0) <= 512, "TMEM columns");
   static constexpr int kKBox = kBK * 128;              // 128 keys x 64 columns
   static constexpr int kQBox = kBQ * 128;              // kBQ queries x 64 columns
   static constexpr int kKBytes = (D / 64) * kKBox;
@@ -82,7 +85,7 @@ struct Cfg {
   static constexpr int kStatBytes = 2 * kBQ * 4;       // lse2 and delta of a query tile
   static constexpr int kK = 0;
   static constexpr int kV = kK + kKBytes;
-  static constexpr int kQ = kV + kKBytes;
+  static constexpr int kQ = kV + (kVTmem ? 0 : kKBytes);
   static constexpr int kDO = kQ + kNQ * kQBytes;
   static constexpr int kDs = kDO + kNDO * kQBytes;
   static constexpr int kStat = kDs + kDsBytes;
@@ -92,6 +95,7 @@ struct Cfg {
 
 struct Params {
   __nv_bfloat16 *dq, *dk, *dv;
+  const __nv_bfloat16* v;
   long long q_sb, q_sh, q_ss;        // element strides of q, o, do, dq (batch, head, row)
   long long k_sb, k_sh, k_ss;        // and of k, v, dk, dv
   const float* stats;                // [batch * hq][nq][lse2, delta][kBQ]
@@ -259,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                    const Params p) {
   using C = Cfg<D>;
   extern __shared__ __align__(1024) uint8_t smem[];  // no room is left to round its start up
-  __shared__ uint64_t bar_unit_full[2], bar_unit_empty[2], bar_kv_full, bar_kv_empty, bar_q_full[2], bar_q_empty[2],
+  __shared__ uint64_t bar_unit_full[2], bar_unit_empty[2], bar_kv_full, bar_kv_empty, bar_v, bar_q_full[2], bar_q_empty[2],
       bar_do_full[2], bar_do_empty[2], bar_s, bar_p, bar_dp, bar_ds, bar_dq, bar_dqfree, bar_acc, bar_accfree, bar_drain;
   __shared__ int unit_ring[2];
   __shared__ uint32_t tmem_base_shared;
@@ -283,6 +287,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(&bar_kv_full, 1);
     mbar_init(&bar_kv_empty, 1);
+    mbar_init(&bar_v, kSoftmaxWarps);
     mbar_init(&bar_s, 1);
     mbar_init(&bar_p, kSoftmaxWarps);
     mbar_init(&bar_dp, 1);
@@ -357,10 +362,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                   ok = false;
                   break;
                 }
-                mbar_arrive_expect_tx(&bar_kv_full, 2 * C::kKBytes);
+                mbar_arrive_expect_tx(&bar_kv_full, (C::kVTmem ? 1 : 2) * C::kKBytes);
                 for (int bx = 0; bx < D / 64; ++bx)
                   tma_load_4d(smem + C::kK + bx * C::kKBox, &map_k, &bar_kv_full, bx * 64, x.j * kBK, x.kvh, x.b);
-                for (int bx = 0; bx < D / 64; ++bx)
+                for (int bx = 0; !C::kVTmem && bx < D / 64; ++bx)
                   tma_load_4d(smem + C::kV + bx * C::kKBox, &map_v, &bar_kv_full, bx * 64, x.j * kBK, x.kvh, x.b);
                 ++loads;
               }
@@ -404,6 +409,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           umma_bf16_ss(tb + col, ad + (((kk >> 2) * C::kKBox + (kk & 3) * 32) >> 4), bd + (((kk >> 2) * C::kQBox + (kk & 3) * 32) >> 4),
                        idesc_s, kk > 0 ? 1u : 0u);
       };
+      // the same with V in TMEM
+      auto issue_dp_tmem = [&](uint32_t b) {
+        const uint64_t bd = make_sdesc_sw128(b, 16, 1024);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_bf16_ts(tb + C::kColDp, tb + C::kColV + kk * 8, bd + (((kk >> 2) * C::kQBox + (kk & 3) * 32) >> 4), idesc_s,
+                       kk > 0 ? 1u : 0u);
+      };
       bool ok = true;
       int g = 0;          // steps of earlier units
       int active = 0;     // earlier units with steps (K/V and accumulator phases)
@@ -435,11 +448,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t q_addr = q_base + qs * C::kQBytes, do_addr = do_base + dos * C::kQBytes;
           // dP(t); its columns hold dQ(t-1) until the dQ warps have read it
           ok = wait(&bar_do_full[dos], (gt / C::kNDO) & 1, kDevTimeoutTma) &&
-               (!C::kAlias || gt == 0 || wait(&bar_dqfree, (gt - 1) & 1, kDevTimeoutPipe));
+               (!C::kAlias || gt == 0 || wait(&bar_dqfree, (gt - 1) & 1, kDevTimeoutPipe)) &&
+               (!C::kVTmem || t > 0 || wait(&bar_v, active & 1, kDevTimeoutPipe));
           if (!ok) break;
           tc_fence_after();
           if (leader) {
-            issue_scores(v_addr, do_addr, C::kColDp);
+            if constexpr (C::kVTmem)
+              issue_dp_tmem(do_addr);
+            else
+              issue_scores(v_addr, do_addr, C::kColDp);
             umma_commit(&bar_dp);
           }
           __syncwarp();
@@ -459,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             umma_commit(&bar_do_empty[dos]);
           }
           __syncwarp();
-          if (C::kAhead && t + 1 < x.steps) {
+          if (t + 1 < x.steps) {
             ok = issue_s(gt + 1);
             if (!ok) break;
           }
@@ -486,7 +503,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             umma_commit(&bar_q_empty[qs]);
           }
           __syncwarp();
-          if (!C::kAhead && t + 1 < x.steps) ok = issue_s(gt + 1);
         }
         if (!ok) break;
         if (leader) {
@@ -617,6 +633,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Unit x = decode_unit<D>(p, u);
       const int key = x.j * kBK + row;
       const bool ragged = x.j * kBK + kBK > p.skv;  // keys behind the last one
+      if (C::kVTmem && x.steps > 0) {
+        // this warpgroup's half of V's columns, a row per thread; the previous unit's MMAs are complete (bar_acc)
+        const uint4* src = reinterpret_cast<const uint4*>(p.v + x.b * p.k_sb + x.kvh * p.k_sh + key * p.k_ss + wg * (D / 2));
+#pragma unroll
+        for (int part = 0; part < D / 128; ++part) {
+          uint32_t v[32];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint4 w = key < p.skv ? __ldg(src + part * 8 + e) : make_uint4(0u, 0u, 0u, 0u);
+            v[4 * e] = w.x;
+            v[4 * e + 1] = w.y;
+            v[4 * e + 2] = w.z;
+            v[4 * e + 3] = w.w;
+          }
+          tmem_st32(lanes + C::kColV + wg * (D / 4) + part * 32, v);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar_v);
+      }
       for (int i = p.nq - 1; ok && i >= x.i_min; --i) {
         for (int h = 0; h < p.group; ++h, ++g) {
           const int qs = g % C::kNQ;
@@ -853,6 +890,7 @@ int launch(const void* dout, const void* q, const void* k, const void* v, const 
 
   Params p{};
   p.dq = static_cast<__nv_bfloat16*>(dq);
+  p.v = static_cast<const __nv_bfloat16*>(v);
   p.dk = static_cast<__nv_bfloat16*>(dk);
   p.dv = static_cast<__nv_bfloat16*>(dv);
   const bool bhsd = layout == TOKMIX_LAYOUT_BHSD;
