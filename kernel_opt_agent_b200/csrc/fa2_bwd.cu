@@ -6,7 +6,7 @@
 // dk and dv are summed over the query heads that share a key/value head.  P is formed again from
 // q, k and lse, so the forward keeps one number per row instead of the S x S matrix.
 //
-// Two launches:
+// Three launches:
 //   fa2_bwd_prep    delta and lse * log2(e) in rows padded to whole query tiles (padding: +inf, 0,
 //                   so that a padded row's P is 0), the counters below set to 0.
 //   fa2_bwd_kernel  persistent, one CTA per SM.  A unit is a tile of 128 keys of one key/value head: K and V stay in
@@ -21,11 +21,13 @@
 //   A query tile's dQ is the sum over key tiles, that is, over CTAs.  It grows in fp32 in global
 //   memory by vector reductions, in the order of the key tiles: the CTA of key tile j waits for the
 //   turn counter of (query tile, warp) to read j, adds, and sets it to j + 1.  So the bits are the
-//   same every time; the first tile stores instead of adding (no clearing pass) and the last adds
-//   from registers, scales, rounds and writes dq (no closing pass).
+//   same every time; the first tile stores instead of adding (no clearing pass).
 //   Units are taken from a counter in order of (batch, key/value head, key tile): a CTA waits only
 //   for units that were taken earlier, by CTAs that are running, so the waits end with any number
 //   of resident CTAs.  Under the causal mask this order is longest first.
+//   fa2_bwd_dq      dq = c times those sums, rounded, in dq's layout (a single key tile's dQ is written at once: no such
+//                   launch).  The last key tile's CTA could do it in passing, but reading the sums back held its pipeline
+//                   up for 10 000 to 20 000 cycles a tile.
 // Roles (512 threads): warps 0-7 softmax (two warpgroups, each half of a tile's query columns; thread =
 // key row), warps 8-11 dQ (TMEM to global), warp 12 TMA and unit counter, warp 13 TMEM owner and MMA
 // issuer, warps 14-15 idle (setmaxnreg works on whole warpgroups).
@@ -79,6 +81,7 @@ struct Cfg {
   static_assert(kColV + (kVTmem ? D / 2 : 0) <= 512, "TMEM columns");
   static constexpr int kKBox = kBK * 128;              // 128 keys x 64 columns
   static constexpr int kQBox = kBQ * 128;              // kBQ queries x 64 columns
+  static constexpr int kBoxes = kDH / 64;              // boxes of the columns of dV, dK
   static constexpr int kKBytes = (D / 64) * kKBox;
   static constexpr int kQBytes = (D / 64) * kQBox;
   static constexpr int kDsBytes = kBK * kBQ * 2;       // boxes of 128 keys x 64 queries
@@ -161,6 +164,16 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
+
+// A tile from shared memory to a tensor (rows outside it are left out), in a bulk group of this thread
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* src, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map),
+               "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z), "r"(w)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 __device__ __forceinline__ void red_add_v4(float* dst, float a, float b, float c, float d) {
   asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(dst), "f"(a), "f"(b), "f"(c), "f"(d)
@@ -260,7 +273,7 @@ template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
     fa2_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
                    const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                   const Params p) {
+                   const __grid_constant__ CUtensorMap map_dk, const __grid_constant__ CUtensorMap map_dv, const Params p) {
   using C = Cfg<D>;
   extern __shared__ __align__(1024) uint8_t smem[];  // no room is left to round its start up
   __shared__ uint64_t bar_unit_full[2], bar_unit_empty[2], bar_kv_full, bar_kv_empty, bar_v, bar_q_full[2], bar_q_empty[2],
@@ -556,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = false;
             break;
           }
-          if (x.j + 1 < count) {
+          if (p.nk > 1) {
             if (x.j == 0) {
 #pragma unroll
               for (int c = 0; c < C::kDqCols / 4; ++c)
@@ -569,23 +582,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 red_add_v4(acc + c * 512, __uint_as_float(v[4 * c]), __uint_as_float(v[4 * c + 1]),
                            __uint_as_float(v[4 * c + 2]), __uint_as_float(v[4 * c + 3]));
             }
-            __syncwarp();
-            if (lane == 0) {
-              __threadfence();
-              asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(turn), "r"(static_cast<uint32_t>(x.j + 1)) : "memory");
-            }
-          } else {
-            // the last key tile: the sum is complete
-            if (x.j > 0) {
-#pragma unroll
-              for (int c = 0; c < C::kDqCols / 4; ++c) {
-                const float4 a = __ldcg(reinterpret_cast<const float4*>(acc + c * 512));
-                v[4 * c] = __float_as_uint(a.x + __uint_as_float(v[4 * c]));
-                v[4 * c + 1] = __float_as_uint(a.y + __uint_as_float(v[4 * c + 1]));
-                v[4 * c + 2] = __float_as_uint(a.z + __uint_as_float(v[4 * c + 2]));
-                v[4 * c + 3] = __float_as_uint(a.w + __uint_as_float(v[4 * c + 3]));
+            if (x.j + 1 < count) {
+              __syncwarp();
+              if (lane == 0) {
+                __threadfence();
+                asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(turn), "r"(static_cast<uint32_t>(x.j + 1)) : "memory");
               }
             }
+          } else {  // one key tile: the sum is complete
             __nv_bfloat16* out = p.dq + x.b * p.q_sb + head * p.q_sh + static_cast<long long>(i) * C::kBQ * p.q_ss +
                                  x.half * C::kDH;
             const int rows = min(C::kBQ, p.sq - i * C::kBQ);
@@ -612,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------------ softmax warps, epilogue of dV and dK
     asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     const int wg = warp >> 2;
-    const int row = (warp & 3) * 32 + lane;  // key of the tile (epilogue)
+    const int row = (warp & 3) * 32 + lane;  // key of the tile
     const uint32_t lanes = tmem_addr(tbase, (warp & 3) * 32, 0);
     const uint32_t col_s = lanes + C::kColS + wg * C::kHalfQ;
     const uint32_t col_dp = lanes + C::kColDp + wg * C::kHalfQ;
@@ -623,12 +627,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int st_row = (warp & 3) * 32 + ((lane >> 3) & 1) * 8 + (lane & 7);
     const int st_piece = (lane >> 4) + (C::kHalfQ == 64 ? 0 : wg * 4);
     const float c = p.scale_log2;
+    constexpr bool kOwnBox = C::kBQ == 128;  // a box of dS per warpgroup
+    constexpr int kEpiThreads = kOwnBox ? 128 : 256, kEpiRounds = kOwnBox ? C::kBoxes : 2 * C::kBoxes;
+    const int kEpiBarrier = kOwnBox ? 1 + wg : 1;
     bool ok = true;
     int g = 0, active = 0;
-    for (int r = 0; ok; ++r) {
+    for (int r = 0;; ++r) {
       const int u = __shfl_sync(0xffffffffu, lane == 0 ? next_unit(r, ok) : 0, 0);
       ok = __all_sync(0xffffffffu, ok);
-      if (!ok || u < 0) break;
+      if (!ok || u < 0) {
+        named_sync_and(kEpiBarrier, kEpiThreads, ok);  // this round's arrival (see the epilogue)
+        break;
+      }
       if (lane == 0) mbar_arrive(&bar_unit_empty[r & 1]);
       const Unit x = decode_unit<D>(p, u);
       const int key = x.j * kBK + row;
@@ -760,45 +770,58 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) mbar_arrive(&bar_ds);
         }
       }
+      // Epilogue: dV and dK, 64 columns at a time, through the dS buffer (the MMAs that read it are complete) to TMA
+      // stores, which clip the rows behind the last key.  With two boxes of dS warpgroup 0 takes dV and warpgroup 1 dK;
+      // with one both take half of each box.  (Rows written by their threads, 16 bytes at a stride, took 9600 cycles
+      // at D 128.)  Every warp comes here once per unit, whether its waits ran out or not, so none is left at a barrier.
+      if (ok && x.steps > 0)
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar_acc, active & 1, p.status, kDevTimeoutMma));
+      ok = named_sync_and(kEpiBarrier, kEpiThreads, ok);
       if (!ok) break;
-      // epilogue: warpgroup 0 writes dV, warpgroup 1 dK; a tile that no query sees gets zeros
-      if (x.steps > 0) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&bar_acc, active & 1, p.status, kDevTimeoutMma))) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-      }
-      const float mul = wg == 0 ? 1.0f : p.scale;
-      __nv_bfloat16* out = (wg == 0 ? p.dv : p.dk) + x.b * p.k_sb + x.kvh * p.k_sh + key * p.k_ss + x.half * C::kDH;
-#pragma unroll 1
-      for (int dc = 0; dc < C::kDH; dc += 32) {
-        uint32_t a[32];
+      tc_fence_after();
+      for (int round = 0; round < kEpiRounds; ++round) {
+        const int which = kOwnBox ? wg : round / C::kBoxes;  // 0: dV, 1: dK
+        const int box = kOwnBox ? round : round % C::kBoxes;
+        const float mul = which == 0 ? 1.0f : p.scale;
+        const uint32_t from = lanes + (which == 0 ? C::kColDv : C::kColDk) + box * 64 + (kOwnBox ? 0 : wg * C::kHalfQ);
+        uint32_t a[2][4 * kGroups];
         if (x.steps > 0) {
-          tmem_ld32(lanes + (wg == 0 ? C::kColDv : C::kColDk) + dc, a);
-        } else {
+          tmem_ld_frag<kGroups>(from, a[0]);
+          tmem_ld_frag<kGroups>(from + (16u << 16), a[1]);
+          tmem_wait_ld();
+        } else {  // a tile that no query sees
 #pragma unroll
-          for (int e = 0; e < 32; ++e) a[e] = 0u;
+          for (int e = 0; e < 4 * kGroups; ++e) a[0][e] = a[1][e] = 0u;
         }
-        if (key < p.skv) {
-          uint4* dst = reinterpret_cast<uint4*>(out + dc);
 #pragma unroll
-          for (int v4 = 0; v4 < 4; ++v4) {
+        for (int h16 = 0; h16 < 2; ++h16) {
+#pragma unroll
+          for (int n = 0; n < kGroups; n += 2) {
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              w[e] = pack_bf16x2(__uint_as_float(a[v4 * 8 + 2 * e]) * mul, __uint_as_float(a[v4 * 8 + 2 * e + 1]) * mul);
-            dst[v4] = make_uint4(w[0], w[1], w[2], w[3]);
+              w[e] = pack_bf16x2(__uint_as_float(a[h16][4 * n + 2 * e]) * mul, __uint_as_float(a[h16][4 * n + 2 * e + 1]) * mul);
+            st_matrix_x4(ds_base + sw128_offset(st_row + h16 * 16, (st_piece + n) * 16), w);
           }
         }
-      }
-      if (x.steps > 0) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar_accfree);
-        ++active;
+        if (round == kEpiRounds - 1 && x.steps > 0) {  // the accumulators are read
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar_accfree);
+          ++active;
+        }
+        fence_async_smem();
+        named_sync_and(kEpiBarrier, kEpiThreads, true);
+        if ((threadIdx.x & (kEpiThreads - 1)) == 0) {
+          tma_store_4d(which == 0 ? &map_dv : &map_dk, smem + C::kDs + (kOwnBox ? wg * C::kKBox : 0), x.half * C::kDH + box * 64,
+                       x.j * kBK, x.kvh, x.b);
+          bulk_commit();
+          bulk_wait_read();
+        }
+        named_sync_and(kEpiBarrier, kEpiThreads, true);
       }
     }
+    if ((threadIdx.x & (kEpiThreads - 1)) == 0) bulk_wait();
   }
 
   tc_fence_before();
@@ -848,6 +871,43 @@ __global__ void __launch_bounds__(256) fa2_bwd_prep(const __nv_bfloat16* __restr
   }
 }
 
+// dq from the sums over all key tiles: scaled, rounded, in dq's layout.  A block takes 32 TMEM columns of a tile.
+template <int D>
+__global__ void __launch_bounds__(128) fa2_bwd_dq(const Params p) {
+  using C = Cfg<D>;
+  wait_previous_kernels();
+  const long long tile = blockIdx.x;
+  const int c0 = blockIdx.y * 32;
+  const int half = static_cast<int>(tile % C::kSplit);
+  const long long t = tile / C::kSplit;
+  const int i = static_cast<int>(t % p.nq);
+  const long long bh = t / p.nq;
+  const float4* acc = reinterpret_cast<const float4*>(p.acc + tile * (C::kDqCols * 128)) + (c0 / 4) * 128 + threadIdx.x;
+  float4 v[8];
+#pragma unroll
+  for (int c = 0; c < 8; ++c) v[c] = __ldcs(acc + c * 128);
+  __nv_bfloat16* out = p.dq + (bh / p.hq) * p.q_sb + (bh % p.hq) * p.q_sh + static_cast<long long>(i) * C::kBQ * p.q_ss + half * C::kDH;
+  const int rows = min(C::kBQ, p.sq - i * C::kBQ);
+  if constexpr (C::kTransDq) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const float x[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int q = c0 + 4 * c + e;
+        if (q < rows) out[q * p.q_ss + threadIdx.x] = __float2bfloat16_rn(x[e] * p.scale);
+      }
+    }
+  } else if (static_cast<int>(threadIdx.x) < rows) {
+    uint4* dst = reinterpret_cast<uint4*>(out + threadIdx.x * p.q_ss + c0);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      dst[c] = make_uint4(pack_bf16x2(v[2 * c].x * p.scale, v[2 * c].y * p.scale), pack_bf16x2(v[2 * c].z * p.scale, v[2 * c].w * p.scale),
+                          pack_bf16x2(v[2 * c + 1].x * p.scale, v[2 * c + 1].y * p.scale),
+                          pack_bf16x2(v[2 * c + 1].z * p.scale, v[2 * c + 1].w * p.scale));
+  }
+}
+
 struct Sizes {
   long long counters, stats, acc, total;  // bytes
 };
@@ -883,9 +943,9 @@ int launch(const void* dout, const void* q, const void* k, const void* v, const 
     uint32_t box[4] = {64, rows, 1, 1};
     return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   };
-  CUtensorMap mq, mdo, mk, mv;
+  CUtensorMap mq, mdo, mk, mv, mdk, mdv;
   if (!make(&mq, q, sq, hq, C::kBQ) || !make(&mdo, dout, sq, hq, C::kBQ) || !make(&mk, k, skv, hkv, kBK) ||
-      !make(&mv, v, skv, hkv, kBK))
+      !make(&mv, v, skv, hkv, kBK) || !make(&mdk, dk, skv, hkv, kBK) || !make(&mdv, dv, skv, hkv, kBK))
     return TOKMIX_ERR_INVALID_ARGUMENT;
 
   Params p{};
@@ -928,6 +988,8 @@ int launch(const void* dout, const void* q, const void* k, const void* v, const 
   const int side_by_side = p.group > 1 ? 8 : 4;
   p.wave = (std::max(1, device_sm_count()) + side_by_side - 1) / side_by_side;
 
+  const long long tiles = static_cast<long long>(batch) * hq * p.nq * C::kSplit;
+  if (tiles > 0x7FFFFFFFll) return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_fa2_bwd: too many tiles (%lld)", tiles);
   const long long rows = static_cast<long long>(batch) * hq * p.nq * C::kBQ;
   const long long blocks = (rows * (D / 8) + 255) / 256;
   if (blocks > 0x7FFFFFFFll) return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_fa2_bwd: too many rows (%lld)", rows);
@@ -941,8 +1003,10 @@ int launch(const void* dout, const void* q, const void* k, const void* v, const 
   if (e == cudaSuccess) {
     const int grid = static_cast<int>(std::min<long long>(units, std::max(1, device_sm_count())));
     e = launch_overlapped(&fa2_bwd_kernel<D>, dim3(static_cast<unsigned>(grid)), dim3(kThreads),
-                          static_cast<size_t>(smem_bytes), stream, mq, mdo, mk, mv, p);
+                          static_cast<size_t>(smem_bytes), stream, mq, mdo, mk, mv, mdk, mdv, p);
   }
+  if (e == cudaSuccess && p.nk > 1)
+    e = launch_overlapped(&fa2_bwd_dq<D>, dim3(static_cast<unsigned>(tiles), C::kDqCols / 32), dim3(128), 0, stream, p);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(TOKMIX_ERR_LAUNCH, "tokmix_fa2_bwd: %s", cudaGetErrorString(e));
