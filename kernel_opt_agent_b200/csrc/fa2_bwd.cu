@@ -20,7 +20,7 @@
 //     dQ   = dS K      (SS; A is the same dS^T tile read MN-major)
 //   A query tile's dQ is the sum over key tiles, that is, over CTAs.  It grows in fp32 in global
 //   memory by vector reductions, in the order of the key tiles: the CTA of key tile j waits for the
-//   turn counter of (query tile, warp) to read j, adds, and sets it to j + 1.  So the bits are the
+//   query tile's turn counter to read j, adds, and sets it to j + 1.  So the bits are the
 //   same every time; the first tile stores instead of adding (no clearing pass).
 //   Units are taken from a counter in order of (batch, key/value head, key tile): a CTA waits only
 //   for units that were taken earlier, by CTAs that are running, so the waits end with any number
@@ -30,7 +30,7 @@
 //                   up for 10 000 to 20 000 cycles a tile.
 // Roles (512 threads): warps 0-7 softmax (two warpgroups, each half of a tile's query columns; thread =
 // key row), warps 8-11 dQ (TMEM to global), warp 12 TMA and unit counter, warp 13 TMEM owner and MMA
-// issuer, warps 14-15 idle (setmaxnreg works on whole warpgroups).
+// issuer, warps 14 and 15 pass on and wait for the turns of the dQ sums.
 // Order of the MMAs:  dP(t) dV(t) S(t+1) dQ(t) dK(t) | dP(t+1) ...: while the softmax warps form P
 // the tensor core has dQ and dK to do, and while they form dS it has dV and the next S.
 //
@@ -56,8 +56,8 @@ namespace fa2b {
 constexpr int kBK = 128;             // keys per unit
 constexpr int kThreads = 512;
 constexpr int kSoftmaxWarps = 8, kDqWarps = 4;
-constexpr int kWarpTma = 12, kWarpMma = 13;
-constexpr int kUnitReaders = 1 + kSoftmaxWarps + kDqWarps;
+constexpr int kWarpTma = 12, kWarpMma = 13, kWarpPass = 14, kWarpTurn = 15;
+constexpr int kUnitReaders = 3 + kSoftmaxWarps + kDqWarps;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D>
@@ -72,6 +72,10 @@ struct Cfg {
   static constexpr bool kTransDq = D == 256;           // dQ^T: lanes are columns of dq, columns are queries
   static constexpr int kDqCols = kTransDq ? kBQ : kDH; // TMEM columns of dQ
   static constexpr int kHalfQ = kBQ / 2;               // query columns of a softmax warpgroup
+  // Cycles between 8 KB of reductions: an SM sends about 25 bytes a cycle, and reductions that wait for that keep the
+  // tensor core from shared memory and TMA requests in the queue (D 128, 64 KB a step: B4 Hq32 Hkv8 S8192 took 6809 us
+  // without, 6325 with 320 cycles, 6623 with 440).  Half as much a step (D 64, 256) needs none.
+  static constexpr int kPace = D == 128 ? 320 : 0;
   static constexpr uint32_t kColS = 0;
   static constexpr uint32_t kColDp = kBQ;
   static constexpr uint32_t kColDq = kAlias ? kColDp : 2 * kBQ;
@@ -103,11 +107,11 @@ struct Params {
   long long k_sb, k_sh, k_ss;        // and of k, v, dk, dv
   const float* stats;                // [batch * hq][nq][lse2, delta][kBQ]
   float* acc;                        // [batch * hq][nq][split][kDqCols / 4][128][4]
-  uint32_t* turns;                   // [batch * hq][nq][split][4]
+  uint32_t* turns;                   // [batch * hq][nq][split]
   uint32_t* ticket;
   int batch, hq, hkv, group, sq, skv, nq, nk;
   int units;
-  int wave;                          // (batch, key/value head, half) rows whose key tiles are interleaved
+  int wave;                          // the order of the units, see Unit
   int causal;
   float scale, scale_log2;
   uint32_t* status;
@@ -180,26 +184,21 @@ __device__ __forceinline__ void red_add_v4(float* dst, float a, float b, float c
                : "memory");
 }
 
-// Whole warp: waits (bounded) until the turn counter reads `want`; lane 0 polls.
+// Waits (bounded) until the turn counter reads `want`.
 __device__ __forceinline__ bool wait_turn(const uint32_t* turn, uint32_t want, uint32_t* status) {
-  bool ok = true;
-  if (lane_id() == 0) {
-    const unsigned long long t0 = global_timer_ns();
-    while (true) {
-      uint32_t v;
-      asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(turn) : "memory");
-      if (v == want) break;
-      if (cta_abort_flag() != 0u) { ok = false; break; }
-      if (global_timer_ns() - t0 > kWaitTimeoutNs) {
-        record_status(status, kDevTimeoutPipe);
-        cta_abort_flag() = 1u;
-        ok = false;
-        break;
-      }
-      __nanosleep(20);
+  const unsigned long long t0 = global_timer_ns();
+  while (true) {
+    uint32_t v;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(turn) : "memory");
+    if (v == want) return true;
+    if (cta_abort_flag() != 0u) return false;
+    if (global_timer_ns() - t0 > kWaitTimeoutNs) {
+      record_status(status, kDevTimeoutPipe);
+      cta_abort_flag() = 1u;
+      return false;
     }
+    __nanosleep(20);
   }
-  return __all_sync(0xffffffffu, ok);
 }
 
 // 16 lanes x 8 N columns of TMEM, dealt out like an mma accumulator: thread l gets, of every 8 columns i,
@@ -277,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using C = Cfg<D>;
   extern __shared__ __align__(1024) uint8_t smem[];  // no room is left to round its start up
   __shared__ uint64_t bar_unit_full[2], bar_unit_empty[2], bar_kv_full, bar_kv_empty, bar_v, bar_q_full[2], bar_q_empty[2],
-      bar_do_full[2], bar_do_empty[2], bar_s, bar_p, bar_dp, bar_ds, bar_dq, bar_dqfree, bar_acc, bar_accfree, bar_drain;
+      bar_do_full[2], bar_do_empty[2], bar_s, bar_p, bar_dp, bar_ds, bar_dq, bar_dqfree, bar_turn[2], bar_added[2], bar_passed[2], bar_acc, bar_accfree, bar_drain;
   __shared__ int unit_ring[2];
   __shared__ uint32_t tmem_base_shared;
 
@@ -297,6 +296,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bar_q_empty[i], 1);
       mbar_init(&bar_do_full[i], 1);
       mbar_init(&bar_do_empty[i], 1);
+      mbar_init(&bar_turn[i], 1);
+      mbar_init(&bar_added[i], kDqWarps);
+      mbar_init(&bar_passed[i], 1);
     }
     mbar_init(&bar_kv_full, 1);
     mbar_init(&bar_kv_empty, 1);
@@ -532,6 +534,42 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_drain(&bar_drain, 0);
       }
       __syncwarp();
+    } else if (lane == 0) {
+      // ---------------------------------------------------------------- turns of the dQ sums
+      // kWarpTurn waits for a step's turn, a step or two ahead of the dQ warps' additions; kWarpPass waits for
+      // those, for their arrival in L2 (the fence: 1700 cycles, which the dQ warps need not stand still for),
+      // and passes the turn on.
+      const bool pass = warp == kWarpPass;
+      bool ok = true;
+      int g = 0;
+      for (int r = 0; ok; ++r) {
+        const int u = next_unit(r, ok);
+        if (!ok || u < 0) break;
+        mbar_arrive(&bar_unit_empty[r & 1]);
+        if (p.nk == 1) continue;  // no sums
+        const Unit x = decode_unit<D>(p, u);
+        for (int i = p.nq - 1; ok && i >= x.i_min; --i) {
+          const int count = contributors<D>(p, i);
+          for (int h = 0; h < p.group; ++h, ++g) {
+            const long long bh = static_cast<long long>(x.b) * p.hq + x.kvh * p.group + h;
+            uint32_t* turn = p.turns + (bh * p.nq + i) * C::kSplit + x.half;
+            if (pass) {
+              ok = mbar_wait(&bar_added[g & 1], (g >> 1) & 1, p.status, kDevTimeoutPipe);
+              if (!ok) break;
+              if (x.j + 1 < count) {
+                __threadfence();
+                asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(turn), "r"(static_cast<uint32_t>(x.j + 1)) : "memory");
+              }
+              mbar_arrive(&bar_passed[g & 1]);
+            } else {
+              ok = (g < 2 || mbar_wait(&bar_passed[g & 1], ((g >> 1) - 1) & 1, p.status, kDevTimeoutPipe)) &&
+                   (x.j == 0 || wait_turn(turn, static_cast<uint32_t>(x.j), p.status));
+              if (!ok) break;
+              mbar_arrive(&bar_turn[g & 1]);
+            }
+          }
+        }
+      }
     }
   } else if (warp >= kSoftmaxWarps) {
     // ------------------------------------------------------------------ dQ: TMEM -> global, in turn
@@ -552,8 +590,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int head = x.kvh * p.group + h;
           const long long bh = static_cast<long long>(x.b) * p.hq + head;
           const long long tile = (bh * p.nq + i) * C::kSplit + x.half;
-          uint32_t* turn = p.turns + tile * 4 + wq;
-          const int count = contributors<D>(p, i);
           if (!__all_sync(0xffffffffu, mbar_wait(&bar_dq, g & 1, p.status, kDevTimeoutMma))) {
             ok = false;
             break;
@@ -565,11 +601,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&bar_dqfree);
           float* acc = p.acc + tile * (C::kDqCols * 128) + row * 4;
-          if (x.j > 0 && !wait_turn(turn, static_cast<uint32_t>(x.j), p.status)) {
-            ok = false;
-            break;
-          }
           if (p.nk > 1) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&bar_turn[g & 1], (g >> 1) & 1, p.status, kDevTimeoutPipe))) {
+              ok = false;
+              break;
+            }
             if (x.j == 0) {
 #pragma unroll
               for (int c = 0; c < C::kDqCols / 4; ++c)
@@ -578,17 +614,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                                    __uint_as_float(v[4 * c + 3])));
             } else {
 #pragma unroll
-              for (int c = 0; c < C::kDqCols / 4; ++c)
+              for (int c = 0; c < C::kDqCols / 4; ++c) {
+                if (C::kPace > 0 && c % 4 == 0 && c > 0)
+                  for (const long long t0 = clock64(); clock64() - t0 < C::kPace;) {}
                 red_add_v4(acc + c * 512, __uint_as_float(v[4 * c]), __uint_as_float(v[4 * c + 1]),
                            __uint_as_float(v[4 * c + 2]), __uint_as_float(v[4 * c + 3]));
-            }
-            if (x.j + 1 < count) {
-              __syncwarp();
-              if (lane == 0) {
-                __threadfence();
-                asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(turn), "r"(static_cast<uint32_t>(x.j + 1)) : "memory");
               }
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar_added[g & 1]);
           } else {  // one key tile: the sum is complete
             __nv_bfloat16* out = p.dq + x.b * p.q_sb + head * p.q_sh + static_cast<long long>(i) * C::kBQ * p.q_ss +
                                  x.half * C::kDH;
@@ -918,7 +952,7 @@ Sizes sizes(long long batch, long long hq, long long sq, long long skv) {
   const long long tiles = batch * hq * ((sq + C::kBQ - 1) / C::kBQ);
   auto up = [](long long n) { return (n + 255) / 256 * 256; };
   Sizes s{};
-  s.counters = up((1 + tiles * C::kSplit * 4) * 4);
+  s.counters = up((1 + tiles * C::kSplit) * 4);
   s.stats = up(tiles * C::kStatBytes);
   s.acc = skv > kBK ? tiles * C::kSplit * C::kDqCols * 128 * 4 : 0;  // one key tile: dq is written at once
   s.total = s.counters + s.stats + s.acc;
@@ -982,11 +1016,10 @@ int launch(const void* dout, const void* q, const void* k, const void* v, const 
   if (units > 0x3FFFFFFFll || steps > 0x3FFFFFFFll)
     return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_fa2_bwd: too many tiles (%lld x %lld)", units, steps);
   p.units = static_cast<int>(units);
-  // CTAs of a row run side by side and share its tiles of Q, dO and dQ in L2, each a turn behind the one before:
-  // 4 to a row, 8 where several heads give the turns more time (B4 Hq32 Hkv8 S8192 D128: 6970 us at 4, 6759 at 8,
-  // 6900 at 16; B8 H8 S2048 D128: 298 at 4, 358 at 8, 466 at 16).
-  const int side_by_side = p.group > 1 ? 8 : 4;
-  p.wave = (std::max(1, device_sm_count()) + side_by_side - 1) / side_by_side;
+  // The rows of a wave fill the SMs with 4 key tiles each, 8 where several heads give the turns more time (B4 Hq32
+  // Hkv8 S8192 D128: 6842 us at 4, 6623 at 8, 6779 at 16; B8 H8 S2048 D128: 281 at 2, 282 at 4, 341 at 8).
+  const int share = p.group > 1 ? 8 : 4;
+  p.wave = (std::max(1, device_sm_count()) + share - 1) / share;
 
   const long long tiles = static_cast<long long>(batch) * hq * p.nq * C::kSplit;
   if (tiles > 0x7FFFFFFFll) return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_fa2_bwd: too many tiles (%lld)", tiles);
