@@ -89,8 +89,9 @@ int tokmix_fa2_bwd(const void* dout, const void* q, const void* k, const void* v
                    int head_dim, int layout, int causal, float sm_scale, void* workspace, long long workspace_bytes,
                    uint32_t* status, void* stream);
 
-/* Workspace size of tokmix_fa2_bwd in bytes (-1 for bad arguments). */
-long long tokmix_fa2_bwd_workspace_bytes(int batch, int heads_q, int seqlen_q, int seqlen_kv, int head_dim);
+/* Workspace size of tokmix_fa2_bwd in bytes on the current device (-1 for bad arguments). */
+long long tokmix_fa2_bwd_workspace_bytes(int batch, int heads_q, int heads_kv, int seqlen_q, int seqlen_kv, int head_dim,
+                                         int causal);
 
 /* Steps before the recurrence that the GDN prefill entry points can do inside their first stage
  * (the `gates` argument; NULL = neither).  The reference takes normalised q, k and ready g, beta

@@ -49,7 +49,7 @@ SIGNATURES = {
     "tokmix_fa2_fwd": (_I, [_VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _I, _F, _VP, _VP]),
     "tokmix_fa2_fwd_lse": (_I, [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _I, _F, _VP, _VP]),
     "tokmix_fa2_bwd": (_I, [_VP] * 9 + [_I] * 8 + [_F, _VP, _LL, _VP, _VP]),
-    "tokmix_fa2_bwd_workspace_bytes": (_LL, [_I, _I, _I, _I, _I]),
+    "tokmix_fa2_bwd_workspace_bytes": (_LL, [_I] * 7),
     "tokmix_gdn_prefill": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _F, _I, _VP,
                                 _VP, _VP]),
     "tokmix_gdn_prefill_noalloc": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _F, _I, _VP,

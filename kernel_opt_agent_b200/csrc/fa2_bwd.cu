@@ -25,8 +25,8 @@
 //   Units are taken from a counter in order of (batch, key/value head, key tile): a CTA waits only
 //   for units that were taken earlier, by CTAs that are running, so the waits end with any number
 //   of resident CTAs.  Under the causal mask this order is longest first.
-//   fa2_bwd_dq      dq = c times those sums, rounded, in dq's layout (a single key tile's dQ is written at once: no such
-//                   launch).  The last key tile's CTA could do it in passing, but reading the sums back held its pipeline
+//   fa2_bwd_finish  dq = c times those sums, rounded, in dq's layout, and dV and dK of key tiles that came in parts (with
+//                   a single key tile, whose dQ is written at once, and no parts, no such launch).  The last key tile's CTA could do it in passing, but reading the sums back held its pipeline
 //                   up for 10 000 to 20 000 cycles a tile.
 // Roles (512 threads): warps 0-7 softmax (two warpgroups, each half of a tile's query columns; thread =
 // key row), warps 8-11 dQ (TMEM to global), warp 12 TMA and unit counter, warp 13 TMEM owner and MMA
@@ -58,6 +58,7 @@ constexpr int kThreads = 512;
 constexpr int kSoftmaxWarps = 8, kDqWarps = 4;
 constexpr int kWarpTma = 12, kWarpMma = 13, kWarpPass = 14, kWarpTurn = 15;
 constexpr int kUnitReaders = 3 + kSoftmaxWarps + kDqWarps;
+constexpr int kMaxParted = 256;      // key tiles of a row that may come in parts
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D>
@@ -106,23 +107,35 @@ struct Params {
   long long q_sb, q_sh, q_ss;        // element strides of q, o, do, dq (batch, head, row)
   long long k_sb, k_sh, k_ss;        // and of k, v, dk, dv
   const float* stats;                // [batch * hq][nq][lse2, delta][kBQ]
-  float* acc;                        // [batch * hq][nq][split][kDqCols / 4][128][4]
-  uint32_t* turns;                   // [batch * hq][nq][split]
+  int streams;                       // sums that a query tile's dQ is gathered in: key tile j adds to sum j % streams
+  float* acc;                        // [streams][batch * hq][nq][split][kDqCols / 4][128][4]
+  uint32_t* turns;                   // [streams][batch * hq][nq][split]
+  long long tiles;                   // batch * hq * nq * split
   uint32_t* ticket;
   int batch, hq, hkv, group, sq, skv, nq, nk;
   int units;
   int wave;                          // the order of the units, see Unit
+  int per_row;                       // units of a row: nk, or with parts first[nk]
+  int part_tiles;                    // query tiles of a part
+  float* partial;                    // [rows][per_row][dV, dK][kDH / 4][128][4]
+  uint16_t first[kMaxParted + 1];    // with parts: the first unit of each key tile in its row
   int causal;
   float scale, scale_log2;
   uint32_t* status;
 };
 
-// One unit: key tile j of (b, kvh), column half `half`; its steps visit the query tiles nq-1 .. i_min, each for
-// every query head of the group (heads inside tiles: head by head, a later and shorter unit could not
-// pass the earlier one into the next head, B2 Hq16 Hkv2 S4096 D256 took 2490 us).  Units are numbered wave by wave: within a wave of p.wave
-// (b, kvh, half) rows, all their first key tiles, then all their second ones, and so on.
+// One unit: key tile j of (b, kvh), column half `half`.  The steps of a key tile visit the query tiles nq-1 .. i_min,
+// each for every query head of the group (heads inside tiles: head by head, a later and shorter unit could not
+// pass the earlier one into the next head, B2 Hq16 Hkv2 S4096 D256 took 2490 us for 1744).  Where key tiles are too
+// few to fill the GPU a unit is one of `parts` parts of a tile's steps, p.part_tiles query tiles each (cut at the same query
+// tiles for every key tile: their turns go with each other), and leaves its dV and dK in fp32 for fa2_bwd_finish to
+// add.  Units are numbered wave by wave: within a wave of p.wave (b, kvh, half) rows, all
+// their first units, then all their second ones, and so on.
 struct Unit {
-  int b, kvh, j, half, i_min, steps;
+  int b, kvh, j, half;
+  int i0, steps;         // first query tile, number of steps
+  int parts;
+  long long slot;        // of p.partial
 };
 
 template <int D>
@@ -130,18 +143,45 @@ __device__ __forceinline__ Unit decode_unit(const Params& p, int u) {
   using C = Cfg<D>;
   Unit x;
   const int rows = p.batch * p.hkv * C::kSplit;
-  const int first = u / (p.wave * p.nk) * p.wave;  // first row of the wave
+  const int first = u / (p.wave * p.per_row) * p.wave;  // first row of the wave
   const int in_wave = min(p.wave, rows - first);
-  u -= first * p.nk;
-  x.j = u / in_wave;
-  int row = first + u - x.j * in_wave;
+  u -= first * p.per_row;
+  const int v = u / in_wave;
+  int row = first + u - v * in_wave;
+  x.slot = static_cast<long long>(row) * p.per_row + v;
   x.half = row % C::kSplit;
   row /= C::kSplit;
   x.kvh = row % p.hkv;
   x.b = row / p.hkv;
-  x.i_min = p.causal ? x.j * (kBK / C::kBQ) : 0;
-  x.steps = max(0, p.nq - x.i_min) * p.group;
+  int part = 0;
+  x.j = v;
+  x.parts = 1;
+  if (p.partial != nullptr) {
+    int lo = 0, hi = p.nk;  // first[lo] <= v < first[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (p.first[mid] <= v)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    x.j = lo;
+    part = v - p.first[lo];
+    x.parts = p.first[lo + 1] - p.first[lo];
+  }
+  const int all = max(0, p.nq - (p.causal ? x.j * (kBK / C::kBQ) : 0));  // query tiles
+  const int skip = part * p.part_tiles;
+  x.i0 = p.nq - 1 - skip;
+  x.steps = (x.parts > 1 ? min(p.part_tiles, all - skip) : all) * p.group;
   return x;
+}
+
+// The step after (i, h)
+__device__ __forceinline__ void next_step(const Params& p, int& i, int& h) {
+  if (++h == p.group) {
+    h = 0;
+    --i;
+  }
 }
 
 // number of key tiles that add to query tile i
@@ -355,9 +395,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive(&bar_unit_full[r & 1]);
           if (u < 0) break;
           const Unit x = decode_unit<D>(p, u);
-          int t = 0;
-          for (int i = p.nq - 1; ok && i >= x.i_min; --i) {
-            for (int h = 0; h < p.group; ++h, ++t, ++g) {
+          {
+            int i = x.i0, h = 0;
+            for (int t = 0; t < x.steps; ++t, ++g, next_step(p, i, h)) {
               const int head = x.kvh * p.group + h;
               const long long bh = static_cast<long long>(x.b) * p.hq + head;
               const int qs = g % C::kNQ, ds = g % C::kNDO;
@@ -548,22 +588,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(&bar_unit_empty[r & 1]);
         if (p.nk == 1) continue;  // no sums
         const Unit x = decode_unit<D>(p, u);
-        for (int i = p.nq - 1; ok && i >= x.i_min; --i) {
-          const int count = contributors<D>(p, i);
-          for (int h = 0; h < p.group; ++h, ++g) {
+        uint32_t* turns = p.turns + x.j % p.streams * p.tiles;
+        const uint32_t rank = x.j / p.streams;
+        {
+          int i = x.i0, h = 0;
+          for (int t = 0; t < x.steps; ++t, ++g, next_step(p, i, h)) {
+            const int count = contributors<D>(p, i);
             const long long bh = static_cast<long long>(x.b) * p.hq + x.kvh * p.group + h;
-            uint32_t* turn = p.turns + (bh * p.nq + i) * C::kSplit + x.half;
+            uint32_t* turn = turns + (bh * p.nq + i) * C::kSplit + x.half;
             if (pass) {
               ok = mbar_wait(&bar_added[g & 1], (g >> 1) & 1, p.status, kDevTimeoutPipe);
               if (!ok) break;
-              if (x.j + 1 < count) {
+              if (x.j + p.streams < count) {
                 __threadfence();
-                asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(turn), "r"(static_cast<uint32_t>(x.j + 1)) : "memory");
+                asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(turn), "r"(rank + 1) : "memory");
               }
               mbar_arrive(&bar_passed[g & 1]);
             } else {
               ok = (g < 2 || mbar_wait(&bar_passed[g & 1], ((g >> 1) - 1) & 1, p.status, kDevTimeoutPipe)) &&
-                   (x.j == 0 || wait_turn(turn, static_cast<uint32_t>(x.j), p.status));
+                   (rank == 0 || wait_turn(turn, rank, p.status));
               if (!ok) break;
               mbar_arrive(&bar_turn[g & 1]);
             }
@@ -585,8 +628,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok || u < 0) break;
       if (lane == 0) mbar_arrive(&bar_unit_empty[r & 1]);
       const Unit x = decode_unit<D>(p, u);
-      for (int i = p.nq - 1; ok && i >= x.i_min; --i) {
-        for (int h = 0; h < p.group; ++h, ++g) {
+      {
+        int i = x.i0, h = 0;
+        for (int t = 0; t < x.steps; ++t, ++g, next_step(p, i, h)) {
           const int head = x.kvh * p.group + h;
           const long long bh = static_cast<long long>(x.b) * p.hq + head;
           const long long tile = (bh * p.nq + i) * C::kSplit + x.half;
@@ -600,13 +644,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bar_dqfree);
-          float* acc = p.acc + tile * (C::kDqCols * 128) + row * 4;
+          float* acc = p.acc + (x.j % p.streams * p.tiles + tile) * (C::kDqCols * 128) + row * 4;
           if (p.nk > 1) {
             if (!__all_sync(0xffffffffu, mbar_wait(&bar_turn[g & 1], (g >> 1) & 1, p.status, kDevTimeoutPipe))) {
               ok = false;
               break;
             }
-            if (x.j == 0) {
+            if (x.j < p.streams) {
 #pragma unroll
               for (int c = 0; c < C::kDqCols / 4; ++c)
                 __stcg(reinterpret_cast<float4*>(acc + c * 512),
@@ -698,8 +742,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar_v);
       }
-      for (int i = p.nq - 1; ok && i >= x.i_min; --i) {
-        for (int h = 0; h < p.group; ++h, ++g) {
+      {
+        int i = x.i0, h = 0;
+        for (int t = 0; t < x.steps; ++t, ++g, next_step(p, i, h)) {
           const int qs = g % C::kNQ;
           if (!__all_sync(0xffffffffu, mbar_wait(&bar_q_full[qs], (g / C::kNQ) & 1, p.status, kDevTimeoutTma) &&
                                            mbar_wait(&bar_s, g & 1, p.status, kDevTimeoutMma))) {
@@ -813,6 +858,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = named_sync_and(kEpiBarrier, kEpiThreads, ok);
       if (!ok) break;
       tc_fence_after();
+      if (x.parts > 1) {  // a part: fp32, as fa2_bwd_finish reads it; warpgroup 0 dV, warpgroup 1 dK
+        float* dst = p.partial + (x.slot * 2 + wg) * (C::kDH * 128) + row * 4;
+#pragma unroll 1
+        for (int dc = 0; dc < C::kDH; dc += 32) {
+          uint32_t a[32];
+          tmem_ld32(lanes + (wg == 0 ? C::kColDv : C::kColDk) + dc, a);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            __stcg(reinterpret_cast<float4*>(dst + (dc / 4 + e) * 512),
+                   make_float4(__uint_as_float(a[4 * e]), __uint_as_float(a[4 * e + 1]), __uint_as_float(a[4 * e + 2]),
+                               __uint_as_float(a[4 * e + 3])));
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar_accfree);
+        ++active;
+        continue;
+      }
       for (int round = 0; round < kEpiRounds; ++round) {
         const int which = kOwnBox ? wg : round / C::kBoxes;  // 0: dV, 1: dK
         const int box = kOwnBox ? round : round % C::kBoxes;
@@ -905,58 +968,172 @@ __global__ void __launch_bounds__(256) fa2_bwd_prep(const __nv_bfloat16* __restr
   }
 }
 
-// dq from the sums over all key tiles: scaled, rounded, in dq's layout.  A block takes 32 TMEM columns of a tile.
+__device__ __forceinline__ void store_row(__nv_bfloat16* out, const float4 (&v)[8], float mul) {
+  uint4* dst = reinterpret_cast<uint4*>(out);
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    dst[c] = make_uint4(pack_bf16x2(v[2 * c].x * mul, v[2 * c].y * mul), pack_bf16x2(v[2 * c].z * mul, v[2 * c].w * mul),
+                        pack_bf16x2(v[2 * c + 1].x * mul, v[2 * c + 1].y * mul),
+                        pack_bf16x2(v[2 * c + 1].z * mul, v[2 * c + 1].w * mul));
+}
+
+// dq from the sums over all key tiles: scaled, rounded, in dq's layout; a block takes 32 TMEM columns of a tile.  Behind
+// those blocks, dV and dK of key tiles that came in parts: the parts added in order, a block 32 columns of one of the
+// two.
 template <int D>
-__global__ void __launch_bounds__(128) fa2_bwd_dq(const Params p) {
+__global__ void __launch_bounds__(128) fa2_bwd_finish(const __grid_constant__ Params p, const int dq_blocks) {
   using C = Cfg<D>;
   wait_previous_kernels();
-  const long long tile = blockIdx.x;
-  const int c0 = blockIdx.y * 32;
-  const int half = static_cast<int>(tile % C::kSplit);
-  const long long t = tile / C::kSplit;
-  const int i = static_cast<int>(t % p.nq);
-  const long long bh = t / p.nq;
-  const float4* acc = reinterpret_cast<const float4*>(p.acc + tile * (C::kDqCols * 128)) + (c0 / 4) * 128 + threadIdx.x;
+  const int row = threadIdx.x;
+  int block = static_cast<int>(blockIdx.x);
   float4 v[8];
+  if (block < dq_blocks) {
+    const long long tile = block / (C::kDqCols / 32);
+    const int c0 = block % (C::kDqCols / 32) * 32;
+    const int half = static_cast<int>(tile % C::kSplit);
+    const long long t = tile / C::kSplit;
+    const int i = static_cast<int>(t % p.nq);
+    const long long bh = t / p.nq;
+    const float4* acc = reinterpret_cast<const float4*>(p.acc + tile * (C::kDqCols * 128)) + (c0 / 4) * 128 + row;
 #pragma unroll
-  for (int c = 0; c < 8; ++c) v[c] = __ldcs(acc + c * 128);
-  __nv_bfloat16* out = p.dq + (bh / p.hq) * p.q_sb + (bh % p.hq) * p.q_sh + static_cast<long long>(i) * C::kBQ * p.q_ss + half * C::kDH;
-  const int rows = min(C::kBQ, p.sq - i * C::kBQ);
-  if constexpr (C::kTransDq) {
+    for (int c = 0; c < 8; ++c) v[c] = __ldcs(acc + c * 128);
+    const int sums = min(p.streams, contributors<D>(p, i));
+    for (int q = 1; q < sums; ++q) {
+      acc += p.tiles * (C::kDqCols * 128 / 4);
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      const float x[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int q = c0 + 4 * c + e;
-        if (q < rows) out[q * p.q_ss + threadIdx.x] = __float2bfloat16_rn(x[e] * p.scale);
+      for (int c = 0; c < 8; ++c) {
+        const float4 w = __ldcs(acc + c * 128);
+        v[c] = make_float4(v[c].x + w.x, v[c].y + w.y, v[c].z + w.z, v[c].w + w.w);
       }
     }
-  } else if (static_cast<int>(threadIdx.x) < rows) {
-    uint4* dst = reinterpret_cast<uint4*>(out + threadIdx.x * p.q_ss + c0);
+    __nv_bfloat16* out = p.dq + (bh / p.hq) * p.q_sb + (bh % p.hq) * p.q_sh + static_cast<long long>(i) * C::kBQ * p.q_ss + half * C::kDH;
+    const int rows = min(C::kBQ, p.sq - i * C::kBQ);
+    if constexpr (C::kTransDq) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      dst[c] = make_uint4(pack_bf16x2(v[2 * c].x * p.scale, v[2 * c].y * p.scale), pack_bf16x2(v[2 * c].z * p.scale, v[2 * c].w * p.scale),
-                          pack_bf16x2(v[2 * c + 1].x * p.scale, v[2 * c + 1].y * p.scale),
-                          pack_bf16x2(v[2 * c + 1].z * p.scale, v[2 * c + 1].w * p.scale));
+      for (int c = 0; c < 8; ++c) {
+        const float x[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int q = c0 + 4 * c + e;
+          if (q < rows) out[q * p.q_ss + row] = __float2bfloat16_rn(x[e] * p.scale);
+        }
+      }
+    } else if (row < rows) {
+      store_row(out + row * p.q_ss + c0, v, p.scale);
+    }
+    return;
   }
+  block -= dq_blocks;
+  const int c0 = block % (C::kDH / 32) * 32;
+  block /= C::kDH / 32;
+  const int which = block & 1;  // 0: dV, 1: dK
+  block >>= 1;
+  const int j = block % p.nk;
+  int r = block / p.nk;
+  const int parts = p.first[j + 1] - p.first[j];
+  if (parts == 1) return;
+  const float4* src = reinterpret_cast<const float4*>(p.partial + ((static_cast<long long>(r) * p.per_row + p.first[j]) * 2 + which) *
+                                                                      (C::kDH * 128)) +
+                      (c0 / 4) * 128 + row;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) v[c] = __ldcs(src + c * 128);
+  for (int q = 1; q < parts; ++q) {
+    src += 2 * (C::kDH * 128) / 4;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const float4 w = __ldcs(src + c * 128);
+      v[c] = make_float4(v[c].x + w.x, v[c].y + w.y, v[c].z + w.z, v[c].w + w.w);
+    }
+  }
+  const int half = r % C::kSplit;
+  r /= C::kSplit;
+  const long long key = static_cast<long long>(j) * kBK + row;
+  __nv_bfloat16* out = (which == 0 ? p.dv : p.dk) + (r / p.hkv) * p.k_sb + (r % p.hkv) * p.k_sh + key * p.k_ss + half * C::kDH + c0;
+  if (key < p.skv) store_row(out, v, which == 0 ? 1.0f : p.scale);
+}
+
+// How a call is cut.
+struct Plan {
+  int part_tiles;                    // query tiles of a part (0: whole key tiles)
+  int per_row;                       // units of a row
+  int streams;
+  uint16_t first[kMaxParted + 1];
+};
+
+// Parts cost their fp32 way through memory and pay where key tiles are few: the time of a cut, in steps, is the
+// longest unit or the mean load of an SM with what a unit costs beside its steps (2) and what the ends of the SMs' queues differ by
+// (a sixth of the longest unit, causal units being sorted by length; half of it otherwise), and the joining of the parts.
+// (D 128: B1 Hq32 Hkv8 S2048, 128 key tiles of up to 64 steps: 211 us whole, 103 in parts.)
+template <int D>
+Plan plan(int batch, int hkv, int group, int nq, int nk, int causal) {
+  using C = Cfg<D>;
+  Plan best{};
+  best.per_row = nk;
+  const long long rows = static_cast<long long>(batch) * hkv * C::kSplit;
+  const int sms = device_sm_count() > 0 ? device_sm_count() : 148;
+  // A row's CTAs that start at once add to the same query tiles one behind the other, about 3 us each: where
+  // a row's key tiles mostly start at once, dQ is gathered in several sums (B3 Hq12 Hkv4 1000 x 1531 D64, 12 key tiles: 105
+  // us with one sum, 84 with 2, 79 with 4).  Longer calls lose more to the wider sums than to the turns.
+  best.streams = rows * nk > 2LL * sms ? 1 : nk < 4 ? std::max(1, nk) : std::min(4, nk / 4);
+  if (nk > kMaxParted || rows * nk >= 8LL * sms) return best;  // enough whole tiles
+  auto tiles = [&](int j) { return std::max(0, nq - (causal ? j * (kBK / C::kBQ) : 0)); };
+  auto parts_of = [&](int j, int part_tiles) { return std::max(1, (tiles(j) + part_tiles - 1) / part_tiles); };
+  double total = 0.0;
+  for (int j = 0; j < nk; ++j) total += static_cast<double>(tiles(j)) * group * rows;
+  double best_time = 0.0;
+  for (int cut = 1; cut <= 16 && cut <= nq; ++cut) {
+    const int part_tiles = (nq + cut - 1) / cut;
+    long long units = 0, parts = 0;
+    for (int j = 0; j < nk; ++j) {
+      const int n = parts_of(j, part_tiles);
+      units += n;
+      parts += n > 1 ? n : 0;
+    }
+    if (units > 0xFFFF) break;
+    const double longest = static_cast<double>(part_tiles) * group;
+    const double joined = static_cast<double>(parts) * rows * (2.0 * C::kDH * 128 * 4) * 2.0;  // bytes written and read
+    const double mean = (total + 2.0 * static_cast<double>(units) * rows) / sms;
+    const double time = std::max(longest + 2.0, mean + longest / (causal ? 6 : 2)) +
+                        (parts > 0 ? 1.0 + joined / 8e6 : 0.0);  // a step is about 2 us, in which 8 MB pass
+    if (cut == 1 || time < 0.85 * best_time) {
+      best_time = time;
+      best.part_tiles = parts > 0 ? part_tiles : 0;
+      best.per_row = static_cast<int>(units);
+    }
+  }
+  if (best.part_tiles > 0) {
+    int at = 0;
+    for (int j = 0; j < nk; ++j) {
+      best.first[j] = static_cast<uint16_t>(at);
+      at += parts_of(j, best.part_tiles);
+    }
+    best.first[nk] = static_cast<uint16_t>(at);
+  }
+  return best;
 }
 
 struct Sizes {
-  long long counters, stats, acc, total;  // bytes
+  long long counters, stats, acc, partial, total;  // bytes
 };
 
 template <int D>
-Sizes sizes(long long batch, long long hq, long long sq, long long skv) {
+Sizes sizes(long long batch, long long hq, long long hkv, long long sq, long long skv, const Plan& plan) {
   using C = Cfg<D>;
   const long long tiles = batch * hq * ((sq + C::kBQ - 1) / C::kBQ);
   auto up = [](long long n) { return (n + 255) / 256 * 256; };
   Sizes s{};
-  s.counters = up((1 + tiles * C::kSplit) * 4);
+  s.counters = up((1 + plan.streams * tiles * C::kSplit) * 4);
   s.stats = up(tiles * C::kStatBytes);
-  s.acc = skv > kBK ? tiles * C::kSplit * C::kDqCols * 128 * 4 : 0;  // one key tile: dq is written at once
-  s.total = s.counters + s.stats + s.acc;
+  s.acc = skv > kBK ? plan.streams * tiles * C::kSplit * C::kDqCols * 128 * 4 : 0;  // one key tile: dq is written at once
+  s.partial = plan.part_tiles > 0 ? batch * hkv * C::kSplit * plan.per_row * (2LL * C::kDH * 128 * 4) : 0;
+  s.total = s.counters + s.stats + s.acc + s.partial;
   return s;
+}
+
+template <int D>
+Plan plan_of(int batch, int hq, int hkv, int sq, int skv, int causal) {
+  return plan<D>(batch, hkv, hq / hkv, static_cast<int>((static_cast<long long>(sq) + Cfg<D>::kBQ - 1) / Cfg<D>::kBQ),
+                 static_cast<int>((static_cast<long long>(skv) + kBK - 1) / kBK), causal);
 }
 
 template <int D>
@@ -964,7 +1141,8 @@ int launch(const void* dout, const void* q, const void* k, const void* v, const 
            void* dk, void* dv, int batch, int hq, int hkv, int sq, int skv, int layout, int causal, float sm_scale,
            void* workspace, long long workspace_bytes, uint32_t* status, cudaStream_t stream) {
   using C = Cfg<D>;
-  const Sizes sz = sizes<D>(batch, hq, sq, skv);
+  const Plan cut = plan_of<D>(batch, hq, hkv, sq, skv, causal);
+  const Sizes sz = sizes<D>(batch, hq, hkv, sq, skv, cut);
   if (workspace == nullptr || workspace_bytes < sz.total || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
     return fail(TOKMIX_ERR_INVALID_ARGUMENT, "tokmix_fa2_bwd: needs a 16-byte aligned workspace of %lld bytes", sz.total);
   // 4-D tensor maps over (d, seq, head, batch); the layout only changes the strides.
@@ -1003,6 +1181,8 @@ int launch(const void* dout, const void* q, const void* k, const void* v, const 
   p.nq = (sq + C::kBQ - 1) / C::kBQ;
   p.nk = (skv + kBK - 1) / kBK;
   p.causal = causal ? 1 : 0;
+  const long long tiles = static_cast<long long>(batch) * hq * p.nq * C::kSplit;
+  if (tiles > 0xFFFFFFFll) return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_fa2_bwd: too many tiles (%lld)", tiles);
   p.scale = sm_scale;
   p.scale_log2 = sm_scale * kLog2e;
   p.status = status;
@@ -1011,7 +1191,15 @@ int launch(const void* dout, const void* q, const void* k, const void* v, const 
   p.turns = p.ticket + 1;
   p.stats = reinterpret_cast<const float*>(ws + sz.counters);
   p.acc = reinterpret_cast<float*>(ws + sz.counters + sz.stats);
-  const long long units = static_cast<long long>(batch) * hkv * p.nk * C::kSplit;
+  p.per_row = cut.per_row;
+  p.streams = cut.streams;
+  p.part_tiles = cut.part_tiles;
+  p.tiles = tiles;
+  if (cut.part_tiles > 0) {
+    p.partial = reinterpret_cast<float*>(ws + sz.counters + sz.stats + sz.acc);
+    std::copy(cut.first, cut.first + p.nk + 1, p.first);
+  }
+  const long long units = static_cast<long long>(batch) * hkv * C::kSplit * p.per_row;
   const long long steps = static_cast<long long>(p.nq) * p.group;
   if (units > 0x3FFFFFFFll || steps > 0x3FFFFFFFll)
     return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_fa2_bwd: too many tiles (%lld x %lld)", units, steps);
@@ -1021,8 +1209,6 @@ int launch(const void* dout, const void* q, const void* k, const void* v, const 
   const int share = p.group > 1 ? 8 : 4;
   p.wave = (std::max(1, device_sm_count()) + share - 1) / share;
 
-  const long long tiles = static_cast<long long>(batch) * hq * p.nq * C::kSplit;
-  if (tiles > 0x7FFFFFFFll) return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_fa2_bwd: too many tiles (%lld)", tiles);
   const long long rows = static_cast<long long>(batch) * hq * p.nq * C::kBQ;
   const long long blocks = (rows * (D / 8) + 255) / 256;
   if (blocks > 0x7FFFFFFFll) return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_fa2_bwd: too many rows (%lld)", rows);
@@ -1038,8 +1224,11 @@ int launch(const void* dout, const void* q, const void* k, const void* v, const 
     e = launch_overlapped(&fa2_bwd_kernel<D>, dim3(static_cast<unsigned>(grid)), dim3(kThreads),
                           static_cast<size_t>(smem_bytes), stream, mq, mdo, mk, mv, mdk, mdv, p);
   }
-  if (e == cudaSuccess && p.nk > 1)
-    e = launch_overlapped(&fa2_bwd_dq<D>, dim3(static_cast<unsigned>(tiles), C::kDqCols / 32), dim3(128), 0, stream, p);
+  const long long dq_blocks = p.nk > 1 ? tiles * (C::kDqCols / 32) : 0;
+  const long long join_blocks = cut.part_tiles > 0 ? static_cast<long long>(batch) * hkv * C::kSplit * p.nk * 2 * (C::kDH / 32) : 0;
+  if (e == cudaSuccess && dq_blocks + join_blocks > 0)
+    e = launch_overlapped(&fa2_bwd_finish<D>, dim3(static_cast<unsigned>(dq_blocks + join_blocks)), dim3(128), 0, stream, p,
+                          static_cast<int>(dq_blocks));
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(TOKMIX_ERR_LAUNCH, "tokmix_fa2_bwd: %s", cudaGetErrorString(e));
@@ -1056,13 +1245,18 @@ auto by_head_dim(int head_dim, F64 f64, F128 f128, F256 f256, decltype(f64()) ot
 }  // namespace fa2b
 }  // namespace tokmix
 
-extern "C" long long tokmix_fa2_bwd_workspace_bytes(int batch, int heads_q, int seqlen_q, int seqlen_kv, int head_dim) {
+extern "C" long long tokmix_fa2_bwd_workspace_bytes(int batch, int heads_q, int heads_kv, int seqlen_q, int seqlen_kv,
+                                                    int head_dim, int causal) {
   using namespace tokmix::fa2b;
-  if (batch < 0 || heads_q <= 0 || seqlen_q < 0 || seqlen_kv < 0) return -1;
+  if (batch < 0 || heads_q <= 0 || heads_kv <= 0 || heads_q % heads_kv != 0 || seqlen_q < 0 || seqlen_kv < 0) return -1;
+  auto need = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    return sizes<D>(batch, heads_q, heads_kv, seqlen_q, seqlen_kv, plan_of<D>(batch, heads_q, heads_kv, seqlen_q, seqlen_kv, causal))
+        .total;
+  };
   return by_head_dim(
-      head_dim, [&] { return sizes<64>(batch, heads_q, seqlen_q, seqlen_kv).total; },
-      [&] { return sizes<128>(batch, heads_q, seqlen_q, seqlen_kv).total; },
-      [&] { return sizes<256>(batch, heads_q, seqlen_q, seqlen_kv).total; }, -1LL);
+      head_dim, [&] { return need(std::integral_constant<int, 64>()); }, [&] { return need(std::integral_constant<int, 128>()); },
+      [&] { return need(std::integral_constant<int, 256>()); }, -1LL);
 }
 
 extern "C" int tokmix_fa2_bwd(const void* dout, const void* q, const void* k, const void* v, const void* o,

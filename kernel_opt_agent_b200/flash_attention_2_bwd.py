@@ -43,7 +43,7 @@ def kernel_fn(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
     do, q, k, v, o, lse = (_lib.aligned(t) for t in (do, q, k, v, o, lse))
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     lib, dev = _lib.load(), q.device
-    need = lib.tokmix_fa2_bwd_workspace_bytes(batch, heads, sq, skv, d) if q.numel() else 0
+    need = _lib.call_on(dev, lib.tokmix_fa2_bwd_workspace_bytes, batch, heads, heads_kv, sq, skv, d, 1 if causal else 0) if q.numel() else 0
     # from the allocator on every call: calls on several streams and captured graphs do not share it
     workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
     status = _lib.host_status_ptr(dev, "flash_attention_2_bwd")

@@ -34,12 +34,14 @@ def test_attention_gradient_rejects_bad_arguments(changes, code):
 def test_attention_gradient_workspace():
     need = _lib.load().tokmix_fa2_bwd_workspace_bytes
     for d in (64, 128, 256):
-        assert need(2, 4, 1000, 1000, d) >= 2 * 4 * 1000 * d * 4     # a sum in fp32 per element of dq
-        assert need(2, 4, 1000, 128, d) < 2 * 4 * 1000 * d * 4       # one key tile: none
-    assert need(0, 4, 10, 10, 64) >= 0 and need(1, 1, 0, 10, 64) >= 0
-    assert need(-1, 4, 10, 10, 64) == -1 and need(1, 0, 10, 10, 64) == -1 and need(1, 1, 10, 10, 96) == -1
+        assert need(8, 32, 32, 1000, 1000, d, 1) >= 8 * 32 * 1000 * d * 4     # a sum in fp32 per element of dq
+        assert need(8, 32, 32, 1000, 128, d, 1) < 8 * 32 * 1000 * d * 4       # one key tile: none
+        assert need(1, 8, 1, 2048, 2048, d, 1) > 8 * 2048 * d * 4             # few key tiles: parts of dk and dv beside them
+    assert need(0, 4, 2, 10, 10, 64, 1) >= 0 and need(1, 1, 1, 0, 10, 64, 0) >= 0
+    assert need(-1, 4, 2, 10, 10, 64, 1) == -1 and need(1, 0, 1, 10, 10, 64, 1) == -1 and need(1, 1, 1, 10, 10, 96, 1) == -1
+    assert need(1, 3, 2, 10, 10, 64, 1) == -1
     # a long batch: sizes beyond 32 bits
-    assert need(64, 64, 65536, 65536, 256) >= 64 * 64 * 65536 * 256 * 4
+    assert need(64, 64, 64, 65536, 65536, 256, 1) >= 64 * 64 * 65536 * 256 * 4
 
 
 def test_attention_forward_with_lse_rejects_bad_arguments():
