@@ -19,6 +19,7 @@ and this in one differentiable call."""
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -29,27 +30,37 @@ from . import flash_attention_2 as _forward
 KERNEL_TYPE = "flash_attention_2_bwd"
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(batch: int, heads: int, heads_kv: int, sq: int, skv: int, d: int, causal: int, device: torch.device) -> int:
+    need = _lib.call_on(device, _lib.load().tokmix_fa2_bwd_workspace_bytes, batch, heads, heads_kv, sq, skv, d, causal)
+    return max(need, 0)  # bad sizes: the call itself says which
+
+
 def kernel_fn(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
               causal: bool = True, sm_scale: float | None = None, *, layout: str = "bhsd"):
     q, k, v, hd, sd = _forward._validate_inputs(q, k, v, layout)
-    for name, t in (("do", do), ("o", o)):
-        if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:
-            raise ValueError(f"{name} must be a bfloat16 tensor shaped like q on its device")
-    batch, heads, heads_kv, sq, skv, d = q.shape[0], q.shape[hd], k.shape[hd], q.shape[sd], k.shape[sd], q.shape[3]
-    if lse.shape != (batch, heads, sq) or lse.dtype != torch.float32 or lse.device != q.device:
+    shape, dtype, dev = q.shape, q.dtype, q.device
+    if do.shape != shape or do.dtype != dtype or do.device != dev:
+        raise ValueError("do must be a bfloat16 tensor shaped like q on its device")
+    if o.shape != shape or o.dtype != dtype or o.device != dev:
+        raise ValueError("o must be a bfloat16 tensor shaped like q on its device")
+    batch, heads, sq, d = shape[0], shape[hd], shape[sd], shape[3]
+    heads_kv, skv = k.shape[hd], k.shape[sd]
+    if lse.shape != (batch, heads, sq) or lse.dtype != torch.float32 or lse.device != dev:
         raise ValueError("lse must be float32 [batch, heads, seq_len] on the device of q")
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(d)
-    do, q, k, v, o, lse = (_lib.aligned(t) for t in (do, q, k, v, o, lse))
+    do, q, k, v, o, lse = (_lib.aligned(do), _lib.aligned(q), _lib.aligned(k), _lib.aligned(v), _lib.aligned(o),
+                           _lib.aligned(lse))
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-    lib, dev = _lib.load(), q.device
-    need = _lib.call_on(dev, lib.tokmix_fa2_bwd_workspace_bytes, batch, heads, heads_kv, sq, skv, d, 1 if causal else 0) if q.numel() else 0
+    causal = 1 if causal else 0
+    need = _workspace_bytes(batch, heads, heads_kv, sq, skv, d, causal, dev) if batch and sq else 0
     # from the allocator on every call: calls on several streams and captured graphs do not share it
-    workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    workspace = _lib.empty((need or 1,), torch.uint8, dev)
     status = _lib.host_status_ptr(dev, "flash_attention_2_bwd")
-    rc = _lib.call_on(dev, lib.tokmix_fa2_bwd, do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+    rc = _lib.call_on(dev, _lib.load().tokmix_fa2_bwd, do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
                       lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), batch, heads, heads_kv, sq, skv, d,
-                      _lib.LAYOUT_BHSD if layout == "bhsd" else _lib.LAYOUT_BSHD, 1 if causal else 0, float(sm_scale),
+                      _lib.LAYOUT_BHSD if layout == "bhsd" else _lib.LAYOUT_BSHD, causal, float(sm_scale),
                       workspace.data_ptr(), need, status, _lib.stream_ptr(dev))
     if rc:
         _lib.check(rc, "flash_attention_2_bwd")

@@ -57,21 +57,24 @@ def _pair_axis(half: int, sections: tuple, interleaved: bool):
 
 def describe(q, k, q_weight, k_weight, cos, sin, positions, eps, nope_dim, sections, interleaved):
     """Checks a call; returns its C description (without outputs) and the tensors it points to."""
-    if q.ndim != 4 or k.ndim != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+    qs, ks, dev, dtype = q.shape, k.shape, q.device, q.dtype
+    if len(qs) != 4 or len(ks) != 4 or qs[0] != ks[0] or qs[1] != ks[1] or qs[3] != ks[3]:
         raise ValueError("q and k must be [B, S, heads, D] with equal B, S and D")
-    batch, seq, hq, d = q.shape
-    hk, dev, dtype = k.shape[2], q.device, q.dtype
+    batch, seq, hq, d = qs
+    hk = ks[2]
     if dtype not in _kv8.IO_DTYPES or k.dtype != dtype:
         raise ValueError("q and k must both be bfloat16 or both float16")
     if d not in HEAD_DIMS or hq == 0 or hk == 0:
         raise ValueError(f"head_dim must be one of {HEAD_DIMS}, with at least one head of each kind")
     if batch >= 1 << 31 or seq >= 1 << 31:
         raise ValueError("fewer than 2^31 sequences and tokens per sequence")
-    if not q.is_cuda or any(t.device != dev for t in (k, q_weight, k_weight, cos, sin)):
+    if not q.is_cuda or k.device != dev or q_weight.device != dev or k_weight.device != dev or cos.device != dev or (
+            sin.device != dev):
         raise ValueError("all tensors must be CUDA tensors on one device")
+    wtype = q_weight.dtype
     if q_weight.shape != (d,) or k_weight.shape != (d,):
         raise ValueError(f"q_weight and k_weight must be [{d}]")
-    if q_weight.dtype != k_weight.dtype or q_weight.dtype not in (dtype, torch.float32):
+    if k_weight.dtype != wtype or wtype not in (dtype, torch.float32):
         raise ValueError("q_weight and k_weight must have the type of q or be float32")
     if cos.ndim != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
         raise ValueError("cos and sin must be float32 [rows, pairs]")
@@ -86,8 +89,7 @@ def describe(q, k, q_weight, k_weight, cos, sin, positions, eps, nope_dim, secti
         raise ValueError("cos and sin need between 1 and 2^31 - 1 rows")
     axes, pair_axis = 1, None
     if sections is not None:
-        sections = tuple(int(n) for n in sections)
-        pair_axis, axes = _pair_axis(half, sections, bool(interleaved)), len(sections)
+        pair_axis, axes = _pair_axis(half, tuple(sections), bool(interleaved)), len(sections)
     elif interleaved:
         raise ValueError("interleaved needs sections")
     if positions is None:
@@ -107,7 +109,7 @@ def describe(q, k, q_weight, k_weight, cos, sin, positions, eps, nope_dim, secti
                            sin.data_ptr(), positions.data_ptr() if positions is not None else None,
                            ctypes.addressof(pair_axis) if axes > 1 else None, None, None, None, None, *qs, *ks,
                            0, 0, 0, 0, 0, 0, batch, seq, hq, hk, d, half, nope_dim, axes, rows, _kv8.IO_DTYPES[dtype],
-                           _lib.DTYPE_FP32 if q_weight.dtype == torch.float32 else _kv8.IO_DTYPES[dtype], eps)
+                           _lib.DTYPE_FP32 if wtype == torch.float32 else _kv8.IO_DTYPES[dtype], eps)
     return args, (q, k, q_weight, k_weight, cos, sin, positions, pair_axis)
 
 
@@ -116,8 +118,8 @@ def kernel_fn(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight
               nope_dim: int | None = None, sections: tuple | None = None, interleaved: bool = False):
     args, keep = describe(q, k, q_weight, k_weight, cos, sin, positions, eps, nope_dim, sections, interleaved)
     dev = q.device
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    k_out = torch.empty(k.shape, dtype=q.dtype, device=dev)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     args.q_out, args.k_out = q_out.data_ptr(), k_out.data_ptr()
     status = _lib.host_status_ptr(dev, "qk_norm_rope")
     rc = _lib.call_on(dev, _lib.load().tokmix_qk_norm_rope_fwd, ctypes.byref(args), status, _lib.stream_ptr(dev))

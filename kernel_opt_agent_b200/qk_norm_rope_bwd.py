@@ -18,6 +18,7 @@ an order that sizes alone decide (the same bits every time) and rounded to the w
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -28,27 +29,31 @@ from .qk_norm_rope import check_device_status  # noqa: F401
 KERNEL_TYPE = "qk_norm_rope_bwd"
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(tokens: int, heads_q: int, heads_k: int, head_dim: int, device: torch.device) -> int:
+    return _lib.call_on(device, _lib.load().tokmix_qk_norm_rope_bwd_workspace_bytes, tokens, heads_q, heads_k, head_dim)
+
+
 def kernel_fn(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
               k_weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None = None, *,
               eps: float = 1e-6, nope_dim: int | None = None, sections: tuple | None = None, interleaved: bool = False):
     args, keep = _forward.describe(q, k, q_weight, k_weight, cos, sin, positions, eps, nope_dim, sections, interleaved)
-    for name, t, x in (("dq_out", dq_out, q), ("dk_out", dk_out, k)):
-        if t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
-            raise ValueError(f"{name} must have the shape, type and device of {name[1]}")
-    dev = q.device
+    dev, dtype = q.device, q.dtype
+    if dq_out.shape != q.shape or dq_out.dtype != dtype or dq_out.device != dev:
+        raise ValueError("dq_out must have the shape, type and device of q")
+    if dk_out.shape != k.shape or dk_out.dtype != dtype or dk_out.device != dev:
+        raise ValueError("dk_out must have the shape, type and device of k")
     dq_out, (args.dq_batch_stride, args.dq_token_stride, args.dq_head_stride) = _kv8.token_strides(dq_out)
     dk_out, (args.dk_batch_stride, args.dk_token_stride, args.dk_head_stride) = _kv8.token_strides(dk_out)
     args.dq, args.dk = dq_out.data_ptr(), dk_out.data_ptr()
-    dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    dk = torch.empty(k.shape, dtype=q.dtype, device=dev)
+    dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    dk = torch.empty_like(k, memory_format=torch.contiguous_format)
     args.q_out, args.k_out = dq.data_ptr(), dk.data_ptr()
     dqw, dkw = torch.empty_like(keep[2]), torch.empty_like(keep[3])
-    lib = _lib.load()
-    need = _lib.call_on(dev, lib.tokmix_qk_norm_rope_bwd_workspace_bytes, q.shape[0] * q.shape[1], q.shape[2], k.shape[2],
-                        q.shape[3])
-    ws = _lib.empty((max(need, 1),), torch.uint8, dev)  # per call: calls may overlap on other streams
+    need = _workspace_bytes(args.batch * args.seqlen, args.heads_q, args.heads_k, args.head_dim, dev)
+    ws = _lib.empty((need or 1,), torch.uint8, dev)  # per call: calls may overlap on other streams
     status = _lib.host_status_ptr(dev, "qk_norm_rope")
-    rc = _lib.call_on(dev, lib.tokmix_qk_norm_rope_bwd, ctypes.byref(args), dqw.data_ptr(), dkw.data_ptr(), ws.data_ptr(),
+    rc = _lib.call_on(dev, _lib.load().tokmix_qk_norm_rope_bwd, ctypes.byref(args), dqw.data_ptr(), dkw.data_ptr(), ws.data_ptr(),
                       need, status, _lib.stream_ptr(dev))
     del keep
     if rc:
