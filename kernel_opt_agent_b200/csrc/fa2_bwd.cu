@@ -7,7 +7,7 @@
 // q, k and lse, so the forward keeps one number per row instead of the S x S matrix.
 //
 // Three launches:
-//   fa2_bwd_prep    delta and lse * log2(e) in rows padded to whole query tiles (padding: +inf, 0,
+//   fa2_bwd_prep    -delta and -lse * log2(e) in rows padded to whole query tiles (padding: 0, -inf,
 //                   so that a padded row's P is 0), the counters below set to 0.
 //   fa2_bwd_kernel  persistent, one CTA per SM.  A unit is a tile of 128 keys of one key/value head: K and V stay in
 //                   shared memory, the tiles of BQ queries of every query head of the group pass by
@@ -239,6 +239,34 @@ __device__ __forceinline__ bool wait_turn(const uint32_t* turn, uint32_t want, u
     }
     __nanosleep(20);
   }
+}
+
+// Two fp32 values in a register pair, and Blackwell's arithmetic on them
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pair2(uint32_t a, uint32_t b) {
+  F2 v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b));
+  return v;
+}
+__device__ __forceinline__ float2 split2(F2 v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
 // 16 lanes x 8 N columns of TMEM, dealt out like an mma accumulator: thread l gets, of every 8 columns i,
@@ -704,7 +732,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t ds_base = smem_u32(smem + C::kDs + (C::kHalfQ == 64 ? wg * C::kKBox : 0));
     const int st_row = (warp & 3) * 32 + ((lane >> 3) & 1) * 8 + (lane & 7);
     const int st_piece = (lane >> 4) + (C::kHalfQ == 64 ? 0 : wg * 4);
-    const float c = p.scale_log2;
+    const F2 c2 = pair2(__float_as_uint(p.scale_log2), __float_as_uint(p.scale_log2));
     constexpr bool kOwnBox = C::kBQ == 128;  // a box of dS per warpgroup
     constexpr int kEpiThreads = kOwnBox ? 128 : 256, kEpiRounds = kOwnBox ? C::kBoxes : 2 * C::kBoxes;
     const int kEpiBarrier = kOwnBox ? 1 + wg : 1;
@@ -753,9 +781,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           tc_fence_after();
           // this lane's two query columns of every group of 8
-          const float2* lse2 = reinterpret_cast<const float2*>(smem + C::kStat + qs * C::kStatBytes) + wg * (C::kHalfQ / 2) +
-                               (lane & 3);
-          const float2* delta = lse2 + C::kBQ / 2;
+          const F2* lse2 = reinterpret_cast<const F2*>(smem + C::kStat + qs * C::kStatBytes) + wg * (C::kHalfQ / 2) + (lane & 3);
+          const F2* delta = lse2 + C::kBQ / 2;
           const int q0 = i * C::kBQ + wg * C::kHalfQ;
           const bool masked = ragged || (p.causal && q0 < x.j * kBK + kBK - 1);
           // fragment (h16, rg): key (warp & 3) * 32 + h16 * 16 + rg * 8 + lane / 4
@@ -764,7 +791,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld_frag<kGroups>(col_s, raw[0]);
           tmem_ld_frag<kGroups>(col_s + (16u << 16), raw[1]);
           float pr[2][4 * kGroups];
-          float2 st[kGroups];
+          F2 st[kGroups];
 #pragma unroll
           for (int n = 0; n < kGroups; ++n) st[n] = lse2[4 * n];
           tmem_wait_ld();
@@ -775,8 +802,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int rg = 0; rg < 2; ++rg) {
                 const int e = 4 * n + 2 * rg;
-                pr[h16][e] = ex2_approx(fmaf(__uint_as_float(raw[h16][e]), c, -st[n].x));
-                pr[h16][e + 1] = ex2_approx(fmaf(__uint_as_float(raw[h16][e + 1]), c, -st[n].y));
+                const float2 x = split2(fma2(pair2(raw[h16][e], raw[h16][e + 1]), c2, st[n]));
+                pr[h16][e] = ex2_approx(x.x);
+                pr[h16][e + 1] = ex2_approx(x.y);
               }
             }
             if (masked) {
@@ -819,8 +847,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int rg = 0; rg < 2; ++rg) {
                 const int e = 4 * n + 2 * rg;
-                ds[e] = pr[h16][e] * (__uint_as_float(raw[h16][e]) - st[n].x);
-                ds[e + 1] = pr[h16][e + 1] * (__uint_as_float(raw[h16][e + 1]) - st[n].y);
+                const float2 x = split2(mul2(pair2(__float_as_uint(pr[h16][e]), __float_as_uint(pr[h16][e + 1])),
+                                             add2(pair2(raw[h16][e], raw[h16][e + 1]), st[n])));
+                ds[e] = x.x;
+                ds[e + 1] = x.y;
               }
             }
             if (masked) {  // dP may be infinite or NaN there
@@ -929,7 +959,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// delta = sum do * o and lse * log2(e) of every row, in rows padded to whole query tiles; D / 8
+// delta = sum do * o and lse * log2(e) of every row, both negated, in rows padded to whole query tiles; D / 8
 // lanes a row, 16 bytes a lane.  Also sets the unit counter and the turn counters to 0.
 template <int D>
 __global__ void __launch_bounds__(256) fa2_bwd_prep(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ dout,
@@ -963,8 +993,8 @@ __global__ void __launch_bounds__(256) fa2_bwd_prep(const __nv_bfloat16* __restr
   if (in && part == 0) {
     const int tile = i / C::kBQ, in_tile = i - tile * C::kBQ;
     float* s = stats + (bh * (sq_pad / C::kBQ) + tile) * (2 * C::kBQ) + in_tile;
-    s[0] = i < sq ? lse[bh * sq + i] * kLog2e : INFINITY;
-    s[C::kBQ] = sum;
+    s[0] = i < sq ? -lse[bh * sq + i] * kLog2e : -INFINITY;
+    s[C::kBQ] = -sum;
   }
 }
 
