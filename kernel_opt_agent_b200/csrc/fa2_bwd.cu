@@ -74,9 +74,9 @@ struct Cfg {
   static constexpr int kDqCols = kTransDq ? kBQ : kDH; // TMEM columns of dQ
   static constexpr int kHalfQ = kBQ / 2;               // query columns of a softmax warpgroup
   // Cycles between 8 KB of reductions: an SM sends about 25 bytes a cycle, and reductions that wait for that keep the
-  // tensor core from shared memory and TMA requests in the queue (D 128, 64 KB a step: B4 Hq32 Hkv8 S8192 took 6809 us
-  // without, 6325 with 320 cycles, 6623 with 440).  Half as much a step (D 64, 256) needs none.
-  static constexpr int kPace = D == 128 ? 320 : 0;
+  // tensor core from shared memory and TMA requests in the queue (B4 Hq32 Hkv8 S8192: D 128 6809 us without, 6158 with
+  // 288, 6623 with 440; D 64 4199 without, 4025 with 320, 4200 with 800; D 256 gains nothing).
+  static constexpr int kPace = D == 128 ? 288 : D == 64 ? 320 : 0;
   static constexpr uint32_t kColS = 0;
   static constexpr uint32_t kColDp = kBQ;
   static constexpr uint32_t kColDq = kAlias ? kColDp : 2 * kBQ;
@@ -968,6 +968,7 @@ __global__ void __launch_bounds__(256) fa2_bwd_prep(const __nv_bfloat16* __restr
                                                     int sq, int sq_pad, int hq, long long sb, long long sh, long long ss) {
   using C = Cfg<D>;
   constexpr int kLanes = D / 8;
+  allow_next_kernel();
   wait_previous_kernels();
   const long long t = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
   for (long long i = t; i < n_counters; i += static_cast<long long>(gridDim.x) * 256) counters[i] = 0u;
@@ -1091,9 +1092,11 @@ struct Plan {
 };
 
 // Parts cost their fp32 way through memory and pay where key tiles are few: the time of a cut, in steps, is the
-// longest unit or the mean load of an SM with what a unit costs beside its steps (2) and what the ends of the SMs' queues differ by
-// (a sixth of the longest unit, causal units being sorted by length; half of it otherwise), and the joining of the parts.
-// (D 128: B1 Hq32 Hkv8 S2048, 128 key tiles of up to 64 steps: 211 us whole, 103 in parts.)
+// longest unit, the turns of a query tile's dQ, or the mean load of an SM with what a unit costs beside its steps (2) and what
+// the ends of the SMs' queues differ by (a sixth of the longest unit, causal units being sorted by length; half of it
+// otherwise), and the joining of the parts.  Whole and cut, us: B1 Hq32 Hkv8 S2048 D128 213, 136 (2 parts); B1 Hq32 Hkv4
+// S1024 D128 195, 63 (8); B1 Hq16 Hkv2 S4096 D256 1290, 699 (2); where a cut does not pay, B2 Hq16 Hkv2 S4096 D256
+// 1404, 1483 (2).
 template <int D>
 Plan plan(int batch, int hkv, int group, int nq, int nk, int causal) {
   using C = Cfg<D>;
@@ -1123,8 +1126,9 @@ Plan plan(int batch, int hkv, int group, int nq, int nk, int causal) {
     const double longest = static_cast<double>(part_tiles) * group;
     const double joined = static_cast<double>(parts) * rows * (2.0 * C::kDH * 128 * 4) * 2.0;  // bytes written and read
     const double mean = (total + 2.0 * static_cast<double>(units) * rows) / sms;
-    const double time = std::max(longest + 2.0, mean + longest / (causal ? 6 : 2)) +
-                        (parts > 0 ? 1.0 + joined / 8e6 : 0.0);  // a step is about 2 us, in which 8 MB pass
+    const double turns = 1.5 * nk / best.streams;
+    const double time = std::max({longest + 2.0, turns, mean + longest / (causal ? 6 : 2)}) +
+                        (parts > 0 ? (nk > 1 ? 0.5 : 1.0) + joined / 8e6 : 0.0);  // a step is about 2 us, in which 8 MB pass
     if (cut == 1 || time < 0.85 * best_time) {
       best_time = time;
       best.part_tiles = parts > 0 ? part_tiles : 0;

@@ -63,6 +63,9 @@ cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_
 #ifdef __CUDACC__
 // Everything earlier in the stream has completed and its writes are visible.
 __device__ __forceinline__ void wait_previous_kernels() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// The next kernel of the stream, if launched by launch_overlapped, may start its set-up once every block of this one has
+// come here (otherwise: once they end).
+__device__ __forceinline__ void allow_next_kernel() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 #endif
 
 // The GDN stage-1 options (tokmix_gdn_stage1): whether gates / q-k normalisation are requested,
