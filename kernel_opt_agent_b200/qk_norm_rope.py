@@ -38,6 +38,7 @@ from . import _kv8, _lib
 KERNEL_TYPE = "qk_norm_rope"
 HEAD_DIMS = (64, 128, 256)
 MAX_AXES = 4
+_NO_STRIDES = (0,) * 6
 
 
 @functools.lru_cache(maxsize=64)
@@ -55,8 +56,9 @@ def _pair_axis(half: int, sections: tuple, interleaved: bool):
     return (ctypes.c_uint8 * half)(*axis)
 
 
-def describe(q, k, q_weight, k_weight, cos, sin, positions, eps, nope_dim, sections, interleaved):
-    """Checks a call; returns its C description (without outputs) and the tensors it points to."""
+def describe(q, k, q_weight, k_weight, cos, sin, positions, eps, nope_dim, sections, interleaved, grads=None):
+    """Checks a call (of the gradient, with grads = (dq_out, dk_out)) and allocates its outputs; returns its C
+    description, the outputs and the tensors it points to."""
     qs, ks, dev, dtype = q.shape, k.shape, q.device, q.dtype
     if len(qs) != 4 or len(ks) != 4 or qs[0] != ks[0] or qs[1] != ks[1] or qs[3] != ks[3]:
         raise ValueError("q and k must be [B, S, heads, D] with equal B, S and D")
@@ -102,25 +104,36 @@ def describe(q, k, q_weight, k_weight, cos, sin, positions, eps, nope_dim, secti
         if positions.dtype != torch.int32 or positions.shape != shape or positions.device != dev:
             raise ValueError(f"positions must be int32 {list(shape)} on the device of q")
         positions = positions.contiguous()
-    q, qs = _kv8.token_strides(q)
-    k, ks = _kv8.token_strides(k)
-    cos, sin, q_weight, k_weight = (_lib.aligned(t) for t in (cos, sin, q_weight, k_weight))
+    dq = dk = None
+    gs = _NO_STRIDES
+    if grads is not None:
+        dq, dk = grads
+        if dq.shape != qs or dq.dtype != dtype or dq.device != dev:
+            raise ValueError("dq_out must have the shape, type and device of q")
+        if dk.shape != ks or dk.dtype != dtype or dk.device != dev:
+            raise ValueError("dk_out must have the shape, type and device of k")
+        dq, gq = _kv8.token_strides(dq)
+        dk, gk = _kv8.token_strides(dk)
+        gs = gq + gk
+    q, sq = _kv8.token_strides(q)
+    k, sk = _kv8.token_strides(k)
+    cos, sin, q_weight, k_weight = _lib.aligned(cos), _lib.aligned(sin), _lib.aligned(q_weight), _lib.aligned(k_weight)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     args = _lib.QkNormRope(q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(),
-                           sin.data_ptr(), positions.data_ptr() if positions is not None else None,
-                           ctypes.addressof(pair_axis) if axes > 1 else None, None, None, None, None, *qs, *ks,
-                           0, 0, 0, 0, 0, 0, batch, seq, hq, hk, d, half, nope_dim, axes, rows, _kv8.IO_DTYPES[dtype],
+                           sin.data_ptr(), None if positions is None else positions.data_ptr(),
+                           ctypes.addressof(pair_axis) if axes > 1 else None, None if dq is None else dq.data_ptr(),
+                           None if dk is None else dk.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), *sq, *sk, *gs,
+                           batch, seq, hq, hk, d, half, nope_dim, axes, rows, _kv8.IO_DTYPES[dtype],
                            _lib.DTYPE_FP32 if wtype == torch.float32 else _kv8.IO_DTYPES[dtype], eps)
-    return args, (q, k, q_weight, k_weight, cos, sin, positions, pair_axis)
+    return args, q_out, k_out, (q, k, q_weight, k_weight, cos, sin, positions, pair_axis, dq, dk)
 
 
 def kernel_fn(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor,
               sin: torch.Tensor, positions: torch.Tensor | None = None, *, eps: float = 1e-6,
               nope_dim: int | None = None, sections: tuple | None = None, interleaved: bool = False):
-    args, keep = describe(q, k, q_weight, k_weight, cos, sin, positions, eps, nope_dim, sections, interleaved)
+    args, q_out, k_out, keep = describe(q, k, q_weight, k_weight, cos, sin, positions, eps, nope_dim, sections, interleaved)
     dev = q.device
-    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
-    args.q_out, args.k_out = q_out.data_ptr(), k_out.data_ptr()
     status = _lib.host_status_ptr(dev, "qk_norm_rope")
     rc = _lib.call_on(dev, _lib.load().tokmix_qk_norm_rope_fwd, ctypes.byref(args), status, _lib.stream_ptr(dev))
     del keep

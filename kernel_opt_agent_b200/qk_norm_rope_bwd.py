@@ -22,7 +22,7 @@ import functools
 
 import torch
 
-from . import _kv8, _lib
+from . import _lib
 from . import qk_norm_rope as _forward
 from .qk_norm_rope import check_device_status  # noqa: F401
 
@@ -37,18 +37,9 @@ def _workspace_bytes(tokens: int, heads_q: int, heads_k: int, head_dim: int, dev
 def kernel_fn(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
               k_weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None = None, *,
               eps: float = 1e-6, nope_dim: int | None = None, sections: tuple | None = None, interleaved: bool = False):
-    args, keep = _forward.describe(q, k, q_weight, k_weight, cos, sin, positions, eps, nope_dim, sections, interleaved)
-    dev, dtype = q.device, q.dtype
-    if dq_out.shape != q.shape or dq_out.dtype != dtype or dq_out.device != dev:
-        raise ValueError("dq_out must have the shape, type and device of q")
-    if dk_out.shape != k.shape or dk_out.dtype != dtype or dk_out.device != dev:
-        raise ValueError("dk_out must have the shape, type and device of k")
-    dq_out, (args.dq_batch_stride, args.dq_token_stride, args.dq_head_stride) = _kv8.token_strides(dq_out)
-    dk_out, (args.dk_batch_stride, args.dk_token_stride, args.dk_head_stride) = _kv8.token_strides(dk_out)
-    args.dq, args.dk = dq_out.data_ptr(), dk_out.data_ptr()
-    dq = torch.empty_like(q, memory_format=torch.contiguous_format)
-    dk = torch.empty_like(k, memory_format=torch.contiguous_format)
-    args.q_out, args.k_out = dq.data_ptr(), dk.data_ptr()
+    args, dq, dk, keep = _forward.describe(q, k, q_weight, k_weight, cos, sin, positions, eps, nope_dim, sections, interleaved,
+                                           (dq_out, dk_out))
+    dev = q.device
     dqw, dkw = torch.empty_like(keep[2]), torch.empty_like(keep[3])
     need = _workspace_bytes(args.batch * args.seqlen, args.heads_q, args.heads_k, args.head_dim, dev)
     ws = _lib.empty((need or 1,), torch.uint8, dev)  # per call: calls may overlap on other streams
