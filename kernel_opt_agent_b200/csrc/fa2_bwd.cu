@@ -9,30 +9,36 @@
 // Three launches:
 //   fa2_bwd_prep    -delta and -lse * log2(e) in rows padded to whole query tiles (padding: 0, -inf,
 //                   so that a padded row's P is 0), the counters below set to 0.
-//   fa2_bwd_kernel  persistent, one CTA per SM.  A unit is a tile of 128 keys of one key/value head: K and V stay in
-//                   shared memory, the tiles of BQ queries of every query head of the group pass by
-//                   (last tile first), and dK and dV grow in TMEM.  Scores are held transposed, keys
-//                   along the 128 TMEM lanes:
+//   fa2_bwd_kernel  persistent, one CTA per SM.  A unit is a tile of 128 keys of one key/value head: K and V
+//                   stay in shared memory, the tiles of kBQ queries of every query head of the group
+//                   pass by (last tile first), and dK and dV grow in TMEM.  Scores are held
+//                   transposed, keys along the 128 TMEM lanes:
 //     S^T  = K Q^T     (SS)            P^T = 2^(c log2e S^T - lse2), bf16, over S^T's own columns
 //     dV  += P^T dO    (A from TMEM)
 //     dP^T = V dO^T    (SS)            dS^T = P^T * (dP^T - delta), bf16, into shared memory
 //     dK  += dS^T Q    (SS)
 //     dQ   = dS K      (SS; A is the same dS^T tile read MN-major)
 //   A query tile's dQ is the sum over key tiles, that is, over CTAs.  It grows in fp32 in global
-//   memory by vector reductions, in the order of the key tiles: the CTA of key tile j waits for the
-//   query tile's turn counter to read j, adds, and sets it to j + 1.  So the bits are the
-//   same every time; the first tile stores instead of adding (no clearing pass).
-//   Units are taken from a counter in order of (batch, key/value head, key tile): a CTA waits only
-//   for units that were taken earlier, by CTAs that are running, so the waits end with any number
-//   of resident CTAs.  Under the causal mask this order is longest first.
-//   fa2_bwd_finish  dq = c times those sums, rounded, in dq's layout, and dV and dK of key tiles that came in parts (with
-//                   a single key tile, whose dQ is written at once, and no parts, no such launch).  The last key tile's CTA could do it in passing, but reading the sums back held its pipeline
-//                   up for 10 000 to 20 000 cycles a tile.
-// Roles (512 threads): warps 0-7 softmax (two warpgroups, each half of a tile's query columns; thread =
-// key row), warps 8-11 dQ (TMEM to global), warp 12 TMA and unit counter, warp 13 TMEM owner and MMA
-// issuer, warps 14 and 15 pass on and wait for the turns of the dQ sums.
+//   memory by vector reductions, in the order of the key tiles: a CTA waits until the query tile's
+//   turn counter names its key tile, adds, and passes the turn on.  So the bits are the same every
+//   time; the first tile stores instead of adding (no clearing pass).
+//   Units are taken from a counter in an order in which a unit waits only for units taken earlier, by
+//   CTAs that are running, so the waits end with any number of resident CTAs.
+//   fa2_bwd_finish  dq = c times those sums, rounded, in dq's layout, and dV and dK of key tiles that came
+//                   in parts.  (The last key tile's CTA could finish dq in passing, but reading the sums back held its pipeline
+//                   up for 10 000 to 20 000 cycles a tile.  With a single key tile dQ is written at once.)
+// Roles (512 threads): warps 0-7 softmax (two warpgroups, each half of a tile's query columns; TMEM is read in
+// the layout of mma accumulators, in which a lane has two of every 8 columns: a lane that owned a row read every row
+// statistic as a broadcast, 1400 of a step's cycles of shared memory), warps 8-11 dQ (TMEM to global), warp 12 TMA
+// and unit counter, warp 13 TMEM owner and MMA issuer, warps 14 and 15 pass on and wait for the turns of the dQ
+// sums.
 // Order of the MMAs:  dP(t) dV(t) S(t+1) dQ(t) dK(t) | dP(t+1) ...: while the softmax warps form P
 // the tensor core has dQ and dK to do, and while they form dS it has dV and the next S.
+//
+// What bounds it (D 128, a step of 128 queries x 128 keys, cycles): the tensor core 2560, shared memory about 3200, sending
+// 64 KB of dQ 2600 at the 25 bytes a cycle that an SM sends; measured 4300 to 4600, and under sustained load the
+// clock, which falls at 1000 W.  B4 Hq32 Hkv8 S8192 causal 6.2 to 6.3 ms, 870 to 890 TFLOP/s of 1384 sustained; without dQ's way to
+// memory it took 5.0 ms.
 //
 // head_dim 256: dV and dK of 128 keys alone would fill TMEM (2 x 256 columns), so a unit takes half
 // of their columns (and of dQ's) and forms S and dP whole; queries come in tiles of 64.  V stays in
