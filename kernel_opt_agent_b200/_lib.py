@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes
 import os
 import pathlib
+import struct
 import threading
 
 import torch
@@ -109,6 +110,10 @@ class QkNormRope(ctypes.Structure):
     _fields_ += [(n, _I) for n in ("batch", "seqlen", "heads_q", "heads_k", "head_dim", "half", "nope", "axes", "table_rows",
                                    "dtype", "weight_dtype")]
     _fields_ += [("eps", _F)]
+
+
+# the same as bytes: packing them takes 0.7 us, filling in the ctypes structure 2.3
+QK_NORM_ROPE = struct.Struct("@" + "".join({_VP: "P", _LL: "q", _I: "i", _F: "f"}[t] for _, t in QkNormRope._fields_))
 
 
 _lib = None

@@ -58,7 +58,7 @@ def _pair_axis(half: int, sections: tuple, interleaved: bool):
 
 def describe(q, k, q_weight, k_weight, cos, sin, positions, eps, nope_dim, sections, interleaved, grads=None):
     """Checks a call (of the gradient, with grads = (dq_out, dk_out)) and allocates its outputs; returns its C
-    description, the outputs and the tensors it points to."""
+    description as bytes, the outputs and the tensors it points to."""
     qs, ks, dev, dtype = q.shape, k.shape, q.device, q.dtype
     if len(qs) != 4 or len(ks) != 4 or qs[0] != ks[0] or qs[1] != ks[1] or qs[3] != ks[3]:
         raise ValueError("q and k must be [B, S, heads, D] with equal B, S and D")
@@ -120,12 +120,12 @@ def describe(q, k, q_weight, k_weight, cos, sin, positions, eps, nope_dim, secti
     cos, sin, q_weight, k_weight = _lib.aligned(cos), _lib.aligned(sin), _lib.aligned(q_weight), _lib.aligned(k_weight)
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
-    args = _lib.QkNormRope(q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(),
-                           sin.data_ptr(), None if positions is None else positions.data_ptr(),
-                           ctypes.addressof(pair_axis) if axes > 1 else None, None if dq is None else dq.data_ptr(),
-                           None if dk is None else dk.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), *sq, *sk, *gs,
-                           batch, seq, hq, hk, d, half, nope_dim, axes, rows, _kv8.IO_DTYPES[dtype],
-                           _lib.DTYPE_FP32 if wtype == torch.float32 else _kv8.IO_DTYPES[dtype], eps)
+    args = _lib.QK_NORM_ROPE.pack(
+        q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+        0 if positions is None else positions.data_ptr(), ctypes.addressof(pair_axis) if axes > 1 else 0,
+        0 if dq is None else dq.data_ptr(), 0 if dk is None else dk.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), *sq, *sk, *gs,
+        batch, seq, hq, hk, d, half, nope_dim, axes, rows, _kv8.IO_DTYPES[dtype],
+        _lib.DTYPE_FP32 if wtype == torch.float32 else _kv8.IO_DTYPES[dtype], eps)
     return args, q_out, k_out, (q, k, q_weight, k_weight, cos, sin, positions, pair_axis, dq, dk)
 
 
@@ -135,7 +135,7 @@ def kernel_fn(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight
     args, q_out, k_out, keep = describe(q, k, q_weight, k_weight, cos, sin, positions, eps, nope_dim, sections, interleaved)
     dev = q.device
     status = _lib.host_status_ptr(dev, "qk_norm_rope")
-    rc = _lib.call_on(dev, _lib.load().tokmix_qk_norm_rope_fwd, ctypes.byref(args), status, _lib.stream_ptr(dev))
+    rc = _lib.call_on(dev, _lib.load().tokmix_qk_norm_rope_fwd, args, status, _lib.stream_ptr(dev))
     del keep
     if rc:
         _lib.check(rc, "qk_norm_rope")

@@ -17,7 +17,6 @@ an order that sizes alone decide (the same bits every time) and rounded to the w
 
 from __future__ import annotations
 
-import ctypes
 import functools
 
 import torch
@@ -41,10 +40,11 @@ def kernel_fn(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor, k: to
                                            (dq_out, dk_out))
     dev = q.device
     dqw, dkw = torch.empty_like(keep[2]), torch.empty_like(keep[3])
-    need = _workspace_bytes(args.batch * args.seqlen, args.heads_q, args.heads_k, args.head_dim, dev)
+    batch, seq, hq, d = q.shape
+    need = _workspace_bytes(batch * seq, hq, k.shape[2], d, dev)
     ws = _lib.empty((need or 1,), torch.uint8, dev)  # per call: calls may overlap on other streams
     status = _lib.host_status_ptr(dev, "qk_norm_rope")
-    rc = _lib.call_on(dev, _lib.load().tokmix_qk_norm_rope_bwd, ctypes.byref(args), dqw.data_ptr(), dkw.data_ptr(), ws.data_ptr(),
+    rc = _lib.call_on(dev, _lib.load().tokmix_qk_norm_rope_bwd, args, dqw.data_ptr(), dkw.data_ptr(), ws.data_ptr(),
                       need, status, _lib.stream_ptr(dev))
     del keep
     if rc:

@@ -152,3 +152,9 @@ def test_rope_modules_raise_on_cpu(changes):
         qk_norm_rope.kernel_fn(**args)
     with pytest.raises(ValueError):
         qk_norm_rope_bwd.kernel_fn(args["q"], args["k"], **args)
+
+
+def test_rope_description_as_bytes():
+    """The module packs the C description's fields; the structure of the same fields has the same bytes."""
+    values = list(range(1, len(_lib.QkNormRope._fields_))) + [0.5]
+    assert bytes(_lib.QkNormRope(*values)) == _lib.QK_NORM_ROPE.pack(*values)
