@@ -62,7 +62,7 @@ namespace fa2b {
 constexpr int kBK = 128;             // keys per unit
 constexpr int kThreads = 512;
 constexpr int kSoftmaxWarps = 8, kDqWarps = 4;
-constexpr int kWarpTma = 12, kWarpMma = 13, kWarpPass = 14, kWarpTurn = 15;
+constexpr int kWarpTma = 12, kWarpMma = 13, kWarpPass = 14;  // and 15
 constexpr int kUnitReaders = 3 + kSoftmaxWarps + kDqWarps;
 constexpr int kMaxParted = 256;      // key tiles of a row that may come in parts
 constexpr float kLog2e = 1.4426950408889634f;
@@ -72,17 +72,22 @@ struct Cfg {
   static constexpr int kBQ = D == 256 ? 64 : 128;      // queries per step
   static constexpr int kDH = D < 128 ? D : 128;        // columns of dV, dK and dQ that a unit forms
   static constexpr int kSplit = D / kDH;
-  static constexpr int kNQ = 2;                        // stages of Q, and of the row statistics
-  static constexpr int kNDO = 2;                       // stages of dO
+  // Step g + 2 takes the buffers of step g crosswise.  dO(g) is done with after dV, early in the step, and leaves its buffer to
+  // Q(g + 2), which the next step already wants for its scores; Q(g) is done with at the step's end and leaves its buffer
+  // to dO(g + 2).  So both are asked for a step ahead of their use (a load takes 1500 to 2000 cycles beside the reductions)
+  // instead of half a step and one and a half.  B2 Hq16 Hkv2 S4096 D256 1433 us without, 1215 with; B4 Hq32 Hkv8 S8192 D64
+  // 4117, 4000 to 4066; D 128, whose steps are long enough, 6200 to 6300, 6310 to 6340.
+  static constexpr bool kCross = D != 128;
   static constexpr bool kAlias = D >= 128;             // dQ in dP's columns
   static constexpr bool kVTmem = D == 256;             // V in TMEM, as the A operand of dP
   static constexpr bool kTransDq = D == 256;           // dQ^T: lanes are columns of dq, columns are queries
   static constexpr int kDqCols = kTransDq ? kBQ : kDH; // TMEM columns of dQ
   static constexpr int kHalfQ = kBQ / 2;               // query columns of a softmax warpgroup
   // Cycles between 8 KB of reductions: an SM sends about 25 bytes a cycle, and reductions that wait for that keep the
-  // tensor core from shared memory and TMA requests in the queue (B4 Hq32 Hkv8 S8192: D 128 6809 us without, 6158 with
-  // 288, 6623 with 440; D 64 4199 without, 4025 with 320, 4200 with 800; D 256 gains nothing).
-  static constexpr int kPace = D == 128 ? 288 : D == 64 ? 320 : 0;
+  // tensor core from shared memory and TMA requests in the queue (B4 Hq32 Hkv8 S8192: D 128 6809 us without, 6200
+  // with 288, 6155 with 304, 6300 with 320, 6623 with 440; D 64 4199 without, 4025 with 320, 4200 with 800; B2 Hq16 Hkv2
+  // S4096 D256 1218 without, 1195 with 300, 1215 with 500).  Half as many at half the distance gains nothing.
+  static constexpr int kPace = D == 128 ? 304 : D == 64 ? 320 : 300;
   static constexpr uint32_t kColS = 0;
   static constexpr uint32_t kColDp = kBQ;
   static constexpr uint32_t kColDq = kAlias ? kColDp : 2 * kBQ;
@@ -96,14 +101,14 @@ struct Cfg {
   static constexpr int kKBytes = (D / 64) * kKBox;
   static constexpr int kQBytes = (D / 64) * kQBox;
   static constexpr int kDsBytes = kBK * kBQ * 2;       // boxes of 128 keys x 64 queries
-  static constexpr int kStatBytes = 2 * kBQ * 4;       // lse2 and delta of a query tile
+  static constexpr int kRowBytes = kBQ * 4;            // lse2 or delta of a query tile
   static constexpr int kK = 0;
   static constexpr int kV = kK + kKBytes;
   static constexpr int kQ = kV + (kVTmem ? 0 : kKBytes);
-  static constexpr int kDO = kQ + kNQ * kQBytes;
-  static constexpr int kDs = kDO + kNDO * kQBytes;
-  static constexpr int kStat = kDs + kDsBytes;
-  static constexpr int kBytes = kStat + kNQ * kStatBytes;
+  static constexpr int kDs = kQ + 4 * kQBytes;         // four buffers of Q and dO, see q_buffer
+  static constexpr int kLse = kDs + kDsBytes;          // two stages
+  static constexpr int kDelta = kLse + 2 * kRowBytes;  // two stages
+  static constexpr int kBytes = kDelta + 2 * kRowBytes;
   static_assert(kBytes + 1024 <= 227 * 1024, "shared memory");  // 1024: the barriers, rounded up to the tiles' alignment
 };
 
@@ -188,6 +193,16 @@ __device__ __forceinline__ void next_step(const Params& p, int& i, int& h) {
     h = 0;
     --i;
   }
+}
+
+// Buffers of step g's Q and dO: steps g and g + 2 share a pair.
+template <int D>
+__device__ __forceinline__ int q_buffer(int g) {
+  return (g & 1) * 2 + (Cfg<D>::kCross ? (g >> 1) & 1 : 0);
+}
+template <int D>
+__device__ __forceinline__ int do_buffer(int g) {
+  return q_buffer<D>(g) ^ 1;
 }
 
 // number of key tiles that add to query tile i
@@ -350,7 +365,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   using C = Cfg<D>;
   extern __shared__ __align__(1024) uint8_t smem[];  // no room is left to round its start up
   __shared__ uint64_t bar_unit_full[2], bar_unit_empty[2], bar_kv_full, bar_kv_empty, bar_v, bar_q_full[2], bar_q_empty[2],
-      bar_do_full[2], bar_do_empty[2], bar_s, bar_p, bar_dp, bar_ds, bar_dq, bar_dqfree, bar_turn[2], bar_added[2], bar_passed[2], bar_acc, bar_accfree, bar_drain;
+      bar_do_full[2], bar_do_empty[2], bar_s, bar_p, bar_dp, bar_ds, bar_dq, bar_dqfree, bar_turn[2], bar_added[2], bar_passed[2], bar_acc, bar_accfree,
+      bar_drain;
   __shared__ int unit_ring[2];
   __shared__ uint32_t tmem_base_shared;
 
@@ -434,17 +450,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int t = 0; t < x.steps; ++t, ++g, next_step(p, i, h)) {
               const int head = x.kvh * p.group + h;
               const long long bh = static_cast<long long>(x.b) * p.hq + head;
-              const int qs = g % C::kNQ, ds = g % C::kNDO;
-              if (g >= C::kNQ && !mbar_wait(&bar_q_empty[qs], (g / C::kNQ - 1) & 1, p.status, kDevTimeoutPipe)) {
+              const int st = g & 1;
+              if (g >= 2 && !mbar_wait(&(C::kCross ? bar_do_empty : bar_q_empty)[st], ((g >> 1) - 1) & 1, p.status, kDevTimeoutPipe)) {
                 ok = false;
                 break;
               }
-              mbar_arrive_expect_tx(&bar_q_full[qs], C::kQBytes + C::kStatBytes);
+              mbar_arrive_expect_tx(&bar_q_full[st], C::kQBytes + C::kRowBytes);
               for (int bx = 0; bx < D / 64; ++bx)
-                tma_load_4d(smem + C::kQ + qs * C::kQBytes + bx * C::kQBox, &map_q, &bar_q_full[qs], bx * 64, i * C::kBQ,
+                tma_load_4d(smem + C::kQ + q_buffer<D>(g) * C::kQBytes + bx * C::kQBox, &map_q, &bar_q_full[st], bx * 64, i * C::kBQ,
                             head, x.b);
-              bulk_load(smem + C::kStat + qs * C::kStatBytes, p.stats + (bh * p.nq + i) * (2 * C::kBQ), C::kStatBytes,
-                        &bar_q_full[qs]);
+              const float* rows = p.stats + (bh * p.nq + i) * (2 * C::kBQ);
+              bulk_load(smem + C::kLse + st * C::kRowBytes, rows, C::kRowBytes, &bar_q_full[st]);
               q_issued = g + 1;
               if (t == 0) {
                 if (loads > 0 && !mbar_wait(&bar_kv_empty, (loads - 1) & 1, p.status, kDevTimeoutPipe)) {
@@ -458,23 +474,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                   tma_load_4d(smem + C::kV + bx * C::kKBox, &map_v, &bar_kv_full, bx * 64, x.j * kBK, x.kvh, x.b);
                 ++loads;
               }
-              if (g >= C::kNDO && !mbar_wait(&bar_do_empty[ds], (g / C::kNDO - 1) & 1, p.status, kDevTimeoutPipe)) {
+              if (g >= 2 && !mbar_wait(&(C::kCross ? bar_q_empty : bar_do_empty)[st], ((g >> 1) - 1) & 1, p.status, kDevTimeoutPipe)) {
                 ok = false;
                 break;
               }
-              mbar_arrive_expect_tx(&bar_do_full[ds], C::kQBytes);
+              mbar_arrive_expect_tx(&bar_do_full[st], C::kQBytes + C::kRowBytes);
               for (int bx = 0; bx < D / 64; ++bx)
-                tma_load_4d(smem + C::kDO + ds * C::kQBytes + bx * C::kQBox, &map_do, &bar_do_full[ds], bx * 64,
+                tma_load_4d(smem + C::kQ + do_buffer<D>(g) * C::kQBytes + bx * C::kQBox, &map_do, &bar_do_full[st], bx * 64,
                             i * C::kBQ, head, x.b);
+              bulk_load(smem + C::kDelta + st * C::kRowBytes, rows + C::kBQ, C::kRowBytes, &bar_do_full[st]);
               do_issued = g + 1;
             }
           }
         }
         // before the CTA retires, let the last loads land (bounded; a no-op on the normal path)
         if (loads > 0) mbar_drain(&bar_kv_full, (loads - 1) & 1);
-        for (int t = max(0, q_issued - C::kNQ); t < q_issued; ++t) mbar_drain(&bar_q_full[t % C::kNQ], (t / C::kNQ) & 1);
-        for (int t = max(0, do_issued - C::kNDO); t < do_issued; ++t)
-          mbar_drain(&bar_do_full[t % C::kNDO], (t / C::kNDO) & 1);
+        for (int t = max(0, q_issued - 2); t < q_issued; ++t) mbar_drain(&bar_q_full[t & 1], (t >> 1) & 1);
+        for (int t = max(0, do_issued - 2); t < do_issued; ++t) mbar_drain(&bar_do_full[t & 1], (t >> 1) & 1);
       }
       __syncwarp();
     } else if (warp == kWarpMma) {
@@ -489,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t base = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
       const bool leader = elect_one();
       const uint32_t k_addr = base + C::kK, v_addr = base + C::kV, ds_addr = base + C::kDs;
-      const uint32_t q_base = base + C::kQ, do_base = base + C::kDO;
+      const uint32_t q_base = base + C::kQ;
       // X^T = A B^T over head_dim: S^T = K Q^T, dP^T = V dO^T (all K-major)
       auto issue_scores = [&](uint32_t a, uint32_t b, uint32_t col) {
         const uint64_t ad = make_sdesc_sw128(a, 16, 1024), bd = make_sdesc_sw128(b, 16, 1024);
@@ -521,11 +537,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (x.steps == 0) continue;
         const uint32_t half_k = x.half * (C::kDH / 64) * C::kKBox, half_q = x.half * (C::kDH / 64) * C::kQBox;
         auto issue_s = [&](int gs) -> bool {
-          const int st = gs % C::kNQ;
-          if (!wait(&bar_q_full[st], (gs / C::kNQ) & 1, kDevTimeoutTma)) return false;
+          if (!wait(&bar_q_full[gs & 1], (gs >> 1) & 1, kDevTimeoutTma)) return false;
           tc_fence_after();
           if (leader) {
-            issue_scores(k_addr, q_base + st * C::kQBytes, C::kColS);
+            issue_scores(k_addr, q_base + q_buffer<D>(gs) * C::kQBytes, C::kColS);
             umma_commit(&bar_s);
           }
           __syncwarp();
@@ -533,10 +548,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         ok = wait(&bar_kv_full, active & 1, kDevTimeoutTma) && issue_s(g);
         for (int t = 0; ok && t < x.steps; ++t) {
-          const int gt = g + t, qs = gt % C::kNQ, dos = gt % C::kNDO;
-          const uint32_t q_addr = q_base + qs * C::kQBytes, do_addr = do_base + dos * C::kQBytes;
+          const int gt = g + t, st = gt & 1;
+          const uint32_t q_addr = q_base + q_buffer<D>(gt) * C::kQBytes, do_addr = q_base + do_buffer<D>(gt) * C::kQBytes;
           // dP(t); its columns hold dQ(t-1) until the dQ warps have read it
-          ok = wait(&bar_do_full[dos], (gt / C::kNDO) & 1, kDevTimeoutTma) &&
+          ok = wait(&bar_do_full[st], (gt >> 1) & 1, kDevTimeoutTma) &&
                (!C::kAlias || gt == 0 || wait(&bar_dqfree, (gt - 1) & 1, kDevTimeoutPipe)) &&
                (!C::kVTmem || t > 0 || wait(&bar_v, active & 1, kDevTimeoutPipe));
           if (!ok) break;
@@ -562,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               umma_bf16_ts(tb + C::kColDv, tb + C::kColS + (kk / per) * C::kHalfQ + (kk % per) * 8, bd + ((kk * 2048) >> 4),
                            idesc_kv, (t > 0 || kk > 0) ? 1u : 0u);
             }
-            umma_commit(&bar_do_empty[dos]);
+            umma_commit(&bar_do_empty[st]);
           }
           __syncwarp();
           if (t + 1 < x.steps) {
@@ -589,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int kk = 0; kk < C::kBQ / 16; ++kk)
               umma_bf16_ss(tb + C::kColDk, dsk + (((kk >> 2) * C::kKBox + (kk & 3) * 32) >> 4), qd + ((kk * 2048) >> 4), idesc_kv,
                            (t > 0 || kk > 0) ? 1u : 0u);
-            umma_commit(&bar_q_empty[qs]);
+            umma_commit(&bar_q_empty[st]);
           }
           __syncwarp();
         }
@@ -610,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
     } else if (lane == 0) {
       // ---------------------------------------------------------------- turns of the dQ sums
-      // kWarpTurn waits for a step's turn, a step or two ahead of the dQ warps' additions; kWarpPass waits for
+      // Warp 15 waits for a step's turn, a step or two ahead of the dQ warps' additions; kWarpPass waits for
       // those, for their arrival in L2 (the fence: 1700 cycles, which the dQ warps need not stand still for),
       // and passes the turn on.
       const bool pass = warp == kWarpPass;
@@ -779,16 +794,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       {
         int i = x.i0, h = 0;
         for (int t = 0; t < x.steps; ++t, ++g, next_step(p, i, h)) {
-          const int qs = g % C::kNQ;
-          if (!__all_sync(0xffffffffu, mbar_wait(&bar_q_full[qs], (g / C::kNQ) & 1, p.status, kDevTimeoutTma) &&
+          if (!__all_sync(0xffffffffu, mbar_wait(&bar_q_full[g & 1], (g >> 1) & 1, p.status, kDevTimeoutTma) &&
                                            mbar_wait(&bar_s, g & 1, p.status, kDevTimeoutMma))) {
             ok = false;
             break;
           }
           tc_fence_after();
           // this lane's two query columns of every group of 8
-          const F2* lse2 = reinterpret_cast<const F2*>(smem + C::kStat + qs * C::kStatBytes) + wg * (C::kHalfQ / 2) + (lane & 3);
-          const F2* delta = lse2 + C::kBQ / 2;
+          const F2* lse2 = reinterpret_cast<const F2*>(smem + C::kLse + (g & 1) * C::kRowBytes) + wg * (C::kHalfQ / 2) + (lane & 3);
+          const F2* delta = lse2 + C::kBQ;  // behind both stages of lse2
           const int q0 = i * C::kBQ + wg * C::kHalfQ;
           const bool masked = ragged || (p.causal && q0 < x.j * kBK + kBK - 1);
           // fragment (h16, rg): key (warp & 3) * 32 + h16 * 16 + rg * 8 + lane / 4
@@ -835,6 +849,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bar_p);
+          if (!__all_sync(0xffffffffu, mbar_wait(&bar_do_full[g & 1], (g >> 1) & 1, p.status, kDevTimeoutTma))) {
+            ok = false;
+            break;
+          }
 #pragma unroll
           for (int n = 0; n < kGroups; ++n) st[n] = delta[4 * n];
           if (!__all_sync(0xffffffffu, mbar_wait(&bar_dp, g & 1, p.status, kDevTimeoutMma))) {
@@ -1102,7 +1120,7 @@ struct Plan {
 // the ends of the SMs' queues differ by (a sixth of the longest unit, causal units being sorted by length; half of it
 // otherwise), and the joining of the parts.  Whole and cut, us: B1 Hq32 Hkv8 S2048 D128 213, 136 (2 parts); B1 Hq32 Hkv4
 // S1024 D128 195, 63 (8); B1 Hq16 Hkv2 S4096 D256 1290, 699 (2); where a cut does not pay, B2 Hq16 Hkv2 S4096 D256
-// 1404, 1483 (2).
+// 1195, 1250 (2).
 template <int D>
 Plan plan(int batch, int hkv, int group, int nq, int nk, int causal) {
   using C = Cfg<D>;
@@ -1163,7 +1181,7 @@ Sizes sizes(long long batch, long long hq, long long hkv, long long sq, long lon
   auto up = [](long long n) { return (n + 255) / 256 * 256; };
   Sizes s{};
   s.counters = up((1 + plan.streams * tiles * C::kSplit) * 4);
-  s.stats = up(tiles * C::kStatBytes);
+  s.stats = up(tiles * 2 * C::kRowBytes);
   s.acc = skv > kBK ? plan.streams * tiles * C::kSplit * C::kDqCols * 128 * 4 : 0;  // one key tile: dq is written at once
   s.partial = plan.part_tiles > 0 ? batch * hkv * C::kSplit * plan.per_row * (2LL * C::kDH * 128 * 4) : 0;
   s.total = s.counters + s.stats + s.acc + s.partial;
