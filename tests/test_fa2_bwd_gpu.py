@@ -10,6 +10,7 @@ their absolute sums, which the bound adds, as it does P's: the exponent c s - ls
 """
 
 import math
+import threading
 
 import pytest
 import torch
@@ -263,6 +264,32 @@ def test_calls_on_two_streams_and_in_graphs(cuda_device):
         torch.cuda.synchronize()
         for o, i in zip(outs, pick):
             assert all(torch.equal(a, b) for a, b in zip(o, want[i]))
+
+
+def test_first_call_of_a_thread(cuda_device):
+    """A thread that has made no CUDA call yet, as autograd's may be when all its memory comes from the allocator's cache."""
+    q, k, v, do = make(1, 4, 2, 300, 300, 128, "bhsd", seed=12)
+
+    def both():
+        o, lse = fa2.kernel_fn(q, k, v, True, return_lse=True)
+        return (o, *bwd.kernel_fn(do, q, k, v, o, lse, True))
+
+    want = both()
+    both()  # leaves its blocks in the cache
+    got = []
+
+    def run():
+        try:
+            got.extend(both())
+        except Exception as e:  # shown by the assertions
+            got.append(e)
+
+    thread = threading.Thread(target=run)
+    thread.start()
+    thread.join()
+    assert len(got) == 4, got
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_masked_infinities_stay_out(cuda_device):
