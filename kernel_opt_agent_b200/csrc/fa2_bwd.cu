@@ -27,13 +27,13 @@
 //   fa2_bwd_finish  dq = c times those sums, rounded, in dq's layout, and dV and dK of key tiles that came
 //                   in parts.  (The last key tile's CTA could finish dq in passing, but reading the sums back held its pipeline
 //                   up for 10 000 to 20 000 cycles a tile.  With a single key tile dQ is written at once.)
-// Roles (512 threads): warps 0-7 softmax (two warpgroups, each half of a tile's query columns; TMEM is read in
-// the layout of mma accumulators, in which a lane has two of every 8 columns: a lane that owned a row read every row
-// statistic as a broadcast, 1400 of a step's cycles of shared memory), warps 8-11 dQ (TMEM to global), warp 12 TMA
-// and unit counter, warp 13 TMEM owner and MMA issuer, warps 14 and 15 pass on and wait for the turns of the dQ
-// sums.
+// Roles: two softmax warpgroups (four at D 64), each a share of a tile's query columns (TMEM is read in the layout of mma
+// accumulators, in which a lane has two of every 8 columns: a lane that owned a row read every row statistic as a broadcast,
+// 1400 of a step's cycles of shared memory); four dQ warps (TMEM to global); a warp each for TMA and the unit counter, for the
+// MMAs and TMEM, for passing on and for awaiting the turns of the dQ sums.
 // Order of the MMAs:  dP(t) dV(t) S(t+1) dQ(t) dK(t) | dP(t+1) ...: while the softmax warps form P
-// the tensor core has dQ and dK to do, and while they form dS it has dV and the next S.
+// the tensor core has dQ and dK to do, and while they form dS it has dV and the next S.  At D 64, where dQ has columns of
+// its own, dP(t+1) goes before dQ(t).
 //
 // What bounds it (D 128, a step of 128 queries x 128 keys, cycles): the tensor core 2560, shared memory about 3200, sending
 // 64 KB of dQ 2600 at the 25 bytes a cycle that an SM sends; measured 4300 to 4600, and under sustained load the
@@ -60,10 +60,7 @@ namespace tokmix {
 namespace fa2b {
 
 constexpr int kBK = 128;             // keys per unit
-constexpr int kThreads = 512;
-constexpr int kSoftmaxWarps = 8, kDqWarps = 4;
-constexpr int kWarpTma = 12, kWarpMma = 13, kWarpPass = 14;  // and 15
-constexpr int kUnitReaders = 3 + kSoftmaxWarps + kDqWarps;
+constexpr int kDqWarps = 4;
 constexpr int kMaxParted = 256;      // key tiles of a row that may come in parts
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -82,7 +79,21 @@ struct Cfg {
   static constexpr bool kVTmem = D == 256;             // V in TMEM, as the A operand of dP
   static constexpr bool kTransDq = D == 256;           // dQ^T: lanes are columns of dq, columns are queries
   static constexpr int kDqCols = kTransDq ? kBQ : kDH; // TMEM columns of dQ
-  static constexpr int kHalfQ = kBQ / 2;               // query columns of a softmax warpgroup
+  // Softmax warpgroups.  At D 64 the softmax is longer than the products, and four hide each other's latencies better (with dP(t+1)
+  // before dQ(t); one without the other gains less or loses).  Two and four, us, 128 queries a tile: B3 Hq12 Hkv4
+  // 1000 x 1531 79.5, 73.9; B1 Hq32 Hkv8 S2048 97.5, 94.7; B4 Hq16 Hkv4 S1024 63.3, 60.8; B8 Hq8 S2048 186.5, 185.9; B16 Hq12
+  // S512 without mask 103.7, 105.7; B4 Hq32 Hkv8 S8192, at the power limit, 4115, 4178.
+  static constexpr int kGroups = D == 64 ? 4 : 2;
+  static constexpr int kGroupQ = kBQ / kGroups;        // query columns of one
+  static constexpr int kSoftmaxWarps = 4 * kGroups;
+  static constexpr int kWarpTma = kSoftmaxWarps + kDqWarps, kWarpMma = kWarpTma + 1, kWarpPass = kWarpTma + 2;
+  static constexpr int kThreads = (kWarpTma + 4) * 32;
+  static constexpr int kUnitReaders = 3 + kSoftmaxWarps + kDqWarps;
+  // registers of the softmax, dQ and other warps, which share those that the CTA is launched with
+  static constexpr int kSoftmaxRegs = kGroups == 4 ? 88 : 144, kDqRegs = kGroups == 4 ? 88 : 152,
+                       kOtherRegs = kGroups == 4 ? 40 : 64;
+  static_assert(kSoftmaxWarps * kSoftmaxRegs + kDqWarps * kDqRegs + 4 * kOtherRegs <= kThreads / 32 * (65536 / kThreads / 8 * 8),
+                "registers");
   // Cycles between 8 KB of reductions: an SM sends about 25 bytes a cycle, and reductions that wait for that keep the
   // tensor core from shared memory and TMA requests in the queue (B4 Hq32 Hkv8 S8192: D 128 6809 us without, 6200
   // with 288, 6155 with 304, 6300 with 320, 6623 with 440; D 64 4199 without, 4025 with 320, 4200 with 800; B2 Hq16 Hkv2
@@ -101,12 +112,13 @@ struct Cfg {
   static constexpr int kKBytes = (D / 64) * kKBox;
   static constexpr int kQBytes = (D / 64) * kQBox;
   static constexpr int kDsBytes = kBK * kBQ * 2;       // boxes of 128 keys x 64 queries
+  static constexpr int kDsBuffers = kAlias ? 1 : 2;    // dP(t + 1), and with it dS(t + 1), does not wait for dQ(t) and dK(t)
   static constexpr int kRowBytes = kBQ * 4;            // lse2 or delta of a query tile
   static constexpr int kK = 0;
   static constexpr int kV = kK + kKBytes;
   static constexpr int kQ = kV + (kVTmem ? 0 : kKBytes);
   static constexpr int kDs = kQ + 4 * kQBytes;         // four buffers of Q and dO, see q_buffer
-  static constexpr int kLse = kDs + kDsBytes;          // two stages
+  static constexpr int kLse = kDs + kDsBuffers * kDsBytes;          // two stages
   static constexpr int kDelta = kLse + 2 * kRowBytes;  // two stages
   static constexpr int kBytes = kDelta + 2 * kRowBytes;
   static_assert(kBytes + 1024 <= 227 * 1024, "shared memory");  // 1024: the barriers, rounded up to the tiles' alignment
@@ -358,15 +370,15 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[N]) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     fa2_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
                    const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                    const __grid_constant__ CUtensorMap map_dk, const __grid_constant__ CUtensorMap map_dv, const Params p) {
   using C = Cfg<D>;
   extern __shared__ __align__(1024) uint8_t smem[];  // no room is left to round its start up
   __shared__ uint64_t bar_unit_full[2], bar_unit_empty[2], bar_kv_full, bar_kv_empty, bar_v, bar_q_full[2], bar_q_empty[2],
-      bar_do_full[2], bar_do_empty[2], bar_s, bar_p, bar_dp, bar_ds, bar_dq, bar_dqfree, bar_turn[2], bar_added[2], bar_passed[2], bar_acc, bar_accfree,
-      bar_drain;
+      bar_do_full[2], bar_do_empty[2], bar_s, bar_p, bar_dp, bar_ds, bar_dq, bar_dqfree, bar_turn[2], bar_added[2],
+      bar_passed[2], bar_acc, bar_accfree, bar_drain;
   __shared__ int unit_ring[2];
   __shared__ uint32_t tmem_base_shared;
 
@@ -381,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     cta_abort_flag() = 0u;
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar_unit_full[i], 1);
-      mbar_init(&bar_unit_empty[i], kUnitReaders);
+      mbar_init(&bar_unit_empty[i], C::kUnitReaders);
       mbar_init(&bar_q_full[i], 1);
       mbar_init(&bar_q_empty[i], 1);
       mbar_init(&bar_do_full[i], 1);
@@ -392,19 +404,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(&bar_kv_full, 1);
     mbar_init(&bar_kv_empty, 1);
-    mbar_init(&bar_v, kSoftmaxWarps);
+    mbar_init(&bar_v, C::kSoftmaxWarps);
     mbar_init(&bar_s, 1);
-    mbar_init(&bar_p, kSoftmaxWarps);
+    mbar_init(&bar_p, C::kSoftmaxWarps);
     mbar_init(&bar_dp, 1);
-    mbar_init(&bar_ds, kSoftmaxWarps);
+    mbar_init(&bar_ds, C::kSoftmaxWarps);
     mbar_init(&bar_dq, 1);
     mbar_init(&bar_dqfree, kDqWarps);
     mbar_init(&bar_acc, 1);
-    mbar_init(&bar_accfree, kSoftmaxWarps);
+    mbar_init(&bar_accfree, C::kSoftmaxWarps);
     mbar_init(&bar_drain, 1);
     fence_barrier_init();
   }
-  if (warp == kWarpMma) {
+  if (warp == C::kWarpMma) {
     tmem_alloc(&tmem_base_shared, 512);
     tmem_relinquish();
   }
@@ -423,9 +435,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     return *reinterpret_cast<volatile int*>(&unit_ring[r & 1]);
   };
 
-  if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == kWarpTma) {
+  if (warp >= C::kWarpTma) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+    if (warp == C::kWarpTma) {
       // ---------------------------------------------------------------- unit counter, TMA
       if (lane == 0) {
         tma_prefetch_desc(&map_q);
@@ -493,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int t = max(0, do_issued - 2); t < do_issued; ++t) mbar_drain(&bar_do_full[t & 1], (t >> 1) & 1);
       }
       __syncwarp();
-    } else if (warp == kWarpMma) {
+    } else if (warp == C::kWarpMma) {
       // ---------------------------------------------------------------- MMA issuer
       // The whole warp walks the steps and waits, one elected lane issues: so addresses and
       // descriptors are warp-uniform (issued from a branch of one lane, an MMA took 75 to 135 cycles
@@ -504,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t tb = __shfl_sync(0xffffffffu, tbase, 0);
       const uint32_t base = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
       const bool leader = elect_one();
-      const uint32_t k_addr = base + C::kK, v_addr = base + C::kV, ds_addr = base + C::kDs;
+      const uint32_t k_addr = base + C::kK, v_addr = base + C::kV;
       const uint32_t q_base = base + C::kQ;
       // X^T = A B^T over head_dim: S^T = K Q^T, dP^T = V dO^T (all K-major)
       auto issue_scores = [&](uint32_t a, uint32_t b, uint32_t col) {
@@ -546,24 +558,31 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           return true;
         };
+        auto issue_dp = [&](int gs) {
+          if (leader) {
+            const uint32_t b = q_base + do_buffer<D>(gs) * C::kQBytes;
+            if constexpr (C::kVTmem)
+              issue_dp_tmem(b);
+            else
+              issue_scores(v_addr, b, C::kColDp);
+            umma_commit(&bar_dp);
+          }
+          __syncwarp();
+        };
         ok = wait(&bar_kv_full, active & 1, kDevTimeoutTma) && issue_s(g);
         for (int t = 0; ok && t < x.steps; ++t) {
           const int gt = g + t, st = gt & 1;
           const uint32_t q_addr = q_base + q_buffer<D>(gt) * C::kQBytes, do_addr = q_base + do_buffer<D>(gt) * C::kQBytes;
-          // dP(t); its columns hold dQ(t-1) until the dQ warps have read it
-          ok = wait(&bar_do_full[st], (gt >> 1) & 1, kDevTimeoutTma) &&
-               (!C::kAlias || gt == 0 || wait(&bar_dqfree, (gt - 1) & 1, kDevTimeoutPipe)) &&
-               (!C::kVTmem || t > 0 || wait(&bar_v, active & 1, kDevTimeoutPipe));
-          if (!ok) break;
-          tc_fence_after();
-          if (leader) {
-            if constexpr (C::kVTmem)
-              issue_dp_tmem(do_addr);
-            else
-              issue_scores(v_addr, do_addr, C::kColDp);
-            umma_commit(&bar_dp);
+          // dP(t); at D >= 128 its columns hold dQ(t-1) until the dQ warps have read it, at D 64 it was issued in front of
+          // dQ(t-1)
+          if (C::kAlias || t == 0) {
+            ok = wait(&bar_do_full[st], (gt >> 1) & 1, kDevTimeoutTma) &&
+                 (!C::kAlias || gt == 0 || wait(&bar_dqfree, (gt - 1) & 1, kDevTimeoutPipe)) &&
+                 (!C::kVTmem || t > 0 || wait(&bar_v, active & 1, kDevTimeoutPipe));
+            if (!ok) break;
+            tc_fence_after();
+            issue_dp(gt);
           }
-          __syncwarp();
           // dV += P^T dO; the first overwrites an accumulator that the previous unit's epilogue has read
           ok = wait(&bar_p, gt & 1, kDevTimeoutPipe) &&
                (t > 0 || active == 0 || wait(&bar_accfree, (active - 1) & 1, kDevTimeoutPipe));
@@ -573,8 +592,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint64_t bd = make_sdesc_sw128(do_addr + half_q, C::kQBox, 1024);
 #pragma unroll
             for (int kk = 0; kk < C::kBQ / 16; ++kk) {
-              constexpr int per = C::kHalfQ / 16;  // steps in a warpgroup's part of P
-              umma_bf16_ts(tb + C::kColDv, tb + C::kColS + (kk / per) * C::kHalfQ + (kk % per) * 8, bd + ((kk * 2048) >> 4),
+              constexpr int per = C::kGroupQ / 16;  // steps in a warpgroup's part of P
+              umma_bf16_ts(tb + C::kColDv, tb + C::kColS + (kk / per) * C::kGroupQ + (kk % per) * 8, bd + ((kk * 2048) >> 4),
                            idesc_kv, (t > 0 || kk > 0) ? 1u : 0u);
             }
             umma_commit(&bar_do_empty[st]);
@@ -584,11 +603,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = issue_s(gt + 1);
             if (!ok) break;
           }
-          ok = wait(&bar_ds, gt & 1, kDevTimeoutPipe) &&
-               (C::kAlias || gt == 0 || wait(&bar_dqfree, (gt - 1) & 1, kDevTimeoutPipe));
+          ok = wait(&bar_ds, gt & 1, kDevTimeoutPipe);
           if (!ok) break;
+          if constexpr (!C::kAlias) {
+            if (t + 1 < x.steps) {
+              ok = wait(&bar_do_full[st ^ 1], ((gt + 1) >> 1) & 1, kDevTimeoutTma);
+              if (!ok) break;
+              tc_fence_after();
+              issue_dp(gt + 1);
+            }
+            ok = gt == 0 || wait(&bar_dqfree, (gt - 1) & 1, kDevTimeoutPipe);
+            if (!ok) break;
+          }
           tc_fence_after();
           if (leader) {
+            const uint32_t ds_addr = base + C::kDs + (C::kDsBuffers == 2 ? st * C::kDsBytes : 0);
             // dQ = dS K (or its transpose)
             const uint64_t dsd = make_sdesc_sw128(ds_addr, C::kKBox, 1024);
             const uint64_t kd = make_sdesc_sw128(k_addr + half_k, C::kKBox, 1024);
@@ -625,10 +654,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
     } else if (lane == 0) {
       // ---------------------------------------------------------------- turns of the dQ sums
-      // Warp 15 waits for a step's turn, a step or two ahead of the dQ warps' additions; kWarpPass waits for
+      // The last warp waits for a step's turn, a step or two ahead of the dQ warps' additions; kWarpPass waits for
       // those, for their arrival in L2 (the fence: 1700 cycles, which the dQ warps need not stand still for),
       // and passes the turn on.
-      const bool pass = warp == kWarpPass;
+      const bool pass = warp == C::kWarpPass;
       bool ok = true;
       int g = 0;
       for (int r = 0; ok; ++r) {
@@ -663,9 +692,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-  } else if (warp >= kSoftmaxWarps) {
+  } else if (warp >= C::kSoftmaxWarps) {
     // ------------------------------------------------------------------ dQ: TMEM -> global, in turn
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kDqRegs));
     const int wq = warp & 3;
     const int row = wq * 32 + lane;  // TMEM lane: a query of the tile, or (transposed) a column of dq
     const uint32_t col = tmem_addr(tbase, wq * 32, C::kColDq);
@@ -741,22 +770,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ------------------------------------------------------------------ softmax warps, epilogue of dV and dK
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
     const int wg = warp >> 2;
     const int row = (warp & 3) * 32 + lane;  // key of the tile
     const uint32_t lanes = tmem_addr(tbase, (warp & 3) * 32, 0);
-    const uint32_t col_s = lanes + C::kColS + wg * C::kHalfQ;
-    const uint32_t col_dp = lanes + C::kColDp + wg * C::kHalfQ;
-    constexpr int kGroups = C::kHalfQ / 8;  // groups of 8 query columns
+    const uint32_t col_s = lanes + C::kColS + wg * C::kGroupQ;
+    const uint32_t col_dp = lanes + C::kColDp + wg * C::kGroupQ;
+    constexpr int kCols8 = C::kGroupQ / 8;  // groups of 8 query columns
     // this lane's row and first piece in the matrices it stores: matrix l / 8 is the lower (upper) 8 keys of 16
     // in an even (odd) group of 8 queries
-    const uint32_t ds_base = smem_u32(smem + C::kDs + (C::kHalfQ == 64 ? wg * C::kKBox : 0));
+    const uint32_t ds_base = smem_u32(smem + C::kDs + wg * C::kGroupQ / 64 * C::kKBox);
     const int st_row = (warp & 3) * 32 + ((lane >> 3) & 1) * 8 + (lane & 7);
-    const int st_piece = (lane >> 4) + (C::kHalfQ == 64 ? 0 : wg * 4);
+    const int st_piece = (lane >> 4) + wg * C::kGroupQ % 64 / 8;
     const F2 c2 = pair2(__float_as_uint(p.scale_log2), __float_as_uint(p.scale_log2));
-    constexpr bool kOwnBox = C::kBQ == 128;  // a box of dS per warpgroup
-    constexpr int kEpiThreads = kOwnBox ? 128 : 256, kEpiRounds = kOwnBox ? C::kBoxes : 2 * C::kBoxes;
-    const int kEpiBarrier = kOwnBox ? 1 + wg : 1;
+    // epilogue: the warpgroups that share a box of the dS buffer, and the boxes in use at once
+    constexpr int kSharers = 64 / C::kGroupQ, kSets = C::kGroups / kSharers;
+    constexpr int kEpiThreads = 128 * kSharers, kEpiRounds = 2 * C::kBoxes / kSets;
+    const int set = wg / kSharers, kEpiBarrier = 1 + set;
     bool ok = true;
     int g = 0, active = 0;
     for (int r = 0;; ++r) {
@@ -801,24 +831,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           tc_fence_after();
           // this lane's two query columns of every group of 8
-          const F2* lse2 = reinterpret_cast<const F2*>(smem + C::kLse + (g & 1) * C::kRowBytes) + wg * (C::kHalfQ / 2) + (lane & 3);
+          const F2* lse2 = reinterpret_cast<const F2*>(smem + C::kLse + (g & 1) * C::kRowBytes) + wg * (C::kGroupQ / 2) + (lane & 3);
           const F2* delta = lse2 + C::kBQ;  // behind both stages of lse2
-          const int q0 = i * C::kBQ + wg * C::kHalfQ;
+          const int q0 = i * C::kBQ + wg * C::kGroupQ;
           const bool masked = ragged || (p.causal && q0 < x.j * kBK + kBK - 1);
           // fragment (h16, rg): key (warp & 3) * 32 + h16 * 16 + rg * 8 + lane / 4
           const int key0 = x.j * kBK + (warp & 3) * 32 + (lane >> 2);
-          uint32_t raw[2][4 * kGroups];
-          tmem_ld_frag<kGroups>(col_s, raw[0]);
-          tmem_ld_frag<kGroups>(col_s + (16u << 16), raw[1]);
-          float pr[2][4 * kGroups];
-          F2 st[kGroups];
+          uint32_t raw[2][4 * kCols8];
+          tmem_ld_frag<kCols8>(col_s, raw[0]);
+          tmem_ld_frag<kCols8>(col_s + (16u << 16), raw[1]);
+          float pr[2][4 * kCols8];
+          F2 st[kCols8];
 #pragma unroll
-          for (int n = 0; n < kGroups; ++n) st[n] = lse2[4 * n];
+          for (int n = 0; n < kCols8; ++n) st[n] = lse2[4 * n];
           tmem_wait_ld();
 #pragma unroll
           for (int h16 = 0; h16 < 2; ++h16) {
 #pragma unroll
-            for (int n = 0; n < kGroups; ++n) {
+            for (int n = 0; n < kCols8; ++n) {
 #pragma unroll
               for (int rg = 0; rg < 2; ++rg) {
                 const int e = 4 * n + 2 * rg;
@@ -832,18 +862,18 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int rg = 0; rg < 2; ++rg) {
                 const int key = key0 + h16 * 16 + rg * 8;
                 // query columns before `first` are masked for this key
-                const int first = (key >= p.skv ? C::kHalfQ : (p.causal ? key - q0 : 0)) - 2 * (lane & 3);
+                const int first = (key >= p.skv ? C::kGroupQ : (p.causal ? key - q0 : 0)) - 2 * (lane & 3);
 #pragma unroll
-                for (int n = 0; n < kGroups; ++n) {
+                for (int n = 0; n < kCols8; ++n) {
                   if (8 * n < first) pr[h16][4 * n + 2 * rg] = 0.0f;
                   if (8 * n + 1 < first) pr[h16][4 * n + 2 * rg + 1] = 0.0f;
                 }
               }
             }
-            uint32_t packed[2 * kGroups];
+            uint32_t packed[2 * kCols8];
 #pragma unroll
-            for (int e = 0; e < 2 * kGroups; ++e) packed[e] = pack_bf16x2(pr[h16][2 * e], pr[h16][2 * e + 1]);
-            tmem_st_frag<kGroups>(col_s + (static_cast<uint32_t>(h16 * 16) << 16), packed);
+            for (int e = 0; e < 2 * kCols8; ++e) packed[e] = pack_bf16x2(pr[h16][2 * e], pr[h16][2 * e + 1]);
+            tmem_st_frag<kCols8>(col_s + (static_cast<uint32_t>(h16 * 16) << 16), packed);
           }
           tmem_wait_st();
           tc_fence_before();
@@ -854,20 +884,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
 #pragma unroll
-          for (int n = 0; n < kGroups; ++n) st[n] = delta[4 * n];
+          for (int n = 0; n < kCols8; ++n) st[n] = delta[4 * n];
           if (!__all_sync(0xffffffffu, mbar_wait(&bar_dp, g & 1, p.status, kDevTimeoutMma))) {
             ok = false;
             break;
           }
           tc_fence_after();
-          tmem_ld_frag<kGroups>(col_dp, raw[0]);
-          tmem_ld_frag<kGroups>(col_dp + (16u << 16), raw[1]);
+          tmem_ld_frag<kCols8>(col_dp, raw[0]);
+          tmem_ld_frag<kCols8>(col_dp + (16u << 16), raw[1]);
           tmem_wait_ld();
 #pragma unroll
           for (int h16 = 0; h16 < 2; ++h16) {
-            float ds[4 * kGroups];
+            float ds[4 * kCols8];
 #pragma unroll
-            for (int n = 0; n < kGroups; ++n) {
+            for (int n = 0; n < kCols8; ++n) {
 #pragma unroll
               for (int rg = 0; rg < 2; ++rg) {
                 const int e = 4 * n + 2 * rg;
@@ -881,20 +911,22 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int rg = 0; rg < 2; ++rg) {
                 const int key = key0 + h16 * 16 + rg * 8;
-                const int first = (key >= p.skv ? C::kHalfQ : (p.causal ? key - q0 : 0)) - 2 * (lane & 3);
+                const int first = (key >= p.skv ? C::kGroupQ : (p.causal ? key - q0 : 0)) - 2 * (lane & 3);
 #pragma unroll
-                for (int n = 0; n < kGroups; ++n) {
+                for (int n = 0; n < kCols8; ++n) {
                   if (8 * n < first) ds[4 * n + 2 * rg] = 0.0f;
                   if (8 * n + 1 < first) ds[4 * n + 2 * rg + 1] = 0.0f;
                 }
               }
             }
 #pragma unroll
-            for (int n = 0; n < kGroups; n += 2) {
+            for (int n = 0; n < kCols8; n += 2) {
               uint32_t w[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(ds[4 * n + 2 * e], ds[4 * n + 2 * e + 1]);
-              st_matrix_x4(ds_base + sw128_offset(st_row + h16 * 16, (st_piece + n) * 16), w);
+              st_matrix_x4(ds_base + (C::kDsBuffers == 2 ? (g & 1) * C::kDsBytes : 0) +
+                               sw128_offset(st_row + h16 * 16, (st_piece + n) * 16),
+                           w);
             }
           }
           fence_async_smem();
@@ -904,20 +936,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       // Epilogue: dV and dK, 64 columns at a time, through the dS buffer (the MMAs that read it are complete) to TMA
-      // stores, which clip the rows behind the last key.  With two boxes of dS warpgroup 0 takes dV and warpgroup 1 dK;
-      // with one both take half of each box.  (Rows written by their threads, 16 bytes at a stride, took 9600 cycles
+      // stores, which clip the rows behind the last key.  With two boxes of dS one half of the warpgroups takes dV and the other dK;
+      // with one all take both.  (Rows written by their threads, 16 bytes at a stride, took 9600 cycles
       // at D 128.)  Every warp comes here once per unit, whether its waits ran out or not, so none is left at a barrier.
       if (ok && x.steps > 0)
         ok = __all_sync(0xffffffffu, mbar_wait(&bar_acc, active & 1, p.status, kDevTimeoutMma));
       ok = named_sync_and(kEpiBarrier, kEpiThreads, ok);
       if (!ok) break;
       tc_fence_after();
-      if (x.parts > 1) {  // a part: fp32, as fa2_bwd_finish reads it; warpgroup 0 dV, warpgroup 1 dK
-        float* dst = p.partial + (x.slot * 2 + wg) * (C::kDH * 128) + row * 4;
+      if (x.parts > 1) {  // a part: fp32, as fa2_bwd_finish reads it
+        constexpr int kPerSum = C::kGroups / 2, kCols = C::kDH / kPerSum;
+        float* dst = p.partial + (x.slot * 2 + wg / kPerSum) * (C::kDH * 128) + row * 4;
 #pragma unroll 1
-        for (int dc = 0; dc < C::kDH; dc += 32) {
+        for (int dc = wg % kPerSum * kCols; dc < (wg % kPerSum + 1) * kCols; dc += 32) {
           uint32_t a[32];
-          tmem_ld32(lanes + (wg == 0 ? C::kColDv : C::kColDk) + dc, a);
+          tmem_ld32(lanes + (wg / kPerSum == 0 ? C::kColDv : C::kColDk) + dc, a);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             __stcg(reinterpret_cast<float4*>(dst + (dc / 4 + e) * 512),
@@ -931,23 +964,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         continue;
       }
       for (int round = 0; round < kEpiRounds; ++round) {
-        const int which = kOwnBox ? wg : round / C::kBoxes;  // 0: dV, 1: dK
-        const int box = kOwnBox ? round : round % C::kBoxes;
+        const int which = kSets == 2 ? set : round / C::kBoxes;  // 0: dV, 1: dK
+        const int box = kSets == 2 ? round : round % C::kBoxes;
         const float mul = which == 0 ? 1.0f : p.scale;
-        const uint32_t from = lanes + (which == 0 ? C::kColDv : C::kColDk) + box * 64 + (kOwnBox ? 0 : wg * C::kHalfQ);
-        uint32_t a[2][4 * kGroups];
+        const uint32_t from = lanes + (which == 0 ? C::kColDv : C::kColDk) + box * 64 + wg % kSharers * C::kGroupQ;
+        uint32_t a[2][4 * kCols8];
         if (x.steps > 0) {
-          tmem_ld_frag<kGroups>(from, a[0]);
-          tmem_ld_frag<kGroups>(from + (16u << 16), a[1]);
+          tmem_ld_frag<kCols8>(from, a[0]);
+          tmem_ld_frag<kCols8>(from + (16u << 16), a[1]);
           tmem_wait_ld();
         } else {  // a tile that no query sees
 #pragma unroll
-          for (int e = 0; e < 4 * kGroups; ++e) a[0][e] = a[1][e] = 0u;
+          for (int e = 0; e < 4 * kCols8; ++e) a[0][e] = a[1][e] = 0u;
         }
 #pragma unroll
         for (int h16 = 0; h16 < 2; ++h16) {
 #pragma unroll
-          for (int n = 0; n < kGroups; n += 2) {
+          for (int n = 0; n < kCols8; n += 2) {
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -964,7 +997,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_async_smem();
         named_sync_and(kEpiBarrier, kEpiThreads, true);
         if ((threadIdx.x & (kEpiThreads - 1)) == 0) {
-          tma_store_4d(which == 0 ? &map_dv : &map_dk, smem + C::kDs + (kOwnBox ? wg * C::kKBox : 0), x.half * C::kDH + box * 64,
+          tma_store_4d(which == 0 ? &map_dv : &map_dk, smem + C::kDs + set * C::kKBox, x.half * C::kDH + box * 64,
                        x.j * kBK, x.kvh, x.b);
           bulk_commit();
           bulk_wait_read();
@@ -977,7 +1010,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   tc_fence_before();
   __syncthreads();
-  if (warp == kWarpMma) {
+  if (warp == C::kWarpMma) {
     tc_fence_after();
     tmem_dealloc(tbase, 512);
   }
@@ -1279,7 +1312,7 @@ int launch(const void* dout, const void* q, const void* k, const void* v, const 
                                     p.q_sb, p.q_sh, p.q_ss);
   if (e == cudaSuccess) {
     const int grid = static_cast<int>(std::min<long long>(units, std::max(1, device_sm_count())));
-    e = launch_overlapped(&fa2_bwd_kernel<D>, dim3(static_cast<unsigned>(grid)), dim3(kThreads),
+    e = launch_overlapped(&fa2_bwd_kernel<D>, dim3(static_cast<unsigned>(grid)), dim3(Cfg<D>::kThreads),
                           static_cast<size_t>(smem_bytes), stream, mq, mdo, mk, mv, mdk, mdv, p);
   }
   const long long dq_blocks = p.nk > 1 ? tiles * (C::kDqCols / 32) : 0;
