@@ -242,16 +242,6 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-// A tile from shared memory to a tensor (rows outside it are left out), in a bulk group of this thread
-__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* src, int x, int y, int z, int w) {
-  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map),
-               "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z), "r"(w)
-               : "memory");
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-
 __device__ __forceinline__ void red_add_v4(float* dst, float a, float b, float c, float d) {
   asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(dst), "f"(a), "f"(b), "f"(c), "f"(d)
                : "memory");
@@ -372,8 +362,7 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[N]) {
 template <int D>
 __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     fa2_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
-                   const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                   const __grid_constant__ CUtensorMap map_dk, const __grid_constant__ CUtensorMap map_dv, const Params p) {
+                   const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params p) {
   using C = Cfg<D>;
   extern __shared__ __align__(1024) uint8_t smem[];  // no room is left to round its start up
   __shared__ uint64_t bar_unit_full[2], bar_unit_empty[2], bar_kv_full, bar_kv_empty, bar_v, bar_q_full[2], bar_q_empty[2],
@@ -783,19 +772,16 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     const int st_row = (warp & 3) * 32 + ((lane >> 3) & 1) * 8 + (lane & 7);
     const int st_piece = (lane >> 4) + wg * C::kGroupQ % 64 / 8;
     const F2 c2 = pair2(__float_as_uint(p.scale_log2), __float_as_uint(p.scale_log2));
-    // epilogue: the warpgroups that share a box of the dS buffer, and the boxes in use at once
-    constexpr int kSharers = 64 / C::kGroupQ, kSets = C::kGroups / kSharers;
-    constexpr int kEpiThreads = 128 * kSharers, kEpiRounds = 2 * C::kBoxes / kSets;
-    const int set = wg / kSharers, kEpiBarrier = 1 + set;
+    // epilogue: the warpgroups that share a box of the dS buffer, the boxes in use at once, lanes that store a row
+    constexpr int kSharers = 64 / C::kGroupQ, kSets = C::kGroups / kSharers, kRounds = 2 * C::kBoxes / kSets;
+    constexpr int kRowLanes = C::kGroupQ / 8;
+    const int set = wg / kSharers, first_col = wg * C::kGroupQ % 64;
     bool ok = true;
     int g = 0, active = 0;
     for (int r = 0;; ++r) {
       const int u = __shfl_sync(0xffffffffu, lane == 0 ? next_unit(r, ok) : 0, 0);
       ok = __all_sync(0xffffffffu, ok);
-      if (!ok || u < 0) {
-        named_sync_and(kEpiBarrier, kEpiThreads, ok);  // this round's arrival (see the epilogue)
-        break;
-      }
+      if (!ok || u < 0) break;
       if (lane == 0) mbar_arrive(&bar_unit_empty[r & 1]);
       const Unit x = decode_unit<D>(p, u);
       const int key = x.j * kBK + row;
@@ -935,14 +921,14 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
           if (lane == 0) mbar_arrive(&bar_ds);
         }
       }
-      // Epilogue: dV and dK, 64 columns at a time, through the dS buffer (the MMAs that read it are complete) to TMA
-      // stores, which clip the rows behind the last key.  With two boxes of dS one half of the warpgroups takes dV and the other dK;
-      // with one all take both.  (Rows written by their threads, 16 bytes at a stride, took 9600 cycles
-      // at D 128.)  Every warp comes here once per unit, whether its waits ran out or not, so none is left at a barrier.
-      if (ok && x.steps > 0)
-        ok = __all_sync(0xffffffffu, mbar_wait(&bar_acc, active & 1, p.status, kDevTimeoutMma));
-      ok = named_sync_and(kEpiBarrier, kEpiThreads, ok);
       if (!ok) break;
+      // Epilogue: dV and dK, 64 columns at a time.  A warp turns its 32 keys round in its own rows of the dS buffer (the MMAs
+      // that read it are complete) and stores rows of 128 bytes (64 where two warpgroups share a box).  With two boxes of dS
+      // one half of the warpgroups takes dV and the other dK; with one all take both.  TMA stores from there waited in
+      // the TMA unit behind the next unit's loads, 3500 ns a unit at D 128; rows written by their threads, 16 bytes at a
+      // stride, took 9600 cycles.  One tile of 128 14.1 us with TMA stores, 12.3 so; B3 Hq12 Hkv4 1000 x 1531 D64 73.6, 71.8;
+      // B4 Hq16 Hkv4 S1024 D128 90.8, 89.
+      if (x.steps > 0 && !__all_sync(0xffffffffu, mbar_wait(&bar_acc, active & 1, p.status, kDevTimeoutMma))) break;
       tc_fence_after();
       if (x.parts > 1) {  // a part: fp32, as fa2_bwd_finish reads it
         constexpr int kPerSum = C::kGroups / 2, kCols = C::kDH / kPerSum;
@@ -963,7 +949,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         ++active;
         continue;
       }
-      for (int round = 0; round < kEpiRounds; ++round) {
+      for (int round = 0; round < kRounds; ++round) {
         const int which = kSets == 2 ? set : round / C::kBoxes;  // 0: dV, 1: dK
         const int box = kSets == 2 ? round : round % C::kBoxes;
         const float mul = which == 0 ? 1.0f : p.scale;
@@ -988,24 +974,29 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
             st_matrix_x4(ds_base + sw128_offset(st_row + h16 * 16, (st_piece + n) * 16), w);
           }
         }
-        if (round == kEpiRounds - 1 && x.steps > 0) {  // the accumulators are read
+        if (round == kRounds - 1 && x.steps > 0) {  // the accumulators are read
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bar_accfree);
           ++active;
         }
-        fence_async_smem();
-        named_sync_and(kEpiBarrier, kEpiThreads, true);
-        if ((threadIdx.x & (kEpiThreads - 1)) == 0) {
-          tma_store_4d(which == 0 ? &map_dv : &map_dk, smem + C::kDs + set * C::kKBox, x.half * C::kDH + box * 64,
-                       x.j * kBK, x.kvh, x.b);
-          bulk_commit();
-          bulk_wait_read();
+        __syncwarp();
+        uint4 w[kRowLanes];
+#pragma unroll
+        for (int e = 0; e < kRowLanes; ++e)
+          w[e] = *reinterpret_cast<const uint4*>(
+              smem + C::kDs + set * C::kKBox +
+              sw128_offset((warp & 3) * 32 + (e * 32 + lane) / kRowLanes, first_col * 2 + lane % kRowLanes * 16));
+        __nv_bfloat16* out = (which == 0 ? p.dv : p.dk) + x.b * p.k_sb + x.kvh * p.k_sh + x.half * C::kDH + box * 64 + first_col +
+                             lane % kRowLanes * 8;
+#pragma unroll
+        for (int e = 0; e < kRowLanes; ++e) {
+          const int key = x.j * kBK + (warp & 3) * 32 + (e * 32 + lane) / kRowLanes;
+          if (key < p.skv) *reinterpret_cast<uint4*>(out + key * p.k_ss) = w[e];
         }
-        named_sync_and(kEpiBarrier, kEpiThreads, true);
+        __syncwarp();
       }
     }
-    if ((threadIdx.x & (kEpiThreads - 1)) == 0) bulk_wait();
   }
 
   tc_fence_before();
@@ -1056,13 +1047,22 @@ __global__ void __launch_bounds__(256) fa2_bwd_prep(const __nv_bfloat16* __restr
   }
 }
 
-__device__ __forceinline__ void store_row(__nv_bfloat16* out, const float4 (&v)[8], float mul) {
-  uint4* dst = reinterpret_cast<uint4*>(out);
+// 32 columns of up to 128 rows, a row per thread, turned round so that rows are stored whole
+__device__ __forceinline__ void store_rows(__nv_bfloat16* out, long long stride, int rows, const float4 (&v)[8], float mul) {
+  constexpr int kPitch = 80;  // bytes: 16-byte pieces of eight rows meet in no bank
+  __shared__ __align__(16) uint8_t tile[128 * kPitch];
+  uint4* own = reinterpret_cast<uint4*>(tile + threadIdx.x * kPitch);
 #pragma unroll
   for (int c = 0; c < 4; ++c)
-    dst[c] = make_uint4(pack_bf16x2(v[2 * c].x * mul, v[2 * c].y * mul), pack_bf16x2(v[2 * c].z * mul, v[2 * c].w * mul),
+    own[c] = make_uint4(pack_bf16x2(v[2 * c].x * mul, v[2 * c].y * mul), pack_bf16x2(v[2 * c].z * mul, v[2 * c].w * mul),
                         pack_bf16x2(v[2 * c + 1].x * mul, v[2 * c + 1].y * mul),
                         pack_bf16x2(v[2 * c + 1].z * mul, v[2 * c + 1].w * mul));
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int row = e * 32 + static_cast<int>(threadIdx.x) / 4, piece = threadIdx.x % 4;
+    if (row < rows) reinterpret_cast<uint4*>(out + row * stride)[piece] = *reinterpret_cast<const uint4*>(tile + row * kPitch + piece * 16);
+  }
 }
 
 // dq from the sums over all key tiles: scaled, rounded, in dq's layout; a block takes 32 TMEM columns of a tile.  Behind
@@ -1096,18 +1096,23 @@ __global__ void __launch_bounds__(128) fa2_bwd_finish(const __grid_constant__ Pa
     }
     __nv_bfloat16* out = p.dq + (bh / p.hq) * p.q_sb + (bh % p.hq) * p.q_sh + static_cast<long long>(i) * C::kBQ * p.q_ss + half * C::kDH;
     const int rows = min(C::kBQ, p.sq - i * C::kBQ);
-    if constexpr (C::kTransDq) {
+    if constexpr (C::kTransDq) {  // a thread has a column of 32 queries
+      __shared__ __align__(16) __nv_bfloat16 tile[32][128];
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        const float x[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int q = c0 + 4 * c + e;
-          if (q < rows) out[q * p.q_ss + row] = __float2bfloat16_rn(x[e] * p.scale);
-        }
+        tile[4 * c][row] = __float2bfloat16_rn(v[c].x * p.scale);
+        tile[4 * c + 1][row] = __float2bfloat16_rn(v[c].y * p.scale);
+        tile[4 * c + 2][row] = __float2bfloat16_rn(v[c].z * p.scale);
+        tile[4 * c + 3][row] = __float2bfloat16_rn(v[c].w * p.scale);
       }
-    } else if (row < rows) {
-      store_row(out + row * p.q_ss + c0, v, p.scale);
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int q = e * 8 + row / 16, piece = row % 16;
+        if (c0 + q < rows) reinterpret_cast<uint4*>(out + (c0 + q) * p.q_ss)[piece] = reinterpret_cast<const uint4*>(tile[q])[piece];
+      }
+    } else {
+      store_rows(out + c0, p.q_ss, rows, v, p.scale);
     }
     return;
   }
@@ -1135,9 +1140,9 @@ __global__ void __launch_bounds__(128) fa2_bwd_finish(const __grid_constant__ Pa
   }
   const int half = r % C::kSplit;
   r /= C::kSplit;
-  const long long key = static_cast<long long>(j) * kBK + row;
-  __nv_bfloat16* out = (which == 0 ? p.dv : p.dk) + (r / p.hkv) * p.k_sb + (r % p.hkv) * p.k_sh + key * p.k_ss + half * C::kDH + c0;
-  if (key < p.skv) store_row(out, v, which == 0 ? 1.0f : p.scale);
+  __nv_bfloat16* out = (which == 0 ? p.dv : p.dk) + (r / p.hkv) * p.k_sb + (r % p.hkv) * p.k_sh +
+                       static_cast<long long>(j) * kBK * p.k_ss + half * C::kDH + c0;
+  store_rows(out, p.k_ss, min(kBK, p.skv - j * kBK), v, which == 0 ? 1.0f : p.scale);
 }
 
 // How a call is cut.
@@ -1246,9 +1251,9 @@ int launch(const void* dout, const void* q, const void* k, const void* v, const 
     uint32_t box[4] = {64, rows, 1, 1};
     return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   };
-  CUtensorMap mq, mdo, mk, mv, mdk, mdv;
+  CUtensorMap mq, mdo, mk, mv;
   if (!make(&mq, q, sq, hq, C::kBQ) || !make(&mdo, dout, sq, hq, C::kBQ) || !make(&mk, k, skv, hkv, kBK) ||
-      !make(&mv, v, skv, hkv, kBK) || !make(&mdk, dk, skv, hkv, kBK) || !make(&mdv, dv, skv, hkv, kBK))
+      !make(&mv, v, skv, hkv, kBK))
     return TOKMIX_ERR_INVALID_ARGUMENT;
 
   Params p{};
@@ -1313,7 +1318,7 @@ int launch(const void* dout, const void* q, const void* k, const void* v, const 
   if (e == cudaSuccess) {
     const int grid = static_cast<int>(std::min<long long>(units, std::max(1, device_sm_count())));
     e = launch_overlapped(&fa2_bwd_kernel<D>, dim3(static_cast<unsigned>(grid)), dim3(Cfg<D>::kThreads),
-                          static_cast<size_t>(smem_bytes), stream, mq, mdo, mk, mv, mdk, mdv, p);
+                          static_cast<size_t>(smem_bytes), stream, mq, mdo, mk, mv, p);
   }
   const long long dq_blocks = p.nk > 1 ? tiles * (C::kDqCols / 32) : 0;
   const long long join_blocks = cut.part_tiles > 0 ? static_cast<long long>(batch) * hkv * C::kSplit * p.nk * 2 * (C::kDH / 32) : 0;
