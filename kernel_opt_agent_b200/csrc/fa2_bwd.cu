@@ -1300,10 +1300,16 @@ int launch(const void* dout, const void* q, const void* k, const void* v, const 
   if (units > 0x3FFFFFFFll || steps > 0x3FFFFFFFll)
     return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_fa2_bwd: too many tiles (%lld x %lld)", units, steps);
   p.units = static_cast<int>(units);
-  // The rows of a wave fill the SMs with 4 key tiles each, 8 where several heads give the turns more time (B4 Hq32
-  // Hkv8 S8192 D128: 6842 us at 4, 6623 at 8, 6779 at 16; B8 H8 S2048 D128: 281 at 2, 282 at 4, 341 at 8).
-  const int share = p.group > 1 ? 8 : 4;
-  p.wave = (std::max(1, device_sm_count()) + share - 1) / share;
+  // The rows of a wave fill the SMs with this many key tiles each: fewer wait less for each other's turns, more read the same
+  // queries together.  Several heads give the turns time, and a causal row's tiles are of different length (us, B4 Hq32 Hkv8
+  // S8192 D128 causal: 6842 at 4, 6623 at 8, 6779 at 16; D64 4235 at 4, 4115 at 8; B8 H8 S2048 causal D64: 171 at 1 and 2, 184
+  // at 4, 200 at 6; D128 280, 283, 294).  Without a mask the units are of one length, and those that start at once should be the
+  // same number of key tiles in every row: B16 H12 S512 D64, 192 rows, 86 at 2, 102 at 4; B4 H16 S2048 D128, 64 rows, 486 at
+  // 2 (2.3 a row), 445 at 4, 453 at 6.
+  const int sms = std::max(1, device_sm_count());
+  const long long kv_rows = static_cast<long long>(batch) * hkv * C::kSplit;
+  const int share = p.group > 1 ? 8 : causal || kv_rows >= (sms + 1) / 2 ? 2 : 4;
+  p.wave = (sms + share - 1) / share;
 
   const long long rows = static_cast<long long>(batch) * hq * p.nq * C::kBQ;
   const long long blocks = (rows * (D / 8) + 255) / 256;
