@@ -1167,9 +1167,13 @@ Plan plan(int batch, int hkv, int group, int nq, int nk, int causal) {
   const long long rows = static_cast<long long>(batch) * hkv * C::kSplit;
   const int sms = device_sm_count() > 0 ? device_sm_count() : 148;
   // A row's CTAs that start at once add to the same query tiles one behind the other, about 3 us each: where
-  // a row's key tiles mostly start at once, dQ is gathered in several sums (B3 Hq12 Hkv4 1000 x 1531 D64, 12 key tiles: 105
-  // us with one sum, 84 with 2, 79 with 4).  Longer calls lose more to the wider sums than to the turns.
-  best.streams = rows * nk > 2LL * sms ? 1 : nk < 4 ? std::max(1, nk) : std::min(4, nk / 4);
+  // a row's key tiles mostly start at once, dQ is gathered in several sums, as many as stay in L2 beside the rest, 72 MB.
+  // With 1, 2, 3, 4 sums, us: B3 Hq12 Hkv4 1000 x 1531 D64, 9 MB a sum, 96, 76, 72, -; B1 H2 S16384 D128, 17 MB, 598, 480,
+  // 451, 432; B1 Hq32 Hkv8 S2048 D128, 34 MB, 149, 144, 145, 148; B1 Hq8 Hkv2 S8192 D128, 34 MB, 494, 464, 458, 459; B1 Hq16 Hkv2
+  // S4096 D256, 67 MB, 640, 642, 651, 661; B2 of it, 134 MB, 1187, 1220, 1250, 1265.
+  const long long sum_bytes = std::max(1LL, rows * group * nq * (C::kDqCols * 128 * 4));
+  const long long fit = (72LL << 20) / sum_bytes;
+  best.streams = rows * nk > 2LL * sms ? 1 : static_cast<int>(std::max(1LL, std::min<long long>({fit, 4, nk < 4 ? nk : nk / 4})));
   if (nk > kMaxParted || rows * nk >= 8LL * sms) return best;  // enough whole tiles
   auto tiles = [&](int j) { return std::max(0, nq - (causal ? j * (kBK / C::kBQ) : 0)); };
   auto parts_of = [&](int j, int part_tiles) { return std::max(1, (tiles(j) + part_tiles - 1) / part_tiles); };
