@@ -127,6 +127,26 @@ def test_many_tiles_and_waves(cuda_device, d, group):
     check(3, 4 * group, 4, 1700, 1700, d, True, "bhsd", seed=d)
 
 
+@pytest.mark.parametrize("b,hq,hkv,sq,skv,d,causal", [
+    (1, 8, 1, 2048, 2048, 64, True), (1, 4, 2, 1500, 1100, 128, False), (1, 8, 1, 1024, 1024, 256, True),
+    (1, 1, 1, 4096, 512, 64, False), (1, 2, 1, 2000, 130, 128, True), (1, 3, 3, 1100, 2500, 128, True), (2, 2, 1, 700, 700, 256, False)])
+def test_few_key_tiles(cuda_device, b, hq, hkv, sq, skv, d, causal):
+    """Too few key tiles to fill the GPU: they come in parts that are joined, and dQ in several sums.  The same bits beside
+    other work on the GPU, which changes the order in which the CTAs get on."""
+    check(b, hq, hkv, sq, skv, d, causal, "bhsd", seed=sq)
+    q, k, v, do = make(b, hq, hkv, sq, skv, d, "bhsd", seed=sq)
+    o, lse = fa2.kernel_fn(q, k, v, causal, return_lse=True)
+    want = bwd.kernel_fn(do, q, k, v, o, lse, causal)
+    side, x = torch.cuda.Stream(), torch.randn(2048, 2048, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(4):
+        with torch.cuda.stream(side):
+            x @ x
+        got = bwd.kernel_fn(do, q, k, v, o, lse, causal)
+        assert all(torch.equal(a, c) for a, c in zip(got, want))
+    torch.cuda.synchronize()
+
+
 def test_custom_scale_and_sharp_rows(cuda_device):
     check(1, 4, 2, 300, 300, 128, True, "bhsd", seed=3, scale=0.3)
     check(1, 2, 1, 300, 333, 64, False, "bshd", seed=4, q_scale=6.0)   # weights of nearly one key
