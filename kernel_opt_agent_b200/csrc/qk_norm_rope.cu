@@ -454,12 +454,16 @@ __global__ void __launch_bounds__(kThreads, kBwdPerSm) qk_norm_rope_bwd_kernel(c
           sum += __shfl_xor_sync(0xffffffffu, sum, m);
           dot += __shfl_xor_sync(0xffffffffu, dot, m);
         }
-        const float inv = rsqrtf(sum * (1.0f / D) + p.eps);
-        const float back = -inv * inv * (dot * (1.0f / D));
+        // Where the iteration has no head, its zeros would, without eps, add 0 * inf to the weights' sums.  (Chosen before the sum is
+        // there: no time; a choice behind the root 1.5 %.)
+        const float inv = rsqrtf(fmaf(sum, 1.0f / D, h < r.heads ? p.eps : 1.0f));
+        // x r before r again: without eps, r^2 alone passes fp32's range where x r^2 does not
+        const float back = -inv * (dot * (1.0f / D));
         const F2 inv2 = pair2(inv, inv), back2 = pair2(back, back);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          acc[kind][e] = fma2(g[e], mul2(x[e], inv2), acc[kind][e]);
+          x[e] = mul2(x[e], inv2);
+          acc[kind][e] = fma2(g[e], x[e], acc[kind][e]);
           x[e] = mul2(inv2, fma2(back2, x[e], o[e]));
         }
         if (h < r.heads) *reinterpret_cast<uint4*>(dst) = narrow<T>(x);
