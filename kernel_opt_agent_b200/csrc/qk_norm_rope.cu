@@ -560,10 +560,11 @@ int prepare(const char* who, const tokmix_qk_norm_rope* a, bool backward, Params
     return fail(TOKMIX_ERR_UNSUPPORTED, "%s: bf16 or fp16 tensors with weights of that type or fp32", who);
   if (a->half <= 0 || a->half % 8 != 0 || a->nope < 0 || a->nope % 8 != 0 || a->nope + 2 * a->half > a->head_dim)
     return fail(TOKMIX_ERR_INVALID_ARGUMENT, "%s: half and nope must be multiples of 8 with nope + 2 half <= head_dim", who);
-  if (a->axes < 1 || a->axes > 4 || (a->axes > 1 && (a->positions == nullptr || a->pair_axis == nullptr)))
+  p.tokens = static_cast<long long>(a->batch) * a->seqlen;  // without any, positions may be an empty tensor's address, null
+  if (a->axes < 1 || a->axes > 4 || (a->axes > 1 && ((a->positions == nullptr && p.tokens > 0) || a->pair_axis == nullptr)))
     return fail(TOKMIX_ERR_INVALID_ARGUMENT, "%s: 1 to 4 position axes; several need positions and an axis per pair", who);
   if (!(a->eps >= 0.0f) || !std::isfinite(a->eps)) return fail(TOKMIX_ERR_INVALID_ARGUMENT, "%s: eps must be finite and not negative", who);
-  if (a->table_rows <= 0 || (a->positions == nullptr && a->table_rows < a->seqlen))
+  if (a->table_rows <= 0 || (a->positions == nullptr && p.tokens > 0 && a->table_rows < a->seqlen))
     return fail(TOKMIX_ERR_INVALID_ARGUMENT, "%s: the tables must have a row for every position", who);
   for (const long long s : {a->q_batch_stride, a->q_token_stride, a->q_head_stride, a->k_batch_stride, a->k_token_stride,
                             a->k_head_stride})
@@ -572,7 +573,6 @@ int prepare(const char* who, const tokmix_qk_norm_rope* a, bool backward, Params
     for (const long long s : {a->dq_batch_stride, a->dq_token_stride, a->dq_head_stride, a->dk_batch_stride, a->dk_token_stride,
                               a->dk_head_stride})
       if (s % 8 != 0) return fail(TOKMIX_ERR_INVALID_ARGUMENT, "%s: strides must be multiples of 8 elements", who);
-  p.tokens = static_cast<long long>(a->batch) * a->seqlen;
   if (p.tokens > 0x7FFFFFFFll) return fail(TOKMIX_ERR_UNSUPPORTED, "%s: too many tokens (%lld)", who, p.tokens);
   if (a->heads_q > 65536 || a->heads_k > 65536) return fail(TOKMIX_ERR_UNSUPPORTED, "%s: more than 65536 heads", who);
   if (p.tokens == 0 && !backward) return TOKMIX_OK;
