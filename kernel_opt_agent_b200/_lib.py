@@ -258,7 +258,7 @@ def check_status(device: torch.device, what: str) -> None:
 
 
 class _HostStatus:
-    """A status word in pinned host memory that the kernels of a device store to when they meet bad
+    """A status word in pinned host memory that an operator's kernels store to when they meet bad
     device-side arguments: looking at it costs no launch, copy or synchronisation, so every call
     does, inside a graph capture too."""
 
@@ -268,27 +268,34 @@ class _HostStatus:
         self.word = ctypes.c_uint32.from_address(self.ptr)
 
 
-_host_status: dict[int, _HostStatus] = {}
+# operators with words of their own (an operator and its gradient, or the calls on one cache, share theirs), so that an
+# error is raised by the operator that met it; by device and operator
+_HOST_STATUS_OPERATORS = ("kv8", "qk_norm_rope", "flash_attention_2_bwd")
+_host_status: dict[tuple[int, str], _HostStatus] = {}
 
 
 def host_status_ptr(device: torch.device, what: str) -> int | None:
-    """Raises if an earlier launch on `device` stored a bit in the host status word (and clears it), else
-    its address for the next launch (None for a first call inside a graph capture, where it cannot be
-    allocated).  With TOKMIX_CHECK_STATUS=0 the launch gets it all the same and only explicit checks look at it."""
-    h = _host_status.get(device.index)
+    """Raises if an earlier launch of operator `what` on `device` stored a bit in its host status word (and clears it),
+    else the word's address for the next launch.  The first call of any operator on a device allocates the words of
+    all; inside a graph capture, where they cannot be allocated, it gets None.  With TOKMIX_CHECK_STATUS=0 the launch
+    gets the address all the same and only explicit checks look at the word."""
+    h = _host_status.get((device.index, what))
     if h is None:
         if torch.cuda.is_current_stream_capturing():
             return None
         with _lock:
-            h = _host_status.setdefault(device.index, _HostStatus())
+            for name in _HOST_STATUS_OPERATORS:
+                if (device.index, name) not in _host_status:
+                    _host_status[device.index, name] = _HostStatus()
+        h = _host_status[device.index, what]
     if h.word.value and _STATUS_MODE != "off":
         take_host_status(device, what)
     return h.ptr
 
 
 def take_host_status(device: torch.device, what: str) -> None:
-    """Raises TokmixDeviceError if the host status word of `device` holds a bit; clears it first."""
-    h = _host_status.get(device.index)
+    """Raises TokmixDeviceError if operator `what`'s host status word of `device` holds a bit; clears it first."""
+    h = _host_status.get((device.index, what))
     if h is not None and h.word.value:
         val, h.word.value = h.word.value, 0
         _raise_for(val, what)

@@ -20,7 +20,7 @@ positions: int32 [B, S], the table row of every token; None: its index in its se
 (n_0, .., n_{A-1}), which add up to half (images: time, height, width), positions is [A, B, S] and every pair takes the row of one
 axis: the first n_0 pairs axis 0, the next n_1 axis 1, and so on; or, ``interleaved``, pair j axis j % A while j < A * n_axis
 and axis 0 behind that.  A position outside the tables makes the token's rotated columns NaN and is
-reported as ``TokmixDeviceError`` by a later call or by ``check_device_status``.  Squares are summed in fp32: a row whose
+reported as ``TokmixDeviceError`` by a later call of this module or its gradient's, or by ``check_device_status``.  Squares are summed in fp32: a row whose
 squares add up to 2^128 overflows (magnitudes of 2^60, D 256); with ``eps=0``, which is allowed, a row of zeros is 0 / 0 (NaN, in the
 weights' gradients too), and one of magnitudes below 2^-62 loses digits of its squares, below 2^-74 all of them.
 
