@@ -264,34 +264,6 @@ __device__ __forceinline__ bool wait_turn(const uint32_t* turn, uint32_t want, u
   }
 }
 
-// Two fp32 values in a register pair, and Blackwell's arithmetic on them
-using F2 = unsigned long long;
-__device__ __forceinline__ F2 pair2(uint32_t a, uint32_t b) {
-  F2 v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b));
-  return v;
-}
-__device__ __forceinline__ float2 split2(F2 v) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-  return f;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 // 16 lanes x 8 N columns of TMEM, dealt out like an mma accumulator: thread l gets, of every 8 columns i,
 // r[4i], r[4i+1] = columns 2 (l % 4), + 1 of lane l / 4 and r[4i+2], r[4i+3] the same of lane l / 4 + 8.
 // No wait.
@@ -348,10 +320,8 @@ __device__ __forceinline__ void st_matrix_x4(uint32_t addr, const uint32_t* r) {
 
 template <int N>
 __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[N]) {
-  static_assert(N == 32 || N == 64 || N == 128, "columns");
-  if constexpr (N == 32) {
-    tmem_ld32(addr, r);
-  } else if constexpr (N == 64) {
+  static_assert(N == 64 || N == 128, "columns");
+  if constexpr (N == 64) {
     tmem_ld64(addr, r);
   } else {
     tmem_ld64(addr, *reinterpret_cast<uint32_t(*)[64]>(&r[0]));
@@ -726,7 +696,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
             } else {
 #pragma unroll
               for (int c = 0; c < C::kDqCols / 4; ++c) {
-                if (C::kPace > 0 && c % 4 == 0 && c > 0)
+                if (c % 4 == 0 && c > 0)
                   for (const long long t0 = clock64(); clock64() - t0 < C::kPace;) {}
                 red_add_v4(acc + c * 512, __uint_as_float(v[4 * c]), __uint_as_float(v[4 * c + 1]),
                            __uint_as_float(v[4 * c + 2]), __uint_as_float(v[4 * c + 3]));
@@ -1363,7 +1333,7 @@ int launch(const void* dout, const void* q, const void* k, const void* v, const 
   return check_launch("tokmix_fa2_bwd");
 }
 
-// Checks shared by the entry points; 0 for a head_dim without a kernel
+// The function for a head_dim, or `otherwise` where there is no kernel for it
 template <typename F64, typename F128, typename F256>
 auto by_head_dim(int head_dim, F64 f64, F128 f128, F256 f256, decltype(f64()) otherwise) {
   return head_dim == 64 ? f64() : head_dim == 128 ? f128() : head_dim == 256 ? f256() : otherwise;

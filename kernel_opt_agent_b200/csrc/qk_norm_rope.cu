@@ -10,7 +10,7 @@
 //   dw = sum over rows of g x r,   dx = r (g w - x r^2 mean(g w x))
 //
 // Both are streams: a few flops per byte, bound by HBM (forward 4 bytes an element, backward 6) or, for
-// few rows, by latency.  A row lies in D / 8 lanes, 8 columns (16 bytes) each, so a warp holds 32 / (D / 8) heads
+// few rows, by latency; next to HBM stand the issue slots, so values are computed in pairs.  A row lies in D / 8 lanes, 8 columns (16 bytes) each, so a warp holds 32 / (D / 8) heads
 // of a token at a time (an iteration); sums are butterflies over a row's lanes.  Every warp takes an equal share of all
 // iterations, token by token: the cos and sin of its columns are read once per token and serve its heads.
 // The rows come through a ring of kDepth iterations per warp in shared memory (cp.async, each lane its own 16
@@ -81,30 +81,6 @@ template <>
 __device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
   __half2 v = __floats2half2_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&v);
-}
-
-// Two fp32 values in a register pair, and Blackwell's arithmetic on them (half the instructions; the kernels
-// are issue-bound before they are HBM-bound).
-using F2 = unsigned long long;
-__device__ __forceinline__ F2 pair2(float a, float b) {
-  F2 v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
-  return v;
-}
-__device__ __forceinline__ float2 split2(F2 v) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-  return f;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
 }
 
 template <typename T>

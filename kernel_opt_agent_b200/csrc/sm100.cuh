@@ -416,4 +416,33 @@ __device__ __forceinline__ float max3f(float a, float b, float c) {
   return d;
 }
 
+// Two fp32 values in a register pair, and Blackwell's arithmetic on them (half the instructions)
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pair2(uint32_t a, uint32_t b) {
+  F2 v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b));
+  return v;
+}
+__device__ __forceinline__ F2 pair2(float a, float b) { return pair2(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ float2 split2(F2 v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 }  // namespace tokmix
