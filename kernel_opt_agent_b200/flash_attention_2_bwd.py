@@ -10,9 +10,10 @@ both layouts).  With P = exp(sm_scale q k^T - lse) under the mask and delta = su
     dv = P^T do,   dS = P * (do v^T - delta),   dq = sm_scale dS k,   dk = sm_scale dS^T q
 
 dk and dv are summed over the query heads that share a key/value head.  P and dS enter their products in
-bf16, sums are fp32, and every sum has an order that sizes alone decide: the same bits every time.
-A key or value that no query sees gets zeros.  Tensors that are not contiguous (a gradient that autograd
-expanded, say) are copied first.
+bf16, sums are fp32, and every sum has an order that the sizes and the GPU's number of SMs decide: the same bits every time.
+A key or value that no query sees gets zeros.  What is masked is replaced in P and dS, whose products are then taken whole: a value
+of v that is not finite stays out of the rows that do not see it, one of q, k or do can reach other rows of its tile.
+Tensors that are not contiguous (a gradient that autograd expanded, say) are copied first.
 
 ``kernel_fn`` runs ``tokmix_fa2_bwd`` (``csrc/fa2_bwd.cu``), no fallback.  ``training.attention`` is the forward
 and this in one differentiable call."""

@@ -19,10 +19,12 @@ cos, sin [rows, half] fp32 are tables by position; the 2 * half columns behind t
 positions: int32 [B, S], the table row of every token; None: its index in its sequence.  With ``sections`` =
 (n_0, .., n_{A-1}), which add up to half (images: time, height, width), positions is [A, B, S] and every pair takes the row of one
 axis: the first n_0 pairs axis 0, the next n_1 axis 1, and so on; or, ``interleaved``, pair j axis j % A while j < A * n_axis
-and axis 0 behind that.  A position outside the tables makes the token's rotated columns NaN and is
-reported as ``TokmixDeviceError`` by a later call of this module or its gradient's, or by ``check_device_status``.  Squares are summed in fp32: a row whose
-squares add up to 2^128 overflows (magnitudes of 2^60, D 256); with ``eps=0``, which is allowed, a row of zeros is 0 / 0 (NaN, in the
-weights' gradients too), and one of magnitudes below 2^-62 loses digits of its squares, below 2^-74 all of them.
+and axis 0 behind that.  A position outside the tables makes the token's rotated columns NaN and is reported as
+``TokmixDeviceError`` by a later call of this module or of its gradient, or by ``check_device_status``.
+
+Squares are summed in fp32: a row whose squares add up to 2^128 overflows (magnitudes of 2^60, D 256).  ``eps`` may be 0: a row of
+zeros is then 0 / 0 (NaN, in the weights' gradients too), and one of magnitudes below 2^-62 loses digits of its squares, below 2^-74
+all of them.
 
 ``kernel_fn`` runs ``tokmix_qk_norm_rope_fwd`` (``csrc/qk_norm_rope.cu``), no fallback.  ``training.qk_norm_rope`` is this with
 its gradient (``qk_norm_rope_bwd``) behind autograd."""

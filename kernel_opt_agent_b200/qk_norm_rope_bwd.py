@@ -11,7 +11,7 @@ position's angles:
     dweight = sum over rows of g x r,    dx = r (g weight - x r^2 mean(g weight x))
 
 fp32 arithmetic.  dq, dk are contiguous in the type of q; the weights' gradients are summed over all tokens and heads in fp32 in
-an order that sizes alone decide (the same bits every time) and rounded to the weights' type.
+an order that the sizes and the GPU's number of SMs decide (the same bits every time) and rounded to the weights' type.
 
 ``kernel_fn`` runs ``tokmix_qk_norm_rope_bwd`` (``csrc/qk_norm_rope.cu``), no fallback."""
 

@@ -6,8 +6,8 @@
 
 Each is its plugin modules' ``kernel_fn`` (``qk_norm_rope`` and ``qk_norm_rope_bwd``, ``flash_attention_2`` and
 ``flash_attention_2_bwd``), with their arguments, checks and errors; cos, sin and positions get no gradient.  The gradients
-are those of the first order only.  Between the passes attention keeps q, k, v, its output and one fp32 number per row,
-qk_norm_rope its inputs.
+are those of the first order only, in contiguous tensors.  Between the passes attention keeps q, k, v (copies of those that are not
+contiguous), its output and one fp32 number per row, qk_norm_rope its inputs.
 
 A step that is to be captured into a CUDA graph makes its first calls before the capture (as every module here), and its
 autograd graph inside it; a graph of the same leaves that was built outside should be gone by then (autograd accumulates on
