@@ -1372,10 +1372,10 @@ extern "C" int tokmix_fa2_bwd(const void* dout, const void* q, const void* k, co
     return fail(TOKMIX_ERR_INVALID_ARGUMENT, "tokmix_fa2_bwd: sm_scale must be finite and positive");
   if (head_dim != 64 && head_dim != 128 && head_dim != 256)
     return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_fa2_bwd: head_dim %d not supported (64, 128 or 256)", head_dim);
-  if (std::max(seqlen_q, seqlen_kv) > 0x7FFFFFFF - (fa2b::kBK - 1))  // whole tiles are counted in int
-    return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_fa2_bwd: too many tokens (%d, %d)", seqlen_q, seqlen_kv);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (batch == 0 || (seqlen_q == 0 && seqlen_kv == 0)) return TOKMIX_OK;
+  if (std::max(seqlen_q, seqlen_kv) > 0x7FFFFFFF - (fa2b::kBK - 1))  // whole tiles are counted in int
+    return fail(TOKMIX_ERR_UNSUPPORTED, "tokmix_fa2_bwd: too many tokens (%d, %d)", seqlen_q, seqlen_kv);
   if (seqlen_kv == 0)
     return fail(TOKMIX_ERR_INVALID_ARGUMENT, "tokmix_fa2_bwd: seqlen_kv must be positive when seqlen_q is");
   for (const void* ptr : {k, v, static_cast<const void*>(dk), static_cast<const void*>(dv)})
