@@ -321,7 +321,8 @@ int tokmix_add_rms_norm_quant(const void* x, const void* residual, const void* w
  * of 8, head_dim contiguous, 16-byte aligned.  For every head row x with its weight w [head_dim] (`weight_dtype`: dtype or fp32):
  *   n = x / sqrt(mean x^2 + eps) * w;  y = n with the pairs (j, j + half) of the 2 half columns behind `nope` rotated:
  *   y_j = n_j cos - n_{j+half} sin,  y_{j+half} = n_j sin + n_{j+half} cos
- * in fp32, rounded once; eps >= 0 (with 0, a row of zeros is NaN, in the weights' gradients too).  cos, sin: fp32 [table_rows, half].  positions: the table row of every token, int32 [axes, batch, seqlen], or
+ * in fp32, rounded once; eps >= 0 (with 0, a row of zeros is NaN, in the weights' gradients too).  cos, sin: fp32
+ * [table_rows, half].  positions: the table row of every token, int32 [axes, batch, seqlen], or
  * NULL: the token's index in its sequence (axes 1).  axes 2 to 4: pair j takes its row from axis pair_axis[j] (host memory,
  * half entries, read during the call).  head_dim 64, 128 or 256; half and nope multiples of 8, half > 0.
  * Forward: q_out, k_out contiguous [batch, seqlen, heads, head_dim].  Backward: dq, dk are the gradients of those outputs (strides
@@ -350,8 +351,8 @@ typedef struct tokmix_qk_norm_rope {
 int tokmix_qk_norm_rope_fwd(const tokmix_qk_norm_rope* args, uint32_t* status, void* stream);
 
 /* The gradients; dq_weight, dk_weight [head_dim] in weight_dtype are summed over all tokens and heads in fp32, in an order that
- * the sizes and the device's number of SMs decide.  workspace: tokmix_qk_norm_rope_bwd_workspace_bytes(batch * seqlen, ...) bytes of device memory, 16-byte aligned,
- * not shared by calls that may overlap. */
+ * the sizes and the device's number of SMs decide.  workspace: tokmix_qk_norm_rope_bwd_workspace_bytes(batch * seqlen, ...)
+ * bytes of device memory, 16-byte aligned, not shared by calls that may overlap. */
 int tokmix_qk_norm_rope_bwd(const tokmix_qk_norm_rope* args, void* dq_weight, void* dk_weight, void* workspace,
                             long long workspace_bytes, uint32_t* status, void* stream);
 long long tokmix_qk_norm_rope_bwd_workspace_bytes(long long tokens, int heads_q, int heads_k, int head_dim);

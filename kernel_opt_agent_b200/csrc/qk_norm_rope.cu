@@ -10,8 +10,8 @@
 //   dw = sum over rows of g x r,   dx = r (g w - x r^2 mean(g w x))
 //
 // Both are streams: a few flops per byte, bound by HBM (forward 4 bytes an element, backward 6) or, for
-// few rows, by latency; next to HBM stand the issue slots, so values are computed in pairs.  A row lies in D / 8 lanes, 8 columns (16 bytes) each, so a warp holds 32 / (D / 8) heads
-// of a token at a time (an iteration); sums are butterflies over a row's lanes.  Every warp takes an equal share of all
+// few rows, by latency; next to HBM stand the issue slots, so values are computed in pairs.  A row lies in
+// D / 8 lanes, 8 columns (16 bytes) each, so a warp holds 32 / (D / 8) heads of a token at a time (an iteration); sums are butterflies over a row's lanes.  Every warp takes an equal share of all
 // iterations, token by token: the cos and sin of its columns are read once per token and serve its heads.
 // The rows come through a ring of kDepth iterations per warp in shared memory (cp.async, each lane its own 16
 // bytes), which runs ahead across tokens: what is in flight costs no registers (with loads into registers, 16 warps of 100
