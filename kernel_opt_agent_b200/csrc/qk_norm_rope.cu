@@ -430,8 +430,8 @@ __global__ void __launch_bounds__(kThreads, kBwdPerSm) qk_norm_rope_bwd_kernel(c
           sum += __shfl_xor_sync(0xffffffffu, sum, m);
           dot += __shfl_xor_sync(0xffffffffu, dot, m);
         }
-        // Where the iteration has no head, its zeros would, without eps, add 0 * inf to the weights' sums.  (Chosen before the sum is
-        // there: no time; a choice behind the root 1.5 %.)
+        // Where the iteration has no head, its zeros would, without eps, add 0 * inf to the weights' sums.  Chosen here, before the
+        // sum is there, it takes no time: B2 S4096 Hq16 Hkv2 D256, three axes, 45.8 us (45.7 without it, 46.4 chosen behind the root).
         const float inv = rsqrtf(fmaf(sum, 1.0f / D, h < r.heads ? p.eps : 1.0f));
         // x r before r again: without eps, r^2 alone passes fp32's range where x r^2 does not
         const float back = -inv * (dot * (1.0f / D));
